@@ -51,10 +51,13 @@ FAMILIES: Dict[str, List[str]] = {
     "gemm_mid_tcgen05": ["gemm_mid_tcgen05.cu"],
     "gemm_f32": ["gemm_f32.cu"],
     "gemm_f32_tcgen05": ["gemm_f32_tcgen05.cu"],
+    "microscaling": ["microscaling.cu"],
+    "gemm_mx_tcgen05": ["gemm_mx_tcgen05.cu"],
     "host_core": ["host_core.cpp"],            # the host side's bookkeeping: plain C++, no device code
 }
 HOST_FAMILIES = {"host_core"}
-HEADERS = ["common.cuh", "mma_tiles.cuh", "split_mma.cuh", "tcgen05_attention.cuh", "attention_decode_noalloc.h", "attention_decode_tma.cuh"]
+HEADERS = ["common.cuh", "mma_tiles.cuh", "split_mma.cuh", "tcgen05_attention.cuh", "attention_decode_noalloc.h", "attention_decode_tma.cuh",
+           "microscaling.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

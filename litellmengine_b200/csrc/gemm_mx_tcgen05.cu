@@ -1,0 +1,338 @@
+// y[T, N] = x[T, K] . w[N, K]^T of microscaled operands: rows of 8 bits, weights of 4 (microscaling.cuh has the formats), for any
+// number of rows, on the block-scaled products of the 5th-generation tensor cores (tcgen05.mma.kind::mxf8f6f4.block_scale).
+//
+//   y[t, n] = sum over blocks b of sx[t, b] * sw[n, b] * (sum over the 32 values of b of x * w)
+// The products of e4m3 and e2m1 values and powers of two are exact; the sums are kept in float32.
+//
+// The weights are the left operand (128 features a tile), the tokens the right one (NT of them), so that no lane is spent on tokens
+// that are not there.  A stage is 128 values of K: a box of the weight's tile (8 KB; the copy engine spreads its 4-bit codes over
+// 16 KB, sixteen of them and eight bytes of nothing, as the products read them), a box of the rows, and the pieces of both operands'
+// scales, which the tensor core copies to its own memory in front of the stage's four products.
+// Roles: warp 0 feeds the copy engine, warp 1 issues, warps 2 to 5 take the sums; all six write the result.  Waits are bounded: one that
+// runs out sets status code 12, and the feeding thread waits for its last copies before the CTA ends.
+//   * Few rows: bytes bound the product.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the
+//     parts' order; nothing is left for another kernel and no result depends on timing.  The first weights are on their way before the
+//     CTA waits for the kernel in front.
+//   * Gate and up: a tile is 64 gate features and the 64 up features beside them; act(gate) * up leaves as rows of 8 bits.
+#include "microscaling.cuh"
+#include "tcgen05_attention.cuh"
+
+#define MG_ROWS 128               // features of a tile (gated: 64 of both)
+#define MG_THREADS 192
+#define MG_W_BYTES (MG_ROWS * MX_K)       // of a stage's weights in shared memory
+#define MG_W_READ (MG_W_BYTES / 2)        // the same as the copy engine counts them: what it reads
+#define MG_STATUS 12
+
+__device__ __forceinline__ bool mg_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    for (int i = 0; i < waits; ++i) {
+        if (t5_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    if (atomicCAS(status, 0, MG_STATUS) == 0) status[1] = blockIdx.y;
+    return false;
+}
+__device__ __forceinline__ void mg_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(t5_smem(dst)), "l"(src), "r"(bytes),
+                 "r"(t5_smem(bar)) : "memory");
+}
+// A piece of scales to tensor memory: 32 lanes of 16 bytes, repeated in every quarter of the lanes.
+__device__ __forceinline__ void mg_scales_lead(unsigned lead, unsigned tmem, unsigned long long desc) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(tmem), "l"(desc), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mg_mma_lead(unsigned lead, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc,
+                                            unsigned a_scales, unsigned b_scales, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 q, %7, 0;\n"
+                 " @q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::
+                     "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(lead) : "memory");
+}
+// 32 lanes of 16 bytes without a swizzle, groups of eight lanes 128 bytes apart.
+__device__ __forceinline__ unsigned long long mg_scale_desc(const void* smem) {
+    return static_cast<unsigned long long>((t5_smem(smem) & 0x3FFFF) >> 4) | (static_cast<unsigned long long>(128 >> 4) << 32) | (1ull << 46);
+}
+// Instruction descriptor: A e2m1, B e4m3, both K-major, scales powers of two; `block`: which of the four scales of a word, for both.
+__host__ __device__ constexpr unsigned mg_idesc(int n, unsigned block) {
+    return (block << 4) | (5u << 7) | (0u << 10) | (static_cast<unsigned>(n >> 3) << 17) | (1u << 23) | ((MG_ROWS >> 4) << 24) | (block << 29);
+}
+
+struct MgArgs {
+    const unsigned char *w_scales, *x_scales;
+    void* y;                              // [T, N]; gated: the codes [T, out_kpad]
+    unsigned char* y_scales;              // gated
+    int T, N, ktiles, out_kpad, vec, act, waits;
+    float limit;
+    int32_t* status;
+};
+enum { MG_STORE = 0, MG_ADD = 1, MG_GATED = 2 };
+
+// grid (parts of K, tiles of features, tiles of tokens), a cluster the parts of a tile.
+template <int NT, int STAGES, int MODE, typename TO>
+__global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel(const __grid_constant__ CUtensorMap w_map,
+                                                                               const __grid_constant__ CUtensorMap x_map, const MgArgs a) {
+    constexpr int X_PIECES = NT > 128 ? 2 : 1;
+    constexpr unsigned X_BYTES = NT * MX_K, S_BYTES = (1 + X_PIECES) * MX_PIECE;
+    constexpr unsigned S_COLS = 4 * (1 + X_PIECES), S_COL0 = NT < 32 ? 32 : NT;
+    constexpr unsigned COLS = S_COL0 + STAGES * S_COLS <= 128 ? 128 : S_COL0 + STAGES * S_COLS <= 256 ? 256 : 512;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    unsigned char* x_s = w_s + STAGES * MG_W_BYTES;               // [STAGES][NT][128], 128-byte swizzle like the weights
+    unsigned char* s_s = x_s + STAGES * X_BYTES;                  // [STAGES][weights' piece, rows' pieces]
+    float* sums = reinterpret_cast<float*>(w_s);                  // [NT][128], when the stages have been read
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full;
+    __shared__ unsigned tmem_base_s;
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int part = blockIdx.x, parts = gridDim.x, tile = blockIdx.y, tok0 = blockIdx.z * NT;
+    const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
+        t5_mbar_init(&acc_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    t5_fence_before();
+    __syncthreads();
+    t5_fence_after();
+    pdl_invite();                                                 // not before: this CTA's tensor memory is taken
+    const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
+
+    int issued = 0;                                               // stages that were asked for, in the thread that asks
+    if (warp == 0) {
+        if (lane == 0) {
+            auto weights = [&](int kb) {
+                const int st = kb % STAGES;
+                const long long at = static_cast<long long>(tile) * a.ktiles + kb0 + kb;
+                t5_expect_tx(&full[st], MG_W_READ + X_BYTES + S_BYTES);
+                t5_tma_2d(w_s + st * MG_W_BYTES, &w_map, 0, static_cast<int>(at * MG_ROWS), &full[st]);
+                mg_copy(s_s + st * S_BYTES, a.w_scales + at * MX_PIECE, MX_PIECE, &full[st]);
+            };
+            auto tokens = [&](int kb) {
+                const int st = kb % STAGES;
+                t5_tma_2d(x_s + st * X_BYTES, &x_map, (kb0 + kb) * MX_K, tok0, &full[st]);
+#pragma unroll
+                for (int p = 0; p < X_PIECES; ++p)
+                    mg_copy(s_s + st * S_BYTES + (1 + p) * MX_PIECE, a.x_scales + (static_cast<size_t>(tok0 / 128 + p) * a.ktiles + kb0 + kb) * MX_PIECE,
+                            MX_PIECE, &full[st]);
+            };
+            const int first = min(STAGES, kbs);
+            for (int kb = 0; kb < first; ++kb) weights(kb);       // nobody's output
+            pdl_wait();
+            for (int kb = 0; kb < first; ++kb) tokens(kb);
+            issued = first;
+            for (int kb = STAGES; kb < kbs; ++kb) {
+                if (!mg_wait(&empty[kb % STAGES], (kb / STAGES - 1) & 1, a.waits, &abort_flag, a.status)) break;
+                weights(kb);
+                tokens(kb);
+                issued = kb + 1;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        pdl_wait();
+        const unsigned lead = elect_one();
+        const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024), sd = mg_scale_desc(s_s);
+        bool ok = true;
+#pragma unroll 1
+        for (int kb = 0; kb < kbs; ++kb) {
+            const int st = kb % STAGES;
+            ok = __all_sync(0xffffffffu, mg_wait(&full[st], (kb / STAGES) & 1, a.waits, &abort_flag, a.status));
+            if (!ok) break;
+            const unsigned sc = tmem + S_COL0 + st * S_COLS;      // a place of its own for each stage: earlier products may still read theirs
+#pragma unroll
+            for (int p = 0; p <= X_PIECES; ++p) mg_scales_lead(lead, sc + 4 * p, sd + ((st * S_BYTES + p * MX_PIECE) >> 4));
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                mg_mma_lead(lead, tmem, wd + st * (MG_W_BYTES >> 4) + 2 * k, xd + st * (X_BYTES >> 4) + 2 * k, mg_idesc(NT, k), sc, sc + 4, (kb | k) ? 1u : 0u);
+            t5_commit_lead(lead, &empty[st]);
+        }
+        if (ok) t5_commit_lead(lead, &acc_full);
+    } else {
+        pdl_wait();
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full, 0, a.waits, &abort_flag, a.status));
+        t5_fence_after();
+        if (ok)
+#pragma unroll 1
+            for (int c = 0; c < NT / 16; ++c) {
+                unsigned r[16];
+                t5_ld16(tmem + (static_cast<unsigned>(quarter * 32) << 16) + 16 * c, r);
+                t5_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sums[(16 * c + i) * MG_ROWS + row] = __uint_as_float(r[i]);
+            }
+    }
+    t5_fence_before();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every part's sums are there
+    {
+        const unsigned base = t5_smem(sums);
+        auto total = [&](int at) {                                // the parts' sums in order, four features, all parts' loads in flight at once
+            float4 f[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < parts) {
+                    unsigned addr;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(addr) : "r"(base + 4u * at), "r"(p));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(f[p].x), "=f"(f[p].y), "=f"(f[p].z), "=f"(f[p].w) : "r"(addr));
+                }
+            float4 v = f[0];
+#pragma unroll
+            for (int p = 1; p < 8; ++p)
+                if (p < parts) v.x += f[p].x, v.y += f[p].y, v.z += f[p].z, v.w += f[p].w;
+            return v;
+        };
+        const int toks = min(NT, a.T - tok0);
+        if constexpr (MODE == MG_GATED) {
+            // sixteen lanes a token, four features a lane, eight lanes a block
+            const int f = 4 * (tid & 15), step = MG_THREADS / 16 * parts;
+            unsigned char* codes = static_cast<unsigned char*>(a.y);
+#pragma unroll 1
+            for (int t0 = 0; t0 < toks; t0 += step) {
+                const int tok = t0 + part + (tid >> 4) * parts;
+                const bool there = tok < toks;
+                const float4 g = total((there ? tok : 0) * MG_ROWS + f), u = total((there ? tok : 0) * MG_ROWS + 64 + f);
+                float v[4] = {gated(g.x, u.x, a.act, a.limit), gated(g.y, u.y, a.act, a.limit), gated(g.z, u.z, a.act, a.limit),
+                              gated(g.w, u.w, a.act, a.limit)};
+                unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
+#pragma unroll
+                for (int o = 1; o < 8; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const unsigned scale = mx_scale<MX_E4M3>(most);
+                const float inv = mx_inverse(scale);
+                if (there) {
+                    const size_t t = tok0 + tok;
+                    *reinterpret_cast<unsigned*>(codes + t * a.out_kpad + tile * 64 + f) = mx_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    if ((tid & 7) == 0) a.y_scales[mx_scale_at(t, (tile * 64 + f) / MX_BLOCK, a.out_kpad / MX_K)] = static_cast<unsigned char>(scale);
+                }
+            }
+        } else {
+            TO* y = static_cast<TO*>(a.y);
+            const int f = tile * MG_ROWS + 4 * lane;
+#pragma unroll 2
+            for (int tok = part + warp * parts; tok < toks; tok += MG_THREADS / 32 * parts) {
+                const float4 t = total(tok * MG_ROWS + 4 * lane);
+                float ts[4] = {t.x, t.y, t.z, t.w};
+                TO* to = y + static_cast<size_t>(tok0 + tok) * a.N + f;
+                if (a.vec) {                                      // N a multiple of 4, y aligned
+                    if (f < a.N) {
+                        if constexpr (sizeof(TO) == 4) {
+                            float4 v = t;
+                            if (MODE == MG_ADD) {
+                                const float4 o = *reinterpret_cast<const float4*>(to);
+                                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                            }
+                            *reinterpret_cast<float4*>(to) = v;
+                        } else {
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(ts[0], ts[1]), hi = __floats2bfloat162_rn(ts[2], ts[3]);
+                            *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (f + i < a.N) to[i] = from_f32<TO>(MODE == MG_ADD ? ts[i] + to_f32(to[i]) : ts[i]);
+                }
+            }
+        }
+    }
+    if (tid == 0 && abort_flag)                                   // whoever gave up: what is in flight lands before the CTA goes away
+        for (int kb = max(0, issued - STAGES); kb < issued; ++kb)
+            for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(&full[kb % STAGES], (kb / STAGES) & 1); ++i) {}
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // nobody leaves while its sums are read
+    if (warp == 1) {
+        t5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(COLS) : "memory");
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+static int mg_sms() {                     // of the current device
+    static int sms[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms[dev] = 0;
+    return sms[dev];
+}
+
+// 4-bit codes, tiles of 128 rows of 64 bytes, spread by the copy engine; 8-bit rows [T, kpad] in boxes of NT rows x 128 values.
+static bool mg_maps(CUtensorMap* w_map, CUtensorMap* x_map, const void* w, long long w_rows, const void* x, int T, int kpad, int nt) {
+    CUtensorMap any;
+    if (g_t5_state == 0) (void)t5_encode_2d(&any, w, 64, 64, 64, 64);        // finds the driver's entry point
+    if (g_t5_state < 0 || w_rows >= (1LL << 31)) return false;
+    const cuuint64_t wd[2] = {MX_K, static_cast<cuuint64_t>(w_rows)}, xd[2] = {static_cast<cuuint64_t>(kpad), static_cast<cuuint64_t>(T)};
+    const cuuint64_t ws[1] = {MX_K / 2}, xs[1] = {static_cast<cuuint64_t>(kpad)};
+    const cuuint32_t wb[2] = {MX_K, MG_ROWS}, xb[2] = {MX_K, static_cast<cuuint32_t>(nt)}, es[2] = {1u, 1u};
+    return g_t5_encode(w_map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(w), wd, ws, wb, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS &&
+           g_t5_encode(x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(x), xd, xs, xb, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.
+static int mg_parts(long long tiles, int ktiles, int slots) {
+    int best = 1;
+    while (best < 8 && (best + 1) * tiles <= slots && ktiles / (best + 1) >= 2) ++best;
+    return best;
+}
+
+template <int NT, int STAGES, int MODE, typename TO>
+static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
+    CUtensorMap w_map, x_map;
+    if (!mg_maps(&w_map, &x_map, w, static_cast<long long>(tiles) * a.ktiles * MG_ROWS, x, a.T, a.ktiles * MX_K, NT)) return LLM_REFUSED_SIZE;
+    constexpr size_t smem = static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K + (NT > 128 ? 3 : 2) * MX_PIECE) + 1024;
+    static_assert(static_cast<size_t>(NT) * MG_ROWS * 4 <= static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K), "the sums fit the stages");
+    static_assert(smem <= (NT <= 64 ? 113 : 226) * 1024, "shared memory of an SM");
+    auto kern = linear_mx_kernel<NT, STAGES, MODE, TO>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int tok_tiles = (a.T + NT - 1) / NT, sms = mg_sms();
+    if (tiles > 65535 || tok_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
+    const int parts = mg_parts(static_cast<long long>(tiles) * tok_tiles, a.ktiles, sms * (NT <= 64 ? 2 : 1) * 7 / 8);
+    launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS), smem, s, parts, w_map, x_map, a);
+    return launch_status();
+}
+template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
+    if (a.T <= 16) return mg_launch<16, 5, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 32) return mg_launch<32, 5, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 64) return mg_launch<64, 4, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 128) return mg_launch<128, 6, MODE, TO>(w, tiles, x, a, s);
+    return mg_launch<256, 4, MODE, TO>(w, tiles, x, a, s);
+}
+
+static int mg_check(const void* w, const void* w_scales, const void* x, const void* x_scales, const int32_t* status, int T, int N, int K) {
+    if (N <= 0 || N > (1 << 24) || K <= 0 || K > (1 << 20) || T > (1 << 24)) return LLM_REFUSED_SIZE;
+    if (!aligned16(w) || !aligned16(w_scales) || !aligned16(x) || !aligned16(x_scales) || (reinterpret_cast<uintptr_t>(w) & 31) || status == nullptr)
+        return LLM_REFUSED_ALIGN;
+    return LLM_OK;
+}
+
+// x: rows of 8 bits [T, K]; w: a weight of 4 bits [N, K]; y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
+extern "C" int llm_linear_mx(const void* x, const void* x_scales, const void* w, const void* w_scales, void* y, int out_dtype, int add, int T, int N,
+                             int K, int waits, int32_t* status, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    if (const int rc = mg_check(w, w_scales, x, x_scales, status, T, N, K)) return rc;
+    if ((out_dtype != LLM_DT_F32 && out_dtype != LLM_DT_BF16) || (add && out_dtype != LLM_DT_F32)) return LLM_REFUSED_DTYPE;
+    MgArgs a = {static_cast<const unsigned char*>(w_scales), static_cast<const unsigned char*>(x_scales), y, nullptr, T, N, (K + MX_K - 1) / MX_K, 0,
+                N % 4 == 0 && aligned16(y), 0, waits, 0.0f, status};
+    const int tiles = (N + MG_ROWS - 1) / MG_ROWS;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (add) return mg_rows<MG_ADD, float>(w, tiles, x, a, s);
+    if (out_dtype == LLM_DT_F32) return mg_rows<MG_STORE, float>(w, tiles, x, a, s);
+    return mg_rows<MG_STORE, bf16>(w, tiles, x, a, s);
+}
+
+// w: a gated weight of 4 bits (N gate and N up rows); codes, scales: act(x gate^T) * (x up^T) as rows of 8 bits [T, N].
+extern "C" int llm_linear_mx_silu_mul(const void* x, const void* x_scales, const void* w, const void* w_scales, void* codes, void* scales, int T,
+                                      int N, int K, int act, float limit, int waits, int32_t* status, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    if (const int rc = mg_check(w, w_scales, x, x_scales, status, T, N, K)) return rc;
+    if (act < 0 || act > 2 || (act == 2 && !(limit > 0.0f))) return LLM_REFUSED_SIZE;
+    if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    const int tiles = 2 * ((N + 127) / 128);                      // as the weight has them
+    MgArgs a = {static_cast<const unsigned char*>(w_scales), static_cast<const unsigned char*>(x_scales), codes, static_cast<unsigned char*>(scales), T, N,
+                (K + MX_K - 1) / MX_K, tiles * 64, 0, act, waits, limit, status};
+    return mg_rows<MG_GATED, float>(w, tiles, x, a, reinterpret_cast<cudaStream_t>(stream));
+}

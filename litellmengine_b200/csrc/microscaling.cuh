@@ -1,0 +1,127 @@
+// Microscaled numbers: blocks of 32 neighbouring values of a row share one scale, a power of two, and each value keeps 8 bits
+// (e4m3: sign, four bits of exponent, three of mantissa, up to 448) or 4 (e2m1: up to 6).
+//
+//   scale  the smallest power of two s with max |x| <= largest * s (at least 2^-127), stored as its exponent plus 127
+//   code   x / s to the format's nearest value, ties to even: dividing by s is exact, so this is the only rounding, half a step
+// A block with an infinity or a NaN has the scale 255: all of it reads as NaN.  A block of zeros has scale 0 (2^-127) and codes 0.
+// Such a scale never saturates: a smaller one (the exponent of the largest value) would cut up to a quarter off the largest values.
+//
+// Where the bytes lie: rows are padded with zeros to whole tiles of 128 values, whose four scales are one 32-bit word.  The words of
+// 128 rows are a piece of 512 bytes: the word of row r (of 128) at 16 (r % 32) + 4 (r / 32), which is how the block-scaled tensor-core
+// products take them (32 lanes of 16 bytes).  Pieces lie by tile of 128 rows, then by tile of 128 values.
+//   rows (8 bits): codes [rows][padded k], one byte each
+//   a weight (4 bits): tiles [tile of 128 rows][tile of 128 values][128][64 bytes], the lower half of a byte the earlier value; a
+//   product fetches a tile as one box of 8 KB
+#pragma once
+
+#include "common.cuh"
+
+#define MX_BLOCK 32
+#define MX_K 128                  // values of a tile's row
+#define MX_PIECE 512              // bytes of the scales of 128 rows x 128 values
+#define MX_E2M1 4
+#define MX_E4M3 8
+
+// Where the scale of block `kb` of a row lies (the byte; of kb = 4 n the word).
+__host__ __device__ __forceinline__ size_t mx_scale_at(size_t row, int kb, int ktiles) {
+    return ((row >> 7) * ktiles + (kb >> 2)) * MX_PIECE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3);
+}
+// The stored scale of a block from the bits of its largest magnitude (as integers these are in order, NaN above infinity above all).
+template <int FMT> __device__ __forceinline__ unsigned mx_scale(unsigned most) {
+    constexpr unsigned EXP = FMT == MX_E4M3 ? 8 : 2, MANT = FMT == MX_E4M3 ? 0x600000u : 0x400000u;      // largest: 1.75 * 2^8, 1.5 * 2^2
+    const unsigned e = (most >> 23) + ((most & 0x7fffffu) > MANT ? 1u : 0u);
+    return most >= 0x7f800000u ? 255u : e > EXP ? e - EXP : 0u;
+}
+__device__ __forceinline__ float mx_inverse(unsigned scale) { return __uint_as_float((254u - min(scale, 253u)) << 23); }      // 1 / s, exact
+__device__ __forceinline__ float mx_value(unsigned scale) {
+    return __uint_as_float(scale == 255u ? 0x7fc00000u : scale ? scale << 23 : 0x400000u);
+}
+__device__ __forceinline__ unsigned mx_abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Four values, already divided by their scale: 32 bits of e4m3, 16 bits of e2m1; the first value lowest.
+__device__ __forceinline__ unsigned mx_e4m3x4(float a, float b, float c, float d) {
+    unsigned r;
+    asm("{\n .reg .b16 lo, hi;\n cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n mov.b32 %0, {lo, hi};\n}\n"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+}
+__device__ __forceinline__ unsigned mx_e2m1x8(const float (&v)[8]) {
+    unsigned r;
+    asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}\n"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+// Eight values of 4 bits, or four of 8 bits, as float32 (through 16-bit floats, which hold all of them).
+__device__ __forceinline__ float2 mx_halves(unsigned h) {
+    float2 f;
+    asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n cvt.f32.f16 %0, lo;\n cvt.f32.f16 %1, hi;\n}\n" : "=f"(f.x), "=f"(f.y) : "r"(h));
+    return f;
+}
+__device__ __forceinline__ void mx_from_e2m1x8(unsigned r, float (&v)[8]) {
+    unsigned h[4];
+    asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+        " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}\n" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(r));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = mx_halves(h[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void mx_from_e4m3x4(unsigned r, float* v) {
+    unsigned lo, hi;
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n" : "=r"(lo), "=r"(hi) : "r"(r));
+    const float2 a = mx_halves(lo), b = mx_halves(hi);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+
+// Eight neighbouring values a lane, four lanes a block, sixteen a tile's row: the lane's codes, and the four blocks' scales as one
+// word in every lane of the sixteen.  All lanes of a warp are here.
+template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned& word) {
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, mx_abs_bits(v[i]));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const unsigned scale = mx_scale<FMT>(most);
+    const float inv = mx_inverse(scale);
+    word = scale << (8 * ((threadIdx.x >> 2) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = v[i] * inv;
+    if constexpr (FMT == MX_E2M1) return make_uint2(mx_e2m1x8(q), 0u);
+    else return make_uint2(mx_e4m3x4(q[0], q[1], q[2], q[3]), mx_e4m3x4(q[4], q[5], q[6], q[7]));
+}
+// The row's eight values from column `col` on (a multiple of 8), which lane threadIdx.x % 16 == col / 8 % 16 holds, to rows of 8 bits.
+__device__ __forceinline__ void mx_store_row8(const float (&v)[8], bool there, size_t row, int col, int kpad, unsigned char* codes, unsigned char* scales) {
+    unsigned word;
+    const uint2 c = mx_encode8<MX_E4M3>(v, word);
+    if (!there) return;
+    *reinterpret_cast<uint2*>(codes + row * kpad + col) = c;
+    if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(row, col / MX_BLOCK, kpad / MX_K)) = word;
+}
+// Eight values from column `col` on of a row of `n`; zeros beyond it.  vec: rows of whole, aligned pieces of eight.
+template <typename T> __device__ __forceinline__ void mx_load8(const T* row, int col, int n, int vec, float (&v)[8]) {
+    if (vec) {
+        if (col < n) {
+            load8(row + col, v);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = col + i < n ? to_f32(row[col + i]) : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ void mx_put8(T* row, int col, int n, int vec, const float (&v)[8]) {
+    if (vec) {
+        if (col < n) store8(row + col, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < n) row[col + i] = from_f32<T>(v[i]);
+    }
+}

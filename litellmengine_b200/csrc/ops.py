@@ -2129,7 +2129,8 @@ _stream_status: Dict[str, torch.Tensor] = {}
 
 def stream_status(device) -> torch.Tensor:
     """The status word of the engine's matrix products and of the delta rule (code 8: a bounded wait of a weight-streaming
-    product ran out; 9: of the paired or the float32 tcgen05 product; 11: of the delta rule's tensor-core scan)."""
+    product ran out; 9: of the paired or the float32 tcgen05 product; 11: of the delta rule's tensor-core scan; 12: of a microscaled
+    tcgen05 product)."""
     key = str(device)
     t = _stream_status.get(key)
     if t is None:
@@ -2290,6 +2291,188 @@ def latent_q_product(x: torch.Tensor, weight: torch.Tensor) -> bool:
     (0.81) 89, 89; 2,000 (0.84) 116, 118; 4,000 202, 214; 8 heads, K 384, 1,500 (0.95) 75, 75; 4,000 (0.84) 152, 154."""
     return (x.shape[0] >= PAIR_HEADS_MIN_ROWS and x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0
             and _pair_takes(x, weight, weight.shape[0], "heads"))
+
+
+# ---- microscaled products: rows in 8 bits, weights in 4 -----------------------------------------------
+# A block of 32 neighbouring values of a row shares one scale, the smallest power of two with which its largest magnitude stays
+# within the format's largest value (e4m3 448, e2m1 6); each value is then rounded to the format's nearest.
+# csrc/microscaling.cuh says where the bytes lie.
+MX_BLOCK = 32
+
+
+def _here(*tensors) -> None:
+    """`_dev`, and on the device whose stream the kernel will go to."""
+    _dev(*tensors)
+    now = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != now:
+            raise KernelError(f"tensor on {t.device}, but the current device is cuda:{now}")
+
+
+class MxRows:
+    """Rows [T, K] in 8 bits (e4m3) with a scale per 32 values: what `linear_mx` and `linear_silu_mul_mx` read.  Made by `mx_rows`,
+    `rmsnorm_mx`, `silu_and_mul_mx` and `linear_silu_mul_mx`.  `codes`: uint8 [T, K padded to 128]; `scales`: uint8 pieces of
+    512 bytes; `values` gives the rows as a matrix again."""
+
+    def __init__(self, T: int, K: int, device):
+        self.shape = torch.Size((T, K))
+        self.device = torch.device(device)
+        tiles = -(-K // 128)
+        pieces = 1 if T <= 128 else 2 * (-(-T // 256))            # products of more rows read two pieces at a time
+        self.codes = torch.empty((T, tiles * 128), dtype=torch.uint8, device=device)
+        self.scales = torch.empty((pieces, tiles, 512), dtype=torch.uint8, device=device)
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        T, K = self.shape
+        return _mx_values(self, self.codes, 8, T, K, False, dtype)
+
+
+class MxWeight:
+    """A weight [N, K] in 4 bits (e2m1) with a scale per 32 values along K, 17 / 32 of a byte a value, stored tile by tile.  Made by
+    `mx_weight`; `gated`: it is [gate; up], gate and up rows stored beside each other for `linear_silu_mul_mx`."""
+
+    def __init__(self, N: int, K: int, gated: bool, device):
+        self.shape = torch.Size((N, K))
+        self.gated = gated
+        self.device = torch.device(device)
+        n = _fn("microscaling", "llm_mx_weight_tiles", [c_int, c_int])(N // 2 if gated else N, int(gated))
+        tiles = -(-K // 128)
+        self.codes = torch.empty((n, tiles, 128, 64), dtype=torch.uint8, device=device)
+        self.scales = torch.empty((n, tiles, 512), dtype=torch.uint8, device=device)
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        N, K = self.shape
+        return _mx_values(self, self.codes, 4, N // 2 if self.gated else N, K, self.gated, dtype)
+
+
+def _mx_values(held, codes: torch.Tensor, bits: int, n: int, k: int, gated: bool, dtype: torch.dtype) -> torch.Tensor:
+    _here(codes)
+    out = torch.empty(tuple(held.shape), dtype=dtype, device=codes.device)
+    f = _fn("microscaling", "llm_mx_values", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
+    _check(f(_ptr(codes), _ptr(held.scales), bits, _ptr(out), _dt(out), n, k, int(gated), _stream()), "mx values")
+    return out
+
+
+def mx_weight(weight: torch.Tensor, gated: bool = False) -> MxWeight:
+    """A weight [N, K] (float32 or bfloat16) in 4 bits.  With `gated`, weight is [gate; up] and serves `linear_silu_mul_mx`."""
+    _here(weight)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1 or (gated and weight.shape[0] % 2):
+        raise KernelError("a microscaled weight is a matrix; a gated one has as many gate as up rows")
+    N, K = weight.shape
+    dt = _dt(weight)
+    made = MxWeight(N, K, gated, weight.device)
+    f = _fn("microscaling", "llm_mx_weight", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p])
+    _check(f(_ptr(weight), dt, _ptr(made.codes), _ptr(made.scales), N // 2 if gated else N, K, int(gated), _stream()), "mx_weight")
+    return made
+
+
+def mx_rows(x: torch.Tensor) -> MxRows:
+    """x [T, K] (float32 or bfloat16) as rows of 8 bits."""
+    _here(x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError("microscaled rows are made of a matrix [T, K]")
+    T, K = x.shape
+    dt = _dt(x)
+    made = MxRows(T, K, x.device)
+    f = _fn("microscaling", "llm_mx_rows", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
+    _check(f(_ptr(x), dt, _ptr(made.codes), _ptr(made.scales), T, K, _stream()), "mx_rows")
+    return made
+
+
+def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, delta=None, rows: Optional[torch.Tensor] = None,
+               sum_out: Optional[torch.Tensor] = None) -> MxRows:
+    """rmsnorm(x (+ delta)) * weight over the last dim, in 32-bit, as rows of 8 bits.  `delta` (x's shape, float32 or bfloat16) may
+    be a `PartialSum`, whose k-splits are added as they are read.  `sum_out` (like x, may be x itself) receives x + delta: the
+    residual stream from then on.  `rows` (int32) selects which rows are normalised; it excludes `sum_out`."""
+    parts, part_stride = 1, 0
+    if isinstance(delta, PartialSum):
+        parts, part_stride = delta.parts.shape[0], delta.parts.stride(0)
+        delta = delta.parts[0]
+    _here(x, weight, delta, rows, sum_out)
+    _i32(rows, "rows")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError("rmsnorm_mx wants a matrix [T, H]")
+    T, H = x.shape
+    if weight.dtype != torch.float32 or weight.numel() != H:
+        raise KernelError("norm weight must be float32 of the row length")
+    if delta is not None and delta.shape != x.shape:
+        raise KernelError("delta must have x's shape")
+    if sum_out is not None and (sum_out.shape != x.shape or sum_out.dtype != x.dtype or rows is not None):
+        raise KernelError("the sum goes to a tensor like x, and only where all rows are normalised")
+    n = rows.numel() if rows is not None else T
+    dt, dd = _dt(x), _dt(delta) if delta is not None else 0
+    made = MxRows(n, H, x.device)
+    f = _fn("microscaling", "llm_mx_rmsnorm", [c_void_p, c_int, c_void_p, c_int, c_int, c_longlong, c_void_p, c_float, c_void_p, c_void_p,
+                                               c_void_p, c_void_p, c_int, c_int, c_void_p])
+    _check(f(_ptr(x), dt, _ptr(delta), dd, parts, part_stride, _ptr(weight), float(eps), _ptr(sum_out), _ptr(made.codes), _ptr(made.scales),
+             _ptr(rows), n, H, _stream()), "rmsnorm_mx")
+    return made
+
+
+def silu_and_mul_mx(gate_up, activation: str = "silu", limit: float = 0.0) -> MxRows:
+    """[T, 2I] -> rows of 8 bits [T, I]: act(first half) * second half as in `silu_and_mul`, in 32-bit until it is rounded to 8
+    bits.  A `PartialSum` is added up on the way."""
+    act = ACTIVATIONS[activation]
+    parts, part_stride = 1, 0
+    if isinstance(gate_up, PartialSum):
+        parts, part_stride = gate_up.parts.shape[0], gate_up.parts.stride(0)
+        gate_up = gate_up.parts[0]
+    _here(gate_up)
+    if gate_up.dim() != 2 or gate_up.shape[1] < 2 or gate_up.shape[1] % 2:
+        raise KernelError("gate and up are the halves of a matrix [T, 2I]")
+    T, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    dt = _dt(gate_up)
+    made = MxRows(T, inter, gate_up.device)
+    f = _fn("microscaling", "llm_mx_silu_and_mul", [c_void_p, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p])
+    _check(f(_ptr(gate_up), dt, parts, part_stride, _ptr(made.codes), _ptr(made.scales), T, inter, act, float(limit), _stream()), "silu_and_mul_mx")
+    return made
+
+
+def _mx_operands(x, weight: MxWeight, gated: bool) -> MxRows:
+    if not isinstance(weight, MxWeight) or weight.gated != gated:
+        raise KernelError("the microscaled product takes an MxWeight" + (" made with gated=True" if gated else " that is not a gated one"))
+    if x.shape[-1] != weight.shape[1] or len(x.shape) != 2:
+        raise KernelError("x and weight disagree on K")
+    x = x if isinstance(x, MxRows) else mx_rows(x)
+    _here(x.codes, weight.codes)
+    return x
+
+
+def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, residual: Optional[torch.Tensor] = None,
+              waits: int = STREAM_WAITS) -> torch.Tensor:
+    """x [T, K] @ weight[N, K]^T with the weight in 4 bits and x in 8 (`MxRows`; a matrix is taken to 8 bits first), products exact,
+    sums in float32, on the block-scaled tcgen05 products.  The result is float32 or bfloat16 [T, N]; with `residual` (float32
+    [T, N]) it is added to that in place, which is returned."""
+    x = _mx_operands(x, weight, False)
+    (T, K), N = x.shape, weight.shape[0]
+    if residual is not None:
+        _here(residual)
+        if residual.dtype != torch.float32 or tuple(residual.shape) != (T, N):
+            raise KernelError("the product joins a float32 residual of its shape")
+    y = residual if residual is not None else torch.empty((T, N), dtype=out_dtype, device=x.device)
+    f = _fn("gemm_mx_tcgen05", "llm_linear_mx", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                                                 c_void_p])
+    _check(f(_ptr(x.codes), _ptr(x.scales), _ptr(weight.codes), _ptr(weight.scales), _ptr(y), _dt(y), int(residual is not None), T, N, K, waits,
+             _ptr(stream_status(x.device)), _stream()), "linear_mx")
+    return y
+
+
+def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: float = 0.0, waits: int = STREAM_WAITS) -> MxRows:
+    """act(x @ gate^T) * (x @ up^T) as rows of 8 bits [T, I] for a gated weight [2I, K] in 4 bits, act as in `silu_and_mul`, in the
+    product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits."""
+    act = ACTIVATIONS[activation]
+    x = _mx_operands(x, weight, True)
+    (T, K), inter = x.shape, weight.shape[0] // 2
+    made = MxRows(T, inter, x.device)
+    f = _fn("gemm_mx_tcgen05", "llm_linear_mx_silu_mul", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                                          c_float, c_int, c_void_p, c_void_p])
+    _check(f(_ptr(x.codes), _ptr(x.scales), _ptr(weight.codes), _ptr(weight.scales), _ptr(made.codes), _ptr(made.scales), T, inter, K, act,
+             float(limit), waits, _ptr(stream_status(x.device)), _stream()), "linear_silu_mul_mx")
+    return made
 
 
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:

@@ -24,7 +24,8 @@ STATUS_TEXT = {1: "a token id outside the vocabulary reached the embedding kerne
                6: "a wait on a barrier in the tcgen05 prompt attention kernel ran out",
                8: "a wait on a copy barrier in the weight-streaming product ran out",
                9: "a wait on a barrier in a tcgen05 product (the paired one or the float32 one) ran out",
-               11: "a wait on a copy barrier in the delta rule's tensor-core scan ran out"}
+               11: "a wait on a copy barrier in the delta rule's tensor-core scan ran out",
+               12: "a wait on a barrier in a microscaled tcgen05 product ran out"}
 
 
 class ModelRunner:
