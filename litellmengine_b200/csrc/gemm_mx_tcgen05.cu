@@ -51,8 +51,8 @@ __device__ __forceinline__ unsigned long long mg_scale_desc(const void* smem) {
     return static_cast<unsigned long long>((t5_smem(smem) & 0x3FFFF) >> 4) | (static_cast<unsigned long long>(128 >> 4) << 32) | (1ull << 46);
 }
 // Instruction descriptor: A e2m1, B e4m3, both K-major, scales powers of two; `block`: which of the four scales of a word, for both.
-__host__ __device__ constexpr unsigned mg_idesc(int n, unsigned block) {
-    return (block << 4) | (5u << 7) | (0u << 10) | (static_cast<unsigned>(n >> 3) << 17) | (1u << 23) | ((MG_ROWS >> 4) << 24) | (block << 29);
+__host__ __device__ constexpr unsigned mg_idesc(int m, int n, unsigned block) {
+    return (block << 4) | (5u << 7) | (0u << 10) | (static_cast<unsigned>(n >> 3) << 17) | (1u << 23) | (static_cast<unsigned>(m >> 4) << 24) | (block << 29);
 }
 
 struct MgArgs {
@@ -69,9 +69,7 @@ enum { MG_STORE = 0, MG_ADD = 1, MG_GATED = 2 };
 template <int NT, int STAGES, int MODE, typename TO>
 __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel(const __grid_constant__ CUtensorMap w_map,
                                                                                const __grid_constant__ CUtensorMap x_map, const MgArgs a) {
-    constexpr int X_PIECES = NT > 128 ? 2 : 1;
-    constexpr unsigned X_BYTES = NT * MX_K, S_BYTES = (1 + X_PIECES) * MX_PIECE;
-    constexpr unsigned S_COLS = 4 * (1 + X_PIECES), S_COL0 = NT < 32 ? 32 : NT;
+    constexpr unsigned X_BYTES = NT * MX_K, S_BYTES = 2 * MX_PIECE, S_COLS = 8, S_COL0 = NT < 32 ? 32 : NT;
     constexpr unsigned COLS = S_COL0 + STAGES * S_COLS <= 128 ? 128 : S_COL0 + STAGES * S_COLS <= 256 ? 256 : 512;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
@@ -113,10 +111,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
             auto tokens = [&](int kb) {
                 const int st = kb % STAGES;
                 t5_tma_2d(x_s + st * X_BYTES, &x_map, (kb0 + kb) * MX_K, tok0, &full[st]);
-#pragma unroll
-                for (int p = 0; p < X_PIECES; ++p)
-                    mg_copy(s_s + st * S_BYTES + (1 + p) * MX_PIECE, a.x_scales + (static_cast<size_t>(tok0 / 128 + p) * a.ktiles + kb0 + kb) * MX_PIECE,
-                            MX_PIECE, &full[st]);
+                mg_copy(s_s + st * S_BYTES + MX_PIECE, a.x_scales + (static_cast<size_t>(tok0 / 128) * a.ktiles + kb0 + kb) * MX_PIECE, MX_PIECE, &full[st]);
             };
             const int first = min(STAGES, kbs);
             for (int kb = 0; kb < first; ++kb) weights(kb);       // nobody's output
@@ -143,10 +138,10 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
             if (!ok) break;
             const unsigned sc = tmem + S_COL0 + st * S_COLS;      // a place of its own for each stage: earlier products may still read theirs
 #pragma unroll
-            for (int p = 0; p <= X_PIECES; ++p) mg_scales_lead(lead, sc + 4 * p, sd + ((st * S_BYTES + p * MX_PIECE) >> 4));
+            for (int p = 0; p < 2; ++p) mg_scales_lead(lead, sc + 4 * p, sd + ((st * S_BYTES + p * MX_PIECE) >> 4));
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                mg_mma_lead(lead, tmem, wd + st * (MG_W_BYTES >> 4) + 2 * k, xd + st * (X_BYTES >> 4) + 2 * k, mg_idesc(NT, k), sc, sc + 4, (kb | k) ? 1u : 0u);
+                mg_mma_lead(lead, tmem, wd + st * (MG_W_BYTES >> 4) + 2 * k, xd + st * (X_BYTES >> 4) + 2 * k, mg_idesc(MG_ROWS, NT, k), sc, sc + 4, (kb | k) ? 1u : 0u);
             t5_commit_lead(lead, &empty[st]);
         }
         if (ok) t5_commit_lead(lead, &acc_full);
@@ -248,6 +243,234 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
     }
 }
 
+// ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
+// The two CTAs of a cluster compute a tile of 256 features x NT tokens together (cta_group::2): each brings its own 128 features and half
+// of the tokens, and reads both halves.  The clusters are persistent and hold two accumulators, so that a tile's result is written under the
+// next one's products; 192 tokens leave room for both and for the scales of all stages in tensor memory.  Tiles are numbered token
+// tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.
+#define MP_NT 192
+#define MP_STAGES 6
+#define MP_X_BYTES (MP_NT / 2 * MX_K)
+#define MP_S_BYTES (3 * MX_PIECE)                                 // own weights' scales, both pieces of the rows'
+#define MP_S_COLS 12
+#define MP_TURN (32 * MG_ROWS * 4)                                // 32 tokens' sums, for gate and up to meet
+
+__device__ __forceinline__ unsigned mp_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned mp_map_to(unsigned smem_addr, unsigned rank) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ bool mp_wait_cluster(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    for (int i = 0; i < waits; ++i) {
+        unsigned ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(t5_smem(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    if (atomicCAS(status, 0, MG_STATUS) == 0) status[1] = blockIdx.x;
+    return false;
+}
+// Boxes into this CTA's shared memory, counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void mp_tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::
+                     "r"(t5_smem(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mp_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::
+                     "r"(t5_smem(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mp_commit_lead(unsigned lead, unsigned long long* bar) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+                 " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::
+                     "r"(t5_smem(bar)), "h"(static_cast<unsigned short>(3)), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mp_scales_lead(unsigned lead, unsigned tmem, unsigned long long desc) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(tmem), "l"(desc), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mp_mma_lead(unsigned lead, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc,
+                                            unsigned a_scales, unsigned b_scales, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 q, %7, 0;\n"
+                 " @q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::
+                     "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(lead) : "memory");
+}
+// Whether all of the four epilogue warps say so.
+__device__ __forceinline__ bool mp_all(bool yes) {
+    unsigned r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.aligned.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r) : "r"(static_cast<unsigned>(yes)) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void mp_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+template <int MODE, typename TO>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linear_mx_pair_kernel(
+    const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap ws_map,
+    const __grid_constant__ CUtensorMap xs_map, const MgArgs a, int token_tiles, int tiles) {
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    unsigned char* x_s = w_s + MP_STAGES * MG_W_BYTES;            // [STAGES][96 tokens][128]
+    unsigned char* s_s = x_s + MP_STAGES * MP_X_BYTES;            // [STAGES][three pieces]
+    float* turn = reinterpret_cast<float*>(s_s + MP_STAGES * MP_S_BYTES);      // gated: two of them
+    __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], acc_full[2], acc_empty[2];
+    __shared__ unsigned tmem_base_s;
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const unsigned rank = __shfl_sync(0xffffffffu, mp_rank(), 0);
+    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1, ktiles = a.ktiles;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < MP_STAGES; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 8); }   // 4 epilogue warps of 2 CTAs
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    t5_fence_before();
+    __syncthreads();
+    mp_cluster_sync();                                            // the other CTA's barriers exist before anyone signals them
+    t5_fence_after();
+    pdl_invite();                                                 // not before: tensor memory is taken
+    const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
+    pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const unsigned full_first = mp_map_to(t5_smem(&full[0]), 0);
+            int it = 0;
+            bool ok = true;
+            for (int t = cluster; ok && t < tiles; t += clusters) {
+                const int tok0 = (t % token_tiles) * MP_NT, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
+                for (int kb = 0; kb < ktiles; ++kb, ++it) {
+                    const int s = it % MP_STAGES;
+                    if (it >= MP_STAGES && !mg_wait(&empty[s], (it / MP_STAGES - 1) & 1, a.waits, &abort_flag, a.status)) { ok = false; break; }
+                    if (rank == 0) t5_expect_tx(&full[s], 2 * (MG_W_READ + MP_X_BYTES + MP_S_BYTES));      // both CTAs' boxes
+                    const unsigned bar = full_first + s * 8;
+                    const int at = wt * ktiles + kb;
+                    mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, at * MG_ROWS, bar);
+                    mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at, bar);
+                    mp_tma_2d(x_s + s * MP_X_BYTES, &x_map, kb * MX_K, tok0 + static_cast<int>(rank) * (MP_NT / 2), bar);
+                    mp_tma_3d(s_s + s * MP_S_BYTES + MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
+                }
+            }
+            if (!ok)                                              // let what is in flight land before the CTA goes away
+                for (int n = 0; n < 2000; ++n) __nanosleep(100);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const unsigned lead = elect_one();
+            const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024), sd = mg_scale_desc(s_s);
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int t = cluster; ok && t < tiles; t += clusters, ++n) {
+                const int buf = n & 1;
+                const unsigned off = ((t % token_tiles) * MP_NT % 128) / 32;        // the tile's first token in its piece of scales
+                if (n >= 2) ok = __all_sync(0xffffffffu, mp_wait_cluster(&acc_empty[buf], ((n >> 1) - 1) & 1, a.waits, &abort_flag, a.status));
+                t5_fence_after();
+#pragma unroll 1
+                for (int kb = 0; ok && kb < ktiles; ++kb, ++it) {
+                    const int s = it % MP_STAGES;
+                    ok = __all_sync(0xffffffffu, mg_wait(&full[s], (it / MP_STAGES) & 1, a.waits, &abort_flag, a.status));
+                    if (!ok) break;
+                    const unsigned sc = tmem + 2 * MP_NT + s * MP_S_COLS;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) mp_scales_lead(lead, sc + 4 * p, sd + ((s * MP_S_BYTES + p * MX_PIECE) >> 4));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mp_mma_lead(lead, tmem + buf * MP_NT, wd + s * (MG_W_BYTES >> 4) + 2 * k, xd + s * (MP_X_BYTES >> 4) + 2 * k,
+                                    mg_idesc(2 * MG_ROWS, MP_NT, k), sc, sc + 4 + off, (kb | k) ? 1u : 0u);
+                    mp_commit_lead(lead, &empty[s]);
+                }
+                if (ok) mp_commit_lead(lead, &acc_full[buf]);
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        const unsigned acc_empty_first = mp_map_to(t5_smem(&acc_empty[0]), 0);
+        int n = 0, turns = 0;
+        for (int t = cluster; t < tiles; t += clusters, ++n) {
+            const int buf = n & 1, tok0 = (t % token_tiles) * MP_NT, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
+            const int toks = min(MP_NT, a.T - tok0);
+            bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
+            if (MODE == MG_GATED) ok = mp_all(ok);                // the four warps meet below: they go on or leave together
+            t5_fence_after();
+            const unsigned acc = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * MP_NT;
+            if constexpr (MODE == MG_GATED) {
+                // 32 tokens at a time through shared memory; then sixteen lanes a token, four features a lane, eight lanes a block
+                const int e = tid - 64, f = 4 * (e & 15);
+                unsigned char* codes = static_cast<unsigned char*>(a.y);
+#pragma unroll 1
+                for (int c = 0; c < toks; c += 32, ++turns) {
+                    unsigned r[32];
+                    t5_ld32(acc + c, r);
+                    t5_wait_ld();
+                    float* to = turn + (turns & 1) * (MP_TURN / 4);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) to[i * MG_ROWS + quarter * 32 + lane] = __uint_as_float(r[i]);
+                    asm volatile("bar.sync 1, 128;\n" ::: "memory");      // with two blocks in turn the next writes wait for this one's reads
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int tok = (e >> 4) + 8 * i;
+                        const float4 g = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + f), u = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + 64 + f);
+                        const float v[4] = {gated(g.x, u.x, a.act, a.limit), gated(g.y, u.y, a.act, a.limit), gated(g.z, u.z, a.act, a.limit),
+                                            gated(g.w, u.w, a.act, a.limit)};
+                        unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
+#pragma unroll
+                        for (int o = 1; o < 8; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        const unsigned scale = mx_scale<MX_E4M3>(most);
+                        const float inv = mx_inverse(scale);
+                        if (c + tok < toks) {
+                            const size_t row = tok0 + c + tok;
+                            *reinterpret_cast<unsigned*>(codes + row * a.out_kpad + wt * 64 + f) = mx_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                            if ((e & 7) == 0) a.y_scales[mx_scale_at(row, (wt * 64 + f) / MX_BLOCK, a.out_kpad / MX_K)] = static_cast<unsigned char>(scale);
+                        }
+                    }
+                }
+            } else {
+                // a lane is a feature: a token's 32 features leave side by side
+                const int f = wt * MG_ROWS + quarter * 32 + lane;
+                TO* y = static_cast<TO*>(a.y) + static_cast<size_t>(tok0) * a.N + f;
+#pragma unroll 1
+                for (int c = 0; c < toks; c += 32) {
+                    unsigned r[32];
+                    t5_ld32(acc + c, r);
+                    float old[32];
+                    if (MODE == MG_ADD)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) old[i] = f < a.N && c + i < toks ? to_f32(y[static_cast<size_t>(c + i) * a.N]) : 0.0f;
+                    t5_wait_ld();
+                    if (f < a.N)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (c + i < toks) y[static_cast<size_t>(c + i) * a.N] = from_f32<TO>(MODE == MG_ADD ? __uint_as_float(r[i]) + old[i] : __uint_as_float(r[i]));
+                }
+            }
+            t5_fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
+            if (!ok) break;
+        }
+    }
+    t5_fence_before();
+    __syncthreads();
+    mp_cluster_sync();                                            // nobody signals a CTA that has left
+    if (warp == 1) {
+        t5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
 static int mg_sms() {                     // of the current device
     static int sms[64] = {0};
@@ -257,19 +480,43 @@ static int mg_sms() {                     // of the current device
     return sms[dev];
 }
 
-// 4-bit codes, tiles of 128 rows of 64 bytes, spread by the copy engine; 8-bit rows [T, kpad] in boxes of NT rows x 128 values.
-static bool mg_maps(CUtensorMap* w_map, CUtensorMap* x_map, const void* w, long long w_rows, const void* x, int T, int kpad, int nt) {
+// 4-bit codes, tiles of 128 rows of 64 bytes, spread by the copy engine.
+static bool mg_weight_map(CUtensorMap* map, const void* w, long long rows) {
     CUtensorMap any;
     if (g_t5_state == 0) (void)t5_encode_2d(&any, w, 64, 64, 64, 64);        // finds the driver's entry point
-    if (g_t5_state < 0 || w_rows >= (1LL << 31)) return false;
-    const cuuint64_t wd[2] = {MX_K, static_cast<cuuint64_t>(w_rows)}, xd[2] = {static_cast<cuuint64_t>(kpad), static_cast<cuuint64_t>(T)};
-    const cuuint64_t ws[1] = {MX_K / 2}, xs[1] = {static_cast<cuuint64_t>(kpad)};
-    const cuuint32_t wb[2] = {MX_K, MG_ROWS}, xb[2] = {MX_K, static_cast<cuuint32_t>(nt)}, es[2] = {1u, 1u};
-    return g_t5_encode(w_map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(w), wd, ws, wb, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS &&
-           g_t5_encode(x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(x), xd, xs, xb, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    if (g_t5_state < 0 || rows >= (1LL << 31)) return false;
+    const cuuint64_t dims[2] = {MX_K, static_cast<cuuint64_t>(rows)}, strides[1] = {MX_K / 2};
+    const cuuint32_t box[2] = {MX_K, MG_ROWS}, es[2] = {1u, 1u};
+    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(w), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// 8-bit rows [rows, kpad] in boxes of `box_rows` x 128 values.
+static bool mg_rows_map(CUtensorMap* map, const void* x, int rows, int kpad, int box_rows) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kpad), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(kpad)};
+    const cuuint32_t box[2] = {MX_K, static_cast<cuuint32_t>(box_rows)}, es[2] = {1u, 1u};
+    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(x), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Pieces of scales as lines of 128 words: [tiles of rows][ktiles] in boxes of `box_tiles` neighbouring tiles of rows (three dimensions), or of one line.
+static bool mg_scales_map(CUtensorMap* map, const void* scales, int row_tiles, int ktiles, int box_tiles) {
+    const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(ktiles), static_cast<cuuint64_t>(row_tiles)};
+    const cuuint64_t strides[2] = {MX_PIECE, static_cast<cuuint64_t>(ktiles) * MX_PIECE};
+    const cuuint32_t box[3] = {128, 1, static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
+    const cuuint64_t line_dims[2] = {128, static_cast<cuuint64_t>(ktiles) * static_cast<cuuint64_t>(row_tiles)};
+    if (line_dims[1] >= (1ULL << 31)) return false;
+    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, box_tiles ? 3 : 2, const_cast<void*>(scales), box_tiles ? dims : line_dims, strides, box, es,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows that stand behind a matrix of T rows of 8 bits, so that no box reaches beyond them: whole tiles, whole pieces of scales.
+static int mg_padded_rows(int T) {
+    if (T <= 16) return 16;
+    if (T <= 32) return 32;
+    if (T <= 64) return 64;
+    return T <= 128 ? 128 : (T + 2 * MP_NT - 1) / (2 * MP_NT) * (2 * MP_NT);
+}
+extern "C" int llm_mx_padded_rows(int T) { return mg_padded_rows(T); }
 
 // Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.
 static int mg_parts(long long tiles, int ktiles, int slots) {
@@ -281,8 +528,9 @@ static int mg_parts(long long tiles, int ktiles, int slots) {
 template <int NT, int STAGES, int MODE, typename TO>
 static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
     CUtensorMap w_map, x_map;
-    if (!mg_maps(&w_map, &x_map, w, static_cast<long long>(tiles) * a.ktiles * MG_ROWS, x, a.T, a.ktiles * MX_K, NT)) return LLM_REFUSED_SIZE;
-    constexpr size_t smem = static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K + (NT > 128 ? 3 : 2) * MX_PIECE) + 1024;
+    if (!mg_weight_map(&w_map, w, static_cast<long long>(tiles) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, mg_padded_rows(a.T), a.ktiles * MX_K, NT)) return LLM_REFUSED_SIZE;
+    constexpr size_t smem = static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K + 2 * MX_PIECE) + 1024;
+    static_assert(NT <= 128, "a tile's scales are one piece");
     static_assert(static_cast<size_t>(NT) * MG_ROWS * 4 <= static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K), "the sums fit the stages");
     static_assert(smem <= (NT <= 64 ? 113 : 226) * 1024, "shared memory of an SM");
     auto kern = linear_mx_kernel<NT, STAGES, MODE, TO>;
@@ -294,12 +542,32 @@ static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS), smem, s, parts, w_map, x_map, a);
     return launch_status();
 }
+template <int MODE, typename TO>
+static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
+    CUtensorMap w_map, x_map, ws_map, xs_map;
+    const int padded = mg_padded_rows(a.T), stored = (tiles + 1) / 2 * 2;
+    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles * MX_K, MP_NT / 2) ||
+        !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, 2))
+        return LLM_REFUSED_SIZE;
+    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES + MP_S_BYTES) + (MODE == MG_GATED ? 2 * MP_TURN : 0) + 1024;
+    static_assert(smem <= 226 * 1024, "shared memory of an SM");
+    static_assert(2 * MP_NT + MP_STAGES * MP_S_COLS <= 512, "tensor memory");
+    auto kern = linear_mx_pair_kernel<MODE, TO>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const long long token_tiles = (a.T + MP_NT - 1) / MP_NT, all = token_tiles * (stored / 2);
+    const int slots = mg_sms() / 2;
+    if (slots <= 0 || all > (1LL << 30)) return LLM_REFUSED_SIZE;
+    const int clusters = all < slots ? static_cast<int>(all) : slots;
+    launch_pdl(kern, dim3(2 * clusters), dim3(MG_THREADS), smem, s, w_map, x_map, ws_map, xs_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
+    return launch_status();
+}
 template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
     if (a.T <= 16) return mg_launch<16, 5, MODE, TO>(w, tiles, x, a, s);
     if (a.T <= 32) return mg_launch<32, 5, MODE, TO>(w, tiles, x, a, s);
     if (a.T <= 64) return mg_launch<64, 4, MODE, TO>(w, tiles, x, a, s);
     if (a.T <= 128) return mg_launch<128, 6, MODE, TO>(w, tiles, x, a, s);
-    return mg_launch<256, 4, MODE, TO>(w, tiles, x, a, s);
+    return mp_launch<MODE, TO>(w, tiles, x, a, s);
 }
 
 static int mg_check(const void* w, const void* w_scales, const void* x, const void* x_scales, const int32_t* status, int T, int N, int K) {

@@ -245,9 +245,9 @@ extern "C" int llm_mx_rmsnorm(const void* x, int x_dtype, const void* delta, int
     return LLM_REFUSED_DTYPE;
 }
 
-// Tiles of 128 rows that a weight of N rows has; gated: of N gate and N up rows, an even number of tiles (the product's result is then
-// whole tiles of 128 values).
-extern "C" int llm_mx_weight_tiles(int N, int is_gated) { return is_gated ? 2 * ((N + 127) / 128) : (N + 127) / 128; }
+// Tiles of 128 rows that a weight of N rows (gated: of N gate and N up rows) has: an even number, because products of many rows take two
+// at a time, and because a gated product's result is then whole tiles of 128 values.
+extern "C" int llm_mx_weight_tiles(int N, int is_gated) { return is_gated ? 2 * ((N + 127) / 128) : (N + 255) / 256 * 2; }
 
 // w: [N, K], gated: [2 N, K] = [gate; up].
 extern "C" int llm_mx_weight(const void* w, int dtype, void* tiles, void* scales, int N, int K, int is_gated, uintptr_t stream) {

@@ -2318,9 +2318,9 @@ class MxRows:
         self.shape = torch.Size((T, K))
         self.device = torch.device(device)
         tiles = -(-K // 128)
-        pieces = 1 if T <= 128 else 2 * (-(-T // 256))            # products of more rows read two pieces at a time
-        self.codes = torch.empty((T, tiles * 128), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((pieces, tiles, 512), dtype=torch.uint8, device=device)
+        padded = _fn("gemm_mx_tcgen05", "llm_mx_padded_rows", [c_int])(T)         # the products read whole tiles; nobody minds what stands there
+        self.codes = torch.empty((padded, tiles * 128), dtype=torch.uint8, device=device)[:T]
+        self.scales = torch.empty((-(-padded // 128), tiles, 512), dtype=torch.uint8, device=device)
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         T, K = self.shape

@@ -44,7 +44,7 @@ def test_sizes_types_and_addresses_of_rows():
     assert act(inter=0) == SIZE and act(kind=3) == SIZE and act(kind=2) == SIZE and act(parts=0) == SIZE and act(dt=5) == DTYPE and act(s=P + 8) == ALIGN
     values = lambda fmt=8, dt=1, gated=0, K=64: m.llm_mx_values(v(P), v(P), fmt, v(P), dt, 4, K, gated, v(0))
     assert values(fmt=6) == SIZE and values(gated=1) == SIZE and values(dt=2) == DTYPE and values(K=0) == SIZE
-    assert [m.llm_mx_weight_tiles(n, g) for n, g in ((1, 0), (128, 0), (129, 0), (1, 1), (128, 1), (129, 1))] == [1, 1, 2, 2, 2, 4]
+    assert [m.llm_mx_weight_tiles(n, g) for n, g in ((1, 0), (128, 0), (129, 0), (1, 1), (128, 1), (129, 1))] == [2, 2, 2, 2, 2, 4]
 
 
 def test_sizes_types_and_addresses_of_products():

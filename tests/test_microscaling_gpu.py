@@ -371,4 +371,4 @@ def test_refusals():
     refuses(o.silu_and_mul_mx, x[:, :63].contiguous())
     refuses(X.values, torch.float16)
     assert o.linear_mx(o.mx_rows(x[:0]), W).shape == (0, 128) and o.linear_silu_mul_mx(x[:0], G).values().shape == (0, 64)
-    assert W.nbytes == 128 * 64 + 512 and G.nbytes == 2 * W.nbytes
+    assert W.nbytes == G.nbytes == 2 * (128 * 64 + 512)
