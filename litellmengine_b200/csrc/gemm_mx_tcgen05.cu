@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
 #define MP_X_BYTES (MP_NT / 2 * MX_K)
 #define MP_S_BYTES (3 * MX_PIECE)                                 // own weights' scales, both pieces of the rows'
 #define MP_S_COLS 12
-#define MP_TURN (32 * MG_ROWS * 4)                                // 32 tokens' sums, for gate and up to meet
+#define MP_TURN (32 * MG_ROWS * 4)                                // 32 tokens' sums, on their way out
 
 __device__ __forceinline__ unsigned mp_rank() {
     unsigned r;
@@ -314,12 +314,12 @@ __device__ __forceinline__ void mp_cluster_sync() {
 template <int MODE, typename TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linear_mx_pair_kernel(
     const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap ws_map,
-    const __grid_constant__ CUtensorMap xs_map, const MgArgs a, int token_tiles, int tiles) {
+    const __grid_constant__ CUtensorMap xs_map, const __grid_constant__ CUtensorMap y_map, const MgArgs a, int token_tiles, int tiles) {
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     unsigned char* x_s = w_s + MP_STAGES * MG_W_BYTES;            // [STAGES][96 tokens][128]
     unsigned char* s_s = x_s + MP_STAGES * MP_X_BYTES;            // [STAGES][three pieces]
-    float* turn = reinterpret_cast<float*>(s_s + MP_STAGES * MP_S_BYTES);      // gated: two of them
+    float* turn = reinterpret_cast<float*>(s_s + MP_STAGES * MP_S_BYTES);      // two blocks
     __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], acc_full[2], acc_empty[2];
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag;
@@ -403,7 +403,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
             const int buf = n & 1, tok0 = (t % token_tiles) * MP_NT, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
             const int toks = min(MP_NT, a.T - tok0);
             bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
-            if (MODE == MG_GATED) ok = mp_all(ok);                // the four warps meet below: they go on or leave together
+            ok = mp_all(ok);                                      // the four warps meet below: they go on or leave together
             t5_fence_after();
             const unsigned acc = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * MP_NT;
             if constexpr (MODE == MG_GATED) {
@@ -437,23 +437,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
                         }
                     }
                 }
+            } else if (a.vec) {
+                // 32 tokens at a time through shared memory and out by the copy engine, which also adds and leaves out what is beyond
+                // the matrix.  Stores straight from the lanes (a token's 32 features, 64 bytes) took longer than a tile's products.
+#pragma unroll 1
+                for (int c = 0; c < toks; c += 32, ++turns) {
+                    unsigned r[32];
+                    t5_ld32(acc + c, r);
+                    TO* to = reinterpret_cast<TO*>(turn) + (turns & 1) * (32 * MG_ROWS) + quarter * 32 + lane;
+                    if (tid == 64) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");       // the block before last has been read
+                    t5_wait_ld();
+                    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) to[i * MG_ROWS] = from_f32<TO>(__uint_as_float(r[i]));
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+                    if (tid == 64 && wt * MG_ROWS < a.N) {
+                        const unsigned from = t5_smem(to - (quarter * 32 + lane));
+                        if (MODE == MG_ADD)
+                            asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(from),
+                                         "r"(wt * MG_ROWS), "r"(tok0 + c) : "memory");
+                        else
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(from),
+                                         "r"(wt * MG_ROWS), "r"(tok0 + c) : "memory");
+                    }
+                    if (tid == 64) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+                }
             } else {
-                // a lane is a feature: a token's 32 features leave side by side
+                // rows that the copy engine cannot address: a lane is a feature, a token's 32 features leave side by side
                 const int f = wt * MG_ROWS + quarter * 32 + lane;
                 TO* y = static_cast<TO*>(a.y) + static_cast<size_t>(tok0) * a.N + f;
 #pragma unroll 1
-                for (int c = 0; c < toks; c += 32) {
-                    unsigned r[32];
-                    t5_ld32(acc + c, r);
-                    float old[32];
-                    if (MODE == MG_ADD)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) old[i] = f < a.N && c + i < toks ? to_f32(y[static_cast<size_t>(c + i) * a.N]) : 0.0f;
+                for (int c = 0; c < toks; c += 16) {
+                    unsigned r[16];
+                    t5_ld16(acc + c, r);
                     t5_wait_ld();
                     if (f < a.N)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (c + i < toks) y[static_cast<size_t>(c + i) * a.N] = from_f32<TO>(MODE == MG_ADD ? __uint_as_float(r[i]) + old[i] : __uint_as_float(r[i]));
+                        for (int i = 0; i < 16; ++i)
+                            if (c + i < toks) {
+                                TO* to = y + static_cast<size_t>(c + i) * a.N;
+                                *to = from_f32<TO>(MODE == MG_ADD ? __uint_as_float(r[i]) + to_f32(*to) : __uint_as_float(r[i]));
+                            }
                 }
             }
             t5_fence_before();
@@ -461,6 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
             if (!ok) break;
         }
+        if (tid == 64) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");       // the result is there before this grid is over
     }
     t5_fence_before();
     __syncthreads();
@@ -544,12 +570,21 @@ static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
 }
 template <int MODE, typename TO>
 static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
-    CUtensorMap w_map, x_map, ws_map, xs_map;
+    CUtensorMap w_map, x_map, ws_map, xs_map, y_map = {};
     const int padded = mg_padded_rows(a.T), stored = (tiles + 1) / 2 * 2;
     if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles * MX_K, MP_NT / 2) ||
         !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, 2))
         return LLM_REFUSED_SIZE;
-    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES + MP_S_BYTES) + (MODE == MG_GATED ? 2 * MP_TURN : 0) + 1024;
+    if (MODE != MG_GATED) {                                       // [T, N] in boxes of 32 rows x 128 values
+        a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.N), static_cast<cuuint64_t>(a.T)}, strides[1] = {static_cast<cuuint64_t>(a.N) * sizeof(TO)};
+        const cuuint32_t box[2] = {MG_ROWS, 32}, es[2] = {1u, 1u};
+        if (a.vec && g_t5_encode(&y_map, sizeof(TO) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, strides, box, es,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return LLM_REFUSED_SIZE;
+    }
+    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES + MP_S_BYTES) + 2 * MP_TURN + 1024;
     static_assert(smem <= 226 * 1024, "shared memory of an SM");
     static_assert(2 * MP_NT + MP_STAGES * MP_S_COLS <= 512, "tensor memory");
     auto kern = linear_mx_pair_kernel<MODE, TO>;
@@ -559,7 +594,7 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     const int slots = mg_sms() / 2;
     if (slots <= 0 || all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
-    launch_pdl(kern, dim3(2 * clusters), dim3(MG_THREADS), smem, s, w_map, x_map, ws_map, xs_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
+    launch_pdl(kern, dim3(2 * clusters), dim3(MG_THREADS), smem, s, w_map, x_map, ws_map, xs_map, y_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
     return launch_status();
 }
 template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
