@@ -249,11 +249,13 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
 // next one's products; 192 tokens leave room for both and for the scales of all stages in tensor memory.  Tiles are numbered token
 // tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.
 #define MP_NT 192
-#define MP_STAGES 6
+#define MP_STAGES 7
+#define MP_THREADS 256
 #define MP_X_BYTES (MP_NT / 2 * MX_K)
-#define MP_S_BYTES (3 * MX_PIECE)                                 // own weights' scales, both pieces of the rows'
-#define MP_S_COLS 12
-#define MP_TURN (32 * MG_ROWS * 4)                                // 32 tokens' sums, on their way out
+#define MP_QUAD 4                                                 // stages whose scales come together, two such groups at a time
+#define MP_S_BYTES (MP_QUAD * 3 * MX_PIECE)                       // own weights' scales, then both pieces of the rows'
+#define MP_S_COLS (MP_QUAD * 12)
+#define MP_TURN 8192                                              // a block of sums on their way out
 
 __device__ __forceinline__ unsigned mp_rank() {
     unsigned r;
@@ -312,15 +314,16 @@ __device__ __forceinline__ void mp_cluster_sync() {
 }
 
 template <int MODE, typename TO>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linear_mx_pair_kernel(
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linear_mx_pair_kernel(
     const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap ws_map,
     const __grid_constant__ CUtensorMap xs_map, const __grid_constant__ CUtensorMap y_map, const MgArgs a, int token_tiles, int tiles) {
+    constexpr int CHUNK = MP_TURN / (MG_ROWS * sizeof(TO));       // tokens of a block
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     unsigned char* x_s = w_s + MP_STAGES * MG_W_BYTES;            // [STAGES][96 tokens][128]
-    unsigned char* s_s = x_s + MP_STAGES * MP_X_BYTES;            // [STAGES][three pieces]
-    float* turn = reinterpret_cast<float*>(s_s + MP_STAGES * MP_S_BYTES);      // two blocks
-    __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], acc_full[2], acc_empty[2];
+    unsigned char* s_s = x_s + MP_STAGES * MP_X_BYTES;            // [2][the weights' QUAD pieces, the rows' two times QUAD]
+    float* turn = reinterpret_cast<float*>(s_s + 2 * MP_S_BYTES); // two blocks
+    __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], s_full[2], s_empty[2], acc_full[2], acc_empty[2];
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -328,8 +331,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
     const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1, ktiles = a.ktiles;
     if (tid == 0) {
         abort_flag = 0;
-        for (int s = 0; s < MP_STAGES; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 8); }   // 4 epilogue warps of 2 CTAs
+        for (int s = 0; s < MP_STAGES; ++s) { t5_mbar_init(&full[s], 2); t5_mbar_init(&empty[s], 1); }      // weights and rows
+        for (int s = 0; s < 2; ++s) {
+            t5_mbar_init(&s_full[s], 1);
+            t5_mbar_init(&s_empty[s], 1);
+            t5_mbar_init(&acc_full[s], 1);
+            t5_mbar_init(&acc_empty[s], 8);                       // 4 epilogue warps of 2 CTAs
+        }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
@@ -344,23 +352,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
     pdl_wait();
 
-    if (warp == 0) {
+    if (warp == 0 || warp >= 6) {
+        // Three threads feed: the weights (warp 0), the rows (6) and the scales (7).  Asking for a box takes a thread 80 clocks and a
+        // turn of the loop 150 more; one thread for all of a stage took 650, its four products 400.
         if (lane == 0) {
-            const unsigned full_first = mp_map_to(t5_smem(&full[0]), 0);
-            int it = 0;
+            const bool scales = warp == 7;
+            const unsigned first = mp_map_to(t5_smem(scales ? &s_full[0] : &full[0]), 0);      // the first CTA's barriers
+            unsigned long long* own = scales ? s_full : full;
+            unsigned long long* free = scales ? s_empty : empty;
+            const int ring = scales ? 2 : MP_STAGES, step = scales ? MP_QUAD : 1;
+            const unsigned bytes = 2 * (scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : MP_X_BYTES);      // of both CTAs
+            int s = 0;
+            unsigned phase = 1;                                   // a barrier that was never used passes for the phase before its first
             bool ok = true;
             for (int t = cluster; ok && t < tiles; t += clusters) {
-                const int tok0 = (t % token_tiles) * MP_NT, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
-                for (int kb = 0; kb < ktiles; ++kb, ++it) {
-                    const int s = it % MP_STAGES;
-                    if (it >= MP_STAGES && !mg_wait(&empty[s], (it / MP_STAGES - 1) & 1, a.waits, &abort_flag, a.status)) { ok = false; break; }
-                    if (rank == 0) t5_expect_tx(&full[s], 2 * (MG_W_READ + MP_X_BYTES + MP_S_BYTES));      // both CTAs' boxes
-                    const unsigned bar = full_first + s * 8;
-                    const int at = wt * ktiles + kb;
-                    mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, at * MG_ROWS, bar);
-                    mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at, bar);
-                    mp_tma_2d(x_s + s * MP_X_BYTES, &x_map, kb * MX_K, tok0 + static_cast<int>(rank) * (MP_NT / 2), bar);
-                    mp_tma_3d(s_s + s * MP_S_BYTES + MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
+                const int tok0 = (t % token_tiles) * MP_NT, at = ((t / token_tiles) * 2 + static_cast<int>(rank)) * ktiles;
+#pragma unroll 1
+                for (int kb = 0; kb < ktiles; kb += step) {
+                    if (!mg_wait(&free[s], phase, a.waits, &abort_flag, a.status)) { ok = false; break; }
+                    if (rank == 0) t5_expect_tx(&own[s], bytes);
+                    const unsigned bar = first + s * 8;
+                    if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
+                    else if (warp == 6) mp_tma_2d(x_s + s * MP_X_BYTES, &x_map, kb * MX_K, tok0 + static_cast<int>(rank) * (MP_NT / 2), bar);
+                    else {                                        // what stands behind the last tile of K is read and not used
+                        mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at + kb, bar);
+                        mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
+                    }
+                    if (++s == ring) s = 0, phase ^= 1;
                 }
             }
             if (!ok)                                              // let what is in flight land before the CTA goes away
@@ -371,7 +389,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
         if (rank == 0) {
             const unsigned lead = elect_one();
             const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024), sd = mg_scale_desc(s_s);
-            int it = 0, n = 0;
+            int s = 0, n = 0, quad = 0;
+            unsigned phase = 0;
             bool ok = true;
             for (int t = cluster; ok && t < tiles; t += clusters, ++n) {
                 const int buf = n & 1;
@@ -379,23 +398,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
                 if (n >= 2) ok = __all_sync(0xffffffffu, mp_wait_cluster(&acc_empty[buf], ((n >> 1) - 1) & 1, a.waits, &abort_flag, a.status));
                 t5_fence_after();
 #pragma unroll 1
-                for (int kb = 0; ok && kb < ktiles; ++kb, ++it) {
-                    const int s = it % MP_STAGES;
-                    ok = __all_sync(0xffffffffu, mg_wait(&full[s], (it / MP_STAGES) & 1, a.waits, &abort_flag, a.status));
+                for (int k0 = 0; ok && k0 < ktiles; k0 += MP_QUAD, ++quad) {
+                    const int qs = quad & 1;
+                    ok = __all_sync(0xffffffffu, mg_wait(&s_full[qs], (quad >> 1) & 1, a.waits, &abort_flag, a.status));
                     if (!ok) break;
-                    const unsigned sc = tmem + 2 * MP_NT + s * MP_S_COLS;
+                    // [weights, rows' first piece, rows' second] of each stage; products that read the group before last have run
+                    const unsigned sc0 = tmem + 2 * MP_NT + qs * MP_S_COLS;
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) mp_scales_lead(lead, sc + 4 * p, sd + ((s * MP_S_BYTES + p * MX_PIECE) >> 4));
+                    for (int q = 0; q < MP_QUAD; ++q)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mp_mma_lead(lead, tmem + buf * MP_NT, wd + s * (MG_W_BYTES >> 4) + 2 * k, xd + s * (MP_X_BYTES >> 4) + 2 * k,
-                                    mg_idesc(2 * MG_ROWS, MP_NT, k), sc, sc + 4 + off, (kb | k) ? 1u : 0u);
-                    mp_commit_lead(lead, &empty[s]);
+                        for (int p = 0; p < 3; ++p) mp_scales_lead(lead, sc0 + 12 * q + 4 * p, sd + ((qs * MP_S_BYTES + (p * MP_QUAD + q) * MX_PIECE) >> 4));
+#pragma unroll 1
+                    for (int q = 0; q < min(MP_QUAD, ktiles - k0); ++q) {
+                        ok = __all_sync(0xffffffffu, mg_wait(&full[s], phase, a.waits, &abort_flag, a.status));
+                        if (!ok) break;
+                        const unsigned sc = sc0 + 12 * q;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mp_mma_lead(lead, tmem + buf * MP_NT, wd + s * (MG_W_BYTES >> 4) + 2 * k, xd + s * (MP_X_BYTES >> 4) + 2 * k,
+                                        mg_idesc(2 * MG_ROWS, MP_NT, k), sc, sc + 4 + off, (k0 | q | k) ? 1u : 0u);
+                        mp_commit_lead(lead, &empty[s]);
+                        if (++s == MP_STAGES) s = 0, phase ^= 1;
+                    }
+                    if (ok) mp_commit_lead(lead, &s_empty[qs]);
                 }
                 if (ok) mp_commit_lead(lead, &acc_full[buf]);
             }
         }
-    } else {
+    } else {                                                      // warps 2 to 5
         const int quarter = warp & 3;
         const unsigned acc_empty_first = mp_map_to(t5_smem(&acc_empty[0]), 0);
         int n = 0, turns = 0;
@@ -407,20 +437,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
             t5_fence_after();
             const unsigned acc = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * MP_NT;
             if constexpr (MODE == MG_GATED) {
-                // 32 tokens at a time through shared memory; then sixteen lanes a token, four features a lane, eight lanes a block
+                // 16 tokens at a time through shared memory; then sixteen lanes a token, four features a lane, eight lanes a block
                 const int e = tid - 64, f = 4 * (e & 15);
                 unsigned char* codes = static_cast<unsigned char*>(a.y);
 #pragma unroll 1
-                for (int c = 0; c < toks; c += 32, ++turns) {
-                    unsigned r[32];
-                    t5_ld32(acc + c, r);
+                for (int c = 0; c < toks; c += 16, ++turns) {
+                    unsigned r[16];
+                    t5_ld16(acc + c, r);
                     t5_wait_ld();
                     float* to = turn + (turns & 1) * (MP_TURN / 4);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) to[i * MG_ROWS + quarter * 32 + lane] = __uint_as_float(r[i]);
+                    for (int i = 0; i < 16; ++i) to[i * MG_ROWS + quarter * 32 + lane] = __uint_as_float(r[i]);
                     asm volatile("bar.sync 1, 128;\n" ::: "memory");      // with two blocks in turn the next writes wait for this one's reads
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 2; ++i) {
                         const int tok = (e >> 4) + 8 * i;
                         const float4 g = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + f), u = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + 64 + f);
                         const float v[4] = {gated(g.x, u.x, a.act, a.limit), gated(g.y, u.y, a.act, a.limit), gated(g.z, u.z, a.act, a.limit),
@@ -438,18 +468,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MG_THREADS, 1) linea
                     }
                 }
             } else if (a.vec) {
-                // 32 tokens at a time through shared memory and out by the copy engine, which also adds and leaves out what is beyond
+                // 8 KB at a time through shared memory and out by the copy engine, which also adds and leaves out what is beyond
                 // the matrix.  Stores straight from the lanes (a token's 32 features, 64 bytes) took longer than a tile's products.
 #pragma unroll 1
-                for (int c = 0; c < toks; c += 32, ++turns) {
-                    unsigned r[32];
-                    t5_ld32(acc + c, r);
-                    TO* to = reinterpret_cast<TO*>(turn) + (turns & 1) * (32 * MG_ROWS) + quarter * 32 + lane;
+                for (int c = 0; c < toks; c += CHUNK, ++turns) {
+                    unsigned r[CHUNK];
+                    if constexpr (CHUNK == 32) t5_ld32(acc + c, r);
+                    else t5_ld16(acc + c, r);
+                    TO* to = reinterpret_cast<TO*>(turn) + (turns & 1) * (CHUNK * MG_ROWS) + quarter * 32 + lane;
                     if (tid == 64) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");       // the block before last has been read
                     t5_wait_ld();
                     asm volatile("bar.sync 1, 128;\n" ::: "memory");
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) to[i * MG_ROWS] = from_f32<TO>(__uint_as_float(r[i]));
+                    for (int i = 0; i < CHUNK; ++i) to[i * MG_ROWS] = from_f32<TO>(__uint_as_float(r[i]));
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     asm volatile("bar.sync 1, 128;\n" ::: "memory");
                     if (tid == 64 && wt * MG_ROWS < a.N) {
@@ -523,11 +554,12 @@ static bool mg_rows_map(CUtensorMap* map, const void* x, int rows, int kpad, int
     return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(x), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// Pieces of scales as lines of 128 words: [tiles of rows][ktiles] in boxes of `box_tiles` neighbouring tiles of rows (three dimensions), or of one line.
+// Pieces of scales as lines of 128 words: [tiles of rows][ktiles] in boxes of MP_QUAD lines, of `box_tiles` neighbouring tiles of rows (three
+// dimensions) or of one.
 static bool mg_scales_map(CUtensorMap* map, const void* scales, int row_tiles, int ktiles, int box_tiles) {
     const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(ktiles), static_cast<cuuint64_t>(row_tiles)};
     const cuuint64_t strides[2] = {MX_PIECE, static_cast<cuuint64_t>(ktiles) * MX_PIECE};
-    const cuuint32_t box[3] = {128, 1, static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
+    const cuuint32_t box[3] = {128, MP_QUAD, static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
     const cuuint64_t line_dims[2] = {128, static_cast<cuuint64_t>(ktiles) * static_cast<cuuint64_t>(row_tiles)};
     if (line_dims[1] >= (1ULL << 31)) return false;
     return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, box_tiles ? 3 : 2, const_cast<void*>(scales), box_tiles ? dims : line_dims, strides, box, es,
@@ -575,18 +607,18 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles * MX_K, MP_NT / 2) ||
         !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, 2))
         return LLM_REFUSED_SIZE;
-    if (MODE != MG_GATED) {                                       // [T, N] in boxes of 32 rows x 128 values
+    if (MODE != MG_GATED) {                                       // [T, N] in boxes of 8 KB, 128 values wide
         a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
         const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.N), static_cast<cuuint64_t>(a.T)}, strides[1] = {static_cast<cuuint64_t>(a.N) * sizeof(TO)};
-        const cuuint32_t box[2] = {MG_ROWS, 32}, es[2] = {1u, 1u};
+        const cuuint32_t box[2] = {MG_ROWS, MP_TURN / (MG_ROWS * sizeof(TO))}, es[2] = {1u, 1u};
         if (a.vec && g_t5_encode(&y_map, sizeof(TO) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, strides, box, es,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return LLM_REFUSED_SIZE;
     }
-    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES + MP_S_BYTES) + 2 * MP_TURN + 1024;
-    static_assert(smem <= 226 * 1024, "shared memory of an SM");
-    static_assert(2 * MP_NT + MP_STAGES * MP_S_COLS <= 512, "tensor memory");
+    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES) + 2 * MP_S_BYTES + 2 * MP_TURN + 1024;
+    static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
+    static_assert(2 * MP_NT + 2 * MP_S_COLS <= 512, "tensor memory");
     auto kern = linear_mx_pair_kernel<MODE, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -594,7 +626,7 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     const int slots = mg_sms() / 2;
     if (slots <= 0 || all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
-    launch_pdl(kern, dim3(2 * clusters), dim3(MG_THREADS), smem, s, w_map, x_map, ws_map, xs_map, y_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
+    launch_pdl(kern, dim3(2 * clusters), dim3(MP_THREADS), smem, s, w_map, x_map, ws_map, xs_map, y_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
     return launch_status();
 }
 template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
