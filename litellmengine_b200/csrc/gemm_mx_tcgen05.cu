@@ -59,9 +59,9 @@ struct MgArgs {
     const unsigned char *w_scales, *x_scales;
     void* y;                              // [T, N]; gated: the codes [T, out_kpad]
     unsigned char* y_scales;              // gated
-    int T, N, ktiles, out_kpad, vec, act, waits;
-    float limit;
+    int T, N, ktiles, out_kpad, vec, waits;
     int32_t* status;
+    MxAct act;
 };
 enum { MG_STORE = 0, MG_ADD = 1, MG_GATED = 2 };
 
@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
                 const int tok = t0 + part + (tid >> 4) * parts;
                 const bool there = tok < toks;
                 const float4 g = total((there ? tok : 0) * MG_ROWS + f), u = total((there ? tok : 0) * MG_ROWS + 64 + f);
-                float v[4] = {gated(g.x, u.x, a.act, a.limit), gated(g.y, u.y, a.act, a.limit), gated(g.z, u.z, a.act, a.limit),
-                              gated(g.w, u.w, a.act, a.limit)};
+                float v[4] = {mx_gated(g.x, u.x, a.act), mx_gated(g.y, u.y, a.act), mx_gated(g.z, u.z, a.act),
+                              mx_gated(g.w, u.w, a.act)};
                 unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
 #pragma unroll
                 for (int o = 1; o < 8; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
 // next one's products; 192 tokens leave room for both and for the scales of all stages in tensor memory.  Tiles are numbered token
 // tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.
 #define MP_NT 192
-#define MP_STAGES 7
-#define MP_THREADS 256
+#define MP_STAGES 6
+#define MP_THREADS 384            // weights, products, 4 + 4 warps for the results, rows, scales
 #define MP_X_BYTES (MP_NT / 2 * MX_K)
 #define MP_QUAD 4                                                 // stages whose scales come together, two such groups at a time
 #define MP_S_BYTES (MP_QUAD * 3 * MX_PIECE)                       // own weights' scales, then both pieces of the rows'
@@ -302,11 +302,11 @@ __device__ __forceinline__ void mp_mma_lead(unsigned lead, unsigned d_tmem, unsi
                  " @q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::
                      "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(lead) : "memory");
 }
-// Whether all of the four epilogue warps say so.
-__device__ __forceinline__ bool mp_all(bool yes) {
+// Whether all of the four warps at this barrier say so.
+__device__ __forceinline__ bool mp_all(bool yes, int bar) {
     unsigned r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.aligned.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-                 : "=r"(r) : "r"(static_cast<unsigned>(yes)) : "memory");
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.aligned.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r) : "r"(static_cast<unsigned>(yes)), "r"(bar) : "memory");
     return r != 0;
 }
 __device__ __forceinline__ void mp_cluster_sync() {
@@ -322,7 +322,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     unsigned char* x_s = w_s + MP_STAGES * MG_W_BYTES;            // [STAGES][96 tokens][128]
     unsigned char* s_s = x_s + MP_STAGES * MP_X_BYTES;            // [2][the weights' QUAD pieces, the rows' two times QUAD]
-    float* turn = reinterpret_cast<float*>(s_s + 2 * MP_S_BYTES); // two blocks
+    float* turns_s = reinterpret_cast<float*>(s_s + 2 * MP_S_BYTES);      // two blocks for each half of the result's warps
     __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], s_full[2], s_empty[2], acc_full[2], acc_empty[2];
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag;
@@ -336,7 +336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             t5_mbar_init(&s_full[s], 1);
             t5_mbar_init(&s_empty[s], 1);
             t5_mbar_init(&acc_full[s], 1);
-            t5_mbar_init(&acc_empty[s], 8);                       // 4 epilogue warps of 2 CTAs
+            t5_mbar_init(&acc_empty[s], 16);                      // 8 warps of 2 CTAs
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -352,11 +352,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
     pdl_wait();
 
-    if (warp == 0 || warp >= 6) {
-        // Three threads feed: the weights (warp 0), the rows (6) and the scales (7).  Asking for a box takes a thread 80 clocks and a
+    if (warp == 0 || warp >= 10) {
+        // Three threads feed: the weights (warp 0), the rows (10) and the scales (11).  Asking for a box takes a thread 80 clocks and a
         // turn of the loop 150 more; one thread for all of a stage took 650, its four products 400.
         if (lane == 0) {
-            const bool scales = warp == 7;
+            const bool scales = warp == 11;
             const unsigned first = mp_map_to(t5_smem(scales ? &s_full[0] : &full[0]), 0);      // the first CTA's barriers
             unsigned long long* own = scales ? s_full : full;
             unsigned long long* free = scales ? s_empty : empty;
@@ -373,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                     if (rank == 0) t5_expect_tx(&own[s], bytes);
                     const unsigned bar = first + s * 8;
                     if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
-                    else if (warp == 6) mp_tma_2d(x_s + s * MP_X_BYTES, &x_map, kb * MX_K, tok0 + static_cast<int>(rank) * (MP_NT / 2), bar);
+                    else if (warp == 10) mp_tma_2d(x_s + s * MP_X_BYTES, &x_map, kb * MX_K, tok0 + static_cast<int>(rank) * (MP_NT / 2), bar);
                     else {                                        // what stands behind the last tile of K is read and not used
                         mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at + kb, bar);
                         mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
@@ -425,36 +425,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                 if (ok) mp_commit_lead(lead, &acc_full[buf]);
             }
         }
-    } else {                                                      // warps 2 to 5
-        const int quarter = warp & 3;
+    } else {                                                      
+        // warps 2 to 5 and 6 to 9: two halves that take a tile's blocks of tokens in turn
+        const int quarter = warp & 3, half = (warp - 2) >> 2, e = (tid - 64) & 127;
+        float* turn = turns_s + half * (2 * MP_TURN / 4);
         const unsigned acc_empty_first = mp_map_to(t5_smem(&acc_empty[0]), 0);
         int n = 0, turns = 0;
         for (int t = cluster; t < tiles; t += clusters, ++n) {
             const int buf = n & 1, tok0 = (t % token_tiles) * MP_NT, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
             const int toks = min(MP_NT, a.T - tok0);
             bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
-            ok = mp_all(ok);                                      // the four warps meet below: they go on or leave together
+            ok = mp_all(ok, 1 + half);                            // the four warps meet below: they go on or leave together
             t5_fence_after();
             const unsigned acc = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * MP_NT;
             if constexpr (MODE == MG_GATED) {
                 // 16 tokens at a time through shared memory; then sixteen lanes a token, four features a lane, eight lanes a block
-                const int e = tid - 64, f = 4 * (e & 15);
+                const int f = 4 * (e & 15);
                 unsigned char* codes = static_cast<unsigned char*>(a.y);
 #pragma unroll 1
-                for (int c = 0; c < toks; c += 16, ++turns) {
+                for (int c = 16 * half; c < toks; c += 32, ++turns) {
                     unsigned r[16];
                     t5_ld16(acc + c, r);
                     t5_wait_ld();
                     float* to = turn + (turns & 1) * (MP_TURN / 4);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) to[i * MG_ROWS + quarter * 32 + lane] = __uint_as_float(r[i]);
-                    asm volatile("bar.sync 1, 128;\n" ::: "memory");      // with two blocks in turn the next writes wait for this one's reads
+                    asm volatile("bar.sync %0, 128;\n" ::"r"(1 + half) : "memory");      // with two blocks in turn the next writes wait for this one's reads
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int tok = (e >> 4) + 8 * i;
                         const float4 g = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + f), u = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + 64 + f);
-                        const float v[4] = {gated(g.x, u.x, a.act, a.limit), gated(g.y, u.y, a.act, a.limit), gated(g.z, u.z, a.act, a.limit),
-                                            gated(g.w, u.w, a.act, a.limit)};
+                        const float v[4] = {mx_gated(g.x, u.x, a.act), mx_gated(g.y, u.y, a.act), mx_gated(g.z, u.z, a.act),
+                                            mx_gated(g.w, u.w, a.act)};
                         unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
 #pragma unroll
                         for (int o = 1; o < 8; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -471,19 +473,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                 // 8 KB at a time through shared memory and out by the copy engine, which also adds and leaves out what is beyond
                 // the matrix.  Stores straight from the lanes (a token's 32 features, 64 bytes) took longer than a tile's products.
 #pragma unroll 1
-                for (int c = 0; c < toks; c += CHUNK, ++turns) {
+                for (int c = CHUNK * half; c < toks; c += 2 * CHUNK, ++turns) {
                     unsigned r[CHUNK];
                     if constexpr (CHUNK == 32) t5_ld32(acc + c, r);
                     else t5_ld16(acc + c, r);
                     TO* to = reinterpret_cast<TO*>(turn) + (turns & 1) * (CHUNK * MG_ROWS) + quarter * 32 + lane;
-                    if (tid == 64) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");       // the block before last has been read
+                    if (e == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");       // the block before last has been read
                     t5_wait_ld();
-                    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+                    asm volatile("bar.sync %0, 128;\n" ::"r"(1 + half) : "memory");
 #pragma unroll
                     for (int i = 0; i < CHUNK; ++i) to[i * MG_ROWS] = from_f32<TO>(__uint_as_float(r[i]));
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    asm volatile("bar.sync 1, 128;\n" ::: "memory");
-                    if (tid == 64 && wt * MG_ROWS < a.N) {
+                    asm volatile("bar.sync %0, 128;\n" ::"r"(1 + half) : "memory");
+                    if (e == 0 && wt * MG_ROWS < a.N) {
                         const unsigned from = t5_smem(to - (quarter * 32 + lane));
                         if (MODE == MG_ADD)
                             asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(from),
@@ -492,14 +494,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(from),
                                          "r"(wt * MG_ROWS), "r"(tok0 + c) : "memory");
                     }
-                    if (tid == 64) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+                    if (e == 0) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                 }
             } else {
                 // rows that the copy engine cannot address: a lane is a feature, a token's 32 features leave side by side
                 const int f = wt * MG_ROWS + quarter * 32 + lane;
                 TO* y = static_cast<TO*>(a.y) + static_cast<size_t>(tok0) * a.N + f;
 #pragma unroll 1
-                for (int c = 0; c < toks; c += 16) {
+                for (int c = 16 * half; c < toks; c += 32) {
                     unsigned r[16];
                     t5_ld16(acc + c, r);
                     t5_wait_ld();
@@ -517,7 +519,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
             if (!ok) break;
         }
-        if (tid == 64) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");       // the result is there before this grid is over
+        if (e == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");       // the result is there before this grid is over
     }
     t5_fence_before();
     __syncthreads();
@@ -616,7 +618,7 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return LLM_REFUSED_SIZE;
     }
-    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES) + 2 * MP_S_BYTES + 2 * MP_TURN + 1024;
+    constexpr size_t smem = static_cast<size_t>(MP_STAGES) * (MG_W_BYTES + MP_X_BYTES) + 2 * MP_S_BYTES + 4 * MP_TURN + 1024;
     static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
     static_assert(2 * MP_NT + 2 * MP_S_COLS <= 512, "tensor memory");
     auto kern = linear_mx_pair_kernel<MODE, TO>;
@@ -651,7 +653,7 @@ extern "C" int llm_linear_mx(const void* x, const void* x_scales, const void* w,
     if (const int rc = mg_check(w, w_scales, x, x_scales, status, T, N, K)) return rc;
     if ((out_dtype != LLM_DT_F32 && out_dtype != LLM_DT_BF16) || (add && out_dtype != LLM_DT_F32)) return LLM_REFUSED_DTYPE;
     MgArgs a = {static_cast<const unsigned char*>(w_scales), static_cast<const unsigned char*>(x_scales), y, nullptr, T, N, (K + MX_K - 1) / MX_K, 0,
-                N % 4 == 0 && aligned16(y), 0, waits, 0.0f, status};
+                N % 4 == 0 && aligned16(y), waits, status, {}};
     const int tiles = (N + MG_ROWS - 1) / MG_ROWS;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (add) return mg_rows<MG_ADD, float>(w, tiles, x, a, s);
@@ -664,10 +666,11 @@ extern "C" int llm_linear_mx_silu_mul(const void* x, const void* x_scales, const
                                       int N, int K, int act, float limit, int waits, int32_t* status, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
     if (const int rc = mg_check(w, w_scales, x, x_scales, status, T, N, K)) return rc;
-    if (act < 0 || act > 2 || (act == 2 && !(limit > 0.0f))) return LLM_REFUSED_SIZE;
+    MxAct form;
+    if (!mx_act(act, limit, &form)) return LLM_REFUSED_SIZE;
     if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
     const int tiles = 2 * ((N + 127) / 128);                      // as the weight has them
     MgArgs a = {static_cast<const unsigned char*>(w_scales), static_cast<const unsigned char*>(x_scales), codes, static_cast<unsigned char*>(scales), T, N,
-                (K + MX_K - 1) / MX_K, tiles * 64, 0, act, waits, limit, status};
+                (K + MX_K - 1) / MX_K, tiles * 64, 0, waits, status, form};
     return mg_rows<MG_GATED, float>(w, tiles, x, a, reinterpret_cast<cudaStream_t>(stream));
 }

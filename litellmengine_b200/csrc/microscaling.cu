@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_rows_kernel(const T* __restrict
 template <typename T>
 __global__ void __launch_bounds__(MX_THREADS) mx_act_kernel(const T* __restrict__ gu, unsigned char* __restrict__ codes,
                                                             unsigned char* __restrict__ scales, long long pieces, int inter, int kpad, int vec,
-                                                            int parts, long long part_stride, int act, float limit) {
+                                                            int parts, long long part_stride, const MxAct act) {
     pdl_begin();
     const long long at = blockIdx.x * static_cast<long long>(MX_THREADS) + threadIdx.x;
     const bool there = at < pieces;
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_act_kernel(const T* __restrict_
         for (int i = 0; i < 8; ++i) b[i] += c[i];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = col + i < inter ? gated(a[i], b[i], act, limit) : 0.0f;
+    for (int i = 0; i < 8; ++i) a[i] = col + i < inter ? mx_gated(a[i], b[i], act) : 0.0f;
     mx_store_row8(a, there, row, col, kpad, codes, scales);
 }
 
@@ -194,7 +194,8 @@ extern "C" int llm_mx_rows(const void* x, int dtype, void* codes, void* scales, 
 extern "C" int llm_mx_silu_and_mul(const void* gu, int dtype, int parts, long long part_stride, void* codes, void* scales, int T, int inter, int act,
                                    float limit, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
-    if (inter <= 0 || inter > MX_MOST_K || parts < 1 || act < 0 || act > 2 || (act == 2 && !(limit > 0.0f))) return LLM_REFUSED_SIZE;
+    MxAct form;
+    if (inter <= 0 || inter > MX_MOST_K || parts < 1 || !mx_act(act, limit, &form)) return LLM_REFUSED_SIZE;
     if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
     const int kpad = mx_tiles(inter) * MX_K, vec = inter % 8 == 0 && part_stride % 8 == 0 && aligned16(gu);
     const long long pieces = static_cast<long long>(T) * (kpad / 8);
@@ -203,9 +204,9 @@ extern "C" int llm_mx_silu_and_mul(const void* gu, int dtype, int parts, long lo
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     unsigned char *c = static_cast<unsigned char*>(codes), *sc = static_cast<unsigned char*>(scales);
     if (dtype == LLM_DT_F32)
-        launch_pdl(mx_act_kernel<float>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const float*>(gu), c, sc, pieces, inter, kpad, vec, parts, part_stride, act, limit);
+        launch_pdl(mx_act_kernel<float>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const float*>(gu), c, sc, pieces, inter, kpad, vec, parts, part_stride, form);
     else if (dtype == LLM_DT_BF16)
-        launch_pdl(mx_act_kernel<bf16>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const bf16*>(gu), c, sc, pieces, inter, kpad, vec, parts, part_stride, act, limit);
+        launch_pdl(mx_act_kernel<bf16>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const bf16*>(gu), c, sc, pieces, inter, kpad, vec, parts, part_stride, form);
     else return LLM_REFUSED_DTYPE;
     return launch_status();
 }
