@@ -18,7 +18,7 @@
 #include "tcgen05_attention.cuh"
 
 #define MG_ROWS 128               // features of a tile (gated: 64 of both)
-#define MG_THREADS 192
+#define MG_THREADS 224
 #define MG_W_BYTES (MG_ROWS * MX_K)       // of a stage's weights in shared memory
 #define MG_W_READ (MG_W_BYTES / 2)        // the same as the copy engine counts them: what it reads
 #define MG_STATUS 12
@@ -32,9 +32,9 @@ __device__ __forceinline__ bool mg_wait(unsigned long long* bar, unsigned parity
     if (atomicCAS(status, 0, MG_STATUS) == 0) status[1] = blockIdx.y;
     return false;
 }
-__device__ __forceinline__ void mg_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(t5_smem(dst)), "l"(src), "r"(bytes),
-                 "r"(t5_smem(bar)) : "memory");
+__device__ __forceinline__ void mg_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(t5_smem(dst)), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(t5_smem(bar)) : "memory");
 }
 // A piece of scales to tensor memory: 32 lanes of 16 bytes, repeated in every quarter of the lanes.
 __device__ __forceinline__ void mg_scales_lead(unsigned lead, unsigned tmem, unsigned long long desc) {
@@ -65,18 +65,19 @@ struct MgArgs {
 };
 enum { MG_STORE = 0, MG_ADD = 1, MG_GATED = 2 };
 
-// grid (parts of K, tiles of features, tiles of tokens), a cluster the parts of a tile.
-template <int NT, int STAGES, int MODE, typename TO>
-__global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel(const __grid_constant__ CUtensorMap w_map,
-                                                                               const __grid_constant__ CUtensorMap x_map, const MgArgs a) {
-    constexpr unsigned X_BYTES = NT * MX_K, S_BYTES = 2 * MX_PIECE, S_COLS = 8, S_COL0 = NT < 32 ? 32 : NT;
-    constexpr unsigned COLS = S_COL0 + STAGES * S_COLS <= 128 ? 128 : S_COL0 + STAGES * S_COLS <= 256 ? 256 : 512;
+// grid (parts of K, tiles of features, tiles of tokens), a cluster the parts of a tile.  WS: stages of weights; G: stages whose rows and scales
+// come together, two such groups at a time.
+template <int NT, int WS, int G, int MODE, typename TO>
+__global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                                                                               const __grid_constant__ CUtensorMap ws_map,
+                                                                               const __grid_constant__ CUtensorMap xs_map, const MgArgs a) {
+    constexpr unsigned X_BYTES = NT * MX_K, S_BYTES = G * MX_PIECE, GROUP_BYTES = G * X_BYTES + 2 * S_BYTES;
+    constexpr unsigned S_COL0 = NT < 32 ? 32 : NT, COLS = S_COL0 + 2 * G * 8 <= 128 ? 128 : 256;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-    unsigned char* x_s = w_s + STAGES * MG_W_BYTES;               // [STAGES][NT][128], 128-byte swizzle like the weights
-    unsigned char* s_s = x_s + STAGES * X_BYTES;                  // [STAGES][weights' piece, rows' pieces]
+    unsigned char* g_s = w_s + WS * MG_W_BYTES;                   // [2][G rows' boxes [NT][128], 128-byte swizzle like the weights; weights' pieces, rows' pieces]
     float* sums = reinterpret_cast<float*>(w_s);                  // [NT][128], when the stages have been read
-    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full;
+    __shared__ __align__(8) unsigned long long full[WS], empty[WS], g_full[2], g_empty[2], acc_full;
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -84,7 +85,8 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
     const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0;
     if (tid == 0) {
         abort_flag = 0;
-        for (int s = 0; s < STAGES; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
+        for (int s = 0; s < WS; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&g_full[s], 2); t5_mbar_init(&g_empty[s], 1); }      // the weights' scales; rows and theirs
         t5_mbar_init(&acc_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -98,51 +100,71 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
     pdl_invite();                                                 // not before: this CTA's tensor memory is taken
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
 
-    int issued = 0;                                               // stages that were asked for, in the thread that asks
+    int issued = 0;                                               // stages, or groups, that were asked for, in the threads that ask
     if (warp == 0) {
-        if (lane == 0) {
-            auto weights = [&](int kb) {
-                const int st = kb % STAGES;
-                const long long at = static_cast<long long>(tile) * a.ktiles + kb0 + kb;
-                t5_expect_tx(&full[st], MG_W_READ + X_BYTES + S_BYTES);
-                t5_tma_2d(w_s + st * MG_W_BYTES, &w_map, 0, static_cast<int>(at * MG_ROWS), &full[st]);
-                mg_copy(s_s + st * S_BYTES, a.w_scales + at * MX_PIECE, MX_PIECE, &full[st]);
-            };
-            auto tokens = [&](int kb) {
-                const int st = kb % STAGES;
-                t5_tma_2d(x_s + st * X_BYTES, &x_map, (kb0 + kb) * MX_K, tok0, &full[st]);
-                mg_copy(s_s + st * S_BYTES + MX_PIECE, a.x_scales + (static_cast<size_t>(tok0 / 128) * a.ktiles + kb0 + kb) * MX_PIECE, MX_PIECE, &full[st]);
-            };
-            const int first = min(STAGES, kbs);
-            for (int kb = 0; kb < first; ++kb) weights(kb);       // nobody's output
-            pdl_wait();
-            for (int kb = 0; kb < first; ++kb) tokens(kb);
-            issued = first;
-            for (int kb = STAGES; kb < kbs; ++kb) {
-                if (!mg_wait(&empty[kb % STAGES], (kb / STAGES - 1) & 1, a.waits, &abort_flag, a.status)) break;
-                weights(kb);
-                tokens(kb);
+        if (lane == 0) {                                          // weights and their scales are nobody's output: no wait for the kernel in front
+            int s = 0;
+            unsigned phase = 1;                                   // a barrier that was never used passes for the phase before its first
+            const int at = tile * a.ktiles + kb0;
+#pragma unroll 1
+            for (int kb = 0; kb < kbs; ++kb) {
+                if (kb % G == 0) {                                // what stands behind the part's last stage is read and not used
+                    const int g = kb / G;
+                    if (!mg_wait(&g_empty[g & 1], ((g >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status)) break;
+                    t5_expect_tx(&g_full[g & 1], S_BYTES);
+                    t5_tma_2d(g_s + (g & 1) * GROUP_BYTES + G * X_BYTES, &ws_map, 0, at + kb, &g_full[g & 1]);
+                }
+                if (!mg_wait(&empty[s], phase, a.waits, &abort_flag, a.status)) break;
+                t5_expect_tx(&full[s], MG_W_READ);
+                t5_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, &full[s]);
                 issued = kb + 1;
+                if (++s == WS) s = 0, phase ^= 1;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        if (lane == 0) {
+            pdl_wait();
+#pragma unroll 1
+            for (int g = 0; g * G < kbs; ++g) {
+                unsigned char* to = g_s + (g & 1) * GROUP_BYTES;
+                if (!mg_wait(&g_empty[g & 1], ((g >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status)) break;
+                t5_expect_tx(&g_full[g & 1], G * X_BYTES + S_BYTES);
+                mg_tma_3d(to, &x_map, 0, tok0, kb0 + g * G, &g_full[g & 1]);
+                t5_tma_2d(to + G * X_BYTES + S_BYTES, &xs_map, 0, (tok0 / 128) * a.ktiles + kb0 + g * G, &g_full[g & 1]);
+                issued = g + 1;
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        pdl_wait();
         const unsigned lead = elect_one();
-        const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024), sd = mg_scale_desc(s_s);
+        const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(g_s, 16, 1024), sd = mg_scale_desc(g_s + G * X_BYTES);
         bool ok = true;
+        int s = 0;
+        unsigned phase = 0;
 #pragma unroll 1
-        for (int kb = 0; kb < kbs; ++kb) {
-            const int st = kb % STAGES;
-            ok = __all_sync(0xffffffffu, mg_wait(&full[st], (kb / STAGES) & 1, a.waits, &abort_flag, a.status));
+        for (int k0 = 0; ok && k0 < kbs; k0 += G) {
+            const int g = (k0 / G) & 1;
+            ok = __all_sync(0xffffffffu, mg_wait(&g_full[g], (k0 / G >> 1) & 1, a.waits, &abort_flag, a.status));
             if (!ok) break;
-            const unsigned sc = tmem + S_COL0 + st * S_COLS;      // a place of its own for each stage: earlier products may still read theirs
+            // [weights, rows] of each stage; the products that read the group before last have run
+            const unsigned sc0 = tmem + S_COL0 + g * (G * 8);
 #pragma unroll
-            for (int p = 0; p < 2; ++p) mg_scales_lead(lead, sc + 4 * p, sd + ((st * S_BYTES + p * MX_PIECE) >> 4));
+            for (int q = 0; q < G; ++q)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                mg_mma_lead(lead, tmem, wd + st * (MG_W_BYTES >> 4) + 2 * k, xd + st * (X_BYTES >> 4) + 2 * k, mg_idesc(MG_ROWS, NT, k), sc, sc + 4, (kb | k) ? 1u : 0u);
-            t5_commit_lead(lead, &empty[st]);
+                for (int p = 0; p < 2; ++p) mg_scales_lead(lead, sc0 + 8 * q + 4 * p, sd + ((g * GROUP_BYTES + p * S_BYTES + q * MX_PIECE) >> 4));
+#pragma unroll 1
+            for (int q = 0; q < min(G, kbs - k0); ++q) {
+                ok = __all_sync(0xffffffffu, mg_wait(&full[s], phase, a.waits, &abort_flag, a.status));
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mg_mma_lead(lead, tmem, wd + s * (MG_W_BYTES >> 4) + 2 * k, xd + ((g * GROUP_BYTES + q * X_BYTES) >> 4) + 2 * k, mg_idesc(MG_ROWS, NT, k),
+                                sc0 + 8 * q, sc0 + 8 * q + 4, (k0 | q | k) ? 1u : 0u);
+                t5_commit_lead(lead, &empty[s]);
+                if (++s == WS) s = 0, phase ^= 1;
+            }
+            if (ok) t5_commit_lead(lead, &g_empty[g]);
         }
         if (ok) t5_commit_lead(lead, &acc_full);
     } else {
@@ -233,8 +255,10 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
         }
     }
     if (tid == 0 && abort_flag)                                   // whoever gave up: what is in flight lands before the CTA goes away
-        for (int kb = max(0, issued - STAGES); kb < issued; ++kb)
-            for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(&full[kb % STAGES], (kb / STAGES) & 1); ++i) {}
+        for (int kb = max(0, issued - WS); kb < issued; ++kb)
+            for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(&full[kb % WS], (kb / WS) & 1); ++i) {}
+    if ((tid == 0 || tid == 192) && abort_flag)                   // a group whose other half was never asked for does not fill
+        for (int n = 0; n < 2000; ++n) __nanosleep(100);
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // nobody leaves while its sums are read
     if (warp == 1) {
@@ -373,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                     if (rank == 0) t5_expect_tx(&own[s], bytes);
                     const unsigned bar = first + s * 8;
                     if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
-                    else if (warp == 10) mp_tma_2d(x_s + s * MP_X_BYTES, &x_map, kb * MX_K, tok0 + static_cast<int>(rank) * (MP_NT / 2), bar);
+                    else if (warp == 10) mp_tma_3d(x_s + s * MP_X_BYTES, &x_map, 0, tok0 + static_cast<int>(rank) * (MP_NT / 2), kb, bar);
                     else {                                        // what stands behind the last tile of K is read and not used
                         mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at + kb, bar);
                         mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
@@ -549,19 +573,19 @@ static bool mg_weight_map(CUtensorMap* map, const void* w, long long rows) {
     return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(w), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// 8-bit rows [rows, kpad] in boxes of `box_rows` x 128 values.
-static bool mg_rows_map(CUtensorMap* map, const void* x, int rows, int kpad, int box_rows) {
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kpad), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(kpad)};
-    const cuuint32_t box[2] = {MX_K, static_cast<cuuint32_t>(box_rows)}, es[2] = {1u, 1u};
-    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(x), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+// 8-bit rows [rows, kpad] as [ktiles][rows][128] in boxes of `box_tiles` x `box_rows` x 128 values.
+static bool mg_rows_map(CUtensorMap* map, const void* x, int rows, int ktiles, int box_rows, int box_tiles) {
+    const cuuint64_t dims[3] = {MX_K, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(ktiles)}, strides[2] = {static_cast<cuuint64_t>(ktiles) * MX_K, MX_K};
+    const cuuint32_t box[3] = {MX_K, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
+    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(x), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// Pieces of scales as lines of 128 words: [tiles of rows][ktiles] in boxes of MP_QUAD lines, of `box_tiles` neighbouring tiles of rows (three
+// Pieces of scales as lines of 128 words: [tiles of rows][ktiles] in boxes of `lines` lines, of `box_tiles` neighbouring tiles of rows (three
 // dimensions) or of one.
-static bool mg_scales_map(CUtensorMap* map, const void* scales, int row_tiles, int ktiles, int box_tiles) {
+static bool mg_scales_map(CUtensorMap* map, const void* scales, int row_tiles, int ktiles, int lines, int box_tiles) {
     const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(ktiles), static_cast<cuuint64_t>(row_tiles)};
     const cuuint64_t strides[2] = {MX_PIECE, static_cast<cuuint64_t>(ktiles) * MX_PIECE};
-    const cuuint32_t box[3] = {128, MP_QUAD, static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
+    const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(lines), static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
     const cuuint64_t line_dims[2] = {128, static_cast<cuuint64_t>(ktiles) * static_cast<cuuint64_t>(row_tiles)};
     if (line_dims[1] >= (1ULL << 31)) return false;
     return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, box_tiles ? 3 : 2, const_cast<void*>(scales), box_tiles ? dims : line_dims, strides, box, es,
@@ -585,29 +609,32 @@ static int mg_parts(long long tiles, int ktiles, int slots) {
     return best;
 }
 
-template <int NT, int STAGES, int MODE, typename TO>
+template <int NT, int WS, int G, int MODE, typename TO>
 static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
-    CUtensorMap w_map, x_map;
-    if (!mg_weight_map(&w_map, w, static_cast<long long>(tiles) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, mg_padded_rows(a.T), a.ktiles * MX_K, NT)) return LLM_REFUSED_SIZE;
-    constexpr size_t smem = static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K + 2 * MX_PIECE) + 1024;
+    CUtensorMap w_map, x_map, ws_map, xs_map;
+    const int padded = mg_padded_rows(a.T), stored = (tiles + 1) / 2 * 2;
+    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, NT, G) ||
+        !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, G, 0) || !mg_scales_map(&xs_map, a.x_scales, (padded + 127) / 128, a.ktiles, G, 0))
+        return LLM_REFUSED_SIZE;
+    constexpr size_t smem = static_cast<size_t>(WS) * MG_W_BYTES + 2 * G * (NT * MX_K + 2 * MX_PIECE) + 1024;
     static_assert(NT <= 128, "a tile's scales are one piece");
-    static_assert(static_cast<size_t>(NT) * MG_ROWS * 4 <= static_cast<size_t>(STAGES) * (MG_W_BYTES + NT * MX_K), "the sums fit the stages");
+    static_assert(NT * 4 <= WS * MX_K, "the sums fit the weights' stages");
     static_assert(smem <= (NT <= 64 ? 113 : 226) * 1024, "shared memory of an SM");
-    auto kern = linear_mx_kernel<NT, STAGES, MODE, TO>;
+    auto kern = linear_mx_kernel<NT, WS, G, MODE, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
     const int tok_tiles = (a.T + NT - 1) / NT, sms = mg_sms();
     if (tiles > 65535 || tok_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
     const int parts = mg_parts(static_cast<long long>(tiles) * tok_tiles, a.ktiles, sms * (NT <= 64 ? 2 : 1) * 7 / 8);
-    launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS), smem, s, parts, w_map, x_map, a);
+    launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS), smem, s, parts, w_map, x_map, ws_map, xs_map, a);
     return launch_status();
 }
 template <int MODE, typename TO>
 static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
     CUtensorMap w_map, x_map, ws_map, xs_map, y_map = {};
     const int padded = mg_padded_rows(a.T), stored = (tiles + 1) / 2 * 2;
-    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles * MX_K, MP_NT / 2) ||
-        !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, 2))
+    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, MP_NT / 2, 1) ||
+        !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, MP_QUAD, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, MP_QUAD, 2))
         return LLM_REFUSED_SIZE;
     if (MODE != MG_GATED) {                                       // [T, N] in boxes of 8 KB, 128 values wide
         a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
@@ -632,10 +659,10 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     return launch_status();
 }
 template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
-    if (a.T <= 16) return mg_launch<16, 5, MODE, TO>(w, tiles, x, a, s);
-    if (a.T <= 32) return mg_launch<32, 5, MODE, TO>(w, tiles, x, a, s);
-    if (a.T <= 64) return mg_launch<64, 4, MODE, TO>(w, tiles, x, a, s);
-    if (a.T <= 128) return mg_launch<128, 6, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 16) return mg_launch<16, 5, 4, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 32) return mg_launch<32, 4, 4, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 64) return mg_launch<64, 4, 2, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 128) return mg_launch<128, 8, 2, MODE, TO>(w, tiles, x, a, s);
     return mp_launch<MODE, TO>(w, tiles, x, a, s);
 }
 
