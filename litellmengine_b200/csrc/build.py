@@ -51,8 +51,7 @@ FAMILIES: Dict[str, List[str]] = {
     "gemm_mid_tcgen05": ["gemm_mid_tcgen05.cu"],
     "gemm_f32": ["gemm_f32.cu"],
     "gemm_f32_tcgen05": ["gemm_f32_tcgen05.cu"],
-    "microscaling": ["microscaling.cu"],
-    "gemm_mx_tcgen05": ["gemm_mx_tcgen05.cu"],
+    "microscaling": ["microscaling.cu", "gemm_mx_tcgen05.cu"],
     "host_core": ["host_core.cpp"],            # the host side's bookkeeping: plain C++, no device code
 }
 HOST_FAMILIES = {"host_core"}

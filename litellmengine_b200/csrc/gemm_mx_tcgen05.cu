@@ -555,12 +555,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-static int mg_sms() {                     // of the current device
-    static int sms[64] = {0};
+#define MG_DEVICES 64
+static int mg_device() {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < MG_DEVICES ? dev : -1;
+}
+static int mg_sms(int dev) {
+    static int sms[MG_DEVICES] = {0};
     if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms[dev] = 0;
     return sms[dev];
+}
+// Lets a kernel have its shared memory, once a device (`had`: a flag for each).
+template <typename K> static int mg_allow(K kern, size_t smem, int dev, bool* had) {
+    if (had[dev]) return LLM_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    had[dev] = e == cudaSuccess;
+    return static_cast<int>(e);
 }
 
 // 4-bit codes, tiles of 128 rows of 64 bytes, spread by the copy engine.
@@ -593,15 +603,6 @@ static bool mg_scales_map(CUtensorMap* map, const void* scales, int row_tiles, i
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Rows that stand behind a matrix of T rows of 8 bits, so that no box reaches beyond them: whole tiles, whole pieces of scales.
-static int mg_padded_rows(int T) {
-    if (T <= 16) return 16;
-    if (T <= 32) return 32;
-    if (T <= 64) return 64;
-    return T <= 128 ? 128 : (T + 2 * MP_NT - 1) / (2 * MP_NT) * (2 * MP_NT);
-}
-extern "C" int llm_mx_padded_rows(int T) { return mg_padded_rows(T); }
-
 // Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.
 static int mg_parts(long long tiles, int ktiles, int slots) {
     int best = 1;
@@ -612,7 +613,7 @@ static int mg_parts(long long tiles, int ktiles, int slots) {
 template <int NT, int WS, int G, int MODE, typename TO>
 static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
     CUtensorMap w_map, x_map, ws_map, xs_map;
-    const int padded = mg_padded_rows(a.T), stored = (tiles + 1) / 2 * 2;
+    const int padded = static_cast<int>(mx_padded_rows(a.T)), stored = (tiles + 1) / 2 * 2;
     if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, NT, G) ||
         !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, G, 0) || !mg_scales_map(&xs_map, a.x_scales, (padded + 127) / 128, a.ktiles, G, 0))
         return LLM_REFUSED_SIZE;
@@ -621,9 +622,11 @@ static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     static_assert(NT * 4 <= WS * MX_K, "the sums fit the weights' stages");
     static_assert(smem <= (NT <= 64 ? 113 : 226) * 1024, "shared memory of an SM");
     auto kern = linear_mx_kernel<NT, WS, G, MODE, TO>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const int tok_tiles = (a.T + NT - 1) / NT, sms = mg_sms();
+    static bool had[MG_DEVICES];
+    const int dev = mg_device();
+    if (dev < 0) return LLM_REFUSED_SIZE;
+    if (const int rc = mg_allow(kern, smem, dev, had)) return rc;
+    const int tok_tiles = (a.T + NT - 1) / NT, sms = mg_sms(dev);
     if (tiles > 65535 || tok_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
     const int parts = mg_parts(static_cast<long long>(tiles) * tok_tiles, a.ktiles, sms * (NT <= 64 ? 2 : 1) * 7 / 8);
     launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS), smem, s, parts, w_map, x_map, ws_map, xs_map, a);
@@ -632,7 +635,7 @@ static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
 template <int MODE, typename TO>
 static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
     CUtensorMap w_map, x_map, ws_map, xs_map, y_map = {};
-    const int padded = mg_padded_rows(a.T), stored = (tiles + 1) / 2 * 2;
+    const int padded = static_cast<int>(mx_padded_rows(a.T)), stored = (tiles + 1) / 2 * 2;
     if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, MP_NT / 2, 1) ||
         !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, MP_QUAD, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, MP_QUAD, 2))
         return LLM_REFUSED_SIZE;
@@ -649,10 +652,12 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
     static_assert(2 * MP_NT + 2 * MP_S_COLS <= 512, "tensor memory");
     auto kern = linear_mx_pair_kernel<MODE, TO>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
+    static bool had[MG_DEVICES];
+    const int dev = mg_device();
+    if (dev < 0) return LLM_REFUSED_SIZE;
+    if (const int rc = mg_allow(kern, smem, dev, had)) return rc;
     const long long token_tiles = (a.T + MP_NT - 1) / MP_NT, all = token_tiles * (stored / 2);
-    const int slots = mg_sms() / 2;
+    const int slots = mg_sms(dev) / 2;
     if (slots <= 0 || all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
     launch_pdl(kern, dim3(2 * clusters), dim3(MP_THREADS), smem, s, w_map, x_map, ws_map, xs_map, y_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
@@ -666,38 +671,40 @@ template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, co
     return mp_launch<MODE, TO>(w, tiles, x, a, s);
 }
 
-static int mg_check(const void* w, const void* w_scales, const void* x, const void* x_scales, const int32_t* status, int T, int N, int K) {
+// The rows of 8 bits as the products take them: made of the matrix `plain` first, where there is one.
+static int mg_operands(void* rows, const void* plain, int dtype, const void* w, const void* w_scales, const int32_t* status, int T, int N, int K,
+                       uintptr_t stream) {
     if (N <= 0 || N > (1 << 24) || K <= 0 || K > (1 << 20) || T > (1 << 24)) return LLM_REFUSED_SIZE;
-    if (!aligned16(w) || !aligned16(w_scales) || !aligned16(x) || !aligned16(x_scales) || (reinterpret_cast<uintptr_t>(w) & 31) || status == nullptr)
-        return LLM_REFUSED_ALIGN;
-    return LLM_OK;
+    if (!aligned16(w) || !aligned16(w_scales) || !aligned16(rows) || (reinterpret_cast<uintptr_t>(w) & 31) || status == nullptr) return LLM_REFUSED_ALIGN;
+    return plain ? llm_mx_rows(plain, dtype, rows, T, K, stream) : LLM_OK;
 }
 
-// x: rows of 8 bits [T, K]; w: a weight of 4 bits [N, K]; y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
-extern "C" int llm_linear_mx(const void* x, const void* x_scales, const void* w, const void* w_scales, void* y, int out_dtype, int add, int T, int N,
+// rows: of 8 bits [T, K], or room for them and `plain` a matrix [T, K] of `dtype` that they are made of first; w: a weight of 4 bits [N, K];
+// y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
+extern "C" int llm_linear_mx(void* rows, const void* plain, int dtype, const void* w, const void* w_scales, void* y, int out_dtype, int add, int T, int N,
                              int K, int waits, int32_t* status, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
-    if (const int rc = mg_check(w, w_scales, x, x_scales, status, T, N, K)) return rc;
     if ((out_dtype != LLM_DT_F32 && out_dtype != LLM_DT_BF16) || (add && out_dtype != LLM_DT_F32)) return LLM_REFUSED_DTYPE;
-    MgArgs a = {static_cast<const unsigned char*>(w_scales), static_cast<const unsigned char*>(x_scales), y, nullptr, T, N, (K + MX_K - 1) / MX_K, 0,
-                N % 4 == 0 && aligned16(y), waits, status, {}};
+    if (const int rc = mg_operands(rows, plain, dtype, w, w_scales, status, T, N, K, stream)) return rc;
+    MgArgs a = {static_cast<const unsigned char*>(w_scales), mx_row_scales(rows, T, K), y, nullptr, T, N, mx_tiles(K), 0, N % 4 == 0 && aligned16(y), waits,
+                status, {}};
     const int tiles = (N + MG_ROWS - 1) / MG_ROWS;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (add) return mg_rows<MG_ADD, float>(w, tiles, x, a, s);
-    if (out_dtype == LLM_DT_F32) return mg_rows<MG_STORE, float>(w, tiles, x, a, s);
-    return mg_rows<MG_STORE, bf16>(w, tiles, x, a, s);
+    if (add) return mg_rows<MG_ADD, float>(w, tiles, rows, a, s);
+    if (out_dtype == LLM_DT_F32) return mg_rows<MG_STORE, float>(w, tiles, rows, a, s);
+    return mg_rows<MG_STORE, bf16>(w, tiles, rows, a, s);
 }
 
-// w: a gated weight of 4 bits (N gate and N up rows); codes, scales: act(x gate^T) * (x up^T) as rows of 8 bits [T, N].
-extern "C" int llm_linear_mx_silu_mul(const void* x, const void* x_scales, const void* w, const void* w_scales, void* codes, void* scales, int T,
-                                      int N, int K, int act, float limit, int waits, int32_t* status, uintptr_t stream) {
+// w: a gated weight of 4 bits (N gate and N up rows); made: act(x gate^T) * (x up^T) as rows of 8 bits [T, N].
+extern "C" int llm_linear_mx_silu_mul(void* rows, const void* plain, int dtype, const void* w, const void* w_scales, void* made, int T, int N, int K,
+                                      int act, float limit, int waits, int32_t* status, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
-    if (const int rc = mg_check(w, w_scales, x, x_scales, status, T, N, K)) return rc;
     MxAct form;
     if (!mx_act(act, limit, &form)) return LLM_REFUSED_SIZE;
-    if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    if (!aligned16(made)) return LLM_REFUSED_ALIGN;
+    if (const int rc = mg_operands(rows, plain, dtype, w, w_scales, status, T, N, K, stream)) return rc;
     const int tiles = 2 * ((N + 127) / 128);                      // as the weight has them
-    MgArgs a = {static_cast<const unsigned char*>(w_scales), static_cast<const unsigned char*>(x_scales), codes, static_cast<unsigned char*>(scales), T, N,
-                (K + MX_K - 1) / MX_K, tiles * 64, 0, waits, status, form};
-    return mg_rows<MG_GATED, float>(w, tiles, x, a, reinterpret_cast<cudaStream_t>(stream));
+    MgArgs a = {static_cast<const unsigned char*>(w_scales), mx_row_scales(rows, T, K), made, mx_row_scales(made, T, N), T, N, mx_tiles(K), tiles * 64, 0,
+                waits, status, form};
+    return mg_rows<MG_GATED, float>(w, tiles, rows, a, reinterpret_cast<cudaStream_t>(stream));
 }

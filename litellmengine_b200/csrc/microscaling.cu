@@ -165,7 +165,6 @@ __global__ void __launch_bounds__(MX_THREADS) mx_values_kernel(const unsigned ch
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-static inline int mx_tiles(int k) { return (k + MX_K - 1) / MX_K; }
 #define MX_MOST_K (1 << 20)
 static inline bool mx_grid(long long pieces, unsigned* blocks) {
     const long long b = (pieces + MX_THREADS - 1) / MX_THREADS;
@@ -173,17 +172,17 @@ static inline bool mx_grid(long long pieces, unsigned* blocks) {
     return b > 0 && b <= 0x7fffffffLL;
 }
 
-// x: [T, K] -> codes [T, ktiles * 128], scales [pieces][512].
-extern "C" int llm_mx_rows(const void* x, int dtype, void* codes, void* scales, int T, int K, uintptr_t stream) {
+// x: [T, K] -> rows of 8 bits: codes [padded rows][ktiles * 128], then scales.
+extern "C" int llm_mx_rows(const void* x, int dtype, void* rows, int T, int K, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
     if (K <= 0 || K > MX_MOST_K) return LLM_REFUSED_SIZE;
-    if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
     const int kpad = mx_tiles(K) * MX_K, vec = K % 8 == 0 && aligned16(x);
     const long long pieces = static_cast<long long>(T) * (kpad / 8);
     unsigned blocks;
     if (!mx_grid(pieces, &blocks)) return LLM_REFUSED_SIZE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    unsigned char *c = static_cast<unsigned char*>(codes), *sc = static_cast<unsigned char*>(scales);
+    unsigned char *c = static_cast<unsigned char*>(rows), *sc = mx_row_scales(rows, T, K);
     if (dtype == LLM_DT_F32) launch_pdl(mx_rows_kernel<float>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const float*>(x), c, sc, pieces, K, kpad, vec);
     else if (dtype == LLM_DT_BF16) launch_pdl(mx_rows_kernel<bf16>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const bf16*>(x), c, sc, pieces, K, kpad, vec);
     else return LLM_REFUSED_DTYPE;
@@ -191,18 +190,18 @@ extern "C" int llm_mx_rows(const void* x, int dtype, void* codes, void* scales, 
 }
 
 // gu: [parts][T, 2 * inter] = [gate | up], parts `part_stride` values apart (more than one: float32).
-extern "C" int llm_mx_silu_and_mul(const void* gu, int dtype, int parts, long long part_stride, void* codes, void* scales, int T, int inter, int act,
-                                   float limit, uintptr_t stream) {
+extern "C" int llm_mx_silu_and_mul(const void* gu, int dtype, int parts, long long part_stride, void* rows, int T, int inter, int act, float limit,
+                                   uintptr_t stream) {
     if (T <= 0) return LLM_OK;
     MxAct form;
     if (inter <= 0 || inter > MX_MOST_K || parts < 1 || !mx_act(act, limit, &form)) return LLM_REFUSED_SIZE;
-    if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
     const int kpad = mx_tiles(inter) * MX_K, vec = inter % 8 == 0 && part_stride % 8 == 0 && aligned16(gu);
     const long long pieces = static_cast<long long>(T) * (kpad / 8);
     unsigned blocks;
     if (!mx_grid(pieces, &blocks)) return LLM_REFUSED_SIZE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    unsigned char *c = static_cast<unsigned char*>(codes), *sc = static_cast<unsigned char*>(scales);
+    unsigned char *c = static_cast<unsigned char*>(rows), *sc = mx_row_scales(rows, T, inter);
     if (dtype == LLM_DT_F32)
         launch_pdl(mx_act_kernel<float>, dim3(blocks), dim3(MX_THREADS), 0, s, static_cast<const float*>(gu), c, sc, pieces, inter, kpad, vec, parts, part_stride, form);
     else if (dtype == LLM_DT_BF16)
@@ -230,10 +229,11 @@ static int mx_norm_launch(const void* x, const void* delta, const float* w, void
 
 // x: [*, hidden]; delta: [parts][*, hidden] or null; w: float32 [hidden]; sum_out: like x (may be x) or null; rows: int32 [n] or null.
 extern "C" int llm_mx_rmsnorm(const void* x, int x_dtype, const void* delta, int delta_dtype, int parts, long long part_stride, const float* w,
-                              float eps, void* sum_out, void* codes, void* scales, const int32_t* rows, int n, int hidden, uintptr_t stream) {
+                              float eps, void* sum_out, void* made, const int32_t* rows, int n, int hidden, uintptr_t stream) {
     if (n <= 0) return LLM_OK;
     if (hidden <= 0 || parts < 1 || (sum_out && rows)) return LLM_REFUSED_SIZE;
-    if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    if (!aligned16(made)) return LLM_REFUSED_ALIGN;
+    void *codes = made, *scales = mx_row_scales(made, n, hidden);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (!delta) delta_dtype = LLM_DT_F32;
 #define CASE(k, TX, TD) \

@@ -16,6 +16,8 @@
 
 #include "common.cuh"
 
+#include <cstddef>
+
 #define MX_BLOCK 32
 #define MX_K 128                  // values of a tile's row
 #define MX_PIECE 512              // bytes of the scales of 128 rows x 128 values
@@ -26,6 +28,13 @@
 __host__ __device__ __forceinline__ size_t mx_scale_at(size_t row, int kb, int ktiles) {
     return ((row >> 7) * ktiles + (kb >> 2)) * MX_PIECE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3);
 }
+// Rows that stand behind T rows of 8 bits, so that no box of a product (16, 32, 64 or 128 rows, or 192 of a pair) reaches beyond them, nor
+// beyond whole pieces of scales; the scales stand behind the codes.
+static inline long long mx_padded_rows(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : (T + 383LL) / 384 * 384; }
+static inline int mx_tiles(int k) { return (k + MX_K - 1) / MX_K; }
+static inline unsigned char* mx_row_scales(void* rows, int T, int K) { return static_cast<unsigned char*>(rows) + mx_padded_rows(T) * mx_tiles(K) * MX_K; }
+extern "C" int llm_mx_rows(const void* x, int dtype, void* rows, int T, int K, uintptr_t stream);
+
 // The stored scale of a block from the bits of its largest magnitude (as integers these are in order, NaN above infinity above all).
 template <int FMT> __device__ __forceinline__ unsigned mx_scale(unsigned most) {
     constexpr unsigned EXP = FMT == MX_E4M3 ? 8 : 2, MANT = FMT == MX_E4M3 ? 0x600000u : 0x400000u;      // largest: 1.75 * 2^8, 1.5 * 2^2

@@ -2298,15 +2298,59 @@ def latent_q_product(x: torch.Tensor, weight: torch.Tensor) -> bool:
 # within the format's largest value (e4m3 448, e2m1 6); each value is then rounded to the format's nearest.
 # csrc/microscaling.cuh says where the bytes lie.
 MX_BLOCK = 32
+_mx_calls: Dict[str, object] = {}
+_P, _I, _F, _L = c_void_p, c_int, c_float, c_longlong
+_MX_SIGNATURES = {
+    "llm_mx_rows": ("microscaling", [_P, _I, _P, _I, _I, _P]),
+    "llm_mx_weight": ("microscaling", [_P, _I, _P, _P, _I, _I, _I, _P]),
+    "llm_mx_values": ("microscaling", [_P, _P, _I, _P, _I, _I, _I, _I, _P]),
+    "llm_mx_rmsnorm": ("microscaling", [_P, _I, _P, _I, _I, _L, _P, _F, _P, _P, _P, _I, _I, _P]),
+    "llm_mx_silu_and_mul": ("microscaling", [_P, _I, _I, _L, _P, _I, _I, _I, _F, _P]),
+    "llm_linear_mx": ("microscaling", [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "llm_linear_mx_silu_mul": ("microscaling", [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _P]),
+}
+
+
+def _mx_call(name: str):
+    f = _mx_calls.get(name)
+    if f is None:
+        family, argtypes = _MX_SIGNATURES[name]
+        f = _mx_calls[name] = _fn(family, name, argtypes)
+    return f
 
 
 def _here(*tensors) -> None:
     """`_dev`, and on the device whose stream the kernel will go to."""
-    _dev(*tensors)
-    now = torch.cuda.current_device()
+    now = -1
     for t in tensors:
-        if t is not None and t.device.index != now:
-            raise KernelError(f"tensor on {t.device}, but the current device is cuda:{now}")
+        if t is None:
+            continue
+        at = t.get_device()
+        if at != now:
+            if at < 0:
+                raise KernelError("tensor is not on a CUDA device; the engine has no CPU path")
+            now = torch._C._cuda_getDevice()
+            if at != now:
+                raise KernelError(f"tensor on cuda:{at}, but the current device is cuda:{now}")
+        if not t.is_contiguous():
+            raise KernelError("tensor is not contiguous")
+
+
+_mx_status: Dict[int, torch.Tensor] = {}
+
+
+def _mx_status_ptr(device: torch.device) -> int:
+    t = _mx_status.get(device.index)
+    if t is None:
+        t = _mx_status[device.index] = stream_status(device)
+    return t.data_ptr()
+
+
+def mx_padded_rows(T: int) -> int:
+    """Rows that stand behind T rows of 8 bits: the products read whole tiles, and nobody minds what stands there."""
+    if T <= 128:
+        return 16 if T <= 16 else 32 if T <= 32 else 64 if T <= 64 else 128
+    return (T + 383) // 384 * 384
 
 
 class MxRows:
@@ -2314,29 +2358,47 @@ class MxRows:
     `rmsnorm_mx`, `silu_and_mul_mx` and `linear_silu_mul_mx`.  `codes`: uint8 [T, K padded to 128]; `scales`: uint8 pieces of
     512 bytes; `values` gives the rows as a matrix again."""
 
-    def __init__(self, T: int, K: int, device):
-        self.shape = torch.Size((T, K))
-        self.device = torch.device(device)
-        tiles = -(-K // 128)
-        padded = _fn("gemm_mx_tcgen05", "llm_mx_padded_rows", [c_int])(T)         # the products read whole tiles; nobody minds what stands there
-        self.codes = torch.empty((padded, tiles * 128), dtype=torch.uint8, device=device)[:T]
-        self.scales = torch.empty((-(-padded // 128), tiles, 512), dtype=torch.uint8, device=device)
+    __slots__ = ("shape", "device", "buffer")
+
+    def __init__(self, T: int, K: int, device: torch.device):
+        self.shape = (T, K)
+        self.device = device
+        tiles, padded = (K + 127) // 128, mx_padded_rows(T)
+        # one allocation: the codes, then the scales
+        self.buffer = torch.empty(tiles * (padded * 128 + (padded + 127) // 128 * 512), dtype=torch.uint8, device=device)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        T, K = self.shape
+        tiles = (K + 127) // 128
+        return self.buffer[:T * tiles * 128].view(T, tiles * 128)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        T, K = self.shape
+        tiles, padded = (K + 127) // 128, mx_padded_rows(T)
+        return self.buffer[padded * tiles * 128:].view((padded + 127) // 128, tiles, 512)
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         T, K = self.shape
-        return _mx_values(self, self.codes, 8, T, K, False, dtype)
+        _here(self.buffer)
+        out = torch.empty((T, K), dtype=dtype, device=self.device)
+        at = self.buffer.data_ptr()
+        _check(_mx_call("llm_mx_values")(at, at + mx_padded_rows(T) * ((K + 127) // 128) * 128, 8, out.data_ptr(), _dt(out), T, K, 0, _stream()),
+               "values of rows in 8 bits")
+        return out
 
 
 class MxWeight:
     """A weight [N, K] in 4 bits (e2m1) with a scale per 32 values along K, 17 / 32 of a byte a value, stored tile by tile.  Made by
     `mx_weight`; `gated`: it is [gate; up], gate and up rows stored beside each other for `linear_silu_mul_mx`."""
 
-    def __init__(self, N: int, K: int, gated: bool, device):
-        self.shape = torch.Size((N, K))
+    def __init__(self, N: int, K: int, gated: bool, device: torch.device):
+        self.shape = (N, K)
         self.gated = gated
-        self.device = torch.device(device)
-        n = _fn("microscaling", "llm_mx_weight_tiles", [c_int, c_int])(N // 2 if gated else N, int(gated))
-        tiles = -(-K // 128)
+        self.device = device
+        # tiles of 128 rows: an even number, because products of many rows take two at a time; gated: 64 gate and 64 up rows
+        n, tiles = 2 * (((N // 2 + 127) // 128) if gated else (N + 255) // 256), (K + 127) // 128
         self.codes = torch.empty((n, tiles, 128, 64), dtype=torch.uint8, device=device)
         self.scales = torch.empty((n, tiles, 512), dtype=torch.uint8, device=device)
 
@@ -2346,15 +2408,11 @@ class MxWeight:
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         N, K = self.shape
-        return _mx_values(self, self.codes, 4, N // 2 if self.gated else N, K, self.gated, dtype)
-
-
-def _mx_values(held, codes: torch.Tensor, bits: int, n: int, k: int, gated: bool, dtype: torch.dtype) -> torch.Tensor:
-    _here(codes)
-    out = torch.empty(tuple(held.shape), dtype=dtype, device=codes.device)
-    f = _fn("microscaling", "llm_mx_values", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
-    _check(f(_ptr(codes), _ptr(held.scales), bits, _ptr(out), _dt(out), n, k, int(gated), _stream()), "mx values")
-    return out
+        _here(self.codes)
+        out = torch.empty((N, K), dtype=dtype, device=self.device)
+        _check(_mx_call("llm_mx_values")(self.codes.data_ptr(), self.scales.data_ptr(), 4, out.data_ptr(), _dt(out), N // 2 if self.gated else N, K,
+                                         int(self.gated), _stream()), "values of a weight in 4 bits")
+        return out
 
 
 def mx_weight(weight: torch.Tensor, gated: bool = False) -> MxWeight:
@@ -2365,8 +2423,8 @@ def mx_weight(weight: torch.Tensor, gated: bool = False) -> MxWeight:
     N, K = weight.shape
     dt = _dt(weight)
     made = MxWeight(N, K, gated, weight.device)
-    f = _fn("microscaling", "llm_mx_weight", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p])
-    _check(f(_ptr(weight), dt, _ptr(made.codes), _ptr(made.scales), N // 2 if gated else N, K, int(gated), _stream()), "mx_weight")
+    _check(_mx_call("llm_mx_weight")(weight.data_ptr(), dt, made.codes.data_ptr(), made.scales.data_ptr(), N // 2 if gated else N, K, int(gated),
+                                     _stream()), "mx_weight")
     return made
 
 
@@ -2378,8 +2436,7 @@ def mx_rows(x: torch.Tensor) -> MxRows:
     T, K = x.shape
     dt = _dt(x)
     made = MxRows(T, K, x.device)
-    f = _fn("microscaling", "llm_mx_rows", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
-    _check(f(_ptr(x), dt, _ptr(made.codes), _ptr(made.scales), T, K, _stream()), "mx_rows")
+    _check(_mx_call("llm_mx_rows")(x.data_ptr(), dt, made.buffer.data_ptr(), T, K, _stream()), "mx_rows")
     return made
 
 
@@ -2406,10 +2463,8 @@ def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, delta=None, ro
     n = rows.numel() if rows is not None else T
     dt, dd = _dt(x), _dt(delta) if delta is not None else 0
     made = MxRows(n, H, x.device)
-    f = _fn("microscaling", "llm_mx_rmsnorm", [c_void_p, c_int, c_void_p, c_int, c_int, c_longlong, c_void_p, c_float, c_void_p, c_void_p,
-                                               c_void_p, c_void_p, c_int, c_int, c_void_p])
-    _check(f(_ptr(x), dt, _ptr(delta), dd, parts, part_stride, _ptr(weight), float(eps), _ptr(sum_out), _ptr(made.codes), _ptr(made.scales),
-             _ptr(rows), n, H, _stream()), "rmsnorm_mx")
+    _check(_mx_call("llm_mx_rmsnorm")(x.data_ptr(), dt, _ptr(delta), dd, parts, part_stride, weight.data_ptr(), eps, _ptr(sum_out),
+                                      made.buffer.data_ptr(), _ptr(rows), n, H, _stream()), "rmsnorm_mx")
     return made
 
 
@@ -2427,19 +2482,24 @@ def silu_and_mul_mx(gate_up, activation: str = "silu", limit: float = 0.0) -> Mx
     T, inter = gate_up.shape[0], gate_up.shape[1] // 2
     dt = _dt(gate_up)
     made = MxRows(T, inter, gate_up.device)
-    f = _fn("microscaling", "llm_mx_silu_and_mul", [c_void_p, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p])
-    _check(f(_ptr(gate_up), dt, parts, part_stride, _ptr(made.codes), _ptr(made.scales), T, inter, act, float(limit), _stream()), "silu_and_mul_mx")
+    _check(_mx_call("llm_mx_silu_and_mul")(gate_up.data_ptr(), dt, parts, part_stride, made.buffer.data_ptr(), T, inter, act, limit, _stream()),
+           "silu_and_mul_mx")
     return made
 
 
-def _mx_operands(x, weight: MxWeight, gated: bool) -> MxRows:
+def _mx_operands(x, weight: MxWeight, gated: bool):
+    """(address of a matrix that is still to be taken to 8 bits or None, its dtype, the rows of 8 bits, T, K) of a product's x."""
     if not isinstance(weight, MxWeight) or weight.gated != gated:
         raise KernelError("the microscaled product takes an MxWeight" + (" made with gated=True" if gated else " that is not a gated one"))
-    if x.shape[-1] != weight.shape[1] or len(x.shape) != 2:
+    made = type(x) is MxRows
+    if len(x.shape) != 2 or x.shape[1] != weight.shape[1]:
         raise KernelError("x and weight disagree on K")
-    x = x if isinstance(x, MxRows) else mx_rows(x)
-    _here(x.codes, weight.codes)
-    return x
+    T, K = x.shape
+    if made:
+        _here(x.buffer, weight.codes)
+        return None, 0, x, T, K
+    _here(x, weight.codes)
+    return x.data_ptr(), _dt(x), MxRows(T, K, weight.device), T, K
 
 
 def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, residual: Optional[torch.Tensor] = None,
@@ -2447,17 +2507,19 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
     """x [T, K] @ weight[N, K]^T with the weight in 4 bits and x in 8 (`MxRows`; a matrix is taken to 8 bits first), products exact,
     sums in float32, on the block-scaled tcgen05 products.  The result is float32 or bfloat16 [T, N]; with `residual` (float32
     [T, N]) it is added to that in place, which is returned."""
-    x = _mx_operands(x, weight, False)
-    (T, K), N = x.shape, weight.shape[0]
+    plain, dt, rows, T, K = _mx_operands(x, weight, False)
+    N = weight.shape[0]
     if residual is not None:
         _here(residual)
-        if residual.dtype != torch.float32 or tuple(residual.shape) != (T, N):
+        if residual.dtype != torch.float32 or residual.shape != (T, N):
             raise KernelError("the product joins a float32 residual of its shape")
-    y = residual if residual is not None else torch.empty((T, N), dtype=out_dtype, device=x.device)
-    f = _fn("gemm_mx_tcgen05", "llm_linear_mx", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
-                                                 c_void_p])
-    _check(f(_ptr(x.codes), _ptr(x.scales), _ptr(weight.codes), _ptr(weight.scales), _ptr(y), _dt(y), int(residual is not None), T, N, K, waits,
-             _ptr(stream_status(x.device)), _stream()), "linear_mx")
+        y, od = residual, 0
+    else:
+        y = torch.empty((T, N), dtype=out_dtype, device=weight.device)
+        od = _dt(y)
+    _check(_mx_call("llm_linear_mx")(rows.buffer.data_ptr(), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(), y.data_ptr(), od,
+                                     residual is not None, T, N, K, waits, _mx_status_ptr(weight.device), _stream()), "linear_mx")
+    _mx_count(plain)
     return y
 
 
@@ -2465,14 +2527,19 @@ def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: flo
     """act(x @ gate^T) * (x @ up^T) as rows of 8 bits [T, I] for a gated weight [2I, K] in 4 bits, act as in `silu_and_mul`, in the
     product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits."""
     act = ACTIVATIONS[activation]
-    x = _mx_operands(x, weight, True)
-    (T, K), inter = x.shape, weight.shape[0] // 2
-    made = MxRows(T, inter, x.device)
-    f = _fn("gemm_mx_tcgen05", "llm_linear_mx_silu_mul", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                                                          c_float, c_int, c_void_p, c_void_p])
-    _check(f(_ptr(x.codes), _ptr(x.scales), _ptr(weight.codes), _ptr(weight.scales), _ptr(made.codes), _ptr(made.scales), T, inter, K, act,
-             float(limit), waits, _ptr(stream_status(x.device)), _stream()), "linear_silu_mul_mx")
+    plain, dt, rows, T, K = _mx_operands(x, weight, True)
+    inter = weight.shape[0] // 2
+    made = MxRows(T, inter, weight.device)
+    _check(_mx_call("llm_linear_mx_silu_mul")(rows.buffer.data_ptr(), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(),
+                                              made.buffer.data_ptr(), T, inter, K, act, limit, waits, _mx_status_ptr(weight.device), _stream()),
+           "linear_silu_mul_mx")
+    _mx_count(plain)
     return made
+
+
+def _mx_count(plain) -> None:
+    global launch_count
+    launch_count += plain is not None         # the kernel that takes a matrix to 8 bits
 
 
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:

@@ -34,24 +34,25 @@ P, SIZE, DTYPE, ALIGN = 4096, -1, -2, -3          # an aligned address that noth
 def test_sizes_types_and_addresses_of_rows():
     m, f, ll = lib("microscaling"), ctypes.c_float, ctypes.c_longlong
     v = ctypes.c_void_p
-    rows = lambda x=P, dt=1, c=P, s=P, T=4, K=64: m.llm_mx_rows(v(x), dt, v(c), v(s), T, K, v(0))
-    assert rows(T=0) == 0 and rows(K=0) == SIZE and rows(K=(1 << 20) + 1) == SIZE and rows(c=P + 8) == ALIGN and rows(s=P + 4) == ALIGN and rows(dt=2) == DTYPE
+    rows = lambda dt=1, r=P, T=4, K=64: m.llm_mx_rows(v(P), dt, v(r), T, K, v(0))
+    assert rows(T=0) == 0 and rows(K=0) == SIZE and rows(K=(1 << 20) + 1) == SIZE and rows(r=P + 8) == ALIGN and rows(dt=2) == DTYPE
     weight = lambda dt=1, t=P, s=P, N=4, K=64: m.llm_mx_weight(v(P), dt, v(t), v(s), N, K, 0, v(0))
     assert weight(N=0) == SIZE and weight(K=0) == SIZE and weight(N=(1 << 24) + 1) == SIZE and weight(dt=3) == DTYPE and weight(t=P + 1) == ALIGN
-    norm = lambda dt=0, parts=1, H=64, sum_out=0, rws=0, c=P: m.llm_mx_rmsnorm(v(P), dt, v(P), 0, parts, ll(0), v(P), f(1e-6), v(sum_out), v(c), v(P), v(rws), 4, H, v(0))
-    assert norm(H=0) == SIZE and norm(parts=0) == SIZE and norm(sum_out=P, rws=P) == SIZE and norm(dt=2) == DTYPE and norm(c=P + 2) == ALIGN and norm(H=32769) == SIZE
-    act = lambda dt=1, parts=1, inter=64, kind=0, limit=0.0, s=P: m.llm_mx_silu_and_mul(v(P), dt, parts, ll(0), v(P), v(s), 4, inter, kind, f(limit), v(0))
-    assert act(inter=0) == SIZE and act(kind=3) == SIZE and act(kind=2) == SIZE and act(parts=0) == SIZE and act(dt=5) == DTYPE and act(s=P + 8) == ALIGN
+    norm = lambda dt=0, parts=1, H=64, sum_out=0, rws=0, r=P: m.llm_mx_rmsnorm(v(P), dt, v(P), 0, parts, ll(0), v(P), f(1e-6), v(sum_out), v(r), v(rws), 4, H, v(0))
+    assert norm(H=0) == SIZE and norm(parts=0) == SIZE and norm(sum_out=P, rws=P) == SIZE and norm(dt=2) == DTYPE and norm(r=P + 2) == ALIGN and norm(H=32769) == SIZE
+    act = lambda dt=1, parts=1, inter=64, kind=0, limit=0.0, r=P: m.llm_mx_silu_and_mul(v(P), dt, parts, ll(0), v(r), 4, inter, kind, f(limit), v(0))
+    assert act(inter=0) == SIZE and act(kind=3) == SIZE and act(kind=2) == SIZE and act(parts=0) == SIZE and act(dt=5) == DTYPE and act(r=P + 8) == ALIGN
     values = lambda fmt=8, dt=1, gated=0, K=64: m.llm_mx_values(v(P), v(P), fmt, v(P), dt, 4, K, gated, v(0))
     assert values(fmt=6) == SIZE and values(gated=1) == SIZE and values(dt=2) == DTYPE and values(K=0) == SIZE
     assert [m.llm_mx_weight_tiles(n, g) for n, g in ((1, 0), (128, 0), (129, 0), (1, 1), (128, 1), (129, 1))] == [2, 2, 2, 2, 2, 4]
 
 
 def test_sizes_types_and_addresses_of_products():
-    m, f = lib("gemm_mx_tcgen05"), ctypes.c_float
+    m, f = lib("microscaling"), ctypes.c_float
     v = ctypes.c_void_p
-    y = lambda x=P, w=P, dt=0, add=0, T=4, N=64, K=64, status=P: m.llm_linear_mx(v(x), v(P), v(w), v(P), v(P), dt, add, T, N, K, 1, v(status), v(0))
+    y = lambda x=P, plain=0, xd=1, w=P, dt=0, add=0, T=4, N=64, K=64, status=P: m.llm_linear_mx(v(x), v(plain), xd, v(w), v(P), v(P), dt, add, T, N, K, 1, v(status), v(0))
     assert y(T=0) == 0 and y(N=0) == SIZE and y(K=0) == SIZE and y(K=(1 << 20) + 1) == SIZE and y(T=(1 << 24) + 1) == SIZE
-    assert y(x=P + 8) == ALIGN and y(w=P + 16) == ALIGN and y(status=0) == ALIGN and y(dt=2) == DTYPE and y(dt=1, add=1) == DTYPE
-    g = lambda kind=0, limit=0.0, T=4, N=64, c=P: m.llm_linear_mx_silu_mul(v(P), v(P), v(P), v(P), v(c), v(P), T, N, 64, kind, f(limit), 1, v(P), v(0))
-    assert g(T=0) == 0 and g(N=0) == SIZE and g(kind=3) == SIZE and g(kind=2) == SIZE and g(kind=-1) == SIZE and g(c=P + 8) == ALIGN
+    assert y(x=P + 8) == ALIGN and y(w=P + 16) == ALIGN and y(status=0) == ALIGN and y(dt=2) == DTYPE and y(dt=1, add=1) == DTYPE and y(plain=P, xd=2) == DTYPE
+    g = lambda kind=0, limit=0.0, T=4, N=64, made=P: m.llm_linear_mx_silu_mul(v(P), v(0), 0, v(P), v(P), v(made), T, N, 64, kind, f(limit), 1, v(P), v(0))
+    assert g(T=0) == 0 and g(N=0) == SIZE and g(kind=3) == SIZE and g(kind=2) == SIZE and g(kind=-1) == SIZE and g(made=P + 8) == ALIGN
+    assert [ops.mx_padded_rows(t) for t in (1, 16, 17, 33, 65, 128, 129, 384, 385)] == [16, 16, 32, 64, 128, 128, 384, 384, 768]
