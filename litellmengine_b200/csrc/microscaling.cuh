@@ -111,29 +111,53 @@ __device__ __forceinline__ void mx_store_row8(const float (&v)[8], bool there, s
     *reinterpret_cast<uint2*>(codes + row * kpad + col) = c;
     if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(row, col / MX_BLOCK, kpad / MX_K)) = word;
 }
-// Eight values from column `col` on of a row of `n`; zeros beyond it.  vec: rows of whole, aligned pieces of eight.
-template <typename T> __device__ __forceinline__ void mx_load8(const T* row, int col, int n, int vec, float (&v)[8]) {
-    if (vec) {
-        if (col < n) {
-            load8(row + col, v);
-            return;
-        }
+// Eight values from column `col` on of a row of `n`; zeros beyond it.  vec 8: rows of whole, aligned pieces of eight; 2: of pairs; 1: any.
+__device__ __forceinline__ float2 mx_load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 mx_load2(const bf16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
+__device__ __forceinline__ void mx_store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void mx_store2(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+template <bool FAST, typename T> __device__ __forceinline__ void mx_load8(const T* row, int col, int n, int vec, float (&v)[8]) {
+    if constexpr (FAST) {                                         // vec 8, without a branch around the loads
+        if (col < n) load8(row + col, v);
+        else
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (vec == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            if (col + i < n) {
+                const float2 f = mx_load2(row + col + i);
+                v[i] = f.x, v[i + 1] = f.y;
+            }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = col + i < n ? to_f32(row[col + i]) : 0.0f;
+        for (int i = 0; i < 8; ++i)
+            if (col + i < n) v[i] = to_f32(row[col + i]);
     }
 }
-template <typename T> __device__ __forceinline__ void mx_put8(T* row, int col, int n, int vec, const float (&v)[8]) {
-    if (vec) {
+template <bool FAST, typename T> __device__ __forceinline__ void mx_put8(T* row, int col, int n, int vec, const float (&v)[8]) {
+    if constexpr (FAST) {
         if (col < n) store8(row + col, v);
+    } else if (vec == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            if (col + i < n) mx_store2(row + col + i, v[i], v[i + 1]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (col + i < n) row[col + i] = from_f32<T>(v[i]);
     }
 }
+// How rows of n values of `size` bytes from p on (null: nothing) can be read or written.
+static inline int mx_vec(int n, const void* p, int size) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return n % 8 == 0 && (at & 15) == 0 ? 8 : n % 2 == 0 && (at & (2 * size - 1)) == 0 ? 2 : 1;
+}
+static inline int mx_vec(int a, int b) { return a < b ? a : b; }
 
 // A gated feed-forward's middle, all of its kinds in one form without branches: g * sigmoid(z) * (u + shift), z = g * (alpha + beta g^2), g and u
 // clamped by `limit` (infinity: not).  silu: z = g; the tanh form of gelu is g * sigmoid(2 sqrt(2/pi) (g + 0.044715 g^3)), because

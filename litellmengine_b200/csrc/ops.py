@@ -2321,7 +2321,7 @@ def _mx_call(name: str):
 
 def _here(*tensors) -> None:
     """`_dev`, and on the device whose stream the kernel will go to."""
-    now = -1
+    now = -2
     for t in tensors:
         if t is None:
             continue
