@@ -18,7 +18,8 @@
 #include "tcgen05_attention.cuh"
 
 #define MG_ROWS 128               // features of a tile (gated: 64 of both)
-#define MG_THREADS 224
+#define MG_MAKERS 9               // warps that make rows of a matrix
+#define MG_THREADS(PLAIN) (32 * (2 + ((PLAIN) ? MG_MAKERS : 5)))
 #define MG_W_BYTES (MG_ROWS * MX_K)       // of a stage's weights in shared memory
 #define MG_W_READ (MG_W_BYTES / 2)        // the same as the copy engine counts them: what it reads
 #define MG_STATUS 12
@@ -62,17 +63,23 @@ struct MgArgs {
     int T, N, ktiles, out_kpad, vec, waits;
     int32_t* status;
     MxAct act;
+    const void* plain;                    // a bfloat16 matrix [T, K] that the kernel takes to 8 bits itself
+    int K;
 };
 enum { MG_STORE = 0, MG_ADD = 1, MG_GATED = 2 };
 
 // grid (parts of K, tiles of features, tiles of tokens), a cluster the parts of a tile.  WS: stages of weights; G: stages whose rows and scales
 // come together, two such groups at a time.
-template <int NT, int WS, int G, int MODE, typename TO>
-__global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+// PLAIN: x comes as a matrix, and the warps that will take the sums make the rows of 8 bits of their part of K in shared memory first: one launch
+// and no rows in memory, for steps so short that every CTA can do it while its weights come.
+template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO>
+__global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                                                const __grid_constant__ CUtensorMap ws_map,
                                                                                const __grid_constant__ CUtensorMap xs_map, const MgArgs a) {
+    constexpr int THREADS = MG_THREADS(PLAIN);
     constexpr unsigned X_BYTES = NT * MX_K, S_BYTES = G * MX_PIECE, GROUP_BYTES = G * X_BYTES + 2 * S_BYTES;
-    constexpr unsigned S_COL0 = NT < 32 ? 32 : NT, COLS = S_COL0 + 2 * G * 8 <= 128 ? 128 : 256;
+    constexpr unsigned S_COL0 = NT < 32 ? 32 : NT, COLS = 128;
+    static_assert(S_COL0 + 2 * G * 8 <= COLS, "tensor memory");
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     unsigned char* g_s = w_s + WS * MG_W_BYTES;                   // [2][G rows' boxes [NT][128], 128-byte swizzle like the weights; weights' pieces, rows' pieces]
@@ -82,13 +89,29 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int part = blockIdx.x, parts = gridDim.x, tile = blockIdx.y, tok0 = blockIdx.z * NT;
-    const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0;
+    const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0, early = min(min(WS, 2 * G), kbs);
+    auto weights = [&](int kb, int s) {                           // into stage s; with the first of a group all of its scales
+        const int at = tile * a.ktiles + kb0 + kb;
+        if (kb % G == 0) {                                        // what stands behind the part's last stage is read and not used
+            const int g = (kb / G) & 1;
+            t5_expect_tx(&g_full[g], S_BYTES);
+            t5_tma_2d(g_s + g * GROUP_BYTES + G * X_BYTES, &ws_map, 0, at, &g_full[g]);
+        }
+        t5_expect_tx(&full[s], MG_W_READ);
+        t5_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, at * MG_ROWS, &full[s]);
+    };
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < WS; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { t5_mbar_init(&g_full[s], 2); t5_mbar_init(&g_empty[s], 1); }      // the weights' scales; rows and theirs
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&g_full[s], PLAIN ? 1 + MG_MAKERS : 2); t5_mbar_init(&g_empty[s], 1); }      // the weights' scales; rows and theirs
         t5_mbar_init(&acc_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        // Weights and their scales are nobody's output: the first of them are on their way before anything else, whatever runs in front.
+        for (int kb = 0; kb < early; ++kb) weights(kb, kb);
+    }
+    if (warp == 6 && lane == 0 && !PLAIN) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&x_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&xs_map) : "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(COLS) : "memory");
@@ -102,27 +125,22 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
 
     int issued = 0;                                               // stages, or groups, that were asked for, in the threads that ask
     if (warp == 0) {
-        if (lane == 0) {                                          // weights and their scales are nobody's output: no wait for the kernel in front
-            int s = 0;
-            unsigned phase = 1;                                   // a barrier that was never used passes for the phase before its first
-            const int at = tile * a.ktiles + kb0;
+        if (lane == 0) {
+            int s = early % WS;
+            unsigned phase = early == WS ? 0 : 1;                 // a barrier that was never used passes for the phase before its first
+            issued = early;
 #pragma unroll 1
-            for (int kb = 0; kb < kbs; ++kb) {
-                if (kb % G == 0) {                                // what stands behind the part's last stage is read and not used
-                    const int g = kb / G;
-                    if (!mg_wait(&g_empty[g & 1], ((g >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status)) break;
-                    t5_expect_tx(&g_full[g & 1], S_BYTES);
-                    t5_tma_2d(g_s + (g & 1) * GROUP_BYTES + G * X_BYTES, &ws_map, 0, at + kb, &g_full[g & 1]);
-                }
+            for (int kb = early; kb < kbs; ++kb) {
+                const int g = kb / G;
+                if (kb % G == 0 && !mg_wait(&g_empty[g & 1], ((g >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status)) break;
                 if (!mg_wait(&empty[s], phase, a.waits, &abort_flag, a.status)) break;
-                t5_expect_tx(&full[s], MG_W_READ);
-                t5_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, &full[s]);
+                weights(kb, s);
                 issued = kb + 1;
                 if (++s == WS) s = 0, phase ^= 1;
             }
         }
         __syncwarp();
-    } else if (warp == 6) {
+    } else if (warp == 6 && !PLAIN) {
         if (lane == 0) {
             pdl_wait();
 #pragma unroll 1
@@ -139,6 +157,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
     } else if (warp == 1) {
         const unsigned lead = elect_one();
         const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(g_s, 16, 1024), sd = mg_scale_desc(g_s + G * X_BYTES);
+        const unsigned off = tok0 % 128 / 32;                     // the tile's first token in its piece of scales
         bool ok = true;
         int s = 0;
         unsigned phase = 0;
@@ -160,7 +179,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     mg_mma_lead(lead, tmem, wd + s * (MG_W_BYTES >> 4) + 2 * k, xd + ((g * GROUP_BYTES + q * X_BYTES) >> 4) + 2 * k, mg_idesc(MG_ROWS, NT, k),
-                                sc0 + 8 * q, sc0 + 8 * q + 4, (k0 | q | k) ? 1u : 0u);
+                                sc0 + 8 * q, sc0 + 8 * q + 4 + off, (k0 | q | k) ? 1u : 0u);
                 t5_commit_lead(lead, &empty[s]);
                 if (++s == WS) s = 0, phase ^= 1;
             }
@@ -169,6 +188,53 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
         if (ok) t5_commit_lead(lead, &acc_full);
     } else {
         pdl_wait();
+        if constexpr (PLAIN) {                                    // warps 2 to 6; rows beyond T keep what stands there, nobody minds
+            // A warp takes two stages of a row at a time, sixteen lanes each, and has the next group's values on their way while it makes this one's.
+            static_assert(G % 2 == 0, "stages go in pairs");
+            constexpr int BATCH = (NT * G / 2 + MG_MAKERS - 1) / MG_MAKERS;       // units of a group that a warp has at most
+            const int p = lane & 15, units = a.T * (G / 2);
+            const bf16* x = static_cast<const bf16*>(a.plain) + kb0 * MX_K + (lane >> 4) * MX_K + p * 8;
+            const int left = a.K - kb0 * MX_K - (lane >> 4) * MX_K - p * 8;       // values of the row from the lane's first on
+            uint4 raw[BATCH];
+            auto fetch = [&](int g) {
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const int u = warp - 2 + j * MG_MAKERS, at = (g * G + u % (G / 2) * 2) * MX_K;
+                    raw[j] = u < units && at < left ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(u / (G / 2)) * a.K + at) : make_uint4(0u, 0u, 0u, 0u);
+                }
+            };
+            fetch(0);
+#pragma unroll 1
+            for (int g = 0; g * G < kbs; ++g) {
+                unsigned char* to = g_s + (g & 1) * GROUP_BYTES;
+                if (!__all_sync(0xffffffffu, mg_wait(&g_empty[g & 1], ((g >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status))) break;
+                uint4 now[BATCH];
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) now[j] = raw[j];
+                fetch(g + 1);                                     // beyond the part: not used, and beyond the row not read
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const int u = warp - 2 + j * MG_MAKERS, r = u / (G / 2), q = u % (G / 2) * 2 + (lane >> 4);
+                    if (u >= units) break;                        // for the whole warp
+                    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&now[j]);
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = __bfloat1622float2(h[i]);
+                        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+                    }
+                    unsigned word;
+                    const uint2 c = mx_encode8<MX_E4M3>(v, word);
+                    // the 128-byte swizzle: 16-byte piece i of row r at i ^ (r % 8)
+                    *reinterpret_cast<uint2*>(to + q * X_BYTES + r * MX_K + (((p >> 1) ^ (r & 7)) << 4) + (p & 1) * 8) = c;
+                    if (p == 0) *reinterpret_cast<unsigned*>(to + G * X_BYTES + S_BYTES + q * MX_PIECE + (r & 31) * 16 + (r >> 5) * 4) = word;
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) t5_arrive(&g_full[g & 1]);
+            }
+        }
+        if (warp < 6) {
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full, 0, a.waits, &abort_flag, a.status));
         t5_fence_after();
@@ -181,6 +247,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sums[(16 * c + i) * MG_ROWS + row] = __uint_as_float(r[i]);
             }
+        }
     }
     t5_fence_before();
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every part's sums are there
@@ -204,7 +271,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
         const int toks = min(NT, a.T - tok0);
         if constexpr (MODE == MG_GATED) {
             // sixteen lanes a token, four features a lane, eight lanes a block
-            const int f = 4 * (tid & 15), step = MG_THREADS / 16 * parts;
+            const int f = 4 * (tid & 15), step = THREADS / 16 * parts;
             unsigned char* codes = static_cast<unsigned char*>(a.y);
 #pragma unroll 1
             for (int t0 = 0; t0 < toks; t0 += step) {
@@ -228,7 +295,7 @@ __global__ void __launch_bounds__(MG_THREADS, NT <= 64 ? 2 : 1) linear_mx_kernel
             TO* y = static_cast<TO*>(a.y);
             const int f = tile * MG_ROWS + 4 * lane;
 #pragma unroll 2
-            for (int tok = part + warp * parts; tok < toks; tok += MG_THREADS / 32 * parts) {
+            for (int tok = part + warp * parts; tok < toks; tok += THREADS / 32 * parts) {
                 const float4 t = total(tok * MG_ROWS + 4 * lane);
                 float ts[4] = {t.x, t.y, t.z, t.w};
                 TO* to = y + static_cast<size_t>(tok0 + tok) * a.N + f;
@@ -603,33 +670,48 @@ static bool mg_scales_map(CUtensorMap* map, const void* scales, int row_tiles, i
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.
+// Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.  Two CTAs an SM, less an eighth, because
+// clusters do not fill a group of SMs to the last slot: one row x 4,096 by 6,144 in 4 parts 5.9 us, 5 (240 CTAs) 5.7, 6 (288) 9.5; 8 rows x
+// 2,048 by 12,288 in one 6.9, two (192) 5.9, three (288) 9.7; 8 rows by 2 x 12,288 (192 tiles) in one 13.3, two 18.0.
+static int mg_slots(int sms) { return 2 * sms * 7 / 8; }
 static int mg_parts(long long tiles, int ktiles, int slots) {
     int best = 1;
     while (best < 8 && (best + 1) * tiles <= slots && ktiles / (best + 1) >= 2) ++best;
     return best;
 }
 
-template <int NT, int WS, int G, int MODE, typename TO>
+// Whether more rows than 64 go to pairs of CTAs, or to tiles of 64 rows each of which reads the weights again but whose K may be cut.  By
+// the time that both take, in hundredths of a microsecond beside what they share: a wave of single CTAs 36 a tile of K and 25 a part, a round of
+// pairs 28.  Rows x K by N, us, single / pair: 100 x 4,096 by 4,096 8.5, 13.4; 256 11.3, 13.7; 320 16.3, 13.7; 700 29, 14.3; 160 x 4,096 by 6,144
+// 15.8, 13.5; 256 x 12,288 by 4,096 23.7, 29.7; 320 39.5, 29.8; 700 x 1,024 by 1,024 6.2, 7.1; 1,024 x 1,024 by 2,048 7.8, 7.7; 128 x 2,048 by
+// 12,288 11.2, 10.0; gated 128 x 4,096 by 2 x 12,288 36.5, 27.1 (64 rows: 21.5).
+static bool mg_pairs_pay(int T, int tiles, int ktiles, int sms) {
+    if (T <= 64) return false;
+    const long long single = static_cast<long long>((T + 63) / 64) * tiles, pairs = static_cast<long long>((T + MP_NT - 1) / MP_NT) * ((tiles + 1) / 2);
+    const int parts = mg_parts(single, ktiles, mg_slots(sms));
+    const long long waves = (single * parts + 2 * sms - 1) / (2 * sms), rounds = (pairs + sms / 2 - 1) / (sms / 2);
+    return 36 * waves * ((ktiles + parts - 1) / parts) + 25 * parts > 28 * rounds * ktiles;
+}
+
+template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO>
 static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
-    CUtensorMap w_map, x_map, ws_map, xs_map;
+    CUtensorMap w_map, ws_map, x_map = {}, xs_map = {};
     const int padded = static_cast<int>(mx_padded_rows(a.T)), stored = (tiles + 1) / 2 * 2;
-    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, NT, G) ||
-        !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, G, 0) || !mg_scales_map(&xs_map, a.x_scales, (padded + 127) / 128, a.ktiles, G, 0))
-        return LLM_REFUSED_SIZE;
+    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, G, 0)) return LLM_REFUSED_SIZE;
+    if (!PLAIN && (!mg_rows_map(&x_map, x, padded, a.ktiles, NT, G) || !mg_scales_map(&xs_map, a.x_scales, (padded + 127) / 128, a.ktiles, G, 0))) return LLM_REFUSED_SIZE;
     constexpr size_t smem = static_cast<size_t>(WS) * MG_W_BYTES + 2 * G * (NT * MX_K + 2 * MX_PIECE) + 1024;
-    static_assert(NT <= 128, "a tile's scales are one piece");
+    static_assert(128 % NT == 0, "a tile's scales are in one piece");
     static_assert(NT * 4 <= WS * MX_K, "the sums fit the weights' stages");
-    static_assert(smem <= (NT <= 64 ? 113 : 226) * 1024, "shared memory of an SM");
-    auto kern = linear_mx_kernel<NT, WS, G, MODE, TO>;
+    static_assert(smem <= 113 * 1024, "half of an SM's shared memory");
+    auto kern = linear_mx_kernel<NT, WS, G, PLAIN, MODE, TO>;
     static bool had[MG_DEVICES];
     const int dev = mg_device();
     if (dev < 0) return LLM_REFUSED_SIZE;
     if (const int rc = mg_allow(kern, smem, dev, had)) return rc;
     const int tok_tiles = (a.T + NT - 1) / NT, sms = mg_sms(dev);
     if (tiles > 65535 || tok_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
-    const int parts = mg_parts(static_cast<long long>(tiles) * tok_tiles, a.ktiles, sms * (NT <= 64 ? 2 : 1) * 7 / 8);
-    launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS), smem, s, parts, w_map, x_map, ws_map, xs_map, a);
+    const int parts = mg_parts(static_cast<long long>(tiles) * tok_tiles, a.ktiles, mg_slots(sms));
+    launch_pdl_cluster(kern, dim3(parts, tiles, tok_tiles), dim3(MG_THREADS(PLAIN)), smem, s, parts, w_map, x_map, ws_map, xs_map, a);
     return launch_status();
 }
 template <int MODE, typename TO>
@@ -664,30 +746,46 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     return launch_status();
 }
 template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
-    if (a.T <= 16) return mg_launch<16, 5, 4, MODE, TO>(w, tiles, x, a, s);
-    if (a.T <= 32) return mg_launch<32, 4, 4, MODE, TO>(w, tiles, x, a, s);
-    if (a.T <= 64) return mg_launch<64, 4, 2, MODE, TO>(w, tiles, x, a, s);
-    if (a.T <= 128) return mg_launch<128, 8, 2, MODE, TO>(w, tiles, x, a, s);
-    return mp_launch<MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 16) return a.plain ? mg_launch<16, 5, 4, true, MODE, TO>(w, tiles, x, a, s) : mg_launch<16, 5, 4, false, MODE, TO>(w, tiles, x, a, s);
+    if (a.T <= 32) return mg_launch<32, 4, 4, false, MODE, TO>(w, tiles, x, a, s);
+    const int dev = mg_device(), sms = dev < 0 ? 0 : mg_sms(dev);
+    if (sms < 2) return LLM_REFUSED_SIZE;
+    return mg_pairs_pay(a.T, tiles, a.ktiles, sms) ? mp_launch<MODE, TO>(w, tiles, x, a, s) : mg_launch<64, 4, 2, false, MODE, TO>(w, tiles, x, a, s);
 }
 
-// The rows of 8 bits as the products take them: made of the matrix `plain` first, where there is one.
-static int mg_operands(void* rows, const void* plain, int dtype, const void* w, const void* w_scales, const int32_t* status, int T, int N, int K,
-                       uintptr_t stream) {
+// Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself.
+#define MG_PLAIN_ROWS 16
+extern "C" int llm_linear_mx_takes(const void* plain, int dtype, int T, int K) { return T <= MG_PLAIN_ROWS && dtype == LLM_DT_BF16 && K % 8 == 0 && aligned16(plain); }
+
+// Checks a product's operands and, where there is room for rows beside a matrix `plain`, makes them.
+static int mg_operands(MgArgs* a, void* rows, const void* plain, int dtype, const void* w, const void* w_scales, int T, int N, int K, int waits,
+                       int32_t* status, uintptr_t stream) {
     if (N <= 0 || N > (1 << 24) || K <= 0 || K > (1 << 20) || T > (1 << 24)) return LLM_REFUSED_SIZE;
     if (!aligned16(w) || !aligned16(w_scales) || !aligned16(rows) || (reinterpret_cast<uintptr_t>(w) & 31) || status == nullptr) return LLM_REFUSED_ALIGN;
+    if (plain && dtype != LLM_DT_F32 && dtype != LLM_DT_BF16) return LLM_REFUSED_DTYPE;
+    const bool itself = plain && rows == nullptr;
+    if (itself ? !llm_linear_mx_takes(plain, dtype, T, K) : rows == nullptr) return LLM_REFUSED_ALIGN;
+    *a = {};
+    a->w_scales = static_cast<const unsigned char*>(w_scales);
+    a->T = T, a->N = N, a->K = K, a->ktiles = mx_tiles(K), a->waits = waits, a->status = status;
+    if (itself) {
+        a->plain = plain;
+        return LLM_OK;
+    }
+    a->x_scales = mx_row_scales(rows, T, K);
     return plain ? llm_mx_rows(plain, dtype, rows, T, K, stream) : LLM_OK;
 }
 
-// rows: of 8 bits [T, K], or room for them and `plain` a matrix [T, K] of `dtype` that they are made of first; w: a weight of 4 bits [N, K];
-// y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
+// rows: of 8 bits [T, K], or room for them (null: none, where llm_linear_mx_takes) and `plain` a matrix [T, K] of `dtype`; w: a weight of 4 bits
+// [N, K]; y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
 extern "C" int llm_linear_mx(void* rows, const void* plain, int dtype, const void* w, const void* w_scales, void* y, int out_dtype, int add, int T, int N,
                              int K, int waits, int32_t* status, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
     if ((out_dtype != LLM_DT_F32 && out_dtype != LLM_DT_BF16) || (add && out_dtype != LLM_DT_F32)) return LLM_REFUSED_DTYPE;
-    if (const int rc = mg_operands(rows, plain, dtype, w, w_scales, status, T, N, K, stream)) return rc;
-    MgArgs a = {static_cast<const unsigned char*>(w_scales), mx_row_scales(rows, T, K), y, nullptr, T, N, mx_tiles(K), 0, N % 4 == 0 && aligned16(y), waits,
-                status, {}};
+    MgArgs a;
+    if (const int rc = mg_operands(&a, rows, plain, dtype, w, w_scales, T, N, K, waits, status, stream)) return rc;
+    a.y = y;
+    a.vec = N % 4 == 0 && aligned16(y);
     const int tiles = (N + MG_ROWS - 1) / MG_ROWS;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (add) return mg_rows<MG_ADD, float>(w, tiles, rows, a, s);
@@ -702,9 +800,12 @@ extern "C" int llm_linear_mx_silu_mul(void* rows, const void* plain, int dtype, 
     MxAct form;
     if (!mx_act(act, limit, &form)) return LLM_REFUSED_SIZE;
     if (!aligned16(made)) return LLM_REFUSED_ALIGN;
-    if (const int rc = mg_operands(rows, plain, dtype, w, w_scales, status, T, N, K, stream)) return rc;
+    MgArgs a;
+    if (const int rc = mg_operands(&a, rows, plain, dtype, w, w_scales, T, N, K, waits, status, stream)) return rc;
     const int tiles = 2 * ((N + 127) / 128);                      // as the weight has them
-    MgArgs a = {static_cast<const unsigned char*>(w_scales), mx_row_scales(rows, T, K), made, mx_row_scales(made, T, N), T, N, mx_tiles(K), tiles * 64, 0,
-                waits, status, form};
+    a.y = made;
+    a.y_scales = mx_row_scales(made, T, N);
+    a.out_kpad = tiles * 64;
+    a.act = form;
     return mg_rows<MG_GATED, float>(w, tiles, rows, a, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -28,8 +28,8 @@
 __host__ __device__ __forceinline__ size_t mx_scale_at(size_t row, int kb, int ktiles) {
     return ((row >> 7) * ktiles + (kb >> 2)) * MX_PIECE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3);
 }
-// Rows that stand behind T rows of 8 bits, so that no box of a product (16, 32, 64 or 128 rows, or 192 of a pair) reaches beyond them, nor
-// beyond whole pieces of scales; the scales stand behind the codes.
+// Rows that stand behind T rows of 8 bits, so that hardly a box of a product (16, 32 or 64 rows, or 192 of a pair) reaches beyond them, which takes
+// longer, nor beyond whole pieces of scales; the scales stand behind the codes.
 static inline long long mx_padded_rows(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : (T + 383LL) / 384 * 384; }
 static inline int mx_tiles(int k) { return (k + MX_K - 1) / MX_K; }
 static inline unsigned char* mx_row_scales(void* rows, int T, int K) { return static_cast<unsigned char*>(rows) + mx_padded_rows(T) * mx_tiles(K) * MX_K; }
@@ -122,21 +122,21 @@ template <bool FAST, typename T> __device__ __forceinline__ void mx_load8(const 
         else
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    if (vec == 2) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2)
-            if (col + i < n) {
-                const float2 f = mx_load2(row + col + i);
-                v[i] = f.x, v[i + 1] = f.y;
-            }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + i < n) v[i] = to_f32(row[col + i]);
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (vec == 2) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+                if (col + i < n) {
+                    const float2 f = mx_load2(row + col + i);
+                    v[i] = f.x, v[i + 1] = f.y;
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (col + i < n) v[i] = to_f32(row[col + i]);
+        }
     }
 }
 template <bool FAST, typename T> __device__ __forceinline__ void mx_put8(T* row, int col, int n, int vec, const float (&v)[8]) {

@@ -2298,6 +2298,10 @@ def latent_q_product(x: torch.Tensor, weight: torch.Tensor) -> bool:
 # within the format's largest value (e4m3 448, e2m1 6); each value is then rounded to the format's nearest.
 # csrc/microscaling.cuh says where the bytes lie.
 MX_BLOCK = 32
+# Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself.  In a graph a kernel
+# of its own is faster from a few rows on (16 x 12,288 by 4,096: 9.6 us, 11.6 by the product itself; one row x 4,096 by 6,144: 7.1,
+# 6.2); outside a graph its launch costs the host 6 us.
+MX_PLAIN_ROWS, MX_PLAIN_ROWS_CAPTURED = 16, 4
 _mx_calls: Dict[str, object] = {}
 _P, _I, _F, _L = c_void_p, c_int, c_float, c_longlong
 _MX_SIGNATURES = {
@@ -2488,7 +2492,8 @@ def silu_and_mul_mx(gate_up, activation: str = "silu", limit: float = 0.0) -> Mx
 
 
 def _mx_operands(x, weight: MxWeight, gated: bool):
-    """(address of a matrix that is still to be taken to 8 bits or None, its dtype, the rows of 8 bits, T, K) of a product's x."""
+    """(the rows of 8 bits or room for them, the address of a matrix that they are still to be made of or None, its dtype, T, K) of a
+    product's x."""
     if not isinstance(weight, MxWeight) or weight.gated != gated:
         raise KernelError("the microscaled product takes an MxWeight" + (" made with gated=True" if gated else " that is not a gated one"))
     made = type(x) is MxRows
@@ -2497,9 +2502,12 @@ def _mx_operands(x, weight: MxWeight, gated: bool):
     T, K = x.shape
     if made:
         _here(x.buffer, weight.codes)
-        return None, 0, x, T, K
+        return x.buffer, None, 0, T, K
     _here(x, weight.codes)
-    return x.data_ptr(), _dt(x), MxRows(T, K, weight.device), T, K
+    at, dt = x.data_ptr(), _dt(x)
+    itself = (T <= MX_PLAIN_ROWS and dt == 1 and K % 8 == 0 and at % 16 == 0
+              and (T <= MX_PLAIN_ROWS_CAPTURED or not torch.cuda.is_current_stream_capturing()))
+    return None if itself else MxRows(T, K, weight.device).buffer, at, dt, T, K
 
 
 def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, residual: Optional[torch.Tensor] = None,
@@ -2507,7 +2515,7 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
     """x [T, K] @ weight[N, K]^T with the weight in 4 bits and x in 8 (`MxRows`; a matrix is taken to 8 bits first), products exact,
     sums in float32, on the block-scaled tcgen05 products.  The result is float32 or bfloat16 [T, N]; with `residual` (float32
     [T, N]) it is added to that in place, which is returned."""
-    plain, dt, rows, T, K = _mx_operands(x, weight, False)
+    rows, plain, dt, T, K = _mx_operands(x, weight, False)
     N = weight.shape[0]
     if residual is not None:
         _here(residual)
@@ -2517,9 +2525,10 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
     else:
         y = torch.empty((T, N), dtype=out_dtype, device=weight.device)
         od = _dt(y)
-    _check(_mx_call("llm_linear_mx")(rows.buffer.data_ptr(), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(), y.data_ptr(), od,
+    _check(_mx_call("llm_linear_mx")(_ptr(rows), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(), y.data_ptr(), od,
                                      residual is not None, T, N, K, waits, _mx_status_ptr(weight.device), _stream()), "linear_mx")
-    _mx_count(plain)
+    if plain is not None and rows is not None:
+        _mx_count()
     return y
 
 
@@ -2527,19 +2536,20 @@ def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: flo
     """act(x @ gate^T) * (x @ up^T) as rows of 8 bits [T, I] for a gated weight [2I, K] in 4 bits, act as in `silu_and_mul`, in the
     product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits."""
     act = ACTIVATIONS[activation]
-    plain, dt, rows, T, K = _mx_operands(x, weight, True)
+    rows, plain, dt, T, K = _mx_operands(x, weight, True)
     inter = weight.shape[0] // 2
     made = MxRows(T, inter, weight.device)
-    _check(_mx_call("llm_linear_mx_silu_mul")(rows.buffer.data_ptr(), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(),
+    _check(_mx_call("llm_linear_mx_silu_mul")(_ptr(rows), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(),
                                               made.buffer.data_ptr(), T, inter, K, act, limit, waits, _mx_status_ptr(weight.device), _stream()),
            "linear_silu_mul_mx")
-    _mx_count(plain)
+    if plain is not None and rows is not None:
+        _mx_count()
     return made
 
 
-def _mx_count(plain) -> None:
+def _mx_count() -> None:
     global launch_count
-    launch_count += plain is not None         # the kernel that takes a matrix to 8 bits
+    launch_count += 1                         # the kernel that takes a matrix to 8 bits
 
 
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:

@@ -55,4 +55,7 @@ def test_sizes_types_and_addresses_of_products():
     assert y(x=P + 8) == ALIGN and y(w=P + 16) == ALIGN and y(status=0) == ALIGN and y(dt=2) == DTYPE and y(dt=1, add=1) == DTYPE and y(plain=P, xd=2) == DTYPE
     g = lambda kind=0, limit=0.0, T=4, N=64, made=P: m.llm_linear_mx_silu_mul(v(P), v(0), 0, v(P), v(P), v(made), T, N, 64, kind, f(limit), 1, v(P), v(0))
     assert g(T=0) == 0 and g(N=0) == SIZE and g(kind=3) == SIZE and g(kind=2) == SIZE and g(kind=-1) == SIZE and g(made=P + 8) == ALIGN
+    assert y(x=0) == ALIGN and y(x=0, plain=P, T=17) == ALIGN 
+    takes = lambda T=16, dt=1, K=64, at=P: m.llm_linear_mx_takes(v(at), dt, T, K)
+    assert takes(T=ops.MX_PLAIN_ROWS) and not takes(T=ops.MX_PLAIN_ROWS + 1) and not takes(dt=0) and not takes(K=36) and not takes(at=P + 8)
     assert [ops.mx_padded_rows(t) for t in (1, 16, 17, 33, 65, 128, 129, 384, 385)] == [16, 16, 32, 64, 128, 128, 384, 384, 768]
