@@ -12,7 +12,7 @@ argmax, src/main.cpp:175-178); top-k and top-p are parsed, validated and, as in 
 not applied; --use-kv-cache, --use-paged-kv-cache, --benchmark-interleaved and
 --benchmark-batch-decode are accepted and ignored, because there is one cache (paged) and
 one scheduler; --device takes only CUDA devices.  Added: --dtype, --seed, --random-weights,
---max-total-tokens, --chunk, --max-tokens-per-step, --benchmark-prompt-len.
+--max-total-tokens, --chunk, --max-tokens-per-step, --benchmark-prompt-len, --weight-format.
 """
 from __future__ import annotations
 
@@ -36,6 +36,7 @@ Options:
   --seed <int>             Seed of the sampling stream and of --random-weights, default: 0
   --device <str>           cuda, cuda:N, gpu or auto (there is no CPU path)
   --dtype <str>            bfloat16 (default) or float32
+  --weight-format <str>    stored (default), or mxfp4: attention's and feed-forwards' matrices in 4 bits
   --eos-token-id <int>     Stop generation when this token id is generated
   --page-size <N>          Paged KV cache page size, default 16
   --max-total-tokens <N>   Tokens the cache pool holds, default: prompt + max tokens + 16
@@ -79,6 +80,7 @@ class Args:
     chunk: Optional[int] = None
     max_tokens_per_step: int = 8192
     benchmark_prompt_len: Optional[int] = None
+    weight_format: str = "stored"
 
 
 class ArgError(ValueError):
@@ -92,7 +94,7 @@ _VALUE = {"--model": ("model", str), "--prompt": ("prompt", str), "--input-ids":
           "--benchmark-warmup": ("benchmark_warmup", int), "--page-size": ("page_size", int),
           "--seed": ("seed", int), "--dtype": ("dtype", str), "--max-total-tokens": ("max_total_tokens", int),
           "--chunk": ("chunk", int), "--max-tokens-per-step": ("max_tokens_per_step", int),
-          "--benchmark-prompt-len": ("benchmark_prompt_len", int)}
+          "--benchmark-prompt-len": ("benchmark_prompt_len", int), "--weight-format": ("weight_format", str)}
 _FLAG = {"--verbose": "verbose", "--benchmark": "benchmark", "--use-kv-cache": "use_kv_cache",
          "--use-paged-kv-cache": "use_paged_kv_cache", "--benchmark-interleaved": "benchmark_interleaved",
          "--benchmark-batch-decode": "benchmark_batch_decode", "--random-weights": "random_weights"}
@@ -142,6 +144,10 @@ def parse_args(argv: List[str]) -> Args:
         raise ArgError("--page-size must be positive")
     if a.dtype not in ("bfloat16", "bf16", "float32", "fp32"):
         raise ArgError("--dtype must be bfloat16 or float32")
+    if a.weight_format not in ("stored", "mxfp4"):
+        raise ArgError("--weight-format must be stored or mxfp4")
+    if a.weight_format == "mxfp4" and a.dtype in ("float32", "fp32"):
+        raise ArgError("--weight-format mxfp4 is for --dtype bfloat16")
     return a
 
 
@@ -211,7 +217,7 @@ def _run(args: Args) -> int:
     print("Config:")
     for k, v in (("Model", args.model), ("Prompt", args.prompt), ("Max tokens", args.max_tokens),
                  ("Temperature", args.temperature), ("Top-k", args.top_k), ("Top-p", args.top_p),
-                 ("Seed", args.seed), ("Dtype", args.dtype), ("Eos Token Id", args.eos_token_id if
+                 ("Seed", args.seed), ("Dtype", args.dtype), ("Weights", args.weight_format), ("Eos Token Id", args.eos_token_id if
                                                                args.eos_token_id is not None else -1),
                  ("page_size", args.page_size), ("benchmark", args.benchmark)):
         print(f"  {k + ':':<14}{v}")
@@ -258,7 +264,7 @@ def _run(args: Args) -> int:
     engine = PagedGenerateEngine(
         config if args.random_weights else args.model, dtype=dtype, device=device, page_size=args.page_size,
         max_total_tokens=total, max_requests=max(n_req, 1), max_tokens_per_step=args.max_tokens_per_step,
-        chunk=args.chunk, verbose=args.verbose, seed=args.seed)
+        chunk=args.chunk, verbose=args.verbose, seed=args.seed, weight_format=args.weight_format)
     print("Model initialized.")
     eos = args.eos_token_id if args.eos_token_id is not None else -1
 

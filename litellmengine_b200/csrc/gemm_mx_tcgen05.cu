@@ -9,7 +9,7 @@
 // 16 KB, sixteen of them and eight bytes of nothing, as the products read them), a box of the rows, and the pieces of both operands'
 // scales, which the tensor core copies to its own memory in front of the stage's four products.
 // Roles: warp 0 feeds the copy engine, warp 1 issues, warps 2 to 5 take the sums; all six write the result.  Waits are bounded: one that
-// runs out sets status code 12, and the feeding thread waits for its last copies before the CTA ends.
+// runs out sets status code 9, and the feeding thread waits for its last copies before the CTA ends.
 //   * Few rows: bytes bound the product.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the
 //     parts' order; nothing is left for another kernel and no result depends on timing.  The first weights are on their way before the
 //     CTA waits for the kernel in front.
@@ -22,7 +22,7 @@
 #define MG_THREADS(PLAIN) (32 * (2 + ((PLAIN) ? MG_MAKERS : 5)))
 #define MG_W_BYTES (MG_ROWS * MX_K)       // of a stage's weights in shared memory
 #define MG_W_READ (MG_W_BYTES / 2)        // the same as the copy engine counts them: what it reads
-#define MG_STATUS 12
+#define MG_STATUS 9
 
 __device__ __forceinline__ bool mg_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
     for (int i = 0; i < waits; ++i) {

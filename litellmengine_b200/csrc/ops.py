@@ -2129,8 +2129,7 @@ _stream_status: Dict[str, torch.Tensor] = {}
 
 def stream_status(device) -> torch.Tensor:
     """The status word of the engine's matrix products and of the delta rule (code 8: a bounded wait of a weight-streaming
-    product ran out; 9: of the paired or the float32 tcgen05 product; 11: of the delta rule's tensor-core scan; 12: of a microscaled
-    tcgen05 product)."""
+    product ran out; 9: of the paired, the float32 or a microscaled tcgen05 product; 11: of the delta rule's tensor-core scan)."""
     key = str(device)
     t = _stream_status.get(key)
     if t is None:
@@ -2266,7 +2265,7 @@ def heads_pay(rows: int, weight: torch.Tensor) -> bool:
 
 def heads_product(x: torch.Tensor, weight: torch.Tensor, cache: Optional[torch.Tensor], d: int) -> bool:
     """Whether `linear_pair_heads` takes this q/k/v product, and its tiles fill the clusters well enough to ask `heads_pay`."""
-    return (d == 128 and isinstance(x, torch.Tensor) and x.shape[0] >= PAIR_HEADS_MIN_ROWS and cache is not None and cache.dtype == torch.bfloat16
+    return (d == 128 and isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and x.shape[0] >= PAIR_HEADS_MIN_ROWS and cache is not None and cache.dtype == torch.bfloat16
             and cache.is_contiguous() and x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0
             and _pair_takes(x, weight, weight.shape[0], "heads"))
 
@@ -2553,8 +2552,11 @@ def _mx_count() -> None:
 
 
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:
-    """residual (float32 [T, N]) += x @ weight^T in the product's epilogue, if the paired kernel takes
-    these operands; False, and nothing done, if not."""
+    """residual (float32 [T, N]) += x @ weight^T in the product's epilogue, if the paired kernel or, for a weight in 4 bits, the
+    microscaled one takes these operands; False, and nothing done, if not."""
+    if isinstance(weight, MxWeight):
+        linear_mx(x, weight, residual=residual)
+        return True
     if (residual.dtype != torch.float32 or not residual.is_contiguous() or residual.shape != (x.shape[0], weight.shape[0])
             or not _pair_takes(x, weight, weight.shape[0], "into")):
         return False
@@ -2565,7 +2567,10 @@ def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -
 def linear_silu_mul(x: torch.Tensor, w_gate_up: torch.Tensor, out_dtype: torch.dtype, activation: str = "silu",
                     limit: float = 0.0):
     """act(x @ gate^T) * (x @ up^T) for w_gate_up = [gate; up]: one kernel where the paired product
-    takes it, else the product (which may stay a sum of k-splits) followed by the activation kernel."""
+    takes it, else the product (which may stay a sum of k-splits) followed by the activation kernel.  A weight in 4 bits
+    (`MxWeight`): rows of 8 bits (`MxRows`)."""
+    if isinstance(w_gate_up, MxWeight):
+        return linear_silu_mul_mx(x, w_gate_up, activation=activation, limit=limit)
     if out_dtype == torch.bfloat16 and (isinstance(x, PendingRows) or (x.dtype == torch.bfloat16 and x.is_contiguous() and x.data_ptr() % 16 == 0
                                                                        and small_product(x.shape[0], w_gate_up, gated=True))):
         return linear_small(x, w_gate_up, out_dtype, activation=activation, limit=limit)
@@ -2640,7 +2645,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     src/layers/linear.cu:169-215).  bfloat16 operands accumulate in float32; a float32 weight
     keeps its product in true float32 (no TF32), whatever x is: up to 16 rows in the engine's own streaming kernel, more rows of large matrices
     on the tensor cores as sums of three bfloat16 values each, as near as float32 sums.  bfloat16 weights may be read before the
-    kernel in front of the product in the stream has finished (they are nobody's output); float32 ones are not."""
+    kernel in front of the product in the stream has finished (they are nobody's output); float32 ones are not.  A weight in 4
+    bits (`MxWeight`) goes to `linear_mx`, which also takes `MxRows`."""
+    if isinstance(weight, MxWeight):
+        return linear_mx(x, weight, out_dtype or torch.bfloat16)
     if isinstance(x, PendingRows):
         return linear_small(x, weight, out_dtype or x.dtype)
     _dev(x, weight)

@@ -29,14 +29,16 @@ from .scheduler import ScheduledPortion, Scheduler
 class PagedGenerateEngine:
     def __init__(self, model, dtype: str = "bfloat16", device: str = "cuda:0", page_size: int = 16,
                  max_total_tokens: int = 8192, max_requests: int = 64, max_tokens_per_step: int = 8192,
-                 chunk: Optional[int] = None, verbose: bool = False, seed: int = 0, pipelined: bool = True):
+                 chunk: Optional[int] = None, verbose: bool = False, seed: int = 0, pipelined: bool = True,
+                 weight_format: str = "stored"):
         """`model`: a model folder (config.json + *.safetensors), a typed configuration (random
-        weights from `seed`, drawn on the device), or a ready `ModelRunner`."""
+        weights from `seed`, drawn on the device), or a ready `ModelRunner`.  `weight_format` 'mxfp4': matrices held in
+        4 bits, as `Model` has it (a ready runner's model has its own)."""
         if isinstance(model, ModelRunner):
             self.runner = model
         else:
             kw = dict(dtype=dtype, device=device, page_size=page_size, max_total_tokens=max_total_tokens,
-                      max_requests=max_requests, max_tokens_per_step=max_tokens_per_step)
+                      max_requests=max_requests, max_tokens_per_step=max_tokens_per_step, weight_format=weight_format)
             if isinstance(model, str):
                 self.runner = ModelRunner.from_folder(model, **kw)
             else:

@@ -23,9 +23,8 @@ STATUS_TEXT = {1: "a token id outside the vocabulary reached the embedding kerne
                5: "a wait on a copy barrier in the decode attention kernel ran out",
                6: "a wait on a barrier in the tcgen05 prompt attention kernel ran out",
                8: "a wait on a copy barrier in the weight-streaming product ran out",
-               9: "a wait on a barrier in a tcgen05 product (the paired one or the float32 one) ran out",
-               11: "a wait on a copy barrier in the delta rule's tensor-core scan ran out",
-               12: "a wait on a barrier in a microscaled tcgen05 product ran out"}
+               9: "a wait on a barrier in a tcgen05 product (the paired one, the float32 one or a microscaled one) ran out",
+               11: "a wait on a copy barrier in the delta rule's tensor-core scan ran out"}
 
 
 class ModelRunner:
@@ -91,9 +90,9 @@ class ModelRunner:
 
     # ---- construction ----------------------------------------------------------------------
     @classmethod
-    def from_folder(cls, model_dir: str, dtype="bfloat16", device="cuda", **kw) -> "ModelRunner":
+    def from_folder(cls, model_dir: str, dtype="bfloat16", device="cuda", weight_format: str = "stored", **kw) -> "ModelRunner":
         config = load_config(model_dir)
-        model = Model(config.plan(), dtype=dtype, device=device)
+        model = Model(config.plan(), dtype=dtype, device=device, weight_format=weight_format)
         model.load_weights(SafetensorsSource(model_dir), where=model_dir)
         r = cls(model, **kw)
         r.config = config
@@ -101,9 +100,9 @@ class ModelRunner:
 
     @classmethod
     def from_config(cls, config, seed: int = 0, dtype="bfloat16", device="cuda",
-                    source: Optional[WeightSource] = None, **kw) -> "ModelRunner":
+                    source: Optional[WeightSource] = None, weight_format: str = "stored", **kw) -> "ModelRunner":
         """Random weights drawn on the device (for benchmarks); `source` overrides them."""
-        model = Model(config.plan(), dtype=dtype, device=device)
+        model = Model(config.plan(), dtype=dtype, device=device, weight_format=weight_format)
         if source is None:
             store = torch.bfloat16 if model.dtype == torch.bfloat16 else torch.float32
             source = RandomSource(model.parameters(), seed, store, device=device)

@@ -131,6 +131,11 @@ class AttentionMixer:
         if self.k_norm is not None:
             self.k_norm.load({"weight": t["k_norm.weight"]})
 
+    def hold_in_4_bits(self) -> int:
+        """From now on the projections are held in 4 bits (`ops.MxWeight`).  How many matrices that are."""
+        self.w_qkv, self.w_o = ops.mx_weight(self.w_qkv), ops.mx_weight(self.w_o)
+        return 2
+
     def cache_need(self):
         if not self.spec.has_kv:
             return None
@@ -432,6 +437,13 @@ class GatedAttentionMixer(BranchMixer):
         n_dec = 0 if work is None else (work.padded_rows.shape[0] if padded else work.num_decode)
         n_tiles = 0 if work is None else (work.padded_tiles.shape[0] if padded else work.num_prefill_tiles)
         return decode_key_splits(self.device, n_dec, self.nkv, decode_reach(batch, self.span)) if n_dec and (self._wide or not n_tiles) else 0
+
+    def hold_in_4_bits(self) -> int:
+        """As `AttentionMixer.hold_in_4_bits`; a branch whose matrices its parent has holds none."""
+        if self.w_in is None:
+            return 0
+        self.w_in, self.w_o = ops.mx_weight(self.w_in), ops.mx_weight(self.w_o)
+        return 2
 
     def large_rows(self, between: bool):
         """As `BranchMixer.large_rows`.  Decode steps of 4 layers, us, without and with both: width 4,096, 17 / 24 / 32 requests 430, 400 / 441, 417 / 456,

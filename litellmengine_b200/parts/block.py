@@ -203,14 +203,18 @@ class Block:
 
 
 def _normed(norm, part, h: torch.Tensor, delta, dtype: torch.dtype):
-    """(h + delta, the part's input norm(h + delta)): by the norm's kernel, in place, or left to the part's first product."""
+    """(h + delta, the part's input norm(h + delta)): by the norm's kernel, in place, for a first product with its weight in 4 bits as
+    rows of 8 bits, or left to the part's first product."""
     from ..csrc import ops
-    if (getattr(part, "first_product", None) is not None and h.is_cuda and ops.rows_worth_leaving(h, delta)
-            and speaks_for_forward(norm, "products_apply_it") and speaks_for_forward(part, "first_product")):
+    if getattr(part, "first_product", None) is not None and h.is_cuda and speaks_for_forward(part, "first_product"):
         weight, gated = part.first_product()
-        rows = ops.pending_rows(h, delta, norm, weight, dtype, gated)
-        if rows is not None:
-            return rows.stream, rows
+        if isinstance(weight, ops.MxWeight):
+            if speaks_for_forward(norm, "makes_mx_rows") and (delta is None or isinstance(delta, (torch.Tensor, ops.PartialSum))):
+                return h, norm.forward_mx(h, delta)
+        elif ops.rows_worth_leaving(h, delta) and speaks_for_forward(norm, "products_apply_it"):
+            rows = ops.pending_rows(h, delta, norm, weight, dtype, gated)
+            if rows is not None:
+                return rows.stream, rows
     return h, norm.forward(h, dtype, delta=delta, write_sum=delta is not None)
 
 

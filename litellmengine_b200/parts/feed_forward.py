@@ -52,6 +52,11 @@ class SwiGLU:
         ops.prepare_streaming(self.w_gate_up)       # a tiled copy for decode steps (bfloat16 on a GPU only)
         ops.prepare_streaming(self.w_down)
 
+    def hold_in_4_bits(self) -> int:
+        """From now on the matrices are held in 4 bits (`ops.MxWeight`), and what stands between them are rows of 8 bits."""
+        self.w_gate_up, self.w_down = ops.mx_weight(self.w_gate_up, gated=True), ops.mx_weight(self.w_down)
+        return 2
+
     supports_partials = True   # forward(x, partials_ok=True) may return an ops.PartialSum
     supports_residual = True   # forward(x, residual=h) may add its result to h itself and return None
 

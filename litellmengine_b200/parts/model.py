@@ -33,10 +33,19 @@ class Model:
     kernels and the cache are in the compute dtype (bfloat16 or float32); logits are float32.
     """
 
-    def __init__(self, plan: ModelPlan, dtype="bfloat16", device="cuda"):
+    WEIGHT_FORMATS = ("stored", "mxfp4")
+
+    def __init__(self, plan: ModelPlan, dtype="bfloat16", device="cuda", weight_format: str = "stored"):
+        """`weight_format` 'mxfp4': the matrices of the parts that can (`hold_in_4_bits`: softmax attention's projections, dense
+        feed-forwards) are taken to 4 bits with a scale per 32 values when they are loaded, and multiply rows of 8 bits."""
         plan.validate()
         self.plan = plan
         self.dtype = _compute_dtype(dtype)
+        if weight_format not in self.WEIGHT_FORMATS:
+            raise ValueError(f"weight_format {weight_format!r}: one of {self.WEIGHT_FORMATS}")
+        if weight_format != "stored" and self.dtype != torch.bfloat16:
+            raise ValueError("weights in 4 bits are for bfloat16 models")
+        self.weight_format = weight_format
         self.device = torch.device(device)
         self.blocks: List[Block] = [Block(b, plan.hidden_size, self.dtype, self.device) for b in plan.blocks]
         self.final_norm = lookup("norm", plan.final_norm.kind)(plan.final_norm, plan.hidden_size)
@@ -87,10 +96,15 @@ class Model:
         get = lambda n: fetch_tensor(source, n, params[n], self.dtype, self.device)
         have = set(source.names())
         self.embedding = get(p.embedding_name).contiguous()
+        held = 0
         for spec, block in zip(p.blocks, self.blocks):
             # a tensor that may be absent and is: the part is handed nothing for it
             block.load({n: get(f"{spec.weight_prefix}.{n}") for n, ps in block.parameters().items()
                         if not (ps.optional and f"{spec.weight_prefix}.{n}" not in have)})
+            if self.weight_format == "mxfp4":              # a layer's stored matrices are gone before the next one's come
+                held += sum(part.hold_in_4_bits() for part in block.parts() if hasattr(part, "hold_in_4_bits"))
+        if self.weight_format == "mxfp4" and not held:
+            raise ValueError("weight_format 'mxfp4': no part of this model holds its matrices in 4 bits")
         for norm, prefix in ((self.final_norm, p.final_norm_name), (self.embedding_norm, p.embedding_norm_name)):
             if norm is not None:
                 norm.load({name: get(self._norm_tensor(prefix, k, name)) for k, name in enumerate(norm.parameters())})
@@ -154,6 +168,9 @@ class Model:
                 for v in vars(part).values():
                     if isinstance(v, torch.Tensor) and v.dim() in (2, 3):
                         add(v)
+                    elif isinstance(v, ops.MxWeight):
+                        add(v.codes)
+                        add(v.scales)
         if self.rejoin is not None:
             for w in self.rejoin.matrices():
                 add(w)
@@ -230,5 +247,5 @@ def model_parameters(plan: ModelPlan) -> Dict[str, ParamSpec]:
     return Model(plan, dtype="float32", device="meta").parameters()
 
 
-def build_model(config, dtype="bfloat16", device="cuda") -> Model:
-    return Model(config.plan(), dtype=dtype, device=device)
+def build_model(config, dtype="bfloat16", device="cuda", weight_format: str = "stored") -> Model:
+    return Model(config.plan(), dtype=dtype, device=device, weight_format=weight_format)

@@ -21,6 +21,7 @@ class RMSNorm:
     accepts_partials = True    # `delta` may be an ops.PartialSum: the kernel adds the k-splits as it reads
     accepts_join = True        # and a PendingNormed with a `join`
     products_apply_it = True   # a small product may make this norm's output itself (ops.PendingRows)
+    makes_mx_rows = True       # `forward_mx` gives the output as rows of 8 bits, for products with weights in 4
     center = False             # what a kernel that applies this norm itself needs to know beside weight and eps
 
     def __init__(self, spec: NormSpec, size: int):
@@ -53,6 +54,10 @@ class RMSNorm:
             post = (delta.norm.weight, delta.norm.eps) if delta.norm is not None else None
             return ops.rmsnorm_sandwich(x, y, post, (self.weight, self.eps), out_dtype, rows=rows, join=delta.join)
         return ops.rmsnorm(x, self.weight, self.eps, out_dtype, delta=delta, rows=rows, write_sum=write_sum)
+
+    def forward_mx(self, x: torch.Tensor, delta=None) -> ops.MxRows:
+        """norm(x (+ delta)) as rows of 8 bits; x += delta in place."""
+        return ops.rmsnorm_mx(x, self.weight, self.eps, delta=delta, sum_out=x if delta is not None else None)
 
 
 @register_norm("layernorm")

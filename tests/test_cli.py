@@ -113,3 +113,11 @@ def test_run_prompt_hands_ids_to_the_engine_and_reads_its_new_ids_line(tmp_path)
     both = subprocess.run([sys.executable, os.path.join(root, "bin", "run_prompt"), "--model", str(tmp_path),
                            "--input-ids", "5", "--prompt", "x"], capture_output=True, text=True)
     assert both.returncode != 0 and "exactly one" in both.stderr
+
+
+def test_weight_format():
+    assert cli.parse_args(["--model", "m"]).weight_format == "stored"
+    assert cli.parse_args(["--model", "m", "--weight-format=mxfp4"]).weight_format == "mxfp4"
+    for argv in (["--weight-format", "int4"], ["--weight-format", "mxfp4", "--dtype", "float32"]):
+        with pytest.raises(cli.ArgError, match="--weight-format"):
+            cli.parse_args(["--model", "m"] + argv)

@@ -330,7 +330,7 @@ def test_a_wait_that_runs_out(T, N, K, gated):
         want = run()
         assert status.tolist() == [0, 0]
         run(waits=0)
-        assert status.tolist()[0] == 12
+        assert status.tolist()[0] == 9
         status.zero_()
         for _ in range(3):
             assert torch.equal(run(), want)
