@@ -690,7 +690,7 @@ static bool mg_pairs_pay(int T, int tiles, int ktiles, int sms) {
     const long long single = static_cast<long long>((T + 63) / 64) * tiles, pairs = static_cast<long long>((T + MP_NT - 1) / MP_NT) * ((tiles + 1) / 2);
     const int parts = mg_parts(single, ktiles, mg_slots(sms));
     const long long waves = (single * parts + 2 * sms - 1) / (2 * sms), rounds = (pairs + sms / 2 - 1) / (sms / 2);
-    return 36 * waves * ((ktiles + parts - 1) / parts) + 25 * parts > 28 * rounds * ktiles;
+    return (T + 63) / 64 > 65535 || 36 * waves * ((ktiles + parts - 1) / parts) + 25 * parts > 28 * rounds * ktiles;
 }
 
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO>

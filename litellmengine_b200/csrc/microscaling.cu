@@ -5,6 +5,7 @@
 // Everything is bound by memory: each value is read once and each code written once.  A lane holds eight neighbouring values
 // (16 or 32 bytes a load), a block's largest magnitude takes two exchanges between lanes, and the codes are the converter's.
 #include "microscaling.cuh"
+#include <type_traits>
 
 #define MX_THREADS 256
 
@@ -27,11 +28,26 @@ __global__ void __launch_bounds__(MX_THREADS) mx_rows_kernel(const T* __restrict
     pdl_begin();
     const MxSpan at = mx_span<U>(items, per_row);
     if (!at.there) return;                                        // whole warps
-    float v[U][8];
+    if constexpr (FAST && sizeof(T) == 2) {
+        uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) mx_load8<FAST>(x + at.row * K, at.col + u * 256, K, vec, v[u]);
+        for (int u = 0; u < U; ++u) {
+            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (at.col + u * 256 < K) mx_raw8(x + at.row * K + at.col + u * 256, raw[u]);
+        }
 #pragma unroll
-    for (int u = 0; u < U; ++u) mx_store_row8(v[u], at.col + u * 256 < kpad, at.row, at.col + u * 256, kpad, codes, scales);
+        for (int u = 0; u < U; ++u) {
+            float v[8];
+            mx_raw_values(raw[u], v);
+            mx_store_row8(v, mx_most8(raw[u]), at.col + u * 256 < kpad, at.row, at.col + u * 256, kpad, codes, scales);
+        }
+    } else {
+        float v[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx_load8<FAST>(x + at.row * K, at.col + u * 256, K, vec, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx_store_row8(v[u], mx_most8(v[u]), at.col + u * 256 < kpad, at.row, at.col + u * 256, kpad, codes, scales);
+    }
 }
 
 // ---- rows of 8 bits from act(gate) * up, sums and activation in 32 bits --------------------------------------------
@@ -67,91 +83,203 @@ __global__ void __launch_bounds__(MX_THREADS) mx_act_kernel(const T* __restrict_
         const int col = at.col + u * 256;
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[u][i] = col + i < inter ? mx_gated(a[u][i], b[u][i], act) : 0.0f;
-        mx_store_row8(a[u], col < kpad, at.row, col, kpad, codes, scales);
+        mx_store_row8(a[u], mx_most8(a[u]), col < kpad, at.row, col, kpad, codes, scales);
     }
 }
 
 // ---- rows of 8 bits from rmsnorm(x + delta) * w ---------------------------------------------------------------------
-// One block a row (sum_out may be x: a thread writes what it has read); the row stays in registers between the sum of squares and the codes, CH pieces of eight values a thread.
-template <typename TX, typename TD, int CH, bool FAST>
-__global__ void __launch_bounds__(1024) mx_norm_kernel(const TX* x, const TD* __restrict__ delta, const float* __restrict__ w,
-                                                       TX* sum_out, unsigned char* __restrict__ codes,
-                                                       unsigned char* __restrict__ scales, const int32_t* __restrict__ rows, int hidden, int kpad,
-                                                       float eps, int vec, int parts, long long part_stride) {
-    __shared__ float scratch[32];
-    if (FAST)                                                     // the weights are the model's: on their way before the wait
+// One block a row (sum_out may be x: a thread writes what it has read); the row stays in registers between the sum of squares and the
+// codes, CH pieces of eight values a thread.
+// A value that is a hair off falls to the other side of a border between two codes and comes out a whole step off, an eighth of it.  So
+// everything up to the codes carries what float32 leaves out, where memory bounds the kernel anyway: sums with their remainders, the
+// threads' squares added in 64 bits, the factor in two parts, products with their remainders, and a result rounded to odd (its last
+// bit says that something is beyond it), which makes the rounding to 8 bits the only one.
+__device__ __forceinline__ void mx_two_sum(float a, float b, float& sum, float& rest) {
+    sum = a + b;
+    const float c = sum - a;
+    rest += (a - (sum - c)) + (b - c);
+}
+// v * (ih + il) * g, v with its remainder, rounded to odd: towards zero, and a one as last bit where that is not the whole of it.
+__device__ __forceinline__ float mx_scaled_odd(float v, float rest, float ih, float il, float g) {
+    const float p = v * ih, pe = fmaf(v, ih, -p) + fmaf(rest, ih, v * il), q = p * g, qe = fmaf(pe, g, fmaf(p, g, -q));
+    const float hi = q + qe, lo = qe - (hi - q);
+    const int bits = __float_as_int(hi), odd = (bits + ((__float_as_int(lo) ^ bits) >> 31)) | 1;
+    return fabsf(lo) > 0.0f ? __int_as_float(odd) : hi;           // a NaN passes as it is
+}
+// The codes of a row whose values, with their remainders, the block's threads hold.  scratch: a double a warp, for this row only.
+template <int CH, bool FAST>
+__device__ __forceinline__ void mx_norm_row(float (&v)[CH][8], const float (&rest)[CH][8], const float* w, double* scratch, unsigned char* codes,
+                                            unsigned char* scales, size_t row, int hidden, int kpad, float eps, double per_value, int vec) {
+    float mine = 0.0f;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int col = (c * blockDim.x + threadIdx.x) * 8;
-            if (col < hidden) asm volatile("prefetch.global.L1 [%0];\n" ::"l"(w + col));
-        }
-    pdl_begin();
-    const size_t src = rows ? static_cast<size_t>(rows[blockIdx.x]) : blockIdx.x;
-    const TX* xr = x + src * hidden;
-    float v[CH][8], ss = 0.0f;
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int col = (c * blockDim.x + threadIdx.x) * 8;
-        mx_load8<FAST>(xr, col, hidden, vec, v[c]);
-        if (delta) {
-#pragma unroll 4
-            for (int p = 0; p < parts; ++p) {                     // the sublayer's product may come as its k-splits
-                float d[8];
-                mx_load8<FAST>(delta + src * hidden + p * part_stride, col, hidden, vec, d);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] += d[i];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
-        if (sum_out) mx_put8<FAST>(sum_out + src * hidden, col, hidden, vec, v[c]);
-    }
-    ss = warp_sum(ss);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = ss;
+        for (int i = 0; i < 8; ++i) mine = fmaf(v[c][i], v[c][i], mine);
+    mine = warp_sum(mine);                                        // many partial sums: their roundings average out; what few warps leave is added in 64 bits
+    const int lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+    if (lane == 0) scratch[threadIdx.x >> 5] = mine;
     __syncthreads();
-    ss = warp_sum((threadIdx.x & 31) < ((blockDim.x + 31) >> 5) ? scratch[threadIdx.x & 31] : 0.0f);
-    const float inv = 1.0f / sqrtf(ss / static_cast<float>(hidden) + eps);
+    double ss = lane < warps ? scratch[lane] : 0.0;
+    for (int o = 1; o < warps; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    ss = __shfl_sync(0xffffffffu, ss, 0);
+    const double mean = fma(ss, per_value, static_cast<double>(eps));
+    // 1 / sqrt(mean) in two parts: a first value, and one step of Newton's with its residue taken in full
+    const float mh = static_cast<float>(mean), ml = static_cast<float>(mean - static_cast<double>(mh)), ih = rsqrtf(mh);
+    const float sq = ih * ih, left = fmaf(-mh, sq, 1.0f) - fmaf(mh, fmaf(ih, ih, -sq), ml * sq), il = 0.5f * ih * left;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * blockDim.x + threadIdx.x) * 8;
         float g[8];
         mx_load8<FAST>(w, col, hidden, vec, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] * inv * g[i];
-        mx_store_row8(v[c], col < kpad, blockIdx.x, col, kpad, codes, scales);
+        for (int i = 0; i < 8; ++i) v[c][i] = mx_scaled_odd(v[c][i], rest[c][i], ih, il, g[i]);
+        mx_store_row8(v[c], mx_most8(v[c]), col < kpad, row, col, kpad, codes, scales);
+    }
+}
+template <typename TX, typename TD, int CH, bool FAST>
+__global__ void __launch_bounds__(1024) mx_norm_kernel(const TX* x, const TD* __restrict__ delta, const float* __restrict__ w,
+                                                       TX* sum_out, unsigned char* __restrict__ codes,
+                                                       unsigned char* __restrict__ scales, const int32_t* __restrict__ rows, int hidden, int kpad,
+                                                       float eps, double per_value, int vec, int parts, long long part_stride) {
+    __shared__ double scratch[32];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {                                // the weights are the model's: on their way before the wait
+        const int col = (c * blockDim.x + threadIdx.x) * 8;
+        if (col < hidden) asm volatile("prefetch.global.L1 [%0];\n" ::"l"(w + col));
+    }
+    pdl_begin();
+    const size_t src = rows ? static_cast<size_t>(rows[blockIdx.x]) : blockIdx.x;
+    const TX* xr = x + src * hidden;
+    float v[CH][8], rest[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        mx_load8<FAST>(xr, (c * blockDim.x + threadIdx.x) * 8, hidden, vec, v[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[c][i] = 0.0f;
+    }
+    if (delta)
+#pragma unroll 1
+        for (int p = 0; p < parts; ++p) {                         // the sublayer's product may come as its k-splits
+            float d[CH][8];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) mx_load8<FAST>(delta + src * hidden + p * part_stride, (c * blockDim.x + threadIdx.x) * 8, hidden, vec, d[c]);
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mx_two_sum(v[c][i], d[c][i], v[c][i], rest[c][i]);
+        }
+    if (sum_out)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) mx_put8<FAST>(sum_out + src * hidden, (c * blockDim.x + threadIdx.x) * 8, hidden, vec, v[c]);
+    mx_norm_row<CH, FAST>(v, rest, w, scratch, codes, scales, blockIdx.x, hidden, kpad, eps, per_value, vec);
+}
+
+// The same for many rows of whole, aligned pieces: a block takes every gridDim-th row, and the next one's values are on their way, each warp's own
+// in shared memory (nobody waits for another warp's), while it works on this one.
+template <typename TX, typename TD, int CH>
+__global__ void __launch_bounds__(256) mx_norm_rows_kernel(const TX* x, const TD* __restrict__ delta, const float* __restrict__ w, TX* sum_out,
+                                                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int n, int hidden,
+                                                           int kpad, float eps, double per_value) {
+    constexpr int XB = 256 * sizeof(TX), DB = 256 * sizeof(TD);   // bytes of a warp's 256 values and of what joins them
+    __shared__ double scratch[2][32];
+    extern __shared__ __align__(16) unsigned char next_s[];       // [2][CH][warps][XB + DB]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto at = [&](int buf, int c) { return next_s + ((buf * CH + c) * (blockDim.x >> 5) + warp) * (XB + DB); };
+    auto copy = [&](unsigned char* to, const void* from) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+    };
+    auto fetch = [&](int r, int buf) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = c * blockDim.x * 8 + warp * 256;
+            if (r < n) {
+#pragma unroll
+                for (int b = 0; b < XB; b += 512)
+                    if (col + static_cast<int>((b + lane * 16) / sizeof(TX)) < hidden)
+                        copy(at(buf, c) + b + lane * 16, reinterpret_cast<const char*>(x + static_cast<size_t>(r) * hidden + col) + b + lane * 16);
+                if (delta)
+#pragma unroll
+                    for (int b = 0; b < DB; b += 512)
+                        if (col + static_cast<int>((b + lane * 16) / sizeof(TD)) < hidden)
+                            copy(at(buf, c) + XB + b + lane * 16, reinterpret_cast<const char*>(delta + static_cast<size_t>(r) * hidden + col) + b + lane * 16);
+            }
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+    pdl_begin();
+    fetch(blockIdx.x, 0);
+    int buf = 0;
+#pragma unroll 1
+    for (int r = blockIdx.x; r < n; r += gridDim.x, buf ^= 1) {
+        __syncwarp();                                             // the block's own reads of two rows ago
+        fetch(r + gridDim.x, buf ^ 1);
+        asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+        __syncwarp();
+        float v[CH][8], rest[CH][8];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = rest[c][i] = 0.0f;
+            if (col < hidden) {
+                load8(reinterpret_cast<const TX*>(at(buf, c)) + lane * 8, v[c]);
+                if (delta) {
+                    float d[8];
+                    load8(reinterpret_cast<const TD*>(at(buf, c) + XB) + lane * 8, d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) mx_two_sum(v[c][i], d[i], v[c][i], rest[c][i]);
+                }
+                if (sum_out) store8(sum_out + static_cast<size_t>(r) * hidden + col, v[c]);
+            }
+        }
+        mx_norm_row<CH, true>(v, rest, w, scratch[buf], codes, scales, r, hidden, kpad, eps, per_value, 8);
     }
 }
 
 // ---- weights of 4 bits ----------------------------------------------------------------------------------------------
-// Rows of the tiles.  It does not invite the kernel behind it: products fetch weights before they wait for what is in front of them.
+// Rows of the tiles, U neighbouring ones a warp and 256 values of each: what a warp writes of a tile lies side by side (U times 64 bytes).  It
+// does not invite the kernel behind it: products fetch weights before they wait for what is in front of them.
 template <int U, bool FAST, typename T>
 __global__ void __launch_bounds__(MX_THREADS) mx_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ tiles,
                                                                unsigned char* __restrict__ scales, unsigned items, unsigned per_row, int N, int K, int ktiles,
                                                                int gated_rows, int vec) {
     pdl_wait();
-    const MxSpan at = mx_span<U>(items, per_row);                 // a row of the tiles
-    if (!at.there) return;
-    const long long row = at.row;
-    long long src = row;                                          // of the matrix; gated: [gate; up] of N rows each
-    bool real = row < N;
-    if (gated_rows) {
-        const long long f = (row >> 7) * 64 + (row & 63);
-        real = f < N;
-        src = (row & 64) ? N + f : f;
-    }
-    float v[U][8];
-#pragma unroll
-    for (int u = 0; u < U; ++u) mx_load8<FAST>(w + src * K, real ? at.col + u * 256 : K, K, vec, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int col = at.col + u * 256;
+    const unsigned item = blockIdx.x * (MX_THREADS / 32) + (threadIdx.x >> 5), group = item / per_row;
+    if (item >= items) return;
+    const int col = (item - group * per_row) * 256 + (threadIdx.x & 31) * 8;
+    const unsigned row = group * U;                               // of the tiles; gated: 64 rows of gate, 64 of up from [gate; up] of N rows each
+    const long long first = gated_rows ? (row >> 7) * 64LL + (row & 63) : row, there = N - first;
+    const T* from = w + (gated_rows && (row & 64) ? N + first : first) * K + col;
+    const bool whole = col < ktiles * MX_K;
+    unsigned char* to = tiles + ((static_cast<long long>(row >> 7) * ktiles + (col >> 7)) * 128 + (row & 127)) * 64 + (col & 127) / 2;
+    unsigned char* to_scales = scales + mx_scale_at(row, col / MX_BLOCK, ktiles);
+    auto store = [&](int u, const float (&v)[8], unsigned most) {
         unsigned word;
-        const uint2 c = mx_encode8<MX_E2M1>(v[u], word);
-        if (col < ktiles * MX_K) {
-            const long long tile = (row >> 7) * ktiles + (col >> 7);
-            *reinterpret_cast<unsigned*>(tiles + (tile * 128 + (row & 127)) * 64 + (col & 127) / 2) = c.x;
-            if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(row, col / MX_BLOCK, ktiles)) = word;
+        const uint2 c = mx_encode8<MX_E2M1>(v, most, word);
+        if (whole) {
+            *reinterpret_cast<unsigned*>(to + u * 64) = c.x;
+            if ((threadIdx.x & 15) == 0) *reinterpret_cast<unsigned*>(to_scales + u * 16) = word;
         }
+    };
+    if constexpr (FAST && sizeof(T) == 2) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (u < there && col < K) mx_raw8(from + static_cast<size_t>(u) * K, raw[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float v[8];
+            mx_raw_values(raw[u], v);
+            store(u, v, mx_most8(raw[u]));
+        }
+    } else {
+        float v[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx_load8<FAST>(from + (u < there ? static_cast<size_t>(u) * K : 0) - col, u < there ? col : K, K, vec, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) store(u, v[u], mx_most8(v[u]));
     }
 }
 
@@ -198,6 +326,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_values_kernel(const unsigned ch
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 #define MX_MOST_K (1 << 20)
+#define MX_NORM_ROWS 1024
 // How `rows` rows of n values are cut into warps' items of `u` pieces: four pieces where that leaves enough warps and wastes little.
 struct MxCut {
     int u;
@@ -269,14 +398,28 @@ static int mx_norm_launch(const void* x, const void* delta, const float* w, void
     const int kpad = mx_tiles(hidden) * MX_K;
     const int vec = part_stride % 8 ? 1 : mx_vec(mx_vec(mx_vec(hidden, x, sizeof(TX)), mx_vec(hidden, delta, sizeof(TD))),
                                                  mx_vec(mx_vec(hidden, w, 4), mx_vec(hidden, sum_out, sizeof(TX))));
-    // Few rows: a piece of eight values a thread, as many threads as that takes.  Many: blocks of up to 256 threads with up to four pieces
-    // each, so that more rows are on their way in an SM (4,096 x 4,096: XX us, with a piece a thread YY).
-    const int pieces = kpad / 8, most = n >= 1024 ? 256 : 1024, ch = pieces <= most ? 1 : pieces <= 2 * most ? 2 : 4;
+    // Many rows: blocks that fetch ahead.  Few: a piece of eight values a thread, as many threads as that takes.
+    const int pieces = kpad / 8;
     if (pieces > 4096) return LLM_REFUSED_SIZE;
+    if (n >= MX_NORM_ROWS && vec == 8 && parts == 1 && !rows && pieces <= 1024) {
+        const int ch = pieces <= 256 ? 1 : pieces <= 512 ? 2 : 4, threads = (pieces + ch * 32 - 1) / (ch * 32) * 32;
+        const size_t smem = static_cast<size_t>(2) * ch * threads * 8 * (sizeof(TX) + sizeof(TD));
+        auto kern = ch == 1 ? mx_norm_rows_kernel<TX, TD, 1> : ch == 2 ? mx_norm_rows_kernel<TX, TD, 2> : mx_norm_rows_kernel<TX, TD, 4>;
+        int dev = 0, sms = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return LLM_REFUSED_SIZE;
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return static_cast<int>(e);
+        const int per_sm = static_cast<int>(216 * 1024 / (smem + 1536)), fit = per_sm * threads > 1024 ? 1024 / threads : per_sm;
+        launch_pdl(kern, dim3(n < sms * fit ? n : sms * fit), dim3(threads), smem, s, static_cast<const TX*>(x), static_cast<const TD*>(delta), w,
+                   static_cast<TX*>(sum_out), static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), n, hidden, kpad, eps, 1.0 / hidden);
+        return launch_status();
+    }
+    const int ch = pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : 4;
     auto kern = vec == 8 ? (ch == 1 ? mx_norm_kernel<TX, TD, 1, true> : ch == 2 ? mx_norm_kernel<TX, TD, 2, true> : mx_norm_kernel<TX, TD, 4, true>)
                          : (ch == 1 ? mx_norm_kernel<TX, TD, 1, false> : ch == 2 ? mx_norm_kernel<TX, TD, 2, false> : mx_norm_kernel<TX, TD, 4, false>);
     launch_pdl(kern, dim3(n), dim3((pieces + ch * 32 - 1) / (ch * 32) * 32), 0, s, static_cast<const TX*>(x), static_cast<const TD*>(delta), w,
-               static_cast<TX*>(sum_out), static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), rows, hidden, kpad, eps, vec, parts, part_stride);
+               static_cast<TX*>(sum_out), static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), rows, hidden, kpad, eps, 1.0 / hidden, vec,
+               parts, part_stride);
     return launch_status();
 }
 
@@ -308,8 +451,14 @@ extern "C" int llm_mx_weight(const void* w, int dtype, void* tiles, void* scales
     if (N <= 0 || K <= 0 || K > MX_MOST_K || N > (1 << 24)) return LLM_REFUSED_SIZE;
     if (!aligned16(tiles) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
     const int ktiles = mx_tiles(K), vec = mx_vec(K, w, dtype == LLM_DT_F32 ? 4 : 2);
+    const long long rows = llm_mx_weight_tiles(N, is_gated) * 128LL;
     MxCut cut;
-    if (!mx_cut(llm_mx_weight_tiles(N, is_gated) * 128LL, ktiles * MX_K, &cut)) return LLM_REFUSED_SIZE;
+    cut.per_row = (ktiles + 1) / 2;
+    cut.u = rows * cut.per_row >= 32768 ? 4 : rows * cut.per_row >= 16384 ? 2 : 1;
+    const long long items = rows / cut.u * cut.per_row;
+    if (items > 0x7fffffffLL) return LLM_REFUSED_SIZE;
+    cut.items = static_cast<unsigned>(items);
+    cut.blocks = (cut.items + MX_THREADS / 32 - 1) / (MX_THREADS / 32);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     unsigned char *t = static_cast<unsigned char*>(tiles), *sc = static_cast<unsigned char*>(scales);
 #define F32(U, V) mx_weight_kernel<U, V, float>

@@ -84,12 +84,26 @@ __device__ __forceinline__ void mx_from_e4m3x4(unsigned r, float* v) {
     v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
 }
 
-// Eight neighbouring values a lane, four lanes a block, sixteen a tile's row: the lane's codes, and the four blocks' scales as one
-// word in every lane of the sixteen.  All lanes of a warp are here.
-template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned& word) {
+// Eight values as they lie in memory, read in one or two loads; their largest magnitude's bits (of float32), and themselves.
+__device__ __forceinline__ void mx_raw8(const bf16* p, uint4& raw) { raw = *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ unsigned mx_most8(const uint4& r) {    // two 16-bit magnitudes an instruction
+    const unsigned m = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+    return max(m & 0xffff0000u, m << 16);
+}
+__device__ __forceinline__ void mx_raw_values(const uint4& r, float (&v)[8]) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ unsigned mx_most8(const float (&v)[8]) {
     unsigned most = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max(most, mx_abs_bits(v[i]));
+    return most;
+}
+// Eight neighbouring values a lane, four lanes a block, sixteen a tile's row: the lane's codes, and the four blocks' scales as one
+// word in every lane of the sixteen.  most: of the lane's values.  All lanes of a warp are here.
+template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned most, unsigned& word) {
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
     const unsigned scale = mx_scale<FMT>(most);
@@ -103,10 +117,11 @@ template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[
     if constexpr (FMT == MX_E2M1) return make_uint2(mx_e2m1x8(q), 0u);
     else return make_uint2(mx_e4m3x4(q[0], q[1], q[2], q[3]), mx_e4m3x4(q[4], q[5], q[6], q[7]));
 }
+template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned& word) { return mx_encode8<FMT>(v, mx_most8(v), word); }
 // The row's eight values from column `col` on (a multiple of 8), which lane threadIdx.x % 16 == col / 8 % 16 holds, to rows of 8 bits.
-__device__ __forceinline__ void mx_store_row8(const float (&v)[8], bool there, size_t row, int col, int kpad, unsigned char* codes, unsigned char* scales) {
+__device__ __forceinline__ void mx_store_row8(const float (&v)[8], unsigned most, bool there, size_t row, int col, int kpad, unsigned char* codes, unsigned char* scales) {
     unsigned word;
-    const uint2 c = mx_encode8<MX_E4M3>(v, word);
+    const uint2 c = mx_encode8<MX_E4M3>(v, most, word);
     if (!there) return;
     *reinterpret_cast<uint2*>(codes + row * kpad + col) = c;
     if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(row, col / MX_BLOCK, kpad / MX_K)) = word;
@@ -161,16 +176,18 @@ static inline int mx_vec(int a, int b) { return a < b ? a : b; }
 
 // A gated feed-forward's middle, all of its kinds in one form without branches: g * sigmoid(z) * (u + shift), z = g * (alpha + beta g^2), g and u
 // clamped by `limit` (infinity: not).  silu: z = g; the tanh form of gelu is g * sigmoid(2 sqrt(2/pi) (g + 0.044715 g^3)), because
-// (1 + tanh(z / 2)) / 2 = sigmoid(z); the clamped form: z = 1.702 g, shift 1.  The fast exponential and division are off by about
-// (3 + |z|) 2^-24 of the result, which is rounded to 8 bits next.  With the precise ones and a branch a kind eight values took a
-// thread of the product's result 3,200 clocks, longer than the products.  A NaN stays one.
+// (1 + tanh(z / 2)) / 2 = sigmoid(z); the clamped form: z = 1.702 g, shift 1.  The division is the fast one and a step that squares its
+// error, so that the result is as near as float32 has it: a value that is off crosses a border between two codes more often.  With
+// the compiler's division and a branch a kind eight values took a thread of the product's result 3,200 clocks, longer than the products.
+// A NaN stays one.
 struct MxAct {
     float limit, alpha, beta, shift;
 };
 __device__ __forceinline__ float mx_gated(float g, float u, const MxAct& a) {
     g = g > a.limit ? a.limit : g;
     u = u > a.limit ? a.limit : u < -a.limit ? -a.limit : u;
-    return __fdividef(g, 1.0f + __expf(-g * (a.alpha + a.beta * g * g))) * (u + a.shift);
+    const float d = 1.0f + expf(-g * (a.alpha + a.beta * g * g)), s = __fdividef(1.0f, d), t = fmaf(-d, s, 1.0f);
+    return g * (fabsf(t) <= 1.0f ? fmaf(s, t, s) : s) * (u + a.shift);       // t is none of these where d is infinite or beyond what the fast form takes
 }
 static inline bool mx_act(int kind, float limit, MxAct* a) {
     if (kind < 0 || kind > 2 || (kind == 2 && !(limit > 0.0f))) return false;

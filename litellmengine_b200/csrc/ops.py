@@ -2401,20 +2401,32 @@ class MxWeight:
         self.gated = gated
         self.device = device
         # tiles of 128 rows: an even number, because products of many rows take two at a time; gated: 64 gate and 64 up rows
-        n, tiles = 2 * (((N // 2 + 127) // 128) if gated else (N + 255) // 256), (K + 127) // 128
-        self.codes = torch.empty((n, tiles, 128, 64), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((n, tiles, 512), dtype=torch.uint8, device=device)
+        self.tiles = n, tiles = 2 * (((N // 2 + 127) // 128) if gated else (N + 255) // 256), (K + 127) // 128
+        # one allocation: the codes, then the scales
+        self.buffer = torch.empty(n * tiles * (128 * 64 + 512), dtype=torch.uint8, device=device)
+        self.at = self.buffer.data_ptr()
+        self.scales_at = self.at + n * tiles * 128 * 64
+
+    @property
+    def codes(self) -> torch.Tensor:
+        n, tiles = self.tiles
+        return self.buffer[:n * tiles * 128 * 64].view(n, tiles, 128, 64)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        n, tiles = self.tiles
+        return self.buffer[n * tiles * 128 * 64:].view(n, tiles, 512)
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.buffer.numel()
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         N, K = self.shape
-        _here(self.codes)
+        _here(self.buffer)
         out = torch.empty((N, K), dtype=dtype, device=self.device)
-        _check(_mx_call("llm_mx_values")(self.codes.data_ptr(), self.scales.data_ptr(), 4, out.data_ptr(), _dt(out), N // 2 if self.gated else N, K,
-                                         int(self.gated), _stream()), "values of a weight in 4 bits")
+        _check(_mx_call("llm_mx_values")(self.at, self.scales_at, 4, out.data_ptr(), _dt(out), N // 2 if self.gated else N, K, int(self.gated),
+                                         _stream()), "values of a weight in 4 bits")
         return out
 
 
@@ -2426,8 +2438,7 @@ def mx_weight(weight: torch.Tensor, gated: bool = False) -> MxWeight:
     N, K = weight.shape
     dt = _dt(weight)
     made = MxWeight(N, K, gated, weight.device)
-    _check(_mx_call("llm_mx_weight")(weight.data_ptr(), dt, made.codes.data_ptr(), made.scales.data_ptr(), N // 2 if gated else N, K, int(gated),
-                                     _stream()), "mx_weight")
+    _check(_mx_call("llm_mx_weight")(weight.data_ptr(), dt, made.at, made.scales_at, N // 2 if gated else N, K, int(gated), _stream()), "mx_weight")
     return made
 
 
@@ -2500,9 +2511,9 @@ def _mx_operands(x, weight: MxWeight, gated: bool):
         raise KernelError("x and weight disagree on K")
     T, K = x.shape
     if made:
-        _here(x.buffer, weight.codes)
+        _here(x.buffer, weight.buffer)
         return x.buffer, None, 0, T, K
-    _here(x, weight.codes)
+    _here(x, weight.buffer)
     at, dt = x.data_ptr(), _dt(x)
     itself = (T <= MX_PLAIN_ROWS and dt == 1 and K % 8 == 0 and at % 16 == 0
               and (T <= MX_PLAIN_ROWS_CAPTURED or not torch.cuda.is_current_stream_capturing()))
@@ -2524,7 +2535,7 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
     else:
         y = torch.empty((T, N), dtype=out_dtype, device=weight.device)
         od = _dt(y)
-    _check(_mx_call("llm_linear_mx")(_ptr(rows), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(), y.data_ptr(), od,
+    _check(_mx_call("llm_linear_mx")(_ptr(rows), plain, dt, weight.at, weight.scales_at, y.data_ptr(), od,
                                      residual is not None, T, N, K, waits, _mx_status_ptr(weight.device), _stream()), "linear_mx")
     if plain is not None and rows is not None:
         _mx_count()
@@ -2538,8 +2549,8 @@ def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: flo
     rows, plain, dt, T, K = _mx_operands(x, weight, True)
     inter = weight.shape[0] // 2
     made = MxRows(T, inter, weight.device)
-    _check(_mx_call("llm_linear_mx_silu_mul")(_ptr(rows), plain, dt, weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                              made.buffer.data_ptr(), T, inter, K, act, limit, waits, _mx_status_ptr(weight.device), _stream()),
+    _check(_mx_call("llm_linear_mx_silu_mul")(_ptr(rows), plain, dt, weight.at, weight.scales_at, made.buffer.data_ptr(),
+                                              T, inter, K, act, limit, waits, _mx_status_ptr(weight.device), _stream()),
            "linear_silu_mul_mx")
     if plain is not None and rows is not None:
         _mx_count()

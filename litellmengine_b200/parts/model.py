@@ -169,8 +169,7 @@ class Model:
                     if isinstance(v, torch.Tensor) and v.dim() in (2, 3):
                         add(v)
                     elif isinstance(v, ops.MxWeight):
-                        add(v.codes)
-                        add(v.scales)
+                        add(v.buffer)
         if self.rejoin is not None:
             for w in self.rejoin.matrices():
                 add(w)

@@ -119,7 +119,8 @@ def half_step(n, fmt=8):
     return torch.maximum(n.abs() * 2.0 ** -4, s * 2.0 ** -10)
 
 
-@pytest.mark.parametrize("T,H", [(1, 4096), (3, 1), (2, 33), (130, 200), (257, 1450), (5, 8192), (2, 8200), (3, 20000), (1, 32768)])
+@pytest.mark.parametrize("T,H", [(1, 4096), (3, 1), (2, 33), (130, 200), (257, 1450), (5, 8192), (2, 8200), (3, 20000), (1, 32768), (1024, 8), (1100, 1032),
+                                 (3000, 2048), (1333, 4096), (1025, 8192), (1030, 1450)])
 @pytest.mark.parametrize("pending", ["none", "float32", "bfloat16", "parts"])
 def test_norm(T, H, pending):
     o, g = ops(), gen(T + H)
@@ -133,9 +134,10 @@ def test_norm(T, H, pending):
     elif pending != "none":
         delta = normal(g, T, H).to(getattr(torch, pending))
         total = x + delta.float()
-    v = total.to(F64)
+    # the stream is rounded after each addition; the norm is of what the sum is before that
+    v = x.to(F64) + (0 if delta is None else delta.parts.to(F64).sum(0) if pending == "parts" else delta.to(F64))
     n = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + 1e-6) * w.to(F64)
-    # sums of squares: at most 32 a thread, then 10 halvings; with root, division and two products less than 32 roundings of 2^-24 in all
+    # less than 32 roundings of 2^-24 in all
     near = half_step(n) + n.abs() * 32 * 2.0 ** -24
     out = torch.empty_like(x)
     before = x.clone()
@@ -145,9 +147,15 @@ def test_norm(T, H, pending):
     assert got.codes[:, H:].count_nonzero() == 0
     again = o.rmsnorm_mx(x, w, 1e-6, delta=delta, sum_out=x)      # in place
     assert torch.equal(x, total) and torch.equal(again.values(F32), got.values(F32))
+    if pending in ("float32", "bfloat16") and T < 1000:
+        cut = o.rmsnorm_mx(before[:3].contiguous(), w, 1e-6, delta=delta[:3].contiguous()).values(F32)
+        assert torch.equal(cut, got.values(F32)[:3])              # no row depends on the others
     rows = torch.tensor([T - 1, 0, T // 2, T // 2], dtype=torch.int32, device=DEV)
     picked = o.rmsnorm_mx(total, w, 1e-6, rows=rows).values(F32)
-    assert torch.equal(picked, o.rmsnorm_mx(total, w, 1e-6).values(F32)[rows.long()])
+    assert T > 1000 or torch.equal(picked, o.rmsnorm_mx(total, w, 1e-6).values(F32)[rows.long()])
+    n = total.to(F64)[rows.long()]
+    n = n * torch.rsqrt(n.square().mean(-1, keepdim=True) + 1e-6) * w.to(F64)
+    assert bool(((picked.to(F64) - n).abs() <= half_step(n) + n.abs() * 32 * 2.0 ** -24).all())
 
 
 def test_norm_of_16_bits_and_of_rows_that_are_not_finite():
