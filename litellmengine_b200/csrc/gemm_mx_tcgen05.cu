@@ -441,7 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     t5_fence_after();
     pdl_invite();                                                 // not before: tensor memory is taken
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
-    pdl_wait();
+    if (warp != 0) pdl_wait();                                    // weights are nobody's output
 
     if (warp == 0 || warp >= 10) {
         // Three threads feed: the weights (warp 0), the rows (10) and the scales (11).  Asking for a box takes a thread 80 clocks and a

@@ -2342,6 +2342,11 @@ def _here(*tensors) -> None:
 _mx_status: Dict[int, torch.Tensor] = {}
 
 
+def _mx_matrix(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """`torch.empty` of a matrix, in two thirds of the host's time."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def _mx_status_ptr(device: torch.device) -> int:
     t = _mx_status.get(device.index)
     if t is None:
@@ -2385,8 +2390,7 @@ class MxRows:
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         T, K = self.shape
         _here(self.buffer)
-        out = torch.empty((T, K), dtype=dtype, device=self.device)
-        at = self.buffer.data_ptr()
+        out, at = _mx_matrix(T, K, dtype, self.device), self.buffer.data_ptr()
         _check(_mx_call("llm_mx_values")(at, at + mx_padded_rows(T) * ((K + 127) // 128) * 128, 8, out.data_ptr(), _dt(out), T, K, 0, _stream()),
                "values of rows in 8 bits")
         return out
@@ -2406,6 +2410,7 @@ class MxWeight:
         self.buffer = torch.empty(n * tiles * (128 * 64 + 512), dtype=torch.uint8, device=device)
         self.at = self.buffer.data_ptr()
         self.scales_at = self.at + n * tiles * 128 * 64
+        self.status_at = _mx_status_ptr(device)      # of its products
 
     @property
     def codes(self) -> torch.Tensor:
@@ -2424,7 +2429,7 @@ class MxWeight:
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         N, K = self.shape
         _here(self.buffer)
-        out = torch.empty((N, K), dtype=dtype, device=self.device)
+        out = _mx_matrix(N, K, dtype, self.device)
         _check(_mx_call("llm_mx_values")(self.at, self.scales_at, 4, out.data_ptr(), _dt(out), N // 2 if self.gated else N, K, int(self.gated),
                                          _stream()), "values of a weight in 4 bits")
         return out
@@ -2465,14 +2470,15 @@ def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, delta=None, ro
         delta = delta.parts[0]
     _here(x, weight, delta, rows, sum_out)
     _i32(rows, "rows")
-    if x.dim() != 2 or x.shape[1] < 1:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise KernelError("rmsnorm_mx wants a matrix [T, H]")
-    T, H = x.shape
+    T, H = shape
     if weight.dtype != torch.float32 or weight.numel() != H:
         raise KernelError("norm weight must be float32 of the row length")
-    if delta is not None and delta.shape != x.shape:
+    if delta is not None and delta.shape != shape:
         raise KernelError("delta must have x's shape")
-    if sum_out is not None and (sum_out.shape != x.shape or sum_out.dtype != x.dtype or rows is not None):
+    if sum_out is not None and sum_out is not x and (sum_out.shape != shape or sum_out.dtype != x.dtype) or (sum_out is not None and rows is not None):
         raise KernelError("the sum goes to a tensor like x, and only where all rows are normalised")
     n = rows.numel() if rows is not None else T
     dt, dd = _dt(x), _dt(delta) if delta is not None else 0
@@ -2506,11 +2512,11 @@ def _mx_operands(x, weight: MxWeight, gated: bool):
     product's x."""
     if not isinstance(weight, MxWeight) or weight.gated != gated:
         raise KernelError("the microscaled product takes an MxWeight" + (" made with gated=True" if gated else " that is not a gated one"))
-    made = type(x) is MxRows
-    if len(x.shape) != 2 or x.shape[1] != weight.shape[1]:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != weight.shape[1]:
         raise KernelError("x and weight disagree on K")
-    T, K = x.shape
-    if made:
+    T, K = shape
+    if type(x) is MxRows:
         _here(x.buffer, weight.buffer)
         return x.buffer, None, 0, T, K
     _here(x, weight.buffer)
@@ -2533,10 +2539,10 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
             raise KernelError("the product joins a float32 residual of its shape")
         y, od = residual, 0
     else:
-        y = torch.empty((T, N), dtype=out_dtype, device=weight.device)
+        y = _mx_matrix(T, N, out_dtype, weight.device)
         od = _dt(y)
     _check(_mx_call("llm_linear_mx")(_ptr(rows), plain, dt, weight.at, weight.scales_at, y.data_ptr(), od,
-                                     residual is not None, T, N, K, waits, _mx_status_ptr(weight.device), _stream()), "linear_mx")
+                                     residual is not None, T, N, K, waits, weight.status_at, _stream()), "linear_mx")
     if plain is not None and rows is not None:
         _mx_count()
     return y
@@ -2550,7 +2556,7 @@ def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: flo
     inter = weight.shape[0] // 2
     made = MxRows(T, inter, weight.device)
     _check(_mx_call("llm_linear_mx_silu_mul")(_ptr(rows), plain, dt, weight.at, weight.scales_at, made.buffer.data_ptr(),
-                                              T, inter, K, act, limit, waits, _mx_status_ptr(weight.device), _stream()),
+                                              T, inter, K, act, limit, waits, weight.status_at, _stream()),
            "linear_silu_mul_mx")
     if plain is not None and rows is not None:
         _mx_count()
