@@ -337,9 +337,10 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 // The two CTAs of a cluster compute a tile of 256 features x NT tokens together (cta_group::2): each brings its own 128 features and half
 // of the tokens, and reads both halves.  The clusters are persistent and hold two accumulators, so that a tile's result is written under the
-// next one's products; 192 tokens leave room for both and for the scales of all stages in tensor memory.  Tiles are numbered token
+// next one's products; 192 tokens at most leave room for both and for two groups of scales in tensor
+// memory.  Tiles are numbered token
 // tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.
-#define MP_NT 192
+#define MP_NT 192                 // most tokens of a tile; a launch takes as many as waste least (mp_width)
 #define MP_STAGES 6
 #define MP_THREADS 384            // weights, products, 4 + 4 warps for the results, rows, scales
 #define MP_X_BYTES (MP_NT / 2 * MX_K)
@@ -407,7 +408,7 @@ __device__ __forceinline__ void mp_cluster_sync() {
 template <int MODE, typename TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linear_mx_pair_kernel(
     const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap ws_map,
-    const __grid_constant__ CUtensorMap xs_map, const __grid_constant__ CUtensorMap y_map, const MgArgs a, int token_tiles, int tiles) {
+    const __grid_constant__ CUtensorMap xs_map, const __grid_constant__ CUtensorMap y_map, const MgArgs a, int nt, int token_tiles, int tiles) {
     constexpr int CHUNK = MP_TURN / (MG_ROWS * sizeof(TO));       // tokens of a block
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
@@ -452,19 +453,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             unsigned long long* own = scales ? s_full : full;
             unsigned long long* free = scales ? s_empty : empty;
             const int ring = scales ? 2 : MP_STAGES, step = scales ? MP_QUAD : 1;
-            const unsigned bytes = 2 * (scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : MP_X_BYTES);      // of both CTAs
+            const unsigned bytes = 2 * (scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : nt / 2 * MX_K);      // of both CTAs
             int s = 0;
             unsigned phase = 1;                                   // a barrier that was never used passes for the phase before its first
             bool ok = true;
             for (int t = cluster; ok && t < tiles; t += clusters) {
-                const int tok0 = (t % token_tiles) * MP_NT, at = ((t / token_tiles) * 2 + static_cast<int>(rank)) * ktiles;
+                const int tok0 = (t % token_tiles) * nt, at = ((t / token_tiles) * 2 + static_cast<int>(rank)) * ktiles;
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; kb += step) {
                     if (!mg_wait(&free[s], phase, a.waits, &abort_flag, a.status)) { ok = false; break; }
                     if (rank == 0) t5_expect_tx(&own[s], bytes);
                     const unsigned bar = first + s * 8;
                     if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
-                    else if (warp == 10) mp_tma_3d(x_s + s * MP_X_BYTES, &x_map, 0, tok0 + static_cast<int>(rank) * (MP_NT / 2), kb, bar);
+                    else if (warp == 10) mp_tma_3d(x_s + s * MP_X_BYTES, &x_map, 0, tok0 + static_cast<int>(rank) * (nt / 2), kb, bar);
                     else {                                        // what stands behind the last tile of K is read and not used
                         mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at + kb, bar);
                         mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
@@ -480,12 +481,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
         if (rank == 0) {
             const unsigned lead = elect_one();
             const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024), sd = mg_scale_desc(s_s);
+            const unsigned idesc = mg_idesc(2 * MG_ROWS, nt, 0);
             int s = 0, n = 0, quad = 0;
             unsigned phase = 0;
             bool ok = true;
             for (int t = cluster; ok && t < tiles; t += clusters, ++n) {
                 const int buf = n & 1;
-                const unsigned off = ((t % token_tiles) * MP_NT % 128) / 32;        // the tile's first token in its piece of scales
+                const unsigned off = ((t % token_tiles) * nt % 128) / 32;        // the tile's first token in its piece of scales
                 if (n >= 2) ok = __all_sync(0xffffffffu, mp_wait_cluster(&acc_empty[buf], ((n >> 1) - 1) & 1, a.waits, &abort_flag, a.status));
                 t5_fence_after();
 #pragma unroll 1
@@ -507,7 +509,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             mp_mma_lead(lead, tmem + buf * MP_NT, wd + s * (MG_W_BYTES >> 4) + 2 * k, xd + s * (MP_X_BYTES >> 4) + 2 * k,
-                                        mg_idesc(2 * MG_ROWS, MP_NT, k), sc, sc + 4 + off, (k0 | q | k) ? 1u : 0u);
+                                        idesc | (static_cast<unsigned>(k) << 4) | (static_cast<unsigned>(k) << 29), sc, sc + 4 + off, (k0 | q | k) ? 1u : 0u);
                         mp_commit_lead(lead, &empty[s]);
                         if (++s == MP_STAGES) s = 0, phase ^= 1;
                     }
@@ -523,8 +525,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
         const unsigned acc_empty_first = mp_map_to(t5_smem(&acc_empty[0]), 0);
         int n = 0, turns = 0;
         for (int t = cluster; t < tiles; t += clusters, ++n) {
-            const int buf = n & 1, tok0 = (t % token_tiles) * MP_NT, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
-            const int toks = min(MP_NT, a.T - tok0);
+            const int buf = n & 1, tok0 = (t % token_tiles) * nt, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
+            const int toks = min(nt, a.T - tok0);
             bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
             ok = mp_all(ok, 1 + half);                            // the four warps meet below: they go on or leave together
             t5_fence_after();
@@ -680,17 +682,32 @@ static int mg_parts(long long tiles, int ktiles, int slots) {
     return best;
 }
 
+// How many tokens a pair's tile has: 192, or 128 where the rounds of all tiles take less with them.  A tile of K = 4,096 takes 10.1 us with 192,
+// 8.2 with 128, 7.4 with 64 (its weights' way to shared memory then takes longest): nt + 174.  Multiples of 64, because the products take the scales
+// of a tile's rows from an even column of tensor memory only.
+#define MP_BESIDE 174
+static int mp_width(int T, int tiles, int sms, long long* cost) {
+    int best = 0;
+    for (int nt = MP_NT; nt >= 128; nt -= 64) {
+        const long long all = static_cast<long long>((T + nt - 1) / nt) * ((tiles + 1) / 2), c = (all + sms / 2 - 1) / (sms / 2) * (nt + MP_BESIDE);
+        if (!best || c < *cost) best = nt, *cost = c;
+    }
+    return best;
+}
+
 // Whether more rows than 64 go to pairs of CTAs, or to tiles of 64 rows each of which reads the weights again but whose K may be cut.  By
 // the time that both take, in hundredths of a microsecond beside what they share: a wave of single CTAs 36 a tile of K and 25 a part, a round of
-// pairs 28.  Rows x K by N, us, single / pair: 100 x 4,096 by 4,096 8.5, 13.4; 256 11.3, 13.7; 320 16.3, 13.7; 700 29, 14.3; 160 x 4,096 by 6,144
-// 15.8, 13.5; 256 x 12,288 by 4,096 23.7, 29.7; 320 39.5, 29.8; 700 x 1,024 by 1,024 6.2, 7.1; 1,024 x 1,024 by 2,048 7.8, 7.7; 128 x 2,048 by
-// 12,288 11.2, 10.0; gated 128 x 4,096 by 2 x 12,288 36.5, 27.1 (64 rows: 21.5).
+// pairs with 192 tokens 28.  Rows x K by N, us, single / pair: 100 x 4,096 by 4,096 8.5, 13.4; 256 11.3, 13.7; 320 16.3, 13.7; 700 29, 14.3; 160 x
+// 4,096 by 6,144 15.8, 13.5; 256 x 12,288 by 4,096 23.7, 29.7; 320 39.5, 29.8; 700 x 1,024 by 1,024 6.2, 7.1; 1,024 x 1,024 by 2,048 7.8, 7.7;
+// 128 x 2,048 by 12,288 11.2, 10.0; gated 128 x 4,096 by 2 x 12,288 36.5, 27.1 (64 rows: 21.5).
 static bool mg_pairs_pay(int T, int tiles, int ktiles, int sms) {
     if (T <= 64) return false;
-    const long long single = static_cast<long long>((T + 63) / 64) * tiles, pairs = static_cast<long long>((T + MP_NT - 1) / MP_NT) * ((tiles + 1) / 2);
+    const long long single = static_cast<long long>((T + 63) / 64) * tiles;
     const int parts = mg_parts(single, ktiles, mg_slots(sms));
-    const long long waves = (single * parts + 2 * sms - 1) / (2 * sms), rounds = (pairs + sms / 2 - 1) / (sms / 2);
-    return (T + 63) / 64 > 65535 || 36 * waves * ((ktiles + parts - 1) / parts) + 25 * parts > 28 * rounds * ktiles;
+    const long long waves = (single * parts + 2 * sms - 1) / (2 * sms);
+    long long pairs = 0;
+    (void)mp_width(T, tiles, sms, &pairs);
+    return (T + 63) / 64 > 65535 || 36 * waves * ((ktiles + parts - 1) / parts) + 25 * parts > 28 * pairs * ktiles / (MP_NT + MP_BESIDE);
 }
 
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO>
@@ -717,8 +734,11 @@ static int mg_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
 template <int MODE, typename TO>
 static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStream_t s) {
     CUtensorMap w_map, x_map, ws_map, xs_map, y_map = {};
-    const int padded = static_cast<int>(mx_padded_rows(a.T)), stored = (tiles + 1) / 2 * 2;
-    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, MP_NT / 2, 1) ||
+    const int padded = static_cast<int>(mx_padded_rows(a.T)), stored = (tiles + 1) / 2 * 2, dev = mg_device();
+    if (dev < 0 || mg_sms(dev) < 2) return LLM_REFUSED_SIZE;
+    long long cost = 0;
+    const int nt = mp_width(a.T, tiles, mg_sms(dev), &cost);
+    if (!mg_weight_map(&w_map, w, static_cast<long long>(stored) * a.ktiles * MG_ROWS) || !mg_rows_map(&x_map, x, padded, a.ktiles, nt / 2, 1) ||
         !mg_scales_map(&ws_map, a.w_scales, stored, a.ktiles, MP_QUAD, 0) || !mg_scales_map(&xs_map, a.x_scales, padded / 128, a.ktiles, MP_QUAD, 2))
         return LLM_REFUSED_SIZE;
     if (MODE != MG_GATED) {                                       // [T, N] in boxes of 8 KB, 128 values wide
@@ -735,14 +755,12 @@ static int mp_launch(const void* w, int tiles, const void* x, MgArgs a, cudaStre
     static_assert(2 * MP_NT + 2 * MP_S_COLS <= 512, "tensor memory");
     auto kern = linear_mx_pair_kernel<MODE, TO>;
     static bool had[MG_DEVICES];
-    const int dev = mg_device();
-    if (dev < 0) return LLM_REFUSED_SIZE;
     if (const int rc = mg_allow(kern, smem, dev, had)) return rc;
-    const long long token_tiles = (a.T + MP_NT - 1) / MP_NT, all = token_tiles * (stored / 2);
+    const long long token_tiles = (a.T + nt - 1) / nt, all = token_tiles * (stored / 2);
     const int slots = mg_sms(dev) / 2;
-    if (slots <= 0 || all > (1LL << 30)) return LLM_REFUSED_SIZE;
+    if (all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
-    launch_pdl(kern, dim3(2 * clusters), dim3(MP_THREADS), smem, s, w_map, x_map, ws_map, xs_map, y_map, a, static_cast<int>(token_tiles), static_cast<int>(all));
+    launch_pdl(kern, dim3(2 * clusters), dim3(MP_THREADS), smem, s, w_map, x_map, ws_map, xs_map, y_map, a, nt, static_cast<int>(token_tiles), static_cast<int>(all));
     return launch_status();
 }
 template <int MODE, typename TO> static int mg_rows(const void* w, int tiles, const void* x, const MgArgs& a, cudaStream_t s) {
@@ -808,4 +826,11 @@ extern "C" int llm_linear_mx_silu_mul(void* rows, const void* plain, int dtype, 
     a.out_kpad = tiles * 64;
     a.act = form;
     return mg_rows<MG_GATED, float>(w, tiles, rows, a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// How a product of T rows of 8 bits runs: tokens of a pair's tile, or minus those of a single CTA's.
+extern "C" int llm_linear_mx_way(int T, int N, int K, int is_gated, int sms) {
+    const int tiles = is_gated ? 2 * ((N + 127) / 128) : (N + MG_ROWS - 1) / MG_ROWS;
+    long long cost = 0;
+    return mg_pairs_pay(T, tiles, mx_tiles(K), sms) ? mp_width(T, tiles, sms, &cost) : T <= 16 ? -16 : T <= 32 ? -32 : -64;
 }

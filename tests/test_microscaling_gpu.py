@@ -249,6 +249,45 @@ def test_gated_product(N, K, activation, limit):
     assert o.stream_status(torch.device(DEV)).tolist() == [0, 0]
 
 
+def way(T, N, K, gated=False):
+    o = ops()
+    f = o._fn("microscaling", "llm_linear_mx_way", [o.c_int] * 5)
+    return f(T, N, K, int(gated), torch.cuda.get_device_properties(0).multi_processor_count)
+
+
+@pytest.mark.parametrize("T,N,K,tokens", [(2000, 2501, 1358, 192), (6013, 1003, 264, 192), (1500, 3000, 130, 128), (1201, 4104, 257, 192), (800, 4000, 2000, 128), (500, 4096, 1032, 128),
+                                          (256, 12288, 520, 128), (90, 20000, 1358, 128), (130, 20000, 4104, 192), (577, 4096, 4096, 192)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_pairs(T, N, K, tokens, gated):
+    """Tiles of pairs of CTAs of every width, with ragged rows, features and K, rows whose scales begin in every word of a piece."""
+    o, g = ops(), gen(T + N + K)
+    n = N // 2 if gated else N
+    W = o.mx_weight(normal(g, 2 * n if gated else n, K) * K ** -0.5, gated=gated)
+    w = W.values(F32)
+    x = normal(g, T, K) * torch.exp2(torch.randint(-3, 4, (T, 1), generator=g, device=DEV).float())      # every row its own scales
+    X = o.mx_rows(x)
+    v = X.values(F32)
+    assert gated or way(T, n, K) == tokens
+    sums, off = v.to(F64) @ w.to(F64).T, (K / 32 + 24) * 2.0 ** -23 * carried(v, w)
+    if gated:
+        gate, up = sums[:, :n], sums[:, n:]
+        want = middle(gate, up, 0, 0)
+        slack = (32 * 2.0 ** -24 * (gate.abs() + 1) * (up.abs() + 1) + 1.2 * off[:, :n] * (up.abs() + 1) + 1.2 * off[:, n:] * (gate.abs() + 1))
+        got = o.linear_silu_mul_mx(X, W)
+        assert bool(((got.values(F32).to(F64) - want).abs() <= torch.maximum(half_step(want), half_step(want.abs() + slack)) + slack).all())
+        return
+    got = o.linear_mx(X, W)
+    assert bool(((got.to(F64) - sums).abs() <= off).all())
+    assert torch.equal(o.linear_mx(X, W, BF16), got.to(BF16))
+    stream = normal(g, T, n)
+    total = stream + got
+    assert torch.equal(o.linear_mx(X, W, residual=stream), total)
+    room = torch.full((T + 2, n), 7.0, device=DEV)                # nothing beyond the result's rows is written
+    room[1:-1].zero_()
+    o.linear_mx(X, W, residual=room[1:-1])
+    assert torch.equal(room[1:-1], got) and bool((room[0] == 7).all()) and bool((room[-1] == 7).all())
+
+
 def test_scales_that_are_far_apart():
     """Blocks whose scales differ by up to 2^60 in one row: every product's scale is its own."""
     o, g = ops(), gen(5)
