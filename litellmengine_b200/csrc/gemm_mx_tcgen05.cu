@@ -6,10 +6,10 @@
 //
 // The weights are the left operand (128 features a tile), the tokens the right one (NT of them), so that no lane is spent on tokens
 // that are not there.  A stage is 128 values of K: a box of the weight's tile (8 KB; the copy engine spreads its 4-bit codes over
-// 16 KB, sixteen of them and eight bytes of nothing, as the products read them), a box of the rows, and the pieces of both operands'
-// scales, which the tensor core copies to its own memory in front of the stage's four products.
-// Roles: warp 0 feeds the copy engine, warp 1 issues, warps 2 to 5 take the sums; all six write the result.  Waits are bounded: one that
-// runs out sets status code 9, and the feeding thread waits for its last copies before the CTA ends.
+// 16 KB, sixteen of them and eight bytes of nothing, as the products read them, and counts the 8 KB on its barrier), a box of the rows, and
+// the pieces of both operands' scales, which the tensor core copies to its own memory in front of the stage's four products.
+// Roles here: warp 0 feeds the weights and their scales, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and theirs; all of them write
+// the result.  Waits are bounded: one that runs out sets status code 9, and what is in flight lands before the CTA ends.
 //   * Few rows: bytes bound the product.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the
 //     parts' order; nothing is left for another kernel and no result depends on timing.  The first weights are on their way before the
 //     CTA waits for the kernel in front.
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     pdl_invite();                                                 // not before: this CTA's tensor memory is taken
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
 
-    int issued = 0;                                               // stages, or groups, that were asked for, in the threads that ask
+    int issued = 0;                                               // stages that were asked for, in the thread that asks
     if (warp == 0) {
         if (lane == 0) {
             int s = early % WS;
@@ -150,7 +150,6 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 t5_expect_tx(&g_full[g & 1], G * X_BYTES + S_BYTES);
                 mg_tma_3d(to, &x_map, 0, tok0, kb0 + g * G, &g_full[g & 1]);
                 t5_tma_2d(to + G * X_BYTES + S_BYTES, &xs_map, 0, (tok0 / 128) * a.ktiles + kb0 + g * G, &g_full[g & 1]);
-                issued = g + 1;
             }
         }
         __syncwarp();
@@ -188,7 +187,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         if (ok) t5_commit_lead(lead, &acc_full);
     } else {
         pdl_wait();
-        if constexpr (PLAIN) {                                    // warps 2 to 6; rows beyond T keep what stands there, nobody minds
+        if constexpr (PLAIN) {                                    // warps 2 to 10; rows beyond T keep what stands there, nobody minds
             // A warp takes two stages of a row at a time, sixteen lanes each, and has the next group's values on their way while it makes this one's.
             static_assert(G % 2 == 0, "stages go in pairs");
             constexpr int BATCH = (NT * G / 2 + MG_MAKERS - 1) / MG_MAKERS;       // units of a group that a warp has at most
@@ -235,18 +234,18 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
             }
         }
         if (warp < 6) {
-        const int quarter = warp & 3, row = quarter * 32 + lane;
-        const bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full, 0, a.waits, &abort_flag, a.status));
-        t5_fence_after();
-        if (ok)
+            const int quarter = warp & 3, row = quarter * 32 + lane;
+            const bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full, 0, a.waits, &abort_flag, a.status));
+            t5_fence_after();
+            if (ok)
 #pragma unroll 1
-            for (int c = 0; c < NT / 16; ++c) {
-                unsigned r[16];
-                t5_ld16(tmem + (static_cast<unsigned>(quarter * 32) << 16) + 16 * c, r);
-                t5_wait_ld();
+                for (int c = 0; c < NT / 16; ++c) {
+                    unsigned r[16];
+                    t5_ld16(tmem + (static_cast<unsigned>(quarter * 32) << 16) + 16 * c, r);
+                    t5_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sums[(16 * c + i) * MG_ROWS + row] = __uint_as_float(r[i]);
-            }
+                    for (int i = 0; i < 16; ++i) sums[(16 * c + i) * MG_ROWS + row] = __uint_as_float(r[i]);
+                }
         }
     }
     t5_fence_before();
@@ -337,9 +336,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 // The two CTAs of a cluster compute a tile of 256 features x NT tokens together (cta_group::2): each brings its own 128 features and half
 // of the tokens, and reads both halves.  The clusters are persistent and hold two accumulators, so that a tile's result is written under the
-// next one's products; 192 tokens at most leave room for both and for two groups of scales in tensor
-// memory.  Tiles are numbered token
-// tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.
+// next one's products; 192 tokens at most leave room for both and for two groups of scales in tensor memory.  Tiles are numbered token tile
+// fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.
 #define MP_NT 192                 // most tokens of a tile; a launch takes as many as waste least (mp_width)
 #define MP_STAGES 6
 #define MP_THREADS 384            // weights, products, 4 + 4 warps for the results, rows, scales

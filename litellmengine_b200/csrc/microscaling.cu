@@ -245,12 +245,12 @@ __global__ void __launch_bounds__(MX_THREADS) mx_weight_kernel(const T* __restri
                                                                int gated_rows, int vec) {
     pdl_wait();
     const unsigned item = blockIdx.x * (MX_THREADS / 32) + (threadIdx.x >> 5), group = item / per_row;
-    if (item >= items) return;
+    const bool mine = item < items;                               // whole warps
     const int col = (item - group * per_row) * 256 + (threadIdx.x & 31) * 8;
     const unsigned row = group * U;                               // of the tiles; gated: 64 rows of gate, 64 of up from [gate; up] of N rows each
-    const long long first = gated_rows ? (row >> 7) * 64LL + (row & 63) : row, there = N - first;
+    const long long first = gated_rows ? (row >> 7) * 64LL + (row & 63) : row, there = mine ? N - first : 0;
     const T* from = w + (gated_rows && (row & 64) ? N + first : first) * K + col;
-    const bool whole = col < ktiles * MX_K;
+    const bool whole = mine && col < ktiles * MX_K;
     unsigned char* to = tiles + ((static_cast<long long>(row >> 7) * ktiles + (col >> 7)) * 128 + (row & 127)) * 64 + (col & 127) / 2;
     unsigned char* to_scales = scales + mx_scale_at(row, col / MX_BLOCK, ktiles);
     auto store = [&](int u, const float (&v)[8], unsigned most) {
@@ -281,6 +281,8 @@ __global__ void __launch_bounds__(MX_THREADS) mx_weight_kernel(const T* __restri
 #pragma unroll
         for (int u = 0; u < U; ++u) store(u, v[u], mx_most8(v[u]));
     }
+    __syncthreads();
+    if (threadIdx.x == 0) __threadfence();                        // all of the block's codes are there for a product that reads them before its wait
 }
 
 // ---- the values that codes stand for --------------------------------------------------------------------------------

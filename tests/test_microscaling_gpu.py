@@ -365,7 +365,8 @@ def test_a_feed_forward_of_them_captured_and_replayed(T):
     assert torch.equal(feed_forward(o, h, delta, norm_w, gate_up, down, torch.empty_like(out)), got)
 
 
-@pytest.mark.parametrize("T,N,K,gated", [(4, 4096, 4096, False), (100, 256, 2048, False), (300, 512, 4096, False), (4, 512, 2048, True)])
+@pytest.mark.parametrize("T,N,K,gated", [(4, 4096, 4096, False), (100, 256, 2048, False), (300, 512, 4096, False), (4, 512, 2048, True),
+                                         (2000, 4096, 1024, False), (700, 4001, 1024, False), (2000, 4096, 640, True)])
 def test_a_wait_that_runs_out(T, N, K, gated):
     """Waits without tries: the status is set, the copies land before the blocks end, and the next products are right."""
     o, g = ops(), gen(9)
