@@ -595,14 +595,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                 for (int c = 16 * half; c < toks; c += 32) {
                     unsigned r[16];
                     t5_ld16(acc + c, r);
+                    float old[16];
+                    if (MODE == MG_ADD)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) old[i] = f < a.N && c + i < toks ? to_f32(y[static_cast<size_t>(c + i) * a.N]) : 0.0f;
                     t5_wait_ld();
                     if (f < a.N)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if (c + i < toks) {
-                                TO* to = y + static_cast<size_t>(c + i) * a.N;
-                                *to = from_f32<TO>(MODE == MG_ADD ? __uint_as_float(r[i]) + to_f32(*to) : __uint_as_float(r[i]));
-                            }
+                            if (c + i < toks)
+                                y[static_cast<size_t>(c + i) * a.N] = from_f32<TO>(MODE == MG_ADD ? old[i] + __uint_as_float(r[i]) : __uint_as_float(r[i]));
                 }
             }
             t5_fence_before();
