@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
             int s = early % WS;
             unsigned phase = early == WS ? 0 : 1;                 // a barrier that was never used passes for the phase before its first
             issued = early;
+            if (early < kbs) pdl_wait();                          // the rest waits for products anyway, and these for the kernel in front: no bound on that
 #pragma unroll 1
             for (int kb = early; kb < kbs; ++kb) {
                 const int g = kb / G;
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(g_s, 16, 1024), sd = mg_scale_desc(g_s + G * X_BYTES);
         const unsigned off = tok0 % 128 / 32;                     // the tile's first token in its piece of scales
         bool ok = true;
+        pdl_wait();                                               // the bounded waits below are not for the kernel in front
         int s = 0;
         unsigned phase = 0;
 #pragma unroll 1
@@ -455,10 +457,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             int s = 0;
             unsigned phase = 1;                                   // a barrier that was never used passes for the phase before its first
             bool ok = true;
+            int ahead = warp == 0 ? MP_STAGES : -1;               // boxes of weights that do not wait for the kernel in front
             for (int t = cluster; ok && t < tiles; t += clusters) {
                 const int tok0 = (t % token_tiles) * nt, at = ((t / token_tiles) * 2 + static_cast<int>(rank)) * ktiles;
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; kb += step) {
+                    if (ahead >= 0 && ahead-- == 0) pdl_wait();   // the bounded waits below are not for that kernel
                     if (!mg_wait(&free[s], phase, a.waits, &abort_flag, a.status)) { ok = false; break; }
                     if (rank == 0) t5_expect_tx(&own[s], bytes);
                     const unsigned bar = first + s * 8;

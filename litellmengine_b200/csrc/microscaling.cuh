@@ -176,8 +176,8 @@ static inline int mx_vec(int a, int b) { return a < b ? a : b; }
 
 // A gated feed-forward's middle, all of its kinds in one form without branches: g * sigmoid(z) * (u + shift), z = g * (alpha + beta g^2), g and u
 // clamped by `limit` (infinity: not).  silu: z = g; the tanh form of gelu is g * sigmoid(2 sqrt(2/pi) (g + 0.044715 g^3)), because
-// (1 + tanh(z / 2)) / 2 = sigmoid(z); the clamped form: z = 1.702 g, shift 1.  The division is the fast one and a step that squares its
-// error, so that the result is as near as float32 has it: a value that is off crosses a border between two codes more often.  With
+// (1 + tanh(z / 2)) / 2 = sigmoid(z); the clamped form: z = 1.702 g, shift 1.  The division is the fast one and one of Newton's steps, which
+// squares its error, so that the result is as near as float32 has it: a value that is off crosses a border between two codes more often.  With
 // the compiler's division and a branch a kind eight values took a thread of the product's result 3,200 clocks, longer than the products.
 // A NaN stays one.
 struct MxAct {

@@ -2408,19 +2408,17 @@ class MxWeight:
         self.tiles = n, tiles = 2 * (((N // 2 + 127) // 128) if gated else (N + 255) // 256), (K + 127) // 128
         # one allocation: the codes, then the scales
         self.buffer = torch.empty(n * tiles * (128 * 64 + 512), dtype=torch.uint8, device=device)
-        self.at = self.buffer.data_ptr()
-        self.scales_at = self.at + n * tiles * 128 * 64
-        self.status_at = _mx_status_ptr(device)      # of its products
+        self.scales_behind = n * tiles * 128 * 64
 
     @property
     def codes(self) -> torch.Tensor:
         n, tiles = self.tiles
-        return self.buffer[:n * tiles * 128 * 64].view(n, tiles, 128, 64)
+        return self.buffer[:self.scales_behind].view(n, tiles, 128, 64)
 
     @property
     def scales(self) -> torch.Tensor:
         n, tiles = self.tiles
-        return self.buffer[n * tiles * 128 * 64:].view(n, tiles, 512)
+        return self.buffer[self.scales_behind:].view(n, tiles, 512)
 
     @property
     def nbytes(self) -> int:
@@ -2429,8 +2427,8 @@ class MxWeight:
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         N, K = self.shape
         _here(self.buffer)
-        out = _mx_matrix(N, K, dtype, self.device)
-        _check(_mx_call("llm_mx_values")(self.at, self.scales_at, 4, out.data_ptr(), _dt(out), N // 2 if self.gated else N, K, int(self.gated),
+        out, at = _mx_matrix(N, K, dtype, self.device), self.buffer.data_ptr()
+        _check(_mx_call("llm_mx_values")(at, at + self.scales_behind, 4, out.data_ptr(), _dt(out), N // 2 if self.gated else N, K, int(self.gated),
                                          _stream()), "values of a weight in 4 bits")
         return out
 
@@ -2443,7 +2441,8 @@ def mx_weight(weight: torch.Tensor, gated: bool = False) -> MxWeight:
     N, K = weight.shape
     dt = _dt(weight)
     made = MxWeight(N, K, gated, weight.device)
-    _check(_mx_call("llm_mx_weight")(weight.data_ptr(), dt, made.at, made.scales_at, N // 2 if gated else N, K, int(gated), _stream()), "mx_weight")
+    at = made.buffer.data_ptr()
+    _check(_mx_call("llm_mx_weight")(weight.data_ptr(), dt, at, at + made.scales_behind, N // 2 if gated else N, K, int(gated), _stream()), "mx_weight")
     return made
 
 
@@ -2463,7 +2462,8 @@ def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, delta=None, ro
                sum_out: Optional[torch.Tensor] = None) -> MxRows:
     """rmsnorm(x (+ delta)) * weight over the last dim, in 32-bit, as rows of 8 bits.  `delta` (x's shape, float32 or bfloat16) may
     be a `PartialSum`, whose k-splits are added as they are read.  `sum_out` (like x, may be x itself) receives x + delta: the
-    residual stream from then on.  `rows` (int32) selects which rows are normalised; it excludes `sum_out`."""
+    residual stream from then on.  `rows` (int32) selects which rows are normalised; it excludes `sum_out`.  A row whose sum of
+    squares is beyond float32 comes out as NaN."""
     parts, part_stride = 1, 0
     if isinstance(delta, PartialSum):
         parts, part_stride = delta.parts.shape[0], delta.parts.stride(0)
@@ -2519,6 +2519,8 @@ def _mx_operands(x, weight: MxWeight, gated: bool):
     if type(x) is MxRows:
         _here(x.buffer, weight.buffer)
         return x.buffer, None, 0, T, K
+    if not isinstance(x, torch.Tensor):
+        raise KernelError("the microscaled product takes rows of 8 bits or a matrix")
     _here(x, weight.buffer)
     at, dt = x.data_ptr(), _dt(x)
     itself = (T <= MX_PLAIN_ROWS and dt == 1 and K % 8 == 0 and at % 16 == 0
@@ -2541,8 +2543,9 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
     else:
         y = _mx_matrix(T, N, out_dtype, weight.device)
         od = _dt(y)
-    _check(_mx_call("llm_linear_mx")(_ptr(rows), plain, dt, weight.at, weight.scales_at, y.data_ptr(), od,
-                                     residual is not None, T, N, K, waits, weight.status_at, _stream()), "linear_mx")
+    at = weight.buffer.data_ptr()
+    _check(_mx_call("llm_linear_mx")(_ptr(rows), plain, dt, at, at + weight.scales_behind, y.data_ptr(), od,
+                                     residual is not None, T, N, K, waits, _mx_status_ptr(weight.device), _stream()), "linear_mx")
     if plain is not None and rows is not None:
         _mx_count()
     return y
@@ -2555,8 +2558,9 @@ def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: flo
     rows, plain, dt, T, K = _mx_operands(x, weight, True)
     inter = weight.shape[0] // 2
     made = MxRows(T, inter, weight.device)
-    _check(_mx_call("llm_linear_mx_silu_mul")(_ptr(rows), plain, dt, weight.at, weight.scales_at, made.buffer.data_ptr(),
-                                              T, inter, K, act, limit, waits, weight.status_at, _stream()),
+    at = weight.buffer.data_ptr()
+    _check(_mx_call("llm_linear_mx_silu_mul")(_ptr(rows), plain, dt, at, at + weight.scales_behind, made.buffer.data_ptr(),
+                                              T, inter, K, act, limit, waits, _mx_status_ptr(weight.device), _stream()),
            "linear_silu_mul_mx")
     if plain is not None and rows is not None:
         _mx_count()
@@ -2663,9 +2667,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     keeps its product in true float32 (no TF32), whatever x is: up to 16 rows in the engine's own streaming kernel, more rows of large matrices
     on the tensor cores as sums of three bfloat16 values each, as near as float32 sums.  bfloat16 weights may be read before the
     kernel in front of the product in the stream has finished (they are nobody's output); float32 ones are not.  A weight in 4
-    bits (`MxWeight`) goes to `linear_mx`, which also takes `MxRows`."""
+    bits (`MxWeight`) goes to `linear_mx`, which also takes `MxRows` (their result is bfloat16 without an `out_dtype`)."""
     if isinstance(weight, MxWeight):
-        return linear_mx(x, weight, out_dtype or torch.bfloat16)
+        return linear_mx(x, weight, out_dtype or getattr(x, "dtype", torch.bfloat16))
     if isinstance(x, PendingRows):
         return linear_small(x, weight, out_dtype or x.dtype)
     _dev(x, weight)

@@ -11,7 +11,7 @@ from ..weights.loader import ParamSpec, WeightSource, check_source, fetch_tensor
 from .block import Block, streams_norm
 from .context import StageContext
 from .norms import PendingSum
-from .registry import lookup
+from .registry import lookup, speaks_for_forward
 from .rejoin import REJOINS, AddedEmbedding
 
 
@@ -102,7 +102,7 @@ class Model:
             block.load({n: get(f"{spec.weight_prefix}.{n}") for n, ps in block.parameters().items()
                         if not (ps.optional and f"{spec.weight_prefix}.{n}" not in have)})
             if self.weight_format == "mxfp4":              # a layer's stored matrices are gone before the next one's come
-                held += sum(part.hold_in_4_bits() for part in block.parts() if hasattr(part, "hold_in_4_bits"))
+                held += sum(part.hold_in_4_bits() for part in block.parts() if speaks_for_forward(part, "hold_in_4_bits"))
         if self.weight_format == "mxfp4" and not held:
             raise ValueError("weight_format 'mxfp4': no part of this model holds its matrices in 4 bits")
         for norm, prefix in ((self.final_norm, p.final_norm_name), (self.embedding_norm, p.embedding_norm_name)):

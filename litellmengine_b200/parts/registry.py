@@ -38,6 +38,11 @@ of the one product that reads its input and whether that is a gate/up pair.  The
 hands to that product.  Both are read with `speaks_for_forward`: a class that derives from such a part and has a forward of its own
 says so again or is called as any other.
 
+A mixer or feed-forward whose forward gives its matrices to `ops.linear`, `linear_silu_mul` and `linear_into` only may have
+`hold_in_4_bits()`, which replaces them by `ops.MxWeight`s once they are loaded and says how many those were: models of 4-bit weights call it.
+Where the weight that `first_product()` names is one, a norm with `makes_mx_rows = True` and `forward_mx(h, delta)` hands the part its input
+as `ops.MxRows`.  Both are read with `speaks_for_forward` too.
+
 A mixer or feed-forward whose forward only launches kernels on the current stream (no host
 reads, no loops over host data) may set the class attribute `graph_safe = True`; steps of a
 model whose parts all do are replayed as CUDA graphs, one per (tokens, entries) of a step.  A

@@ -59,3 +59,32 @@ def test_sizes_types_and_addresses_of_products():
     takes = lambda T=16, dt=1, K=64, at=P: m.llm_linear_mx_takes(v(at), dt, T, K)
     assert takes(T=ops.MX_PLAIN_ROWS) and not takes(T=ops.MX_PLAIN_ROWS + 1) and not takes(dt=0) and not takes(K=36) and not takes(at=P + 8)
     assert [ops.mx_padded_rows(t) for t in (1, 16, 17, 33, 65, 128, 129, 384, 385)] == [16, 16, 32, 64, 128, 128, 384, 384, 768]
+
+
+def test_matrices_are_held_in_4_bits_by_parts_that_say_so_of_their_own_forward(monkeypatch):
+    """A part that derives from one with `hold_in_4_bits` and has a forward of its own keeps its matrices, unless it says so again."""
+    import tiny_models as tm
+    from litellmengine_b200.config import config_from_dict
+    from litellmengine_b200.parts import registry
+    from litellmengine_b200.parts.feed_forward import SwiGLU
+    from litellmengine_b200.parts.model import Model
+    from litellmengine_b200.weights import DictSource
+
+    class Own(SwiGLU):
+        def forward(self, x, **k):
+            return x @ self.w_down.t()
+
+    class Again(Own):
+        def hold_in_4_bits(self):
+            return super().hold_in_4_bits()
+
+    monkeypatch.setattr(ops, "mx_weight", lambda w, gated=False: ("4 bits", gated))
+    w = {n: t.to(torch.bfloat16) if t.dim() == 2 else t for n, t in tm.make_weights(tm.TINY_A, 0, bf16_exact=True).items()}
+    kind = next(k for k, c in registry._KINDS["feed_forward"].items() if c is SwiGLU)
+    for cls, held in ((SwiGLU, True), (Own, False), (Again, True)):
+        monkeypatch.setitem(registry._KINDS["feed_forward"], kind, cls)
+        model = Model(config_from_dict(tm.TINY_A).plan(), device="cpu", weight_format="mxfp4")
+        model.load_weights(DictSource(w))
+        for block in model.blocks:
+            assert block.mixer.w_qkv == ("4 bits", False) and type(block.feed_forward) is cls
+            assert isinstance(block.feed_forward.w_down, tuple) == held and isinstance(block.feed_forward.w_gate_up, tuple) == held

@@ -1,5 +1,7 @@
 """Microscaled rows, weights and products against their definition in 64 bits: blocks of 32, the smallest power of two as scale with
 which the largest magnitude fits the format, codes to the nearest (ties to even)."""
+import copy
+
 import pytest
 import torch
 
@@ -418,5 +420,31 @@ def test_refusals():
     refuses(o.rmsnorm_mx, torch.zeros(1, 32769, device=DEV), torch.ones(32769, device=DEV), 1e-6)
     refuses(o.silu_and_mul_mx, x[:, :63].contiguous())
     refuses(X.values, torch.float16)
+    refuses(o.linear_mx, o.PartialSum(x[None]), W)
+    refuses(o.linear, o.PendingRows(x, None, n, 1e-6, BF16), W)
+    refuses(o.linear_silu_mul, o.PendingRows(x, None, n, 1e-6, BF16), G, BF16)
     assert o.linear_mx(o.mx_rows(x[:0]), W).shape == (0, 128) and o.linear_silu_mul_mx(x[:0], G).values().shape == (0, 64)
     assert W.nbytes == G.nbytes == 2 * (128 * 64 + 512)
+
+
+def test_what_a_product_of_the_general_entry_comes_in():
+    o, g = ops(), gen(12)
+    x, W = normal(g, 3, 256), o.mx_weight(normal(g, 200, 256))
+    want = o.linear_mx(x, W)
+    for given, dtype, out in ((x, None, F32), (x, BF16, BF16), (x.to(BF16), None, BF16), (x.to(BF16), F32, F32), (o.mx_rows(x), None, BF16), (o.mx_rows(x), F32, F32)):
+        got = o.linear(given, W, out_dtype=dtype)
+        assert got.dtype == out
+        if given.shape[0] and (isinstance(given, o.MxRows) or given.dtype == F32):
+            assert torch.equal(got, want.to(out))
+
+
+def test_a_copy_of_a_weight_is_a_weight_of_its_own():
+    o, g = ops(), gen(13)
+    x = normal(g, 5, 300)
+    for gated in (False, True):
+        W = o.mx_weight(normal(g, 260, 300), gated=gated)
+        run = (lambda w: o.linear_silu_mul_mx(x, w).values(F32)) if gated else (lambda w: o.linear_mx(x, w))
+        want, values = run(W), W.values(F32)
+        other = copy.deepcopy(W)
+        W.buffer.zero_()
+        assert torch.equal(run(other), want) and torch.equal(other.values(F32), values) and bool((W.values(F32) == 0).all())
