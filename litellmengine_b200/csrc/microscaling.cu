@@ -106,10 +106,27 @@ __device__ __forceinline__ float mx_scaled_odd(float v, float rest, float ih, fl
     const int bits = __float_as_int(hi), odd = (bits + ((__float_as_int(lo) ^ bits) >> 31)) | 1;
     return fabsf(lo) > 0.0f ? __int_as_float(odd) : hi;           // a NaN passes as it is
 }
-// The codes of a row whose values, with their remainders, the block's threads hold.  scratch: a double a warp, for this row only.
-template <int CH, bool FAST>
-__device__ __forceinline__ void mx_norm_row(float (&v)[CH][8], const float (&rest)[CH][8], const float* w, double* scratch, unsigned char* codes,
-                                            unsigned char* scales, size_t row, int hidden, int kpad, float eps, double per_value, int vec) {
+// Only values next to a border need that.  The plain product v * ih * g is off by less than 8 of its last places: v by a half (one sum's remainder),
+// ih by 2 and a half (rsqrtf's bound and the mean's rounding), each product by a half, and a place is up to twice as much of one number as of another.  So
+// where no value of a warp is within 16 places of a border between two codes, nor a block's largest of one between two scales, nor anything in the
+// format's lowest range, the codes of the plain products are those of the carried ones, which few pieces then take: the same codes for
+// 4,096 x 4,096 with a sum pending in 41 us instead of 44, for one row in 2.6 instead of 3.2.
+#define MX_NEAR 16u
+__device__ __forceinline__ bool mx_doubtful(const float (&t)[8], unsigned most, unsigned scale) {
+    unsigned border = ~0u, least = ~0u;                           // places from 16 below a border on, in the upper 20 bits; magnitudes without sign, zeros last
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned b = __float_as_uint(t[i]);
+        border = min(border, b * 4096u - ((0x80000u - MX_NEAR) << 12));
+        least = min(least, b * 2u - 1u);
+    }
+    return border <= (2u * MX_NEAR << 12) || least < 0x3c800000u * 2u - 1u || scale < 32u || (most & 0x7fffffu) - (0x600000u - MX_NEAR) <= 2u * MX_NEAR;
+}
+// The codes of a row whose values the block's threads hold; rests(c, r) gives the remainders of piece c.  scratch: a double a warp, for this row
+// only.  whole: the remainders may be anything (of several sums).
+template <int CH, bool FAST, typename F>
+__device__ __forceinline__ void mx_norm_row(const float (&v)[CH][8], F rests, const float* w, double* scratch, unsigned char* codes,
+                                            unsigned char* scales, size_t row, int hidden, int kpad, float eps, double per_value, int vec, bool whole) {
     float mine = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -129,11 +146,23 @@ __device__ __forceinline__ void mx_norm_row(float (&v)[CH][8], const float (&res
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * blockDim.x + threadIdx.x) * 8;
-        float g[8];
+        float g[8], t[8];
         mx_load8<FAST>(w, col, hidden, vec, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = mx_scaled_odd(v[c][i], rest[c][i], ih, il, g[i]);
-        mx_store_row8(v[c], mx_most8(v[c]), col < kpad, row, col, kpad, codes, scales);
+        for (int i = 0; i < 8; ++i) t[i] = v[c][i] * ih * g[i];
+        unsigned most = mx_block_most(mx_most8(t)), scale = mx_scale<MX_E4M3>(most);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] *= mx_inverse(scale);
+        if (__any_sync(0xffffffffu, whole || mx_doubtful(t, most, scale))) {
+            float r[8];
+            rests(c, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = mx_scaled_odd(v[c][i], r[i], ih, il, g[i]);
+            scale = mx_scale<MX_E4M3>(mx_block_most(mx_most8(t)));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] *= mx_inverse(scale);
+        }
+        mx_store_codes8(make_uint2(mx_e4m3x4(t[0], t[1], t[2], t[3]), mx_e4m3x4(t[4], t[5], t[6], t[7])), mx_word(scale), col < kpad, row, col, kpad, codes, scales);
     }
 }
 template <typename TX, typename TD, int CH, bool FAST>
@@ -171,13 +200,17 @@ __global__ void __launch_bounds__(1024) mx_norm_kernel(const TX* x, const TD* __
     if (sum_out)
 #pragma unroll
         for (int c = 0; c < CH; ++c) mx_put8<FAST>(sum_out + src * hidden, (c * blockDim.x + threadIdx.x) * 8, hidden, vec, v[c]);
-    mx_norm_row<CH, FAST>(v, rest, w, scratch, codes, scales, blockIdx.x, hidden, kpad, eps, per_value, vec);
+    auto rests = [&](int c, float (&r)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = rest[c][i];
+    };
+    mx_norm_row<CH, FAST>(v, rests, w, scratch, codes, scales, blockIdx.x, hidden, kpad, eps, per_value, vec, parts > 1);
 }
 
 // The same for many rows of whole, aligned pieces: a block takes every gridDim-th row, and the next one's values are on their way, each warp's own
 // in shared memory (nobody waits for another warp's), while it works on this one.
 template <typename TX, typename TD, int CH>
-__global__ void __launch_bounds__(256) mx_norm_rows_kernel(const TX* x, const TD* __restrict__ delta, const float* __restrict__ w, TX* sum_out,
+__global__ void __launch_bounds__(256, CH == 4 ? 2 : 4) mx_norm_rows_kernel(const TX* x, const TD* __restrict__ delta, const float* __restrict__ w, TX* sum_out,
                                                            unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int n, int hidden,
                                                            int kpad, float eps, double per_value) {
     constexpr int XB = 256 * sizeof(TX), DB = 256 * sizeof(TD);   // bytes of a warp's 256 values and of what joins them
@@ -215,24 +248,35 @@ __global__ void __launch_bounds__(256) mx_norm_rows_kernel(const TX* x, const TD
         fetch(r + gridDim.x, buf ^ 1);
         asm volatile("cp.async.wait_group 1;\n" ::: "memory");
         __syncwarp();
-        float v[CH][8], rest[CH][8];
+        float v[CH][8];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int col = (c * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[c][i] = rest[c][i] = 0.0f;
+            for (int i = 0; i < 8; ++i) v[c][i] = 0.0f;
             if (col < hidden) {
                 load8(reinterpret_cast<const TX*>(at(buf, c)) + lane * 8, v[c]);
                 if (delta) {
                     float d[8];
                     load8(reinterpret_cast<const TD*>(at(buf, c) + XB) + lane * 8, d);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) mx_two_sum(v[c][i], d[i], v[c][i], rest[c][i]);
+                    for (int i = 0; i < 8; ++i) v[c][i] += d[i];
                 }
                 if (sum_out) store8(sum_out + static_cast<size_t>(r) * hidden + col, v[c]);
             }
         }
-        mx_norm_row<CH, true>(v, rest, w, scratch[buf], codes, scales, r, hidden, kpad, eps, per_value, 8);
+        auto rests = [&](int c, float (&r)[8]) {                  // from what is still in shared memory
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = 0.0f;
+            if (delta && static_cast<int>(c * blockDim.x + threadIdx.x) * 8 < hidden) {
+                float x8[8], d[8];
+                load8(reinterpret_cast<const TX*>(at(buf, c)) + lane * 8, x8);
+                load8(reinterpret_cast<const TD*>(at(buf, c) + XB) + lane * 8, d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mx_two_sum(x8[i], d[i], x8[i], r[i]);
+            }
+        };
+        mx_norm_row<CH, true>(v, rests, w, scratch[buf], codes, scales, r, hidden, kpad, eps, per_value, 8, false);
     }
 }
 
@@ -328,7 +372,9 @@ __global__ void __launch_bounds__(MX_THREADS) mx_values_kernel(const unsigned ch
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 #define MX_MOST_K (1 << 20)
-#define MX_NORM_ROWS 1024
+// Rows from which blocks fetch ahead.  Few / many rows' kernel, us, float32 sum pending: 1,000 x 4,096 16.1 / 14.3, 700 12.1 / 11.4, 592 9.7 / 10.3;
+// 1,000 x 8,192 33.0 / 28.1; 1,200 x 1,024 5.9 / 5.0, 700 4.6 / 4.5, 512 3.9 / 4.1.
+#define MX_NORM_ROWS 640
 // How `rows` rows of n values are cut into warps' items of `u` pieces: four pieces where that leaves enough warps and wastes little.
 struct MxCut {
     int u;

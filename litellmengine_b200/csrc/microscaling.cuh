@@ -103,14 +103,19 @@ __device__ __forceinline__ unsigned mx_most8(const float (&v)[8]) {
 }
 // Eight neighbouring values a lane, four lanes a block, sixteen a tile's row: the lane's codes, and the four blocks' scales as one
 // word in every lane of the sixteen.  most: of the lane's values.  All lanes of a warp are here.
-template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned most, unsigned& word) {
+__device__ __forceinline__ unsigned mx_block_most(unsigned most) {
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const unsigned scale = mx_scale<FMT>(most);
-    const float inv = mx_inverse(scale);
-    word = scale << (8 * ((threadIdx.x >> 2) & 3));
+    return max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+}
+__device__ __forceinline__ unsigned mx_word(unsigned scale) {
+    unsigned word = scale << (8 * ((threadIdx.x >> 2) & 3));
     word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    return word | __shfl_xor_sync(0xffffffffu, word, 8);
+}
+template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned most, unsigned& word) {
+    const unsigned scale = mx_scale<FMT>(mx_block_most(most));
+    const float inv = mx_inverse(scale);
+    word = mx_word(scale);
     float q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = v[i] * inv;
@@ -118,13 +123,16 @@ template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[
     else return make_uint2(mx_e4m3x4(q[0], q[1], q[2], q[3]), mx_e4m3x4(q[4], q[5], q[6], q[7]));
 }
 template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned& word) { return mx_encode8<FMT>(v, mx_most8(v), word); }
+__device__ __forceinline__ void mx_store_codes8(uint2 c, unsigned word, bool there, size_t row, int col, int kpad, unsigned char* codes, unsigned char* scales) {
+    if (!there) return;
+    *reinterpret_cast<uint2*>(codes + row * kpad + col) = c;
+    if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(row, col / MX_BLOCK, kpad / MX_K)) = word;
+}
 // The row's eight values from column `col` on (a multiple of 8), which lane threadIdx.x % 16 == col / 8 % 16 holds, to rows of 8 bits.
 __device__ __forceinline__ void mx_store_row8(const float (&v)[8], unsigned most, bool there, size_t row, int col, int kpad, unsigned char* codes, unsigned char* scales) {
     unsigned word;
     const uint2 c = mx_encode8<MX_E4M3>(v, most, word);
-    if (!there) return;
-    *reinterpret_cast<uint2*>(codes + row * kpad + col) = c;
-    if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(row, col / MX_BLOCK, kpad / MX_K)) = word;
+    mx_store_codes8(c, word, there, row, col, kpad, codes, scales);
 }
 // Eight values from column `col` on of a row of `n`; zeros beyond it.  vec 8: rows of whole, aligned pieces of eight; 2: of pairs; 1: any.
 __device__ __forceinline__ float2 mx_load2(const float* p) { return *reinterpret_cast<const float2*>(p); }

@@ -122,7 +122,8 @@ def half_step(n, fmt=8):
 
 
 @pytest.mark.parametrize("T,H", [(1, 4096), (3, 1), (2, 33), (130, 200), (257, 1450), (5, 8192), (2, 8200), (3, 20000), (1, 32768), (1024, 8), (1100, 1032),
-                                 (3000, 2048), (1333, 4096), (1025, 8192), (1030, 1450)])
+                                 (3000, 2048), (1333, 4096), (1025, 8192), (1030, 1450),
+                                 (639, 512), (640, 512), (700, 8192), (641, 264)])
 @pytest.mark.parametrize("pending", ["none", "float32", "bfloat16", "parts"])
 def test_norm(T, H, pending):
     o, g = ops(), gen(T + H)
@@ -448,3 +449,34 @@ def test_a_copy_of_a_weight_is_a_weight_of_its_own():
         other = copy.deepcopy(W)
         W.buffer.zero_()
         assert torch.equal(run(other), want) and torch.equal(other.values(F32), values) and bool((W.values(F32) == 0).all())
+
+
+@pytest.mark.parametrize("T,H", [(5, 4096), (5, 520), (700, 2048)])
+@pytest.mark.parametrize("pending", [False, True])
+def test_norms_at_borders_between_codes(T, H, pending):
+    """Rows whose normed values lie on, and one or two places beside, the borders between two codes or two scales, and in the lowest
+    range: a float32 product falls to either side of them, the sums of 64 bits say to which."""
+    o, g = ops(), gen(T + H)
+    # a row's largest value, 7, is its blocks' scale; the rest are ties of e4m3 at that scale moved by up to two places
+    ties = torch.tensor([(8 + m + 0.5) / 8 * 2.0 ** e for m in range(8) for e in range(-14, 2)] + [(m + 0.5) * 2.0 ** -15 for m in range(8)], device=DEV)
+    x = ties[torch.randint(len(ties), (T, H), generator=g, device=DEV)]
+    x = x * torch.where(torch.rand(T, H, generator=g, device=DEV) < 0.5, 1.0, -1.0)
+    x = (x.view(torch.int32) + torch.randint(-2, 3, (T, H), generator=g, device=DEV, dtype=torch.int32)).view(F32)
+    x[:, ::32] = 7.0
+    # the mean of squares is made a power of four, so that the borders stay where they are, as near as one value more can do it
+    want, last = 16.0, x[:, 1:].to(F64).square().sum(-1)
+    rest = want * H - last
+    x[:, 0] = torch.where(rest > 0, rest.clamp(min=0).sqrt(), 7.0).float()
+    w = torch.ones(H, device=DEV)
+    delta = None
+    if pending:
+        delta = normal(g, T, H)
+        x = x - delta                                             # rounded: the sum of both is near the border, and its remainder says where
+    v = x.to(F64) + (0 if delta is None else delta.to(F64))
+    n = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + 1e-12) * w.to(F64)
+    got = o.rmsnorm_mx(x, w, 1e-12, delta=delta).values(F32).to(F64)
+    # half a step of each value, and what a sum of squares in float32 leaves: fewer than 32 roundings of 2^-24
+    assert bool(((got - n).abs() <= half_step(n) + n.abs() * 32 * 2.0 ** -24).all())
+    # and hardly any code differs from the rounded exact value: those within 2^-22 of a border
+    sure = (held(n * (1 + 2.0 ** -21), 8) == held(n * (1 - 2.0 ** -21), 8)) & (scales(n * (1 + 2.0 ** -21), 8) == scales(n * (1 - 2.0 ** -21), 8))
+    assert torch.equal(got[sure], held(n, 8)[sure])
