@@ -253,14 +253,15 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         }
     }
     t5_fence_before();
-    // What the warp's first token is added to is on its way while the parts meet.
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    // What the warp's first token is added to is on its way while the parts meet (an 8B-shape decode step of 32 requests 2.23 ms, 2.29 without).
     const int feature = tile * MG_ROWS + 4 * lane, first_tok = part + warp * parts;
     float4 old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if constexpr (MODE == MG_ADD) {
         pdl_wait();                                               // the warps that feed weights have not
         if (a.vec && first_tok < toks && feature < a.N) old = *reinterpret_cast<const float4*>(static_cast<const float*>(a.y) + static_cast<size_t>(tok0 + first_tok) * a.N + feature);
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every part's sums are there
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");       // every part's sums are there
     {
         const unsigned base = t5_smem(sums);
         auto total = [&](int at) {                                // the parts' sums in order, four features, all parts' loads in flight at once
@@ -335,8 +336,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         for (int n = 0; n < 2000; ++n) __nanosleep(100);
     __syncwarp();
     // Nobody leaves while its sums are read.  A thread that is here has all that it read, because it has made what it stored of it (none is read that is
-    // not); the stores themselves need not be out yet, which a release would wait for (one row x 4,096 by 6,144 5.8 us instead of 5.5, an 8B-shape
-    // decode step of 4 requests 1.87 ms instead of 1.82).
+    // not); the stores themselves need not be out yet, which a release would wait for (one row x 4,096 by 6,144 5.5 us, 5.8 with it; an 8B-shape
+    // decode step of 4 requests 1.82 ms, 1.87).
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     if (warp == 1) {
         t5_fence_after();
