@@ -288,16 +288,11 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 const int tok = t0 + part + (tid >> 4) * parts;
                 const bool there = tok < toks;
                 const float4 g = total((there ? tok : 0) * MG_ROWS + f), u = total((there ? tok : 0) * MG_ROWS + 64 + f);
-                float v[4] = {mx_gated(g.x, u.x, a.act), mx_gated(g.y, u.y, a.act), mx_gated(g.z, u.z, a.act),
-                              mx_gated(g.w, u.w, a.act)};
-                unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
-#pragma unroll
-                for (int o = 1; o < 8; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const unsigned scale = mx_scale<MX_E4M3>(most);
-                const float inv = mx_inverse(scale);
+                unsigned scale;
+                const unsigned made = mx_gated_codes<true>(g, u, a.act, scale);
                 if (there) {
                     const size_t t = tok0 + tok;
-                    *reinterpret_cast<unsigned*>(codes + t * a.out_kpad + tile * 64 + f) = mx_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    *reinterpret_cast<unsigned*>(codes + t * a.out_kpad + tile * 64 + f) = made;
                     if ((tid & 7) == 0) a.y_scales[mx_scale_at(t, (tile * 64 + f) / MX_BLOCK, a.out_kpad / MX_K)] = static_cast<unsigned char>(scale);
                 }
             }
@@ -560,16 +555,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                     for (int i = 0; i < 2; ++i) {
                         const int tok = (e >> 4) + 8 * i;
                         const float4 g = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + f), u = *reinterpret_cast<const float4*>(to + tok * MG_ROWS + 64 + f);
-                        const float v[4] = {mx_gated(g.x, u.x, a.act), mx_gated(g.y, u.y, a.act), mx_gated(g.z, u.z, a.act),
-                                            mx_gated(g.w, u.w, a.act)};
-                        unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
-#pragma unroll
-                        for (int o = 1; o < 8; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        const unsigned scale = mx_scale<MX_E4M3>(most);
-                        const float inv = mx_inverse(scale);
+                        unsigned scale;
+                        const unsigned made = mx_gated_codes<false>(g, u, a.act, scale);
                         if (c + tok < toks) {
                             const size_t row = tok0 + c + tok;
-                            *reinterpret_cast<unsigned*>(codes + row * a.out_kpad + wt * 64 + f) = mx_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                            *reinterpret_cast<unsigned*>(codes + row * a.out_kpad + wt * 64 + f) = made;
                             if ((e & 7) == 0) a.y_scales[mx_scale_at(row, (wt * 64 + f) / MX_BLOCK, a.out_kpad / MX_K)] = static_cast<unsigned char>(scale);
                         }
                     }
