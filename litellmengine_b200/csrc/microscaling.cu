@@ -9,37 +9,45 @@
 
 #define MX_THREADS 256
 
-// A warp takes U pieces of 256 neighbouring values of a row, all of them asked for before the first is used: one piece a thread left
+// A warp takes U pieces of 256 (or 512) neighbouring values of a row, all of them asked for before the first is used: one piece a thread left
 // the memory idle (the values of a weight of 12,288 x 4,096 37 us with one, 24 with four), several leave the SMs idle where there is little to do.
 struct MxSpan {
     long long row;
     int col;                              // of the lane's first piece
     bool there;
 };
-template <int U> __device__ __forceinline__ MxSpan mx_span(unsigned items, unsigned per_row) {
+template <int U, int LANE = 8> __device__ __forceinline__ MxSpan mx_span(unsigned items, unsigned per_row) {
     const unsigned w = blockIdx.x * (MX_THREADS / 32) + (threadIdx.x >> 5), row = w / per_row;
-    return {row, static_cast<int>((w - row * per_row) * (U * 256) + (threadIdx.x & 31) * 8), w < items};
+    return {row, static_cast<int>((w - row * per_row) * (U * 32 * LANE) + (threadIdx.x & 31) * LANE), w < items};
 }
 
 // ---- rows of 8 bits from a matrix -----------------------------------------------------------------------------------
 template <int U, bool FAST, typename T>
 __global__ void __launch_bounds__(MX_THREADS) mx_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
                                                              unsigned char* __restrict__ scales, unsigned items, unsigned per_row, int K, int kpad, int vec) {
+    constexpr bool WIDE = FAST && sizeof(T) == 2;
     pdl_begin();
-    const MxSpan at = mx_span<U>(items, per_row);
+    const MxSpan at = mx_span<U, WIDE ? 16 : 8>(items, per_row);
     if (!at.there) return;                                        // whole warps
-    if constexpr (FAST && sizeof(T) == 2) {
-        uint4 raw[U];
+    if constexpr (WIDE) {
+        uint4 raw[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int col = at.col + u * 512 + h * 8;
+                raw[u][h] = make_uint4(0u, 0u, 0u, 0u);
+                if (col < K) mx_raw8(x + at.row * K + col, raw[u][h]);
+            }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            raw[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (at.col + u * 256 < K) mx_raw8(x + at.row * K + at.col + u * 256, raw[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float v[8];
-            mx_raw_values(raw[u], v);
-            mx_store_row8(v, mx_most8(raw[u]), at.col + u * 256 < kpad, at.row, at.col + u * 256, kpad, codes, scales);
+            const int col = at.col + u * 512;
+            unsigned word;
+            const uint4 c = mx_encode16<MX_E4M3>(raw[u][0], raw[u][1], word);
+            if (col < kpad) {
+                *reinterpret_cast<uint4*>(codes + at.row * kpad + col) = c;
+                if ((col & (MX_K - 1)) == 0) *reinterpret_cast<unsigned*>(scales + mx_scale_at(at.row, col / MX_BLOCK, kpad / MX_K)) = word;
+            }
         }
     } else {
         float v[U][8];
@@ -287,10 +295,11 @@ template <int U, bool FAST, typename T>
 __global__ void __launch_bounds__(MX_THREADS) mx_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ tiles,
                                                                unsigned char* __restrict__ scales, unsigned items, unsigned per_row, int N, int K, int ktiles,
                                                                int gated_rows, int vec) {
+    constexpr int LANE = FAST && sizeof(T) == 2 ? 16 : 8;
     pdl_wait();
     const unsigned item = blockIdx.x * (MX_THREADS / 32) + (threadIdx.x >> 5), group = item / per_row;
     const bool mine = item < items;                               // whole warps
-    const int col = (item - group * per_row) * 256 + (threadIdx.x & 31) * 8;
+    const int col = (item - group * per_row) * (32 * LANE) + (threadIdx.x & 31) * LANE;
     const unsigned row = group * U;                               // of the tiles; gated: 64 rows of gate, 64 of up from [gate; up] of N rows each
     const long long first = gated_rows ? (row >> 7) * 64LL + (row & 63) : row, there = mine ? N - first : 0;
     const T* from = w + (gated_rows && (row & 64) ? N + first : first) * K + col;
@@ -305,18 +314,23 @@ __global__ void __launch_bounds__(MX_THREADS) mx_weight_kernel(const T* __restri
             if ((threadIdx.x & 15) == 0) *reinterpret_cast<unsigned*>(to_scales + u * 16) = word;
         }
     };
-    if constexpr (FAST && sizeof(T) == 2) {
-        uint4 raw[U];
+    if constexpr (LANE == 16) {
+        uint4 raw[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                raw[u][h] = make_uint4(0u, 0u, 0u, 0u);
+                if (u < there && col + h * 8 < K) mx_raw8(from + static_cast<size_t>(u) * K + h * 8, raw[u][h]);
+            }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            raw[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (u < there && col < K) mx_raw8(from + static_cast<size_t>(u) * K, raw[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float v[8];
-            mx_raw_values(raw[u], v);
-            store(u, v, mx_most8(raw[u]));
+            unsigned word;
+            const uint4 c = mx_encode16<MX_E2M1>(raw[u][0], raw[u][1], word);
+            if (whole) {
+                *reinterpret_cast<uint2*>(to + u * 64) = make_uint2(c.x, c.y);
+                if ((threadIdx.x & 7) == 0) *reinterpret_cast<unsigned*>(to_scales + u * 16) = word;
+            }
         }
     } else {
         float v[U][8];
@@ -380,8 +394,8 @@ struct MxCut {
     int u;
     unsigned items, per_row, blocks;
 };
-static inline bool mx_cut(long long rows, int n, MxCut* c) {
-    const int pieces = (n + 255) / 256;
+static inline bool mx_cut(long long rows, int n, MxCut* c, int width = 256) {
+    const int pieces = (n + width - 1) / width;
     c->u = rows * pieces >= 32768 && (pieces % 4 == 0 || pieces >= 12) ? 4 : rows * pieces >= 16384 && (pieces % 2 == 0 || pieces >= 7) ? 2 : 1;
     c->per_row = static_cast<unsigned>((pieces + c->u - 1) / c->u);
     const long long items = rows * c->per_row;
@@ -405,7 +419,7 @@ extern "C" int llm_mx_rows(const void* x, int dtype, void* rows, int T, int K, u
     if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
     const int kpad = mx_tiles(K) * MX_K, vec = mx_vec(K, x, dtype == LLM_DT_F32 ? 4 : 2);
     MxCut cut;
-    if (!mx_cut(T, kpad, &cut)) return LLM_REFUSED_SIZE;
+    if (!mx_cut(T, kpad, &cut, vec == 8 && dtype == LLM_DT_BF16 ? 512 : 256)) return LLM_REFUSED_SIZE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     unsigned char *c = static_cast<unsigned char*>(rows), *sc = mx_row_scales(rows, T, K);
 #define F32(U, V) mx_rows_kernel<U, V, float>
@@ -501,7 +515,8 @@ extern "C" int llm_mx_weight(const void* w, int dtype, void* tiles, void* scales
     const int ktiles = mx_tiles(K), vec = mx_vec(K, w, dtype == LLM_DT_F32 ? 4 : 2);
     const long long rows = llm_mx_weight_tiles(N, is_gated) * 128LL;
     MxCut cut;
-    cut.per_row = (ktiles + 1) / 2;
+    const int wide = vec == 8 && dtype == LLM_DT_BF16 ? 4 : 2;   // tiles of K that a warp takes
+    cut.per_row = (ktiles + wide - 1) / wide;
     cut.u = rows * cut.per_row >= 32768 ? 4 : rows * cut.per_row >= 16384 ? 2 : 1;
     const long long items = rows / cut.u * cut.per_row;
     if (items > 0x7fffffffLL) return LLM_REFUSED_SIZE;

@@ -123,6 +123,23 @@ template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[
     else return make_uint2(mx_e4m3x4(q[0], q[1], q[2], q[3]), mx_e4m3x4(q[4], q[5], q[6], q[7]));
 }
 template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], unsigned& word) { return mx_encode8<FMT>(v, mx_most8(v), word); }
+// Sixteen neighbouring values a lane as they lie in memory, two lanes a block, eight a tile's row: the same with half the exchanges and scales.
+template <int FMT> __device__ __forceinline__ uint4 mx_encode16(const uint4& a, const uint4& b, unsigned& word) {
+    unsigned most = max(mx_most8(a), mx_most8(b));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    const unsigned scale = mx_scale<FMT>(most);
+    const float inv = mx_inverse(scale);
+    word = scale << (8 * ((threadIdx.x >> 1) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    float p[8], q[8];
+    mx_raw_values(a, p);
+    mx_raw_values(b, q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] *= inv, q[i] *= inv;
+    if constexpr (FMT == MX_E2M1) return make_uint4(mx_e2m1x8(p), mx_e2m1x8(q), 0u, 0u);
+    else return make_uint4(mx_e4m3x4(p[0], p[1], p[2], p[3]), mx_e4m3x4(p[4], p[5], p[6], p[7]), mx_e4m3x4(q[0], q[1], q[2], q[3]), mx_e4m3x4(q[4], q[5], q[6], q[7]));
+}
 __device__ __forceinline__ void mx_store_codes8(uint2 c, unsigned word, bool there, size_t row, int col, int kpad, unsigned char* codes, unsigned char* scales) {
     if (!there) return;
     *reinterpret_cast<uint2*>(codes + row * kpad + col) = c;
