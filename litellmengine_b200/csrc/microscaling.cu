@@ -389,14 +389,17 @@ __global__ void __launch_bounds__(MX_THREADS) mx_values_kernel(const unsigned ch
 // Rows from which blocks fetch ahead.  Few / many rows' kernel, us, float32 sum pending: 1,000 x 4,096 16.1 / 14.3, 700 12.1 / 11.4, 592 9.7 / 10.3;
 // 1,000 x 8,192 33.0 / 28.1; 1,200 x 1,024 5.9 / 5.0, 700 4.6 / 4.5, 512 3.9 / 4.1.
 #define MX_NORM_ROWS 640
-// How `rows` rows of n values are cut into warps' items of `u` pieces: four pieces where that leaves enough warps and wastes little.
+// How `rows` rows of n values are cut into warps' items of `u` pieces of `width`: several pieces where that leaves enough warps and wastes little; with 512
+// two at most (4,096 x 4,096: one and two 9.1 us, four 9.8; 700 x 4,096: 2.9, 3.6, 4.1).
 struct MxCut {
     int u;
     unsigned items, per_row, blocks;
 };
 static inline bool mx_cut(long long rows, int n, MxCut* c, int width = 256) {
     const int pieces = (n + width - 1) / width;
-    c->u = rows * pieces >= 32768 && (pieces % 4 == 0 || pieces >= 12) ? 4 : rows * pieces >= 16384 && (pieces % 2 == 0 || pieces >= 7) ? 2 : 1;
+    const bool many = rows * pieces >= 32768, two = pieces % 2 == 0 || pieces >= 7;
+    if (width == 512) c->u = many && two ? 2 : 1;
+    else c->u = many && (pieces % 4 == 0 || pieces >= 12) ? 4 : rows * pieces >= 16384 && two ? 2 : 1;
     c->per_row = static_cast<unsigned>((pieces + c->u - 1) / c->u);
     const long long items = rows * c->per_row;
     c->items = static_cast<unsigned>(items);
@@ -423,7 +426,7 @@ extern "C" int llm_mx_rows(const void* x, int dtype, void* rows, int T, int K, u
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     unsigned char *c = static_cast<unsigned char*>(rows), *sc = mx_row_scales(rows, T, K);
 #define F32(U, V) mx_rows_kernel<U, V, float>
-#define B16(U, V) mx_rows_kernel<U, V, bf16>
+#define B16(U, V) mx_rows_kernel<(V && U == 4 ? 2 : U), V, bf16>         // of 512 values two pieces at most
     if (dtype == LLM_DT_F32) MX_GO(F32, static_cast<const float*>(x), c, sc, cut.items, cut.per_row, K, kpad, vec);
     else if (dtype == LLM_DT_BF16) MX_GO(B16, static_cast<const bf16*>(x), c, sc, cut.items, cut.per_row, K, kpad, vec);
     else return LLM_REFUSED_DTYPE;
@@ -517,7 +520,8 @@ extern "C" int llm_mx_weight(const void* w, int dtype, void* tiles, void* scales
     MxCut cut;
     const int wide = vec == 8 && dtype == LLM_DT_BF16 ? 4 : 2;   // tiles of K that a warp takes
     cut.per_row = (ktiles + wide - 1) / wide;
-    cut.u = rows * cut.per_row >= 32768 ? 4 : rows * cut.per_row >= 16384 ? 2 : 1;
+    // rows a warp; of 512 values each 4,096 x 4,096: one 10.2 us, two 8.7, four 9.6; 12,288 x 4,096: 27.5, 22.4, 21.9
+    cut.u = rows * cut.per_row >= (wide == 4 ? 65536 : 32768) ? 4 : rows * cut.per_row >= 16384 ? 2 : 1;
     const long long items = rows / cut.u * cut.per_row;
     if (items > 0x7fffffffLL) return LLM_REFUSED_SIZE;
     cut.items = static_cast<unsigned>(items);
