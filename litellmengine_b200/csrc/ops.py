@@ -2129,7 +2129,11 @@ _stream_status: Dict[str, torch.Tensor] = {}
 
 def stream_status(device) -> torch.Tensor:
     """The status word of the engine's matrix products and of the delta rule (code 8: a bounded wait of a weight-streaming
-    product ran out; 9: of the paired, the float32 or a microscaled tcgen05 product; 11: of the delta rule's tensor-core scan)."""
+    product ran out; 9: of the paired, the float32 or a microscaled tcgen05 product; 11: of the delta rule's tensor-core scan).
+    One word a device: `cuda` is the current one's, as tensors made on `cuda` and the kernels that read them have it."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     key = str(device)
     t = _stream_status.get(key)
     if t is None:
