@@ -9,7 +9,8 @@
 // 16 KB, sixteen of them and eight bytes of nothing, as the products read them, and counts the 8 KB on its barrier), a box of the rows, and
 // the pieces of both operands' scales, which the tensor core copies to its own memory in front of the stage's four products.
 // Roles here: warp 0 feeds the weights and their scales, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and theirs; all of them write
-// the result.  Waits are bounded: one that runs out sets status code 9, and what is in flight lands before the CTA ends.
+// the result.  Waits are bounded: one that runs out sets status code 9, and the copies and products that are under way then end, which is waited for
+// on their own barriers (bounded too), before the CTA does.
 //   * Few rows: bytes bound the product.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the
 //     parts' order; nothing is left for another kernel and no result depends on timing.  The first weights are on their way before the
 //     CTA waits for the kernel in front.
@@ -32,6 +33,14 @@ __device__ __forceinline__ bool mg_wait(unsigned long long* bar, unsigned parity
     *abort_flag = 1;
     if (atomicCAS(status, 0, MG_STATUS) == 0) status[1] = blockIdx.y;
     return false;
+}
+// What was asked for before a wait ran out: its end.
+__device__ __forceinline__ void mg_land(unsigned long long* bar, unsigned parity) {
+    for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(bar, parity); ++i) {}
+}
+// The uses of a ring's barriers that may be under way, of `asked` in all.
+__device__ __forceinline__ void mg_land_ring(unsigned long long* bars, int ring, int asked) {
+    for (int i = max(0, asked - ring); i < asked; ++i) mg_land(&bars[i % ring], (i / ring) & 1);
 }
 __device__ __forceinline__ void mg_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(t5_smem(dst)), "l"(map),
@@ -84,7 +93,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     unsigned char* g_s = w_s + WS * MG_W_BYTES;                   // [2][G rows' boxes [NT][128], 128-byte swizzle like the weights; weights' pieces, rows' pieces]
     float* sums = reinterpret_cast<float*>(w_s);                  // [NT][128], when the stages have been read
-    __shared__ __align__(8) unsigned long long full[WS], empty[WS], g_full[2], g_empty[2], acc_full;
+    // a group's weights' scales and its rows have barriers of their own: each is waited for by itself where the other was never asked for
+    __shared__ __align__(8) unsigned long long full[WS], empty[WS], gw_full[2], gx_full[2], g_empty[2], acc_full, drained;
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -95,8 +105,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         const int at = tile * a.ktiles + kb0 + kb;
         if (kb % G == 0) {                                        // what stands behind the part's last stage is read and not used
             const int g = (kb / G) & 1;
-            t5_expect_tx(&g_full[g], S_BYTES);
-            t5_tma_2d(g_s + g * GROUP_BYTES + G * X_BYTES, &ws_map, 0, at, &g_full[g]);
+            t5_expect_tx(&gw_full[g], S_BYTES);
+            t5_tma_2d(g_s + g * GROUP_BYTES + G * X_BYTES, &ws_map, 0, at, &gw_full[g]);
         }
         t5_expect_tx(&full[s], MG_W_READ);
         t5_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, at * MG_ROWS, &full[s]);
@@ -104,8 +114,9 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < WS; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { t5_mbar_init(&g_full[s], PLAIN ? 1 + MG_MAKERS : 2); t5_mbar_init(&g_empty[s], 1); }      // the weights' scales; rows and theirs
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&gw_full[s], 1); t5_mbar_init(&gx_full[s], PLAIN ? MG_MAKERS : 1); t5_mbar_init(&g_empty[s], 1); }
         t5_mbar_init(&acc_full, 1);
+        t5_mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         // Weights and their scales are nobody's output: the first of them are on their way before anything else, whatever runs in front.
         for (int kb = 0; kb < early; ++kb) weights(kb, kb);
@@ -124,7 +135,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     pdl_invite();                                                 // not before: this CTA's tensor memory is taken
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
 
-    int issued = 0;                                               // stages that were asked for, in the thread that asks
+    int issued = 0;                                               // stages (warp 6: groups) that were asked for, in the thread that asks
     if (warp == 0) {
         if (lane == 0) {
             int s = early % WS;
@@ -149,9 +160,10 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
             for (int g = 0; g * G < kbs; ++g) {
                 unsigned char* to = g_s + (g & 1) * GROUP_BYTES;
                 if (!mg_wait(&g_empty[g & 1], ((g >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status)) break;
-                t5_expect_tx(&g_full[g & 1], G * X_BYTES + S_BYTES);
-                mg_tma_3d(to, &x_map, 0, tok0, kb0 + g * G, &g_full[g & 1]);
-                t5_tma_2d(to + G * X_BYTES + S_BYTES, &xs_map, 0, (tok0 / 128) * a.ktiles + kb0 + g * G, &g_full[g & 1]);
+                t5_expect_tx(&gx_full[g & 1], G * X_BYTES + S_BYTES);
+                mg_tma_3d(to, &x_map, 0, tok0, kb0 + g * G, &gx_full[g & 1]);
+                t5_tma_2d(to + G * X_BYTES + S_BYTES, &xs_map, 0, (tok0 / 128) * a.ktiles + kb0 + g * G, &gx_full[g & 1]);
+                issued = g + 1;
             }
         }
         __syncwarp();
@@ -166,7 +178,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
 #pragma unroll 1
         for (int k0 = 0; ok && k0 < kbs; k0 += G) {
             const int g = (k0 / G) & 1;
-            ok = __all_sync(0xffffffffu, mg_wait(&g_full[g], (k0 / G >> 1) & 1, a.waits, &abort_flag, a.status));
+            const unsigned turn = (k0 / G >> 1) & 1;
+            ok = __all_sync(0xffffffffu, mg_wait(&gw_full[g], turn, a.waits, &abort_flag, a.status) && mg_wait(&gx_full[g], turn, a.waits, &abort_flag, a.status));
             if (!ok) break;
             // [weights, rows] of each stage; the products that read the group before last have run
             const unsigned sc0 = tmem + S_COL0 + g * (G * 8);
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
-                if (lane == 0) t5_arrive(&g_full[g & 1]);
+                if (lane == 0) t5_arrive(&gx_full[g & 1]);
             }
         }
         if (warp < 6) {
@@ -324,11 +337,17 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
             }
         }
     }
-    if (tid == 0 && abort_flag)                                   // whoever gave up: what is in flight lands before the CTA goes away
-        for (int kb = max(0, issued - WS); kb < issued; ++kb)
-            for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(&full[kb % WS], (kb / WS) & 1); ++i) {}
-    if ((tid == 0 || tid == 192) && abort_flag)                   // a group whose other half was never asked for does not fill
-        for (int n = 0; n < 2000; ++n) __nanosleep(100);
+    if (abort_flag) {                                             // whoever gave up: what is under way ends before the CTA goes away
+        if (tid == 0) {
+            mg_land_ring(full, WS, issued);
+            mg_land_ring(gw_full, 2, (issued + G - 1) / G);
+        } else if (!PLAIN && tid == 192) {
+            mg_land_ring(gx_full, 2, issued);
+        } else if (warp == 1) {                                   // the copies of scales and the products, of which there may be none
+            t5_commit_lead(elect_one(), &drained);                // the lane that issued: elect gives the same one for the same lanes
+            mg_land(&drained, 0);
+        }
+    }
     __syncwarp();
     // Nobody leaves while its sums are read.  A thread that is here has all that it read, because it has made what it stored of it (none is read that is
     // not); the stores themselves need not be out yet, which a release would wait for (one row x 4,096 by 6,144 5.5 us, 5.8 with it; an 8B-shape
@@ -364,6 +383,21 @@ __device__ __forceinline__ unsigned mp_map_to(unsigned smem_addr, unsigned rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr), "r"(rank));
     return r;
 }
+// A wait that ran out ends the pair's work, not one CTA's alone: the other one's flag too.
+__device__ __forceinline__ bool mp_give_up(volatile int* abort_flag, int32_t* status) {
+    *abort_flag = 1;
+    const unsigned other = mp_map_to(t5_smem(const_cast<int*>(abort_flag)), mp_rank() ^ 1);
+    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(other), "r"(1u) : "memory");
+    if (atomicCAS(status, 0, MG_STATUS) == 0) status[1] = blockIdx.x;
+    return false;
+}
+__device__ __forceinline__ bool mp_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    for (int i = 0; i < waits; ++i) {
+        if (t5_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    return mp_give_up(abort_flag, status);
+}
 __device__ __forceinline__ bool mp_wait_cluster(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
     for (int i = 0; i < waits; ++i) {
         unsigned ok;
@@ -372,9 +406,7 @@ __device__ __forceinline__ bool mp_wait_cluster(unsigned long long* bar, unsigne
         if (ok) return true;
         if (*abort_flag) return false;
     }
-    *abort_flag = 1;
-    if (atomicCAS(status, 0, MG_STATUS) == 0) status[1] = blockIdx.x;
-    return false;
+    return mp_give_up(abort_flag, status);
 }
 // Boxes into this CTA's shared memory, counted on a barrier of the pair's first CTA.
 __device__ __forceinline__ void mp_tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
@@ -420,9 +452,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     unsigned char* x_s = w_s + MP_STAGES * MG_W_BYTES;            // [STAGES][96 tokens][128]
     unsigned char* s_s = x_s + MP_STAGES * MP_X_BYTES;            // [2][the weights' QUAD pieces, the rows' two times QUAD]
     float* turns_s = reinterpret_cast<float*>(s_s + 2 * MP_S_BYTES);      // two blocks for each half of the result's warps
-    __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], s_full[2], s_empty[2], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) unsigned long long full[MP_STAGES], empty[MP_STAGES], s_full[2], s_empty[2], acc_full[2], acc_empty[2], drained;
     __shared__ unsigned tmem_base_s;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, asked_s[3];                        // asked_s: boxes of weights, of rows and groups of scales that were asked for
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const unsigned rank = __shfl_sync(0xffffffffu, mp_rank(), 0);
     const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1, ktiles = a.ktiles;
@@ -435,6 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             t5_mbar_init(&acc_full[s], 1);
             t5_mbar_init(&acc_empty[s], 16);                      // 8 warps of 2 CTAs
         }
+        t5_mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
@@ -449,16 +482,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
     if (warp != 0) pdl_wait();                                    // weights are nobody's output
 
+    // One box of this thread's (of weights, rows or scales) for tile t and from stage kb on, into place s of its ring.
+    const bool feeds_scales = warp == 11;
+    unsigned long long* const own = feeds_scales ? s_full : full;
+    const unsigned first = mp_map_to(t5_smem(own), 0);            // the first CTA's barriers
+    const int ring = feeds_scales ? 2 : MP_STAGES, step = feeds_scales ? MP_QUAD : 1;
+    auto ask = [&](int tok0, int at, int kb, int s) {
+        const unsigned bytes = 2 * (feeds_scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : nt / 2 * MX_K);      // of both CTAs
+        if (rank == 0) t5_expect_tx(&own[s], bytes);
+        const unsigned bar = first + s * 8;
+        if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
+        else if (warp == 10) mp_tma_3d(x_s + s * MP_X_BYTES, &x_map, 0, tok0 + static_cast<int>(rank) * (nt / 2), kb, bar);
+        else {                                                    // what stands behind the last tile of K is read and not used
+            mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at + kb, bar);
+            mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
+        }
+    };
+    int asked = 0;
+
     if (warp == 0 || warp >= 10) {
         // Three threads feed: the weights (warp 0), the rows (10) and the scales (11).  Asking for a box takes a thread 80 clocks and a
         // turn of the loop 150 more; one thread for all of a stage took 650, its four products 400.
         if (lane == 0) {
-            const bool scales = warp == 11;
-            const unsigned first = mp_map_to(t5_smem(scales ? &s_full[0] : &full[0]), 0);      // the first CTA's barriers
-            unsigned long long* own = scales ? s_full : full;
-            unsigned long long* free = scales ? s_empty : empty;
-            const int ring = scales ? 2 : MP_STAGES, step = scales ? MP_QUAD : 1;
-            const unsigned bytes = 2 * (scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : nt / 2 * MX_K);      // of both CTAs
+            unsigned long long* free = feeds_scales ? s_empty : empty;
             int s = 0;
             unsigned phase = 1;                                   // a barrier that was never used passes for the phase before its first
             bool ok = true;
@@ -468,20 +514,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; kb += step) {
                     if (ahead >= 0 && ahead-- == 0) pdl_wait();   // the bounded waits below are not for that kernel
-                    if (!mg_wait(&free[s], phase, a.waits, &abort_flag, a.status)) { ok = false; break; }
-                    if (rank == 0) t5_expect_tx(&own[s], bytes);
-                    const unsigned bar = first + s * 8;
-                    if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
-                    else if (warp == 10) mp_tma_3d(x_s + s * MP_X_BYTES, &x_map, 0, tok0 + static_cast<int>(rank) * (nt / 2), kb, bar);
-                    else {                                        // what stands behind the last tile of K is read and not used
-                        mp_tma_2d(s_s + s * MP_S_BYTES, &ws_map, 0, at + kb, bar);
-                        mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
-                    }
+                    if (!mp_wait(&free[s], phase, a.waits, &abort_flag, a.status)) { ok = false; break; }
+                    ask(tok0, at, kb, s);
+                    ++asked;
                     if (++s == ring) s = 0, phase ^= 1;
                 }
             }
-            if (!ok)                                              // let what is in flight land before the CTA goes away
-                for (int n = 0; n < 2000; ++n) __nanosleep(100);
+            asked_s[warp == 0 ? 0 : warp - 9] = asked;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -500,7 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
 #pragma unroll 1
                 for (int k0 = 0; ok && k0 < ktiles; k0 += MP_QUAD, ++quad) {
                     const int qs = quad & 1;
-                    ok = __all_sync(0xffffffffu, mg_wait(&s_full[qs], (quad >> 1) & 1, a.waits, &abort_flag, a.status));
+                    ok = __all_sync(0xffffffffu, mp_wait(&s_full[qs], (quad >> 1) & 1, a.waits, &abort_flag, a.status));
                     if (!ok) break;
                     // [weights, rows' first piece, rows' second] of each stage; products that read the group before last have run
                     const unsigned sc0 = tmem + 2 * MP_NT + qs * MP_S_COLS;
@@ -510,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                         for (int p = 0; p < 3; ++p) mp_scales_lead(lead, sc0 + 12 * q + 4 * p, sd + ((qs * MP_S_BYTES + (p * MP_QUAD + q) * MX_PIECE) >> 4));
 #pragma unroll 1
                     for (int q = 0; q < min(MP_QUAD, ktiles - k0); ++q) {
-                        ok = __all_sync(0xffffffffu, mg_wait(&full[s], phase, a.waits, &abort_flag, a.status));
+                        ok = __all_sync(0xffffffffu, mp_wait(&full[s], phase, a.waits, &abort_flag, a.status));
                         if (!ok) break;
                         const unsigned sc = sc0 + 12 * q;
 #pragma unroll
@@ -534,7 +573,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
         for (int t = cluster; t < tiles; t += clusters, ++n) {
             const int buf = n & 1, tok0 = (t % token_tiles) * nt, wt = (t / token_tiles) * 2 + static_cast<int>(rank);
             const int toks = min(nt, a.T - tok0);
-            bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
+            bool ok = __all_sync(0xffffffffu, mp_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
             ok = mp_all(ok, 1 + half);                            // the four warps meet below: they go on or leave together
             t5_fence_after();
             const unsigned acc = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * MP_NT;
@@ -621,6 +660,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     t5_fence_before();
     __syncthreads();
     mp_cluster_sync();                                            // nobody signals a CTA that has left
+    if (abort_flag) {
+        // A wait ran out, both CTAs know it, and what is under way ends before they go away.  A barrier fills when all who bring its bytes have asked: those
+        // who stopped earlier ask for what the others have asked for already, at most a ring's worth, into places that the products have left
+        // (whoever asked first has waited for that).  Then the first CTA's barriers tell when all of it is there, and one more commit when the products are.
+        if ((warp == 0 || warp >= 10) && lane == 0) {
+            int most = 0;
+            for (int who = feeds_scales ? 2 : 0; who < (feeds_scales ? 3 : 2); ++who)
+                for (unsigned r = 0; r < 2; ++r) {
+                    int n;
+                    asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(n) : "r"(mp_map_to(t5_smem(&asked_s[who]), r)) : "memory");
+                    most = max(most, n);
+                }
+            const int steps = (ktiles + step - 1) / step;         // of a tile
+            for (; asked < most; ++asked) {
+                const int t = cluster + asked / steps * clusters;
+                ask((t % token_tiles) * nt, ((t / token_tiles) * 2 + static_cast<int>(rank)) * ktiles, asked % steps * step, asked % ring);
+            }
+            if (rank == 0) mg_land_ring(own, ring, most);
+        } else if (warp == 1) {
+            if (rank == 0) mp_commit_lead(elect_one(), &drained);         // the lane that issued: elect gives the same one for the same lanes
+            mg_land(&drained, 0);
+        }
+        __syncwarp();
+        __syncthreads();
+        mp_cluster_sync();
+    }
     if (warp == 1) {
         t5_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
