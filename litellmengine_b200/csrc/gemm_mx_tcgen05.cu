@@ -10,7 +10,7 @@
 // the pieces of both operands' scales, which the tensor core copies to its own memory in front of the stage's four products.
 // Roles here: warp 0 feeds the weights and their scales, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and theirs; all of them write
 // the result.  Waits are bounded: one that runs out sets status code 9, and the copies and products that are under way then end, which is waited for
-// on their own barriers (bounded too), before the CTA does.
+// on their own barriers (bounded too), before the CTA does; sums that are not there are not stored, nor added to a stream.
 //   * Few rows: bytes bound the product.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the
 //     parts' order; nothing is left for another kernel and no result depends on timing.  The first weights are on their way before the
 //     CTA waits for the kernel in front.
@@ -94,9 +94,9 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     unsigned char* g_s = w_s + WS * MG_W_BYTES;                   // [2][G rows' boxes [NT][128], 128-byte swizzle like the weights; weights' pieces, rows' pieces]
     float* sums = reinterpret_cast<float*>(w_s);                  // [NT][128], when the stages have been read
     // a group's weights' scales and its rows have barriers of their own: each is waited for by itself where the other was never asked for
-    __shared__ __align__(8) unsigned long long full[WS], empty[WS], gw_full[2], gx_full[2], g_empty[2], acc_full, drained;
+    __shared__ __align__(8) unsigned long long full[WS], empty[WS], gw_full[2], gx_full[2], g_empty[2], acc_full, drained, fed;
     __shared__ unsigned tmem_base_s;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, asked_s[2];                        // asked_s: stages of weights, groups of rows that were asked for
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int part = blockIdx.x, parts = gridDim.x, tile = blockIdx.y, tok0 = blockIdx.z * NT;
     const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0, early = min(min(WS, 2 * G), kbs);
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         for (int s = 0; s < 2; ++s) { t5_mbar_init(&gw_full[s], 1); t5_mbar_init(&gx_full[s], PLAIN ? MG_MAKERS : 1); t5_mbar_init(&g_empty[s], 1); }
         t5_mbar_init(&acc_full, 1);
         t5_mbar_init(&drained, 1);
+        t5_mbar_init(&fed, PLAIN ? 1 : 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         // Weights and their scales are nobody's output: the first of them are on their way before anything else, whatever runs in front.
         for (int kb = 0; kb < early; ++kb) weights(kb, kb);
@@ -135,12 +136,10 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     pdl_invite();                                                 // not before: this CTA's tensor memory is taken
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
 
-    int issued = 0;                                               // stages (warp 6: groups) that were asked for, in the thread that asks
     if (warp == 0) {
         if (lane == 0) {
-            int s = early % WS;
+            int issued = early, s = early % WS;
             unsigned phase = early == WS ? 0 : 1;                 // a barrier that was never used passes for the phase before its first
-            issued = early;
             if (early < kbs) pdl_wait();                          // the rest waits for products anyway, and these for the kernel in front: no bound on that
 #pragma unroll 1
             for (int kb = early; kb < kbs; ++kb) {
@@ -151,10 +150,13 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 issued = kb + 1;
                 if (++s == WS) s = 0, phase ^= 1;
             }
+            asked_s[0] = issued;
+            t5_arrive(&fed);
         }
         __syncwarp();
     } else if (warp == 6 && !PLAIN) {
         if (lane == 0) {
+            int issued = 0;
             pdl_wait();
 #pragma unroll 1
             for (int g = 0; g * G < kbs; ++g) {
@@ -165,6 +167,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 t5_tma_2d(to + G * X_BYTES + S_BYTES, &xs_map, 0, (tok0 / 128) * a.ktiles + kb0 + g * G, &gx_full[g & 1]);
                 issued = g + 1;
             }
+            asked_s[1] = issued;
+            t5_arrive(&fed);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
             }
             if (ok) t5_commit_lead(lead, &g_empty[g]);
         }
-        if (ok) t5_commit_lead(lead, &acc_full);
+        t5_commit_lead(lead, ok ? &acc_full : &drained);          // drained: what was issued has ended, and that was not all
     } else {
         pdl_wait();
         if constexpr (PLAIN) {                                    // warps 2 to 10; rows beyond T keep what stands there, nobody minds
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
             const int quarter = warp & 3, row = quarter * 32 + lane;
             const bool ok = __all_sync(0xffffffffu, mg_wait(&acc_full, 0, a.waits, &abort_flag, a.status));
             t5_fence_after();
-            if (ok)
+            if (ok) {
 #pragma unroll 1
                 for (int c = 0; c < NT / 16; ++c) {
                     unsigned r[16];
@@ -263,6 +267,16 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                     for (int i = 0; i < 16; ++i)
                         if (16 * c + i < toks) sums[(16 * c + i) * MG_ROWS + row] = __uint_as_float(r[i]);
                 }
+            } else {
+                // A wait ran out.  Who asks for copies has stopped; the copies (the stages are where the sums go) and the products end; then NaNs tell
+                // whoever adds the parts up that these sums are not there.  Nothing of it is in the way of a product that does not give up.
+                mg_land(&fed, 0);
+                mg_land_ring(full, WS, asked_s[0]);
+                mg_land_ring(gw_full, 2, (asked_s[0] + G - 1) / G);
+                if (!PLAIN) mg_land_ring(gx_full, 2, asked_s[1]);
+                for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(&drained, 0) && !t5_try_wait(&acc_full, 0); ++i) {}
+                for (int i = 0; i < toks; ++i) sums[i * MG_ROWS + row] = __uint_as_float(0x7fffffffu);
+            }
         }
     }
     t5_fence_before();
@@ -292,6 +306,18 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 if (p < parts) v.x += f[p].x, v.y += f[p].y, v.z += f[p].z, v.w += f[p].w;
             return v;
         };
+        // Whether a sum that is NaN (of four neighbouring features all are) is one of a part that gave up.
+        auto missing = [&](float sum) {
+            if (sum == sum) return false;
+            unsigned quit = 0;
+            for (int p = 0; p < parts; ++p) {
+                unsigned addr, flag;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(addr) : "r"(t5_smem(&abort_flag)), "r"(p));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(flag) : "r"(addr));
+                quit |= flag;
+            }
+            return quit != 0;
+        };
         if constexpr (MODE == MG_GATED) {
             // sixteen lanes a token, four features a lane, eight lanes a block
             const int f = 4 * (tid & 15), step = THREADS / 16 * parts;
@@ -303,7 +329,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                 const float4 g = total((there ? tok : 0) * MG_ROWS + f), u = total((there ? tok : 0) * MG_ROWS + 64 + f);
                 unsigned scale;
                 const unsigned made = mx_gated_codes<true>(g, u, a.act, scale);
-                if (there) {
+                if (there && !missing(g.x + u.x)) {               // for all of a block's lanes
                     const size_t t = tok0 + tok;
                     *reinterpret_cast<unsigned*>(codes + t * a.out_kpad + tile * 64 + f) = made;
                     if ((tid & 7) == 0) a.y_scales[mx_scale_at(t, (tile * 64 + f) / MX_BLOCK, a.out_kpad / MX_K)] = static_cast<unsigned char>(scale);
@@ -315,6 +341,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
 #pragma unroll 2
             for (int tok = first_tok; f < a.N && tok < toks; tok += THREADS / 32 * parts) {
                 const float4 t = total(tok * MG_ROWS + 4 * lane);
+                if (missing(t.x)) continue;
                 float ts[4] = {t.x, t.y, t.z, t.w};
                 TO* to = y + static_cast<size_t>(tok0 + tok) * a.N + f;
                 if (a.vec) {                                      // N a multiple of 4, y aligned
@@ -335,17 +362,6 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
                         if (f + i < a.N) to[i] = from_f32<TO>(MODE == MG_ADD ? ts[i] + to_f32(to[i]) : ts[i]);
                 }
             }
-        }
-    }
-    if (abort_flag) {                                             // whoever gave up: what is under way ends before the CTA goes away
-        if (tid == 0) {
-            mg_land_ring(full, WS, issued);
-            mg_land_ring(gw_full, 2, (issued + G - 1) / G);
-        } else if (!PLAIN && tid == 192) {
-            mg_land_ring(gx_full, 2, issued);
-        } else if (warp == 1) {                                   // the copies of scales and the products, of which there may be none
-            t5_commit_lead(elect_one(), &drained);                // the lane that issued: elect gives the same one for the same lanes
-            mg_land(&drained, 0);
         }
     }
     __syncwarp();
@@ -487,8 +503,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
     unsigned long long* const own = feeds_scales ? s_full : full;
     const unsigned first = mp_map_to(t5_smem(own), 0);            // the first CTA's barriers
     const int ring = feeds_scales ? 2 : MP_STAGES, step = feeds_scales ? MP_QUAD : 1;
+    const unsigned bytes = 2 * (feeds_scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : nt / 2 * MX_K);      // of both CTAs
     auto ask = [&](int tok0, int at, int kb, int s) {
-        const unsigned bytes = 2 * (feeds_scales ? MP_S_BYTES : warp == 0 ? MG_W_READ : nt / 2 * MX_K);      // of both CTAs
         if (rank == 0) t5_expect_tx(&own[s], bytes);
         const unsigned bar = first + s * 8;
         if (warp == 0) mp_tma_2d(w_s + s * MG_W_BYTES, &w_map, 0, (at + kb) * MG_ROWS, bar);
@@ -498,7 +514,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             mp_tma_3d(s_s + s * MP_S_BYTES + MP_QUAD * MX_PIECE, &xs_map, 0, kb, tok0 / 128, bar);
         }
     };
-    int asked = 0;
+    const int steps = (ktiles + step - 1) / step;                 // of a tile
+    int asked = 0;                                                // boxes, or groups of scales, in the thread that asks
 
     if (warp == 0 || warp >= 10) {
         // Three threads feed: the weights (warp 0), the rows (10) and the scales (11).  Asking for a box takes a thread 80 clocks and a
@@ -514,12 +531,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; kb += step) {
                     if (ahead >= 0 && ahead-- == 0) pdl_wait();   // the bounded waits below are not for that kernel
-                    if (!mp_wait(&free[s], phase, a.waits, &abort_flag, a.status)) { ok = false; break; }
+                    if (!mp_wait(&free[s], phase, a.waits, &abort_flag, a.status)) {
+                        asked = (t - cluster) / clusters * steps + kb / step;
+                        ok = false;
+                        break;
+                    }
                     ask(tok0, at, kb, s);
-                    ++asked;
                     if (++s == ring) s = 0, phase ^= 1;
                 }
             }
+            if (ok) asked = (tiles - cluster + clusters - 1) / clusters * steps;
             asked_s[warp == 0 ? 0 : warp - 9] = asked;
         }
         __syncwarp();
@@ -575,6 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             const int toks = min(nt, a.T - tok0);
             bool ok = __all_sync(0xffffffffu, mp_wait(&acc_full[buf], (n >> 1) & 1, a.waits, &abort_flag, a.status));
             ok = mp_all(ok, 1 + half);                            // the four warps meet below: they go on or leave together
+            if (!ok) break;                                       // what has not been computed is not stored
             t5_fence_after();
             const unsigned acc = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * MP_NT;
             if constexpr (MODE == MG_GATED) {
@@ -653,7 +675,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
             t5_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
-            if (!ok) break;
         }
         if (e == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");       // the result is there before this grid is over
     }
@@ -672,7 +693,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                     asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(n) : "r"(mp_map_to(t5_smem(&asked_s[who]), r)) : "memory");
                     most = max(most, n);
                 }
-            const int steps = (ktiles + step - 1) / step;         // of a tile
             for (; asked < most; ++asked) {
                 const int t = cluster + asked / steps * clusters;
                 ask((t % token_tiles) * nt, ((t / token_tiles) * 2 + static_cast<int>(rank)) * ktiles, asked % steps * step, asked % ring);

@@ -41,7 +41,9 @@ def test_a_runner_on_cuda_without_an_index_learns_of_it():
 #: single CTAs of every width with K whole and cut, a matrix that the product takes to 8 bits itself, pairs of CTAs with one tile and several
 SIZES = [(4, 4096, 4096, False, False), (4, 512, 2048, True, False), (3, 1000, 4104, False, True), (16, 700, 12288, True, True), (30, 1024, 4096, False, False),
          (64, 12288, 1024, False, False), (64, 512, 4096, True, False), (2000, 4096, 1024, False, False), (2000, 4096, 640, True, False),
-         (600, 4096, 4096, False, False), (700, 4001, 1024, False, False)]
+         (600, 4096, 4096, False, False), (700, 4001, 1024, False, False),
+         # few tiles and a long K: waits for the sums run out among the stages
+         (4, 128, 65536, False, False), (40, 200, 65536, False, False), (20, 64, 65536, True, False), (2, 128, 65536, False, True)]
 #: tries of a wait: from none to enough for most waits, so that products stop in front of their first stage, among the stages, and not at all
 TRIES = [0, 1, 2, 3] + [2 ** n for n in range(2, 14)]
 
@@ -69,3 +71,54 @@ def test_what_is_under_way_ends_with_the_product(T, N, K, gated, plain):
         status.zero_()
     assert ran_out[0] == (0, 9)
     print(T, N, K, gated, plain, "ran out:", [t for t, c in ran_out if c])
+
+
+@pytest.mark.parametrize("T,N,K,plain", [(T, N, K, plain) for T, N, K, gated, plain in SIZES if not gated] + [(129, 4096, 4096, False), (5000, 2560, 1024, False)])
+def test_what_was_not_computed_is_not_added(T, N, K, plain):
+    """A stream that a product was to be added to: without any tries as it was; with some, every value as it was or with its whole sum."""
+    o, g = ops(), gen(T + N + K + 1)
+    W = o.mx_weight(normal(g, N, K) * K ** -0.5)
+    x = normal(g, T, K, dtype=BF16)
+    X = x if plain else o.mx_rows(x)
+    before = normal(g, T, N)
+    total = o.linear_mx(X, W, residual=before.clone())
+    status = o.stream_status(torch.device(DEV))
+    assert status.tolist() == [0, 0] and not torch.equal(total, before)
+    some = 0
+    try:
+        for tries in TRIES:
+            stream = before.clone()
+            o.linear_mx(X, W, residual=stream, waits=tries)
+            code = status.tolist()[0]
+            status.zero_()
+            assert code == 9 or (code == 0 and torch.equal(stream, total)), tries
+            added = stream != before
+            assert bool((stream[added] == total[added]).all()), tries
+            assert tries > 0 or (code == 9 and not bool(added.any()))
+            some += code == 9 and bool(added.any())
+    finally:
+        status.zero_()
+    print(T, N, K, plain, "added in part:", some)
+
+
+@pytest.mark.parametrize("T,N,K,gated", [(4, 4096, 4096, False), (60, 512, 2048, True), (2000, 4096, 1024, False), (2000, 4096, 640, True), (700, 4001, 1024, False)])
+def test_a_result_that_was_not_computed_is_not_written(T, N, K, gated):
+    """The kernels' own entries with room that the test filled: without tries nothing of it changes."""
+    o, g = ops(), gen(T + N + K + 2)
+    W, X = o.mx_weight(normal(g, 2 * N if gated else N, K), gated=gated), o.mx_rows(normal(g, T, K))
+    status = o.stream_status(torch.device(DEV))
+    at = W.buffer.data_ptr()
+    try:
+        if gated:
+            room = o.MxRows(T, N, torch.device(DEV))
+            room.buffer.fill_(77)
+            rc = o._mx_call("llm_linear_mx_silu_mul")(X.buffer.data_ptr(), None, 0, at, at + W.scales_behind, room.buffer.data_ptr(), T, N, K, 0, 0.0, 0, status.data_ptr(),
+                                                      o._stream())
+            kept = bool((room.buffer == 77).all())
+        else:
+            room = torch.full((T, N), 77.0, device=DEV)
+            rc = o._mx_call("llm_linear_mx")(X.buffer.data_ptr(), None, 0, at, at + W.scales_behind, room.data_ptr(), 0, False, T, N, K, 0, status.data_ptr(), o._stream())
+            kept = bool((room == 77).all())
+        assert rc == 0 and status.tolist()[0] == 9 and kept
+    finally:
+        status.zero_()
