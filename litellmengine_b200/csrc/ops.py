@@ -2579,11 +2579,12 @@ def _mx_count() -> None:
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:
     """residual (float32 [T, N]) += x @ weight^T in the product's epilogue, if the paired kernel or, for a weight in 4 bits, the
     microscaled one takes these operands; False, and nothing done, if not."""
+    if residual.dtype != torch.float32 or not residual.is_contiguous() or residual.shape != (x.shape[0], weight.shape[0]):
+        return False
     if isinstance(weight, MxWeight):
         linear_mx(x, weight, residual=residual)
         return True
-    if (residual.dtype != torch.float32 or not residual.is_contiguous() or residual.shape != (x.shape[0], weight.shape[0])
-            or not _pair_takes(x, weight, weight.shape[0], "into")):
+    if not _pair_takes(x, weight, weight.shape[0], "into"):
         return False
     linear_pair(x, weight, torch.float32, out=residual, accumulate=True)
     return True

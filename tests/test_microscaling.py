@@ -88,3 +88,13 @@ def test_matrices_are_held_in_4_bits_by_parts_that_say_so_of_their_own_forward(m
         for block in model.blocks:
             assert block.mixer.w_qkv == ("4 bits", False) and type(block.feed_forward) is cls
             assert isinstance(block.feed_forward.w_down, tuple) == held and isinstance(block.feed_forward.w_gate_up, tuple) == held
+
+
+def test_a_residual_that_the_product_does_not_take_is_declined():
+    """As with stored weights: False, and nothing done, for a residual that is not float32, not contiguous or of another shape."""
+    W = ops.MxWeight(32, 64, False, torch.device("cpu"))
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for residual in (torch.ones(4, 32, dtype=torch.bfloat16), torch.ones(4, 32, dtype=torch.float64), torch.ones(32, 4).t(), torch.ones(4, 64)[:, ::2], torch.ones(4, 31),
+                     torch.ones(5, 32), torch.ones(128)):
+        assert ops.linear_into(x, W, residual) is False and bool((residual == 1).all())
+    refuses(ops.linear_into, x, W, torch.ones(4, 32))             # one that it takes: no device here
