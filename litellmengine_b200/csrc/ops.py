@@ -7,6 +7,7 @@ compiler or library surfaces as `BuildError`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import weakref
@@ -1883,7 +1884,7 @@ TILE_ROWS, TILE_K = 64, 256
 
 
 def begin_model(matrix_bytes: int, device) -> bool:
-    """Called before a model's weights are loaded with the bytes of its bfloat16 matrices: decides
+    """Called before a model's weights are loaded with the bytes of its matrices, bfloat16 or as its parts will hold them: decides
     whether `prepare_streaming` makes tiled copies for them (all of them or none).  `LLM_TILED=on` /
     `off` overrides the rule."""
     global _tiled_allowed
@@ -1896,6 +1897,17 @@ def begin_model(matrix_bytes: int, device) -> bool:
         _, total = torch.cuda.mem_get_info(device)
         _tiled_allowed = matrix_bytes <= _TILED_SHARE * total
     return _tiled_allowed
+
+
+@contextlib.contextmanager
+def no_tiled_copies():
+    """While matrices are loaded that their part will hold in another form: `prepare_streaming` keeps no copies of them."""
+    global _tiled_allowed
+    was, _tiled_allowed = _tiled_allowed, False
+    try:
+        yield
+    finally:
+        _tiled_allowed = was
 
 
 def tile_weight(weight: torch.Tensor) -> torch.Tensor:

@@ -1,6 +1,7 @@
 """A layer put together from its parts, and the arrangements that wire them."""
 from __future__ import annotations
 
+import contextlib
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -180,22 +181,32 @@ class Block:
         """The parts that may offer a prelude, a graph variant or weights to count."""
         return [p for p in (self.mixer, self.feed_forward) if p is not None]
 
-    def parameters(self) -> Dict[str, ParamSpec]:
+    def parameters(self, of=None) -> Dict[str, ParamSpec]:
+        """What the layer's parts (`of`: these of them) have to be loaded with."""
         out = {}
-        for prefix, part in self._children():
+        for prefix, part in self._children() if of is None else [(n, c) for n, c in self._children() if any(c is p for p in of)]:
             for name, p in part.parameters().items():
                 out[f"{prefix}.{name}" if name else prefix] = p      # '' : the tensor is named like the part
         return out
 
-    def load(self, tensors: Dict[str, torch.Tensor]) -> None:
+    def parts_in_4_bits(self):
+        """The parts whose matrices a model of 4-bit weights holds in that form."""
+        return [p for p in self.parts() if speaks_for_forward(p, "hold_in_4_bits")]
+
+    def load(self, tensors: Dict[str, torch.Tensor], in_4_bits: bool = False) -> int:
+        """Bind the tensors; with `in_4_bits` the matrices of `parts_in_4_bits` are held so from then on (how many those were)."""
+        from ..csrc import ops
+        converted = self.parts_in_4_bits() if in_4_bits else []
         for prefix, part in self._children():
             mine = {n[len(prefix) + 1:]: t for n, t in tensors.items() if n.startswith(prefix + ".")}
             if prefix in tensors and "" in part.parameters():
                 mine[""] = tensors[prefix]
-            part.load({n: t for n, t in mine.items() if n in part.parameters()})
+            with ops.no_tiled_copies() if any(part is p for p in converted) else contextlib.nullcontext():      # what is replaced below needs none
+                part.load({n: t for n, t in mine.items() if n in part.parameters()})
         if self.layer_scales is not None or self.branch_scale != 1.0:
             for norm, ls in zip(self._output_norms(), self.layer_scales or (None, None)):
                 norm.scale_output(self.branch_scale if ls is None else ls.weight * self.branch_scale)
+        return sum(part.hold_in_4_bits() for part in converted)
 
     def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor], ctx: StageContext
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:

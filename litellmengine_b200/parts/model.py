@@ -11,7 +11,7 @@ from ..weights.loader import ParamSpec, WeightSource, check_source, fetch_tensor
 from .block import Block, streams_norm
 from .context import StageContext
 from .norms import PendingSum
-from .registry import lookup, speaks_for_forward
+from .registry import lookup
 from .rejoin import REJOINS, AddedEmbedding
 
 
@@ -79,6 +79,12 @@ class Model:
                                        optional_alias=p.embedding_name if p.tie_word_embeddings else None)
         return out
 
+    def _names_in_4_bits(self) -> set:
+        """The tensors whose matrices are held in 4 bits once they are loaded."""
+        if self.weight_format != "mxfp4":
+            return set()
+        return {f"{spec.weight_prefix}.{name}" for spec, block in zip(self.plan.blocks, self.blocks) for name in block.parameters(block.parts_in_4_bits())}
+
     @staticmethod
     def _norm_tensor(prefix: str, k: int, name: str) -> str:
         """A model's own norm: its first tensor is named like the norm itself; further ones (a bias, a scalar) stand beside it."""
@@ -91,7 +97,8 @@ class Model:
         params = self.parameters()
         aliased = check_source(params, source, where)
         if self.dtype == torch.bfloat16:               # one decision for all of the model's matrices
-            ops.begin_model(sum(2 * ps.shape[0] * ps.shape[1] for n, ps in params.items()
+            in_4_bits = self._names_in_4_bits()
+            ops.begin_model(sum(ps.shape[0] * ps.shape[1] * 17 // 32 if n in in_4_bits else 2 * ps.shape[0] * ps.shape[1] for n, ps in params.items()
                                 if len(ps.shape) == 2 and n not in aliased), self.device)
         get = lambda n: fetch_tensor(source, n, params[n], self.dtype, self.device)
         have = set(source.names())
@@ -99,10 +106,9 @@ class Model:
         held = 0
         for spec, block in zip(p.blocks, self.blocks):
             # a tensor that may be absent and is: the part is handed nothing for it
-            block.load({n: get(f"{spec.weight_prefix}.{n}") for n, ps in block.parameters().items()
-                        if not (ps.optional and f"{spec.weight_prefix}.{n}" not in have)})
-            if self.weight_format == "mxfp4":              # a layer's stored matrices are gone before the next one's come
-                held += sum(part.hold_in_4_bits() for part in block.parts() if speaks_for_forward(part, "hold_in_4_bits"))
+            # (in 4 bits: a layer's stored matrices are gone before the next one's come)
+            held += block.load({n: get(f"{spec.weight_prefix}.{n}") for n, ps in block.parameters().items()
+                                if not (ps.optional and f"{spec.weight_prefix}.{n}" not in have)}, in_4_bits=self.weight_format == "mxfp4")
         if self.weight_format == "mxfp4" and not held:
             raise ValueError("weight_format 'mxfp4': no part of this model holds its matrices in 4 bits")
         for norm, prefix in ((self.final_norm, p.final_norm_name), (self.embedding_norm, p.embedding_norm_name)):
