@@ -36,7 +36,7 @@ Options:
   --seed <int>             Seed of the sampling stream and of --random-weights, default: 0
   --device <str>           cuda, cuda:N, gpu or auto (there is no CPU path)
   --dtype <str>            bfloat16 (default) or float32
-  --weight-format <str>    stored (default), or mxfp4: attention's and feed-forwards' matrices in 4 bits
+  --weight-format <str>    stored (default), or mxfp4: softmax attention's and dense feed-forwards' matrices in 4 bits
   --eos-token-id <int>     Stop generation when this token id is generated
   --page-size <N>          Paged KV cache page size, default 16
   --max-total-tokens <N>   Tokens the cache pool holds, default: prompt + max tokens + 16

@@ -8,8 +8,9 @@
 // that are not there.  A stage is 128 values of K: a box of the weight's tile (8 KB; the copy engine spreads its 4-bit codes over
 // 16 KB, sixteen of them and eight bytes of nothing, as the products read them, and counts the 8 KB on its barrier), a box of the rows, and
 // the pieces of both operands' scales, which the tensor core copies to its own memory in front of the stage's four products.
-// Roles here: warp 0 feeds the weights and their scales, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and theirs; all of them write
-// the result.  Waits are bounded: one that runs out sets status code 9, and the copies and products that are under way then end, which is waited for
+// Roles of single CTAs: warp 0 feeds the weights and their scales, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and theirs; all of them write
+// the result.  Of a pair's CTA: warp 0 feeds the weights, 10 the rows and 11 the scales, warp 1 of the first CTA issues, 2 to 5 and 6 to 9 write the result
+// in turns.  Waits are bounded: one that runs out sets status code 9, and the copies and products that are under way then end, which is waited for
 // on their own barriers (bounded too), before the CTA does; sums that are not there are not stored, nor added to a stream.
 //   * Few rows: bytes bound the product.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the
 //     parts' order; nothing is left for another kernel and no result depends on timing.  The first weights are on their way before the
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
     }
     t5_fence_before();
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-    // What the warp's first token is added to is on its way while the parts meet (an 8B-shape decode step of 32 requests 2.23 ms, 2.29 without).
+    // What the warp's first token is added to is on its way while the parts meet (an 8B-shape decode step of 32 requests 2.24 ms, 2.27 without).
     const int feature = tile * MG_ROWS + 4 * lane, first_tok = part + warp * parts;
     float4 old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if constexpr (MODE == MG_ADD) {
@@ -627,7 +628,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MP_THREADS, 1) linea
                 }
             } else if (a.vec) {
                 // 8 KB at a time through shared memory and out by the copy engine, which also adds and leaves out what is beyond
-                // the matrix.  Stores straight from the lanes (a token's 32 features, 64 bytes) took longer than a tile's products.
+                // the matrix.  By it and by stores straight from the lanes (a token's 32 features), us, float32 / bfloat16 / added: 4,096 x 1,024 by 6,144
+                // 37.5, 39.8 / 31.6, 39.4 / 49.6, 69.6; 700 x 4,096 by 4,096 14.5, 14.9 / 13.9, 15.1 / 15.3, 18.8; 2,048 x 4,096 by 4,096 32.0, 32.4 / 29.9,
+                // 30.8 / 35.4, 36.6; 4,096 x 4,096 by 6,144 82.7, 86.2 / 77.0, 78.0 / 90.9, 89.6, and by 24,576, under the power cap, 318, 347 / 316,
+                // 318 / 375, 362: only long additions are a little faster from the lanes.
 #pragma unroll 1
                 for (int c = CHUNK * half; c < toks; c += 2 * CHUNK, ++turns) {
                     unsigned r[CHUNK];

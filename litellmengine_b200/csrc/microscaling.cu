@@ -3,7 +3,8 @@
 //   weights of 4     from a matrix, gate and up rows of a fused matrix 64 by 64 beside each other
 //   values           of either, as float32 or bfloat16
 // Everything is bound by memory: each value is read once and each code written once.  A lane holds eight neighbouring values
-// (16 or 32 bytes a load), a block's largest magnitude takes two exchanges between lanes, and the codes are the converter's.
+// (16 or 32 bytes a load) and a block's largest magnitude takes two exchanges between lanes; of a bfloat16 matrix of whole, aligned pieces sixteen (two
+// loads) and one exchange.  The codes are the converter's.
 #include "microscaling.cuh"
 #include <type_traits>
 
@@ -173,6 +174,8 @@ __device__ __forceinline__ void mx_norm_row(const float (&v)[CH][8], F rests, co
         mx_store_codes8(make_uint2(mx_e4m3x4(t[0], t[1], t[2], t[3]), mx_e4m3x4(t[4], t[5], t[6], t[7])), mx_word(scale), col < kpad, row, col, kpad, codes, scales);
     }
 }
+// Blocks of up to 1,024 threads leave 64 registers a thread: one piece (widths of up to 8,192) fits, of two 12 to 56 bytes are spilled (up to 16,384),
+// of four 368 to 912 (up to 32,768), beside the 64 KB and more that a row then moves.
 template <typename TX, typename TD, int CH, bool FAST>
 __global__ void __launch_bounds__(1024) mx_norm_kernel(const TX* x, const TD* __restrict__ delta, const float* __restrict__ w,
                                                        TX* sum_out, unsigned char* __restrict__ codes,

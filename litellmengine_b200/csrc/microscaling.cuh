@@ -208,7 +208,7 @@ static inline int mx_vec(int a, int b) { return a < b ? a : b; }
 struct MxAct {
     float limit, alpha, beta, shift;
     double alpha64, beta64;
-    unsigned near;                        // places that mx_gated may be off by, twice over
+    unsigned near;                        // places beside a border within which a value is made in 64 bits: more than mx_gated is off by (mx_act)
 };
 __device__ __forceinline__ float mx_gated(float g, float u, const MxAct& a) {
     g = g > a.limit ? a.limit : g;
@@ -227,7 +227,7 @@ static __device__ __noinline__ float mx_gated_carried(float g, float u, double a
 // Codes and scale of four neighbouring features of a token, eight lanes a block.  CARRY: a value beside a border between two codes, or a block whose
 // largest is beside one between two scales, is made in 64 bits, one in 30,000 (the lowest codes, 2^-15 of a block's largest, may be a step off): what
 // is left is the rounding of the sums.  Of 25 million codes 26 are off without it, as with float32 throughout, 11 with it; it costs products of
-// few rows nothing, those of many 5 % (2,045 x 2 x 12,288 x 4,096 167 to 175 us), which do without.
+// few rows nothing, those of many 5 % (2,045 x 2 x 12,288 x 4,096 167 to 175 us), which do without, as rows made of gate and up values in memory do.
 template <bool CARRY> __device__ __forceinline__ unsigned mx_gated_codes(const float4& g, const float4& u, const MxAct& a, unsigned& scale) {
     float v[4] = {mx_gated(g.x, u.x, a), mx_gated(g.y, u.y, a), mx_gated(g.z, u.z, a), mx_gated(g.w, u.w, a)};
     auto largest = [&]() {
@@ -257,7 +257,7 @@ template <bool CARRY> __device__ __forceinline__ unsigned mx_gated_codes(const f
     return mx_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 }
 // mx_gated is off by up to 10 places (expf 2 of 2^-23, the division as much, each other step a half); where its exponent z is itself rounded, by up to 8 more for
-// each of z, which is at most 75 before a value is nothing beside 2^-95.
+// each of z, which is at most 75 before a value is nothing beside 2^-95: 610.  What is taken as beside a border is the next power of two, 16 and 1,024.
 static inline bool mx_act(int kind, float limit, MxAct* a) {
     if (kind < 0 || kind > 2 || (kind == 2 && !(limit > 0.0f))) return false;
     constexpr double gelu = 1.5957691216057308;                   // 2 sqrt(2 / pi)

@@ -2548,7 +2548,8 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
               waits: int = STREAM_WAITS) -> torch.Tensor:
     """x [T, K] @ weight[N, K]^T with the weight in 4 bits and x in 8 (`MxRows`; a matrix is taken to 8 bits first), products exact,
     sums in float32, on the block-scaled tcgen05 products.  The result is float32 or bfloat16 [T, N]; with `residual` (float32
-    [T, N]) it is added to that in place, which is returned."""
+    [T, N]) it is added to that in place, which is returned.  Where a wait runs out (`stream_status`), what was not computed is neither stored nor
+    added."""
     rows, plain, dt, T, K = _mx_operands(x, weight, False)
     N = weight.shape[0]
     if residual is not None:
@@ -2569,7 +2570,9 @@ def linear_mx(x, weight: MxWeight, out_dtype: torch.dtype = torch.float32, resid
 
 def linear_silu_mul_mx(x, weight: MxWeight, activation: str = "silu", limit: float = 0.0, waits: int = STREAM_WAITS) -> MxRows:
     """act(x @ gate^T) * (x @ up^T) as rows of 8 bits [T, I] for a gated weight [2I, K] in 4 bits, act as in `silu_and_mul`, in the
-    product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits."""
+    product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits.  Products of few rows make values beside a border between
+    two codes in 64 bits; those of many, and `silu_and_mul_mx`, do not: one code in a million may be the neighbour of what another number of
+    rows gives."""
     act = ACTIVATIONS[activation]
     rows, plain, dt, T, K = _mx_operands(x, weight, True)
     inter = weight.shape[0] // 2
@@ -2682,7 +2685,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     product `linear_pair`; by default only the gate/up product does, through `linear_silu_mul`) (the reference uses cuBLAS for all its products,
     src/layers/linear.cu:169-215).  bfloat16 operands accumulate in float32; a float32 weight
     keeps its product in true float32 (no TF32), whatever x is: up to 16 rows in the engine's own streaming kernel, more rows of large matrices
-    on the tensor cores as sums of three bfloat16 values each, as near as float32 sums.  bfloat16 weights may be read before the
+    on the tensor cores as sums of three bfloat16 values each, as near as float32 sums.  bfloat16 weights and those in 4 bits may be read before the
     kernel in front of the product in the stream has finished (they are nobody's output); float32 ones are not.  A weight in 4
     bits (`MxWeight`) goes to `linear_mx`, which also takes `MxRows` (their result is bfloat16 without an `out_dtype`)."""
     if isinstance(weight, MxWeight):

@@ -439,9 +439,7 @@ class GatedAttentionMixer(BranchMixer):
         return decode_key_splits(self.device, n_dec, self.nkv, decode_reach(batch, self.span)) if n_dec and (self._wide or not n_tiles) else 0
 
     def hold_in_4_bits(self) -> int:
-        """As `AttentionMixer.hold_in_4_bits`; a branch whose matrices its parent has holds none."""
-        if self.w_in is None:
-            return 0
+        """As `AttentionMixer.hold_in_4_bits`."""
         self.w_in, self.w_o = ops.mx_weight(self.w_in), ops.mx_weight(self.w_o)
         return 2
 

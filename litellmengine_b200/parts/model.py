@@ -37,7 +37,9 @@ class Model:
 
     def __init__(self, plan: ModelPlan, dtype="bfloat16", device="cuda", weight_format: str = "stored"):
         """`weight_format` 'mxfp4': the matrices of the parts that can (`hold_in_4_bits`: softmax attention's projections, dense
-        feed-forwards) are taken to 4 bits with a scale per 32 values when they are loaded, and multiply rows of 8 bits."""
+        feed-forwards) are taken to 4 bits with a scale per 32 values when they are loaded, and multiply rows of 8 bits; all others (routed
+        experts, recurrent and latent mixers, the embedding, the output head) stay as stored.  Layers of width 1,024 lose the products that make
+        their own input by it: decode steps of up to 16 requests take 2 to 9 % longer, larger ones and prompts less time, as all steps of width 2,048 do."""
         plan.validate()
         self.plan = plan
         self.dtype = _compute_dtype(dtype)

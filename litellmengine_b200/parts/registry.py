@@ -39,7 +39,7 @@ hands to that product.  Both are read with `speaks_for_forward`: a class that de
 says so again or is called as any other.
 
 A mixer or feed-forward whose forward gives its matrices to `ops.linear`, `linear_silu_mul` and `linear_into` only may have
-`hold_in_4_bits()`, which replaces them by `ops.MxWeight`s once they are loaded and says how many those were: models of 4-bit weights call it.
+`hold_in_4_bits()`, which replaces them by `ops.MxWeight`s once they are loaded and says how many those were: blocks of models with 4-bit weights call it.
 Where the weight that `first_product()` names is one, a norm with `makes_mx_rows = True` and `forward_mx(h, delta)` hands the part its input
 as `ops.MxRows`.  Both are read with `speaks_for_forward` too.
 
