@@ -227,7 +227,7 @@ static __device__ __noinline__ float mx_gated_carried(float g, float u, double a
 // Codes and scale of four neighbouring features of a token, eight lanes a block.  CARRY: a value beside a border between two codes, or a block whose
 // largest is beside one between two scales, is made in 64 bits, one in 30,000 (the lowest codes, 2^-15 of a block's largest, may be a step off): what
 // is left is the rounding of the sums.  Of 25 million codes 26 are off without it, as with float32 throughout, 11 with it; it costs products of
-// few rows nothing, those of many 5 % (2,045 x 2 x 12,288 x 4,096 167 to 175 us), which do without, as rows made of gate and up values in memory do.
+// few rows nothing, those of many 5 to 33 % (300 x 2 x 4,096 x 4,096 18.3 to 19.3 us, 2,045 x 2 x 12,288 x 4,096 162 to 215), which do without, as rows made of gate and up values in memory do.
 template <bool CARRY> __device__ __forceinline__ unsigned mx_gated_codes(const float4& g, const float4& u, const MxAct& a, unsigned& scale) {
     float v[4] = {mx_gated(g.x, u.x, a), mx_gated(g.y, u.y, a), mx_gated(g.z, u.z, a), mx_gated(g.w, u.w, a)};
     auto largest = [&]() {
