@@ -366,8 +366,8 @@ __global__ void __launch_bounds__(MG_THREADS(PLAIN), 2) linear_mx_kernel(const _
         }
     }
     __syncwarp();
-    // Nobody leaves while its sums are read.  A thread that is here has all that it read, because it has made what it stored of it (none is read that is
-    // not); the stores themselves need not be out yet, which a release would wait for (one row x 4,096 by 6,144 5.5 us, 5.8 with it; an 8B-shape
+    // Nobody leaves while its sums are read.  A thread that is here has all that it read, because it has made what it stored of it, or has seen that it is
+    // NaN and of a part that gave up; the stores themselves need not be out yet, which a release would wait for (one row x 4,096 by 6,144 5.5 us, 5.8 with it; an 8B-shape
     // decode step of 4 requests 1.82 ms, 1.87).
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     if (warp == 1) {
