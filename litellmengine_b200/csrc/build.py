@@ -52,11 +52,14 @@ FAMILIES: Dict[str, List[str]] = {
     "gemm_f32": ["gemm_f32.cu"],
     "gemm_f32_tcgen05": ["gemm_f32_tcgen05.cu"],
     "microscaling": ["microscaling.cu", "gemm_mx_tcgen05.cu"],
+    "blocks_f8": ["f8_blocks.cu", "gemm_f8_tcgen05.cu"],
     "host_core": ["host_core.cpp"],            # the host side's bookkeeping: plain C++, no device code
 }
 HOST_FAMILIES = {"host_core"}
 HEADERS = ["common.cuh", "mma_tiles.cuh", "split_mma.cuh", "tcgen05_attention.cuh", "attention_decode_noalloc.h", "attention_decode_tma.cuh",
            "microscaling.cuh"]
+# Headers of some families only, so that a change of one leaves the others' libraries as they are.
+FAMILY_HEADERS: Dict[str, List[str]] = {"blocks_f8": ["f8_blocks.cuh"]}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
@@ -124,7 +127,7 @@ def _build_dir_locked() -> str:
 
 def _digest(family: str) -> str:
     h = hashlib.sha256()
-    for fn in ([] if family in HOST_FAMILIES else HEADERS) + FAMILIES[family]:
+    for fn in ([] if family in HOST_FAMILIES else HEADERS) + FAMILY_HEADERS.get(family, []) + FAMILIES[family]:
         with open(os.path.join(CSRC, fn), "rb") as f:
             h.update(fn.encode())
             h.update(f.read())

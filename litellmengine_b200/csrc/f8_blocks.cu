@@ -1,0 +1,369 @@
+// What makes rows and weights of 8 bits under float32 scales (f8_blocks.cuh has the format), what reads them back, and what stands around products
+// of rows that are sorted by expert:
+//   rows      from a matrix; a row may go to several places, one for each expert that its token has picked
+//   weights   from a matrix or a stack of them, gate and up rows 64 by 64 beside each other
+//   values    of either, as float32 or bfloat16
+//   sorting   (token, choice) pairs by expert, and the experts' rows cut into tiles
+//   adding up a token's rows, in the order of its choices
+// Everything is bound by memory: each value is read once and each code written once.
+#include "f8_blocks.cuh"
+
+#define F8_THREADS 256
+
+// ---- rows from a matrix ---------------------------------------------------------------------------------------------
+// Sixteen lanes a block of a row, eight values a lane (16 or 32 bytes); a warp takes U times two blocks, all asked for before the first is used.
+template <typename T> struct F8Raw { typedef uint4 type; };
+template <> struct F8Raw<float> { struct type { float v[8]; }; };
+__device__ __forceinline__ unsigned f8_most(const uint4& r) { return mx_most8(r); }
+__device__ __forceinline__ unsigned f8_most(const F8Raw<float>::type& r) { return mx_most8(r.v); }
+__device__ __forceinline__ uint2 f8_codes(const uint4& r, unsigned most, float inverse) { return f8_codes8(r, most, inverse); }
+__device__ __forceinline__ uint2 f8_codes(const F8Raw<float>::type& r, unsigned most, float inverse) { return f8_codes8(r.v, most, inverse); }
+template <bool FAST> __device__ __forceinline__ void f8_load(const bf16* row, int col, int n, uint4& r) {
+    r = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (FAST) {
+        if (col < n) mx_raw8(row + col, r);
+    } else {
+        unsigned short h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < n) h[i] = __bfloat16_as_ushort(row[col + i]);
+        r = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
+}
+template <bool FAST> __device__ __forceinline__ void f8_load(const float* row, int col, int n, F8Raw<float>::type& r) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = 0.0f;
+    if constexpr (FAST) {
+        if (col < n) load8(row + col, r.v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < n) r.v[i] = row[col + i];
+    }
+}
+
+template <int U, bool FAST, typename T>
+__global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, float* __restrict__ scales, unsigned items,
+                                                             unsigned per_row, int K, int ktiles, long long padded, const int32_t* __restrict__ places, int top) {
+    pdl_begin();
+    const unsigned w = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5);
+    if (w >= items) return;                                       // whole warps
+    const unsigned row = w / per_row;
+    const int lane = threadIdx.x & 31, first = (w - row * per_row) * (2 * U) + (lane >> 4);       // of the lane's tiles of K
+    typename F8Raw<T>::type raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) f8_load<FAST>(x + static_cast<size_t>(row) * K, (first + 2 * u) * F8_K + (lane & 15) * 8, K, raw[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int kb = first + 2 * u;
+        const unsigned most = f8_most16(f8_most(raw[u]));
+        const F8Scale s = f8_scale(most);
+        const uint2 c = f8_codes(raw[u], most, s.inverse);
+        if (kb >= ktiles) continue;
+        for (int k = 0; k < top; ++k) {
+            const long long to = places ? static_cast<long long>(places[static_cast<size_t>(row) * top + k]) : static_cast<long long>(row);
+            if (to < 0) continue;                                 // a pick without an expert
+            *reinterpret_cast<uint2*>(codes + (kb * padded + to) * F8_K + (lane & 15) * 8) = c;
+            if ((lane & 15) == 0) scales[kb * padded + to] = s.scale;
+        }
+    }
+}
+
+extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padded, int T, int K, const int32_t* places, int top, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    if (K <= 0 || K > (1 << 20) || T > (1 << 24) || top <= 0 || padded < T) return LLM_REFUSED_SIZE;
+    if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
+    const int ktiles = f8_tiles(K), esz = dtype == LLM_DT_F32 ? 4 : 2;
+    const bool fast = K % 8 == 0 && aligned16(x) && static_cast<long long>(K) * esz % 16 == 0;
+    // four tiles of K a lane where that leaves every SM with enough warps
+    const bool many = static_cast<long long>(T) * ktiles >= 32 * 1024;
+    const unsigned u = many ? 4 : 1, per_row = (ktiles + 2 * u - 1) / (2 * u);
+    const long long items = static_cast<long long>(T) * per_row;
+    if (items >= (1LL << 31)) return LLM_REFUSED_SIZE;
+    const dim3 grid(static_cast<unsigned>((items + F8_THREADS / 32 - 1) / (F8_THREADS / 32)));
+    unsigned char* codes = static_cast<unsigned char*>(rows);
+    float* scales = f8_row_scales(rows, padded, ktiles);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+#define LAUNCH(U, FAST, T_)                                                                                                                       \
+    launch_pdl((f8_rows_kernel<U, FAST, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(x), codes, scales, static_cast<unsigned>(items), per_row, K, \
+               ktiles, padded, places, places ? top : 1)
+#define LAUNCH_T(T_)                                        \
+    if (many) { if (fast) LAUNCH(4, true, T_); else LAUNCH(4, false, T_); } \
+    else { if (fast) LAUNCH(1, true, T_); else LAUNCH(1, false, T_); }
+    if (dtype == LLM_DT_BF16) { LAUNCH_T(bf16) }
+    else if (dtype == LLM_DT_F32) { LAUNCH_T(float) }
+    else return LLM_REFUSED_DTYPE;
+#undef LAUNCH_T
+#undef LAUNCH
+    return launch_status();
+}
+
+// ---- weights --------------------------------------------------------------------------------------------------------
+// A CTA a block of 128 x 128: sixteen lanes a row, two rows a warp and trip, eight trips that are asked for together.  It does not invite the kernel behind
+// it: products fetch weights before they wait for what is in front of them.
+template <bool FAST, typename T>
+__global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ codes, float4* __restrict__ scales, int rows, int K,
+                                                               int tiles, int ktiles, int gate_rows, long long row_stride, long long matrix_stride) {
+    __shared__ unsigned most_s[F8_THREADS / 32];
+    pdl_wait();
+    const int kb = blockIdx.x, block = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T* from = w + blockIdx.z * matrix_stride + static_cast<long long>(block) * 128 * row_stride;
+    const int col = kb * F8_K + (lane & 15) * 8, there = rows - block * 128;
+    const long long stack = static_cast<long long>(blockIdx.z) * tiles;
+    codes += stack * ktiles * F8_TILE + kb * F8_TILE + (lane & 15) * 8;
+    scales += stack * ktiles + kb;
+    if (gate_rows && there <= 0) {                                // one CTA more: the rows of whole tiles that gate and up do not have
+        for (int f = gate_rows + warp * 2 + (lane >> 4); f < tiles * 64; f += F8_THREADS / 16)
+            for (int up = 0; up < 2; ++up) *reinterpret_cast<uint2*>(codes + static_cast<long long>(f >> 6) * ktiles * F8_TILE + (up * 64 + (f & 63)) * F8_K) = make_uint2(0u, 0u);
+        const int empty = (gate_rows + 63) / 64 + threadIdx.x;    // tiles of nothing else
+        if (empty < tiles) scales[static_cast<long long>(empty) * ktiles] = make_float4(F8_LEAST, F8_LEAST, F8_LEAST, 0.0f);
+        return;
+    }
+    typename F8Raw<T>::type raw[8];
+    unsigned most = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int r = u * 16 + warp * 2 + (lane >> 4);
+        f8_load<FAST>(from + r * row_stride, col, r < there ? K : 0, raw[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) most = max(most, f8_most(raw[u]));
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) most_s[warp] = most;
+    __syncthreads();
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < F8_THREADS / 32; ++i) most = max(most, most_s[i]);
+    const F8Scale s = f8_scale(most);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int r = block * 128 + u * 16 + warp * 2 + (lane >> 4), up = gate_rows && r >= gate_rows, f = up ? r - gate_rows : r;
+        const int tile = gate_rows ? f >> 6 : r >> 7, at = gate_rows ? up * 64 + (f & 63) : r & 127;
+        if (!gate_rows || r < rows)
+            *reinterpret_cast<uint2*>(codes + static_cast<long long>(tile) * ktiles * F8_TILE + at * F8_K) = f8_codes(raw[u], most, s.inverse);
+    }
+    if (!gate_rows) {
+        if (threadIdx.x == 0) scales[static_cast<long long>(block) * ktiles] = make_float4(s.scale, s.scale, s.scale, 0.0f);
+    } else if (threadIdx.x < 4) {                                 // the tiles whose gate rows, first up row or last up row lie in this block
+        const int first = block * 128, i = first / 64 + threadIdx.x, j = (first - gate_rows) / 64 - 1 + static_cast<int>(threadIdx.x);
+        if (i * 64 < gate_rows && i * 64 / 128 == block) scales[static_cast<long long>(i) * ktiles].x = s.scale;
+        if (j >= 0 && j * 64 < gate_rows) {
+            if ((gate_rows + j * 64) / 128 == block) scales[static_cast<long long>(j) * ktiles].y = s.scale;
+            if ((gate_rows + min(j * 64 + 63, gate_rows - 1)) / 128 == block) scales[static_cast<long long>(j) * ktiles].z = s.scale;
+        }
+    }
+}
+
+// N: rows of a matrix (gated: of gate); tiles: of 128 rows as the weight has them, an even number.
+extern "C" int llm_f8_weight(const void* w, int dtype, void* codes, void* scales, int E, int N, int K, int tiles, int gated, long long row_stride,
+                             long long matrix_stride, uintptr_t stream) {
+    if (E <= 0 || E > 65535 || N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 20) || tiles != (gated ? 2 * ((N + 127) / 128) : (N + 255) / 256 * 2)) return LLM_REFUSED_SIZE;
+    if (tiles > 65535 || row_stride < 0 || matrix_stride < 0) return LLM_REFUSED_SIZE;
+    if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    const int esz = dtype == LLM_DT_F32 ? 4 : 2;
+    const bool fast = K % 8 == 0 && aligned16(w) && row_stride * esz % 16 == 0 && matrix_stride * esz % 16 == 0;
+    const int rows = gated ? 2 * N : N, blocks = gated ? (rows + 127) / 128 + (N % 128 ? 1 : 0) : tiles;
+    if (blocks > 65535) return LLM_REFUSED_SIZE;
+    const dim3 grid(f8_tiles(K), blocks, E);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+#define LAUNCH(FAST, T_)                                                                                                                              \
+    launch_pdl((f8_weight_kernel<FAST, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(w), static_cast<unsigned char*>(codes), \
+               static_cast<float4*>(scales), rows, K, tiles, f8_tiles(K), gated ? N : 0, row_stride, matrix_stride)
+    if (dtype == LLM_DT_BF16) { if (fast) LAUNCH(true, bf16); else LAUNCH(false, bf16); }
+    else if (dtype == LLM_DT_F32) { if (fast) LAUNCH(true, float); else LAUNCH(false, float); }
+    else return LLM_REFUSED_DTYPE;
+#undef LAUNCH
+    return launch_status();
+}
+
+// ---- values ---------------------------------------------------------------------------------------------------------
+// Eight lanes a tile's row, sixteen codes a lane, U rows a thread asked for together.
+template <int U, bool FAST, typename T>
+__global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned char* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, int rows,
+                                                               int N, int K, int ktiles, int tiles, long long padded, int kind) {
+    // kind 0: rows, 1: a weight, 2: a gated one (N: its gate rows); tiles: of 128 rows
+    pdl_begin();
+    const int kb = blockIdx.x % ktiles, piece = threadIdx.x & 7, col = kb * F8_K + piece * 16;
+    const long long first = static_cast<long long>(blockIdx.x / ktiles) * (U * (F8_THREADS / 8)) + (threadIdx.x >> 3);
+    uint4 c[U];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long r = first + u * (F8_THREADS / 8);
+        c[u] = make_uint4(0u, 0u, 0u, 0u);
+        s[u] = 0.0f;
+        if (r >= rows) continue;
+        if (kind == 0) {
+            c[u] = *reinterpret_cast<const uint4*>(codes + (kb * padded + r) * F8_K + piece * 16);
+            s[u] = scales[kb * padded + r];
+        } else {
+            const int per = kind == 2 ? 2 * N : N;                // rows of a matrix of the stack
+            const long long e = r / per;
+            const int at = static_cast<int>(r - e * per), up = kind == 2 && at >= N, i = up ? at - N : at;
+            const long long tile = e * tiles + (kind == 2 ? (i >> 6) : (i >> 7));
+            const int in = kind == 2 ? up * 64 + (i & 63) : i & 127, which = !up ? 0 : (i & 63) < f8_split(N, i >> 6) ? 1 : 2;
+            c[u] = *reinterpret_cast<const uint4*>(codes + ((tile * ktiles + kb) * 128 + in) * F8_K + piece * 16);
+            s[u] = scales[(tile * ktiles + kb) * 4 + which];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long r = first + u * (F8_THREADS / 8);
+        if (r >= rows || col >= K) continue;
+        float v[16];
+        mx_from_e4m3x4(c[u].x, v);
+        mx_from_e4m3x4(c[u].y, v + 4);
+        mx_from_e4m3x4(c[u].z, v + 8);
+        mx_from_e4m3x4(c[u].w, v + 12);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= s[u];
+        T* to = out + r * K + col;
+#pragma unroll
+        for (int h = 0; h < 16; h += 8) {
+            if (FAST) {
+                if (col + h < K) store8(to + h, *reinterpret_cast<float(*)[8]>(v + h));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (col + h + i < K) to[h + i] = from_f32<T>(v[h + i]);
+            }
+        }
+    }
+}
+
+extern "C" int llm_f8_values(const void* codes, const void* scales, void* out, int dtype, int rows, int N, int K, int tiles, long long padded, int kind, uintptr_t stream) {
+    if (rows <= 0) return LLM_OK;
+    if (K <= 0 || K > (1 << 20) || kind < 0 || kind > 2 || (kind && N <= 0)) return LLM_REFUSED_SIZE;
+    constexpr int U = 4;                                          // 128 rows a CTA
+    const int esz = dtype == LLM_DT_F32 ? 4 : 2, ktiles = f8_tiles(K);
+    const long long blocks = (static_cast<long long>(rows) + 127) / 128 * ktiles;
+    if (blocks >= (1LL << 31)) return LLM_REFUSED_SIZE;
+    const bool fast = K % 8 == 0 && aligned16(out) && static_cast<long long>(K) * esz % 16 == 0;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+#define LAUNCH(FAST, T_)                                                                                                                              \
+    launch_pdl((f8_values_kernel<U, FAST, T_>), dim3(static_cast<unsigned>(blocks)), dim3(F8_THREADS), 0, s, static_cast<const unsigned char*>(codes), \
+               static_cast<const float*>(scales), static_cast<T_*>(out), rows, N, K, ktiles, tiles, padded, kind)
+    if (dtype == LLM_DT_BF16) { if (fast) LAUNCH(true, bf16); else LAUNCH(false, bf16); }
+    else if (dtype == LLM_DT_F32) { if (fast) LAUNCH(true, float); else LAUNCH(false, float); }
+    else return LLM_REFUSED_DTYPE;
+#undef LAUNCH
+    return launch_status();
+}
+
+// ---- rows sorted by expert ------------------------------------------------------------------------------------------
+// One block: counts the picks of each expert, lays the experts' rows one after another, cuts them into items of up to `per` rows, and gives every pick
+// its row: places[pick] (-1 where the pick is no expert), tokens[row], weights[row].  Which of an expert's rows a pick gets is not fixed; no
+// result depends on it, a row's products being its own.
+__global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* __restrict__ ids, const float* __restrict__ weights, int picks, int top, int E, int per,
+                                                       int32_t* __restrict__ counts, int4* __restrict__ items, int32_t* __restrict__ places,
+                                                       int32_t* __restrict__ tokens, float* __restrict__ row_weights) {
+    extern __shared__ int next_s[];                               // [E] picks, then the next row of an expert
+    __shared__ int2 warps_s[32];
+    pdl_begin();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    for (int e = tid; e < E; e += blockDim.x) next_s[e] = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (int p = tid; p < picks; p += blockDim.x) {
+        const int e = ids[p];
+        if (e >= 0 && e < E) atomicAdd(&next_s[e], 1);
+    }
+    __syncthreads();
+    int2 base = make_int2(0, 0);                                  // rows and items of the experts before this round's
+    for (int e0 = 0; e0 < E; e0 += blockDim.x) {
+        const int e = e0 + tid, n = e < E ? next_s[e] : 0;
+        int2 sum = make_int2(n, (n + per - 1) / per);
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int a = __shfl_up_sync(0xffffffffu, sum.x, o), b = __shfl_up_sync(0xffffffffu, sum.y, o);
+            if (lane >= o) sum.x += a, sum.y += b;
+        }
+        if (lane == 31) warps_s[warp] = sum;
+        __syncthreads();
+        int2 total = base;
+        for (int w = 0; w < warps; ++w) {
+            if (w == warp) sum.x += total.x, sum.y += total.y;
+            total.x += warps_s[w].x, total.y += warps_s[w].y;
+        }
+        if (e < E) {
+            const int row = sum.x - n;
+            int item = sum.y - (n + per - 1) / per;
+            next_s[e] = row;
+            for (int at = 0; at < n; at += per) items[item++] = make_int4(e, row + at, min(per, n - at), 0);
+        }
+        base = total;
+        __syncthreads();
+    }
+    if (tid == 0) counts[0] = base.y, counts[1] = base.x;
+#pragma unroll 8
+    for (int p = tid; p < picks; p += blockDim.x) {
+        const int e = ids[p];
+        int r = -1;
+        if (e >= 0 && e < E) {
+            r = atomicAdd(&next_s[e], 1);
+            tokens[r] = p / top;
+            row_weights[r] = weights[p];
+        }
+        places[p] = r;
+    }
+}
+
+extern "C" int llm_f8_sort(const int32_t* ids, const float* weights, int picks, int top, int E, int per, int32_t* counts, void* items, int32_t* places, int32_t* tokens,
+                           float* row_weights, uintptr_t stream) {
+    if (picks <= 0) return LLM_OK;
+    if (E <= 0 || E > 4096 || top <= 0 || per <= 0) return LLM_REFUSED_SIZE;
+    if (!aligned16(items)) return LLM_REFUSED_ALIGN;
+    const int most = picks > E ? picks : E, threads = most >= 1024 ? 1024 : (most + 31) / 32 * 32;
+    launch_pdl(f8_sort_kernel, dim3(1), dim3(threads), E * sizeof(int), reinterpret_cast<cudaStream_t>(stream), ids, weights, picks, top, E, per, counts,
+               static_cast<int4*>(items), places, tokens, row_weights);
+    return launch_status();
+}
+
+// out[token] = base[token] + the token's rows of y in the order of its choices, in 32 bits.
+template <typename TY, typename TO>
+__global__ void __launch_bounds__(128) f8_add_up_kernel(const TY* __restrict__ y, const int32_t* __restrict__ places, TO* __restrict__ out, int N, int top, int vec,
+                                                        const float* __restrict__ base) {
+    pdl_begin();
+    const size_t t = blockIdx.x;
+    if (vec) {
+        const int i = (blockIdx.y * 128 + threadIdx.x) * 8;
+        if (i >= N) return;
+        float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (base) load8(base + t * N + i, sum);
+#pragma unroll 4
+        for (int k = 0; k < top; ++k) {
+            const int r = places[t * top + k];
+            if (r < 0) continue;
+            float v[8];
+            load8(y + static_cast<size_t>(r) * N + i, v);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) sum[c] += v[c];
+        }
+        store8(out + t * N + i, sum);
+    } else {
+        for (int i = blockIdx.y * 128 + threadIdx.x; i < N; i += gridDim.y * 128) {
+            float sum = base ? base[t * N + i] : 0.0f;
+            for (int k = 0; k < top; ++k) {
+                const int r = places[t * top + k];
+                if (r >= 0) sum += to_f32(y[static_cast<size_t>(r) * N + i]);
+            }
+            out[t * N + i] = from_f32<TO>(sum);
+        }
+    }
+}
+
+// y [rows, N] and out [T, N] of one dtype; base (float32 [T, N]) may be null.
+extern "C" int llm_f8_add_up(const void* y, int dtype, const int32_t* places, const float* base, void* out, int T, int N, int top, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    if (N <= 0 || N > (1 << 24) || top <= 0) return LLM_REFUSED_SIZE;
+    const int vec = N % 8 == 0 && aligned16(y) && aligned16(out) && aligned16(base);
+    const dim3 grid(T, (N + 1023) / 1024);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (dtype == LLM_DT_F32)
+        launch_pdl((f8_add_up_kernel<float, float>), grid, dim3(128), 0, s, static_cast<const float*>(y), places, static_cast<float*>(out), N, top, vec, base);
+    else if (dtype == LLM_DT_BF16)
+        launch_pdl((f8_add_up_kernel<bf16, bf16>), grid, dim3(128), 0, s, static_cast<const bf16*>(y), places, static_cast<bf16*>(out), N, top, vec, base);
+    else
+        return LLM_REFUSED_DTYPE;
+    return launch_status();
+}

@@ -1,0 +1,995 @@
+// y[T, N] = x[T, K] . w[N, K]^T of numbers of 8 bits under float32 scales (f8_blocks.cuh has the format), of one matrix or of a stack's matrices by
+// rows sorted by expert, on the 5th-generation tensor cores (tcgen05.mma.kind::f8f6f4).
+//
+//   y[t, n] = sum over tiles b of 128 values of K: sx[t, b] * sw[n / 128, b] * (sum over the 128 values of cx * cw)
+// Products of codes are exact and a tile's sum is the tensor core's, in float32.  The scales are float32 numbers that no product applies, so every tile of K has
+// an accumulator of its own in tensor memory, which other warps take out, multiply and add up in registers while the next ones are computed.
+//   * Few rows: bytes bound the product.  The weights are the left operand (128 features a tile), the rows the right one (NT of them), so that no lane is spent
+//     on rows that are not there.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the parts' order;
+//     nothing is left for another kernel and no result depends on timing.
+//   * Many rows: pairs of CTAs.  The rows are the left operand, so that a lane is a row and its scale one number for 64 or 128 features.
+//   * Gate and up: act(gate) * up leaves as rows of 8 bits, 128 features a scale.
+//   * Rows sorted by expert: an item (up to a tile's rows of one expert) takes the place of a tile of rows; how many there are only the device knows.
+// Waits are bounded: one that runs out sets status code 10, and the copies and products that are under way then end, which is waited for on their own barriers
+// (bounded too), before the CTA does; what was not computed is neither stored nor added.
+#include "f8_blocks.cuh"
+#include "tcgen05_attention.cuh"
+
+#define F8_STATUS 10
+
+__device__ __forceinline__ bool f8_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    for (int i = 0; i < waits; ++i) {
+        if (t5_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    if (atomicCAS(status, 0, F8_STATUS) == 0) status[1] = blockIdx.y;
+    return false;
+}
+// What was asked for before a wait ran out: its end.
+__device__ __forceinline__ void f8_land(unsigned long long* bar, unsigned parity) {
+    for (int i = 0; i < T5_WAIT_LIMIT && !t5_try_wait(bar, parity); ++i) {}
+}
+// The uses of a ring's barriers that may be under way, of `asked` in all.
+__device__ __forceinline__ void f8_land_ring(unsigned long long* bars, int ring, int asked) {
+    for (int i = max(0, asked - ring); i < asked; ++i) f8_land(&bars[i % ring], (i / ring) & 1);
+}
+__device__ __forceinline__ void f8_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(t5_smem(dst)), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(t5_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void f8_mma_lead(unsigned lead, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+                 " @q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::
+                     "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+// Instruction descriptor: e4m3 x e4m3 -> float32, M x N, both K-major.
+__host__ __device__ constexpr unsigned f8_idesc(int m, int n) {
+    return (1u << 4) | (static_cast<unsigned>(n >> 3) << 17) | (static_cast<unsigned>(m >> 4) << 24);
+}
+
+struct F8Args {
+    const float4* w_scales;               // [tiles][ktiles] of a tile's first 64 features, its 65th, its last
+    const float* x_scales;                // [ktiles][x_rows]
+    long long x_rows;
+    void* y;                              // [T, N]; gated: the codes [tiles / 2][y_rows][128]
+    float* y_scales;                      // gated: [tiles / 2][y_rows]
+    long long y_rows;
+    int T, N, K, ktiles, tiles, vec, waits;       // tiles: of a matrix of the stack; N gated: features of the result
+    int32_t* status;
+    MxAct act;
+    const bf16* plain;                    // a matrix [tokens, K] that the kernel takes to 8 bits itself
+    F8Groups groups;
+    int on_input;                         // a row's weight multiplies its gate and up values instead of the result
+};
+enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+#define F8_MAKERS 8               // warps that make rows of a matrix
+#define F8_FEW_THREADS(PLAIN) (32 * (6 + ((PLAIN) ? F8_MAKERS : 1)))
+
+// grid (parts of K, tiles of features, tiles of rows or items), a cluster the parts of a tile.  WS: stages of weights; G: stages whose rows come together, two
+// such groups at a time.  A CTA's tile is 128 features, gated 64 + 64 gate and as many up features, of two tiles of the weight.
+// Warp 0 feeds the weights, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and their scales; or, PLAIN, x comes as a matrix and warps 6 to 13 make
+// the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.
+template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED>
+__global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                                                                         const F8Args a) {
+    constexpr int THREADS = F8_FEW_THREADS(PLAIN), WT = MODE == F8_GATED ? 2 : 1, FEATURES = 128 * WT;
+    constexpr unsigned W_BYTES = WT * F8_TILE, X_BYTES = NT * F8_K, SLOT = NT * WT;
+    constexpr unsigned SLOTS = 256 / SLOT < 4 ? 256 / SLOT : 4, COLS = SLOT * SLOTS < 32 ? 32 : SLOT * SLOTS;      // accumulators in turn; two CTAs share tensor memory
+    static_assert(COLS <= 256 && SLOTS >= 2, "tensor memory");
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    unsigned char* x_s = w_s + WS * W_BYTES;                      // [2][G][NT][128], 128-byte swizzle like the weights
+    float* sx_s = reinterpret_cast<float*>(x_s + 2 * G * X_BYTES);        // [2][G][NT]
+    float* sums = reinterpret_cast<float*>(w_s);                  // [NT][FEATURES], when the stages have been read
+    __shared__ __align__(8) unsigned long long full[WS], empty[WS], x_full[2], x_empty[2], acc_full[SLOTS], acc_empty[SLOTS], drained, fed;
+    __shared__ unsigned tmem_base_s;
+    __shared__ int abort_flag, asked_s[2];                        // asked_s: stages of weights, groups of rows that were asked for
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int part = blockIdx.x, parts = gridDim.x;
+    const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0;
+    int row0 = blockIdx.z * NT, rows = min(NT, a.T - row0), first_tile = blockIdx.y * WT;
+    if constexpr (GROUPED) {
+        pdl_wait();                                               // the items are the kernel's in front
+        if (static_cast<int>(blockIdx.z) >= a.groups.counts[0]) return;       // the whole cluster
+        const int4 item = a.groups.items[blockIdx.z];
+        first_tile += item.x * a.tiles, row0 = item.y, rows = item.z;
+    }
+    const int early = min(WS, kbs);
+    auto weights = [&](int kb, int s) {                           // into stage s
+        t5_expect_tx(&full[s], W_BYTES);
+#pragma unroll
+        for (int w = 0; w < WT; ++w) t5_tma_2d(w_s + s * W_BYTES + w * F8_TILE, &w_map, 0, ((first_tile + w) * a.ktiles + kb0 + kb) * 128, &full[s]);
+    };
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < WS; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&x_full[s], PLAIN ? F8_MAKERS : 2); t5_mbar_init(&x_empty[s], 5); }      // the products and four warps of sums
+        for (int s = 0; s < static_cast<int>(SLOTS); ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 4); }
+        t5_mbar_init(&drained, 1);
+        t5_mbar_init(&fed, PLAIN ? 1 : 2);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        // Weights are nobody's output: the first of them are on their way before anything else, whatever runs in front.
+        for (int kb = 0; kb < early; ++kb) weights(kb, kb);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    t5_fence_before();
+    __syncthreads();
+    t5_fence_after();
+    pdl_invite();                                                 // not before: this CTA's tensor memory is taken
+    const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int issued = early, s = early % WS;
+            unsigned phase = early == WS ? 0 : 1;                 // a barrier that was never used passes for the phase before its first
+            if (early < kbs) pdl_wait();                          // the rest waits for products anyway, and these for the kernel in front: no bound on that
+#pragma unroll 1
+            for (int kb = early; kb < kbs; ++kb) {
+                if (!f8_wait(&empty[s], phase, a.waits, &abort_flag, a.status)) break;
+                weights(kb, s);
+                issued = kb + 1;
+                if (++s == WS) s = 0, phase ^= 1;
+            }
+            asked_s[0] = issued;
+            t5_arrive(&fed);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const unsigned lead = elect_one();
+        const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024);
+        bool ok = true;
+        pdl_wait();                                               // the bounded waits below are not for the kernel in front
+        int s = 0, slot = 0, q = 0, g = 0;
+        unsigned phase = 0, turn = 0, acc_phase = 1;
+#pragma unroll 1
+        for (int kb = 0; kb < kbs; ++kb) {
+            if (q == 0) ok = __all_sync(0xffffffffu, f8_wait(&x_full[g], turn, a.waits, &abort_flag, a.status));
+            ok = ok && __all_sync(0xffffffffu, f8_wait(&acc_empty[slot], acc_phase, a.waits, &abort_flag, a.status) &&
+                                                   f8_wait(&full[s], phase, a.waits, &abort_flag, a.status));
+            if (!ok) break;
+            t5_fence_after();
+#pragma unroll
+            for (int w = 0; w < WT; ++w)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    f8_mma_lead(lead, tmem + slot * SLOT + w * NT, wd + ((s * W_BYTES + w * F8_TILE) >> 4) + 2 * k, xd + (((g * G + q) * X_BYTES) >> 4) + 2 * k,
+                                f8_idesc(128, NT), k ? 1u : 0u);
+            t5_commit_lead(lead, &empty[s]);
+            t5_commit_lead(lead, &acc_full[slot]);
+            if (++s == WS) s = 0, phase ^= 1;
+            if (++slot == static_cast<int>(SLOTS)) slot = 0, acc_phase ^= 1;
+            if (++q == G) {
+                t5_commit_lead(lead, &x_empty[g]);
+                q = 0, g ^= 1;
+                if (g == 0) turn ^= 1;
+            }
+        }
+        t5_commit_lead(lead, &drained);                           // what was issued has ended
+    } else if (warp < 6) {
+        const int quarter = warp & 3, feature = quarter * 32 + lane;
+        pdl_wait();
+        float acc[WT][NT];
+#pragma unroll
+        for (int w = 0; w < WT; ++w)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[w][i] = 0.0f;
+        // A lane has the weights' scales of every 32nd tile of K; of up rows two, where these 64 lie in two blocks.
+        constexpr int WS_ = MODE == F8_GATED ? 2 : 1;
+        float mine[WT][WS_];
+        bool second[WT];
+#pragma unroll
+        for (int w = 0; w < WT; ++w) second[w] = WS_ == 2 && quarter >= 2 && feature - 64 >= f8_split(a.N, blockIdx.y * WT + w);
+        int slot = 0, q = 0, g = 0;
+        unsigned turn = 0, acc_phase = 0;
+        bool ok = true;
+#pragma unroll 1
+        for (int kb = 0; kb < kbs; ++kb) {
+            if ((kb & 31) == 0)
+#pragma unroll
+                for (int w = 0; w < WT; ++w) {
+                    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (kb + lane < kbs) s = a.w_scales[(first_tile + w) * static_cast<long long>(a.ktiles) + kb0 + kb + lane];
+                    mine[w][0] = quarter < 2 ? s.x : s.y;
+                    if (WS_ == 2) mine[w][WS_ - 1] = quarter < 2 ? s.x : s.z;
+                }
+            ok = __all_sync(0xffffffffu, (q || f8_wait(&x_full[g], turn, a.waits, &abort_flag, a.status)) &&
+                                             f8_wait(&acc_full[slot], acc_phase, a.waits, &abort_flag, a.status));
+            if (!ok) break;
+            t5_fence_after();
+            const unsigned at = tmem + (static_cast<unsigned>(quarter * 32) << 16) + slot * SLOT;
+            const float* sx = sx_s + (g * G + q) * NT;
+#pragma unroll
+            for (int w = 0; w < WT; ++w) {
+                float sw = __shfl_sync(0xffffffffu, mine[w][0], kb & 31);
+                if constexpr (WS_ == 2) {
+                    const float other = __shfl_sync(0xffffffffu, mine[w][WS_ - 1], kb & 31);
+                    if (second[w]) sw = other;
+                }
+#pragma unroll
+                for (int c = 0; c < NT; c += 16) {
+                    unsigned r[16];
+                    t5_ld16(at + w * NT + c, r);
+                    t5_wait_ld();
+                    if (w == WT - 1 && c + 16 == NT) {            // all of it is in registers
+                        t5_fence_before();
+                        __syncwarp();
+                        if (lane == 0) t5_arrive(&acc_empty[slot]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 s = *reinterpret_cast<const float4*>(sx + c + i);
+                        acc[w][c + i] = fmaf(__uint_as_float(r[i]), s.x * sw, acc[w][c + i]);
+                        acc[w][c + i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y * sw, acc[w][c + i + 1]);
+                        acc[w][c + i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z * sw, acc[w][c + i + 2]);
+                        acc[w][c + i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w * sw, acc[w][c + i + 3]);
+                    }
+                }
+            }
+            if (++slot == static_cast<int>(SLOTS)) slot = 0, acc_phase ^= 1;
+            if (++q == G) {
+                __syncwarp();
+                if (lane == 0) t5_arrive(&x_empty[g]);
+                q = 0, g ^= 1;
+                if (g == 0) turn ^= 1;
+            }
+        }
+        if (ok) {
+#pragma unroll
+            for (int w = 0; w < WT; ++w)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+                    if (i < rows) sums[i * FEATURES + w * 128 + feature] = acc[w][i];
+        } else {
+            // A wait ran out.  Who asks for copies has stopped; the copies (the stages are where the sums go) and the products end; then NaNs tell
+            // whoever adds the parts up that these sums are not there.  Nothing of it is in the way of a product that does not give up.
+            f8_land(&fed, 0);
+            f8_land_ring(full, WS, asked_s[0]);
+            if (!PLAIN) f8_land_ring(x_full, 2, asked_s[1]);
+            f8_land(&drained, 0);
+            for (int i = 0; i < rows; ++i)
+                for (int w = 0; w < WT; ++w) sums[i * FEATURES + w * 128 + feature] = __uint_as_float(0x7fffffffu);
+        }
+    } else if constexpr (PLAIN) {                                 // rows beyond the last keep what stands there, nobody minds
+        // A warp takes two stages of a row at a time, sixteen lanes each, and has the next group's values on their way while it makes this one's.
+        static_assert(G % 2 == 0, "stages go in pairs");
+        constexpr int BATCH = (NT * G / 2 + F8_MAKERS - 1) / F8_MAKERS;       // units of a group that a warp has at most
+        const int p = lane & 15, units = rows * (G / 2);
+        const int left = a.K - kb0 * F8_K - (lane >> 4) * F8_K - p * 8;       // values of the row from the lane's first on
+        const bf16* from[BATCH];
+        pdl_wait();
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const int u = warp - 6 + j * F8_MAKERS;
+            long long r = 0;
+            if (u < units) r = GROUPED ? a.groups.tokens[row0 + u / (G / 2)] : row0 + u / (G / 2);
+            from[j] = a.plain + r * a.K + kb0 * F8_K + (lane >> 4) * F8_K + p * 8 + u % (G / 2) * 2 * F8_K;
+        }
+        uint4 raw[BATCH];
+        auto fetch = [&](int grp) {
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int u = warp - 6 + j * F8_MAKERS, at = grp * G * F8_K;
+                raw[j] = u < units && at + u % (G / 2) * 2 * F8_K < left ? *reinterpret_cast<const uint4*>(from[j] + at) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int grp = 0; grp * G < kbs; ++grp) {
+            const int g = grp & 1;
+            if (!__all_sync(0xffffffffu, f8_wait(&x_empty[g], ((grp >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status))) break;
+            uint4 now[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) now[j] = raw[j];
+            fetch(grp + 1);                                       // beyond the part: not used, and beyond the row not read
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int u = warp - 6 + j * F8_MAKERS, r = u / (G / 2), q = u % (G / 2) * 2 + (lane >> 4);
+                if (u >= units) break;                            // for the whole warp
+                const unsigned most = f8_most16(mx_most8(now[j]));
+                const F8Scale s = f8_scale(most);
+                // the 128-byte swizzle: 16-byte piece i of row r at i ^ (r % 8)
+                *reinterpret_cast<uint2*>(x_s + (g * G + q) * X_BYTES + r * F8_K + (((p >> 1) ^ (r & 7)) << 4) + (p & 1) * 8) = f8_codes8(now[j], most, s.inverse);
+                if (p == 0) sx_s[(g * G + q) * NT + r] = s.scale;
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) t5_arrive(&x_full[g]);
+        }
+    } else {
+        int issued = 0;
+        pdl_wait();
+#pragma unroll 1
+        for (int grp = 0; grp * G < kbs; ++grp) {
+            const int g = grp & 1, first = kb0 + grp * G;
+            if (!__all_sync(0xffffffffu, f8_wait(&x_empty[g], ((grp >> 1) & 1) ^ 1, a.waits, &abort_flag, a.status))) break;
+            if (lane == 0) {
+                t5_expect_tx(&x_full[g], G * X_BYTES);
+                f8_tma_3d(x_s + g * G * X_BYTES, &x_map, 0, row0, first, &x_full[g]);
+            }
+            constexpr int EACH = (G * NT + 31) / 32;
+            float s[EACH];
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                const int i = lane + 32 * j, kb = first + i / NT;
+                s[j] = i < G * NT && kb < a.ktiles && row0 + i % NT < a.x_rows ? a.x_scales[kb * a.x_rows + row0 + i % NT] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < EACH; ++j)
+                if (lane + 32 * j < G * NT) sx_s[g * G * NT + lane + 32 * j] = s[j];
+            __syncwarp();
+            if (lane == 0) t5_arrive(&x_full[g]);
+            issued = grp + 1;
+        }
+        if (lane == 0) {
+            asked_s[1] = issued;
+            t5_arrive(&fed);
+        }
+        __syncwarp();
+    }
+    t5_fence_before();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    // What the warp's first row is added to is on its way while the parts meet.
+    const int feature = blockIdx.y * 128 + 4 * lane, first_row = part + warp * parts;
+    float4 old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if constexpr (MODE == F8_ADD) {
+        pdl_wait();                                               // the warps that feed weights have not
+        if (a.vec && first_row < rows && feature < a.N) old = *reinterpret_cast<const float4*>(static_cast<const float*>(a.y) + static_cast<size_t>(row0 + first_row) * a.N + feature);
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");       // every part's sums are there
+    {
+        const unsigned base = t5_smem(sums);
+        auto total = [&](int at) {                                // the parts' sums in order, four features, all parts' loads in flight at once
+            float4 f[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < parts) {
+                    unsigned addr;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(addr) : "r"(base + 4u * at), "r"(p));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(f[p].x), "=f"(f[p].y), "=f"(f[p].z), "=f"(f[p].w) : "r"(addr));
+                }
+            float4 v = f[0];
+#pragma unroll
+            for (int p = 1; p < 8; ++p)
+                if (p < parts) v.x += f[p].x, v.y += f[p].y, v.z += f[p].z, v.w += f[p].w;
+            return v;
+        };
+        // Whether a sum that is NaN (of four neighbouring features all are) is one of a part that gave up.
+        auto missing = [&](float sum) {
+            if (sum == sum) return false;
+            unsigned quit = 0;
+            for (int p = 0; p < parts; ++p) {
+                unsigned addr, flag;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(addr) : "r"(t5_smem(&abort_flag)), "r"(p));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(flag) : "r"(addr));
+                quit |= flag;
+            }
+            return quit != 0;
+        };
+        if constexpr (MODE == F8_GATED) {
+            // a warp a row, four features a lane, all of a block
+            const int f = 4 * lane, block = blockIdx.y;
+            unsigned char* codes = static_cast<unsigned char*>(a.y);
+#pragma unroll 1
+            for (int r = first_row; r < rows; r += THREADS / 32 * parts) {
+                float4 g = total(r * FEATURES + (f >> 6) * 128 + (f & 63)), u = total(r * FEATURES + (f >> 6) * 128 + 64 + (f & 63));
+                const bool quit = missing(g.x + u.x);
+                if (GROUPED && a.on_input) {
+                    const float w = a.groups.weights[row0 + r];
+                    g.x *= w, g.y *= w, g.z *= w, g.w *= w, u.x *= w, u.y *= w, u.z *= w, u.w *= w;
+                }
+                const float v[4] = {mx_gated(g.x, u.x, a.act), mx_gated(g.y, u.y, a.act), mx_gated(g.z, u.z, a.act), mx_gated(g.w, u.w, a.act)};
+                unsigned most = max(max(mx_abs_bits(v[0]), mx_abs_bits(v[1])), max(mx_abs_bits(v[2]), mx_abs_bits(v[3])));
+                most = __reduce_max_sync(0xffffffffu, most);
+                const F8Scale s = f8_scale(most);
+                if (!__any_sync(0xffffffffu, quit)) {
+                    const size_t at = block * a.y_rows + row0 + r;
+                    *reinterpret_cast<unsigned*>(codes + at * F8_K + f) = mx_e4m3x4(v[0] * s.inverse, v[1] * s.inverse, v[2] * s.inverse, v[3] * s.inverse);
+                    if (lane == 0) a.y_scales[at] = s.scale;
+                }
+            }
+        } else {
+            TO* y = static_cast<TO*>(a.y);
+            const int f = feature;
+#pragma unroll 2
+            for (int r = first_row; f < a.N && r < rows; r += THREADS / 32 * parts) {
+                const float4 t = total(r * FEATURES + 4 * lane);
+                if (missing(t.x)) continue;
+                float ts[4] = {t.x, t.y, t.z, t.w};
+                if (GROUPED && a.groups.weights) {
+                    const float w = a.groups.weights[row0 + r];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ts[i] *= w;
+                }
+                TO* to = y + static_cast<size_t>(row0 + r) * a.N + f;
+                if (a.vec) {                                      // N a multiple of 4, y aligned
+                    if constexpr (sizeof(TO) == 4) {
+                        float4 v = make_float4(ts[0], ts[1], ts[2], ts[3]);
+                        if (MODE == F8_ADD) {
+                            const float4 o = r == first_row ? old : *reinterpret_cast<const float4*>(to);
+                            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                        }
+                        *reinterpret_cast<float4*>(to) = v;
+                    } else {
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(ts[0], ts[1]), hi = __floats2bfloat162_rn(ts[2], ts[3]);
+                        *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (f + i < a.N) to[i] = from_f32<TO>(MODE == F8_ADD ? ts[i] + to_f32(to[i]) : ts[i]);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    // Nobody leaves while its sums are read.  A thread that is here has all that it read, because it has made what it stored of it, or has seen that it is
+    // NaN and of a part that gave up; the stores themselves need not be out yet, which a release would wait for.
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (warp == 1) {
+        t5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(COLS) : "memory");
+    }
+}
+
+// ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
+// The two CTAs of a cluster compute a tile of 256 rows x 256 features together (cta_group::2): each brings its own 128 rows and half of the features, and
+// reads both halves.  A tile of K's products fill one of two accumulators while 256 threads, a row and 128 features each, take the other out, so that tensor
+// memory is all in use and the sums are in registers.  The clusters are persistent; the products go on into the next tile while the threads
+// write a finished one.  Tiles are numbered row tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.  Of
+// rows sorted by expert the features are fastest: an expert's rows and weights are few.
+#define FP_STAGES 6
+#define FP_THREADS 384            // weights, products, rows, none; 8 warps for the sums
+#define FP_BLOCK 4096             // a warp's rows on their way out: 32 of 128 bytes
+#define FP_SMALL 56               // registers of a thread that takes no sums, and of one that does: (128 * 56 + 256 * 224) = 384 * 168
+#define FP_LARGE 224
+
+__device__ __forceinline__ unsigned fp_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned fp_map_to(unsigned smem_addr, unsigned rank) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr), "r"(rank));
+    return r;
+}
+// A wait that ran out ends the pair's work, not one CTA's alone: the other one's flag too.
+__device__ __forceinline__ bool fp_give_up(volatile int* abort_flag, int32_t* status) {
+    *abort_flag = 1;
+    const unsigned other = fp_map_to(t5_smem(const_cast<int*>(abort_flag)), fp_rank() ^ 1);
+    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(other), "r"(1u) : "memory");
+    if (atomicCAS(status, 0, F8_STATUS) == 0) status[1] = blockIdx.x;
+    return false;
+}
+__device__ __forceinline__ bool fp_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    for (int i = 0; i < waits; ++i) {
+        if (t5_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    return fp_give_up(abort_flag, status);
+}
+__device__ __forceinline__ bool fp_wait_cluster(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    for (int i = 0; i < waits; ++i) {
+        unsigned ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(t5_smem(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+    }
+    return fp_give_up(abort_flag, status);
+}
+// Boxes into this CTA's shared memory, counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void fp_tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::
+                     "r"(t5_smem(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void fp_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::
+                     "r"(t5_smem(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void fp_commit_lead(unsigned lead, unsigned long long* bar) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+                 " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::
+                     "r"(t5_smem(bar)), "h"(static_cast<unsigned short>(3)), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void fp_mma_lead(unsigned lead, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+                 " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::
+                     "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void fp_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// Whether all of the eight warps that take sums say so.
+__device__ __forceinline__ bool fp_all(bool yes) {
+    unsigned r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.aligned.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r) : "r"(static_cast<unsigned>(yes)) : "memory");
+    return r != 0;
+}
+
+// What a tile of the launch is.
+struct FpTile {
+    int row0, rows;                       // of the pair: first, and how many there are from it on (more than 256 where it goes on)
+    int features;                         // number of the 256 features of a matrix
+    int tile;                             // number of this CTA's tile of the weight
+};
+template <bool GROUPED> __device__ __forceinline__ FpTile fp_tile(const F8Args& a, int t, int row_tiles, int rank) {
+    if constexpr (GROUPED) {
+        const int per = a.tiles / 2, i = t / per, f = t - i * per;
+        const int4 item = a.groups.items[i];
+        return {item.y, item.z, f, item.x * a.tiles + 2 * f + rank};
+    } else {
+        const int f = t / row_tiles, r = t - f * row_tiles;
+        return {r * 256, a.T - r * 256, f, 2 * f + rank};
+    }
+}
+
+// SPLIT: gated, and the up features of a tile may lie in two blocks.
+template <int MODE, typename TO, bool GROUPED, bool SPLIT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pair_kernel(const __grid_constant__ CUtensorMap w_map,
+                                                                                         const __grid_constant__ CUtensorMap x_map, const F8Args a, int row_tiles,
+                                                                                         int all_tiles) {
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    unsigned char* x_s = w_s + FP_STAGES * F8_TILE;               // [STAGES][128 rows][128]
+    unsigned char* out_s = x_s + FP_STAGES * F8_TILE;             // a block for each of the eight warps
+    float* most_s = reinterpret_cast<float*>(out_s);              // gated: [2][2][128]
+    __shared__ __align__(8) unsigned long long full[FP_STAGES], empty[FP_STAGES], acc_full[2], acc_empty[2], drained;
+    __shared__ unsigned tmem_base_s;
+    __shared__ int abort_flag, asked_s[2];                        // asked_s: boxes of weights, of rows that were asked for
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const unsigned rank = __shfl_sync(0xffffffffu, fp_rank(), 0);
+    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1, ktiles = a.ktiles;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < FP_STAGES; ++s) { t5_mbar_init(&full[s], 2); t5_mbar_init(&empty[s], 1); }      // weights and rows
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 16); }     // 8 warps of 2 CTAs
+        t5_mbar_init(&drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    t5_fence_before();
+    __syncthreads();
+    fp_cluster_sync();                                            // the other CTA's barriers exist before anyone signals them
+    t5_fence_after();
+    pdl_invite();                                                 // not before: tensor memory is taken
+    const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base_s, 0);
+    if (GROUPED || warp != 0) pdl_wait();                         // weights are nobody's output, the items are
+    const int tiles = GROUPED ? a.groups.counts[0] * (a.tiles / 2) : all_tiles;
+
+    // One box of this thread's (of weights or rows) for tile at and tile of K kb, into stage s.
+    const unsigned first = fp_map_to(t5_smem(full), 0);           // the first CTA's barriers
+    auto ask = [&](const FpTile& at, int kb, int s) {
+        if (rank == 0) t5_expect_tx(&full[s], 2 * F8_TILE);       // of both CTAs
+        const unsigned bar = first + s * 8;
+        if (warp == 0) fp_tma_2d(w_s + s * F8_TILE, &w_map, 0, (at.tile * ktiles + kb) * 128, bar);
+        else fp_tma_3d(x_s + s * F8_TILE, &x_map, 0, at.row0 + static_cast<int>(rank) * 128, kb, bar);
+    };
+    int asked = 0;                                                // boxes, in the thread that asks
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(FP_SMALL));
+        if (warp == 0 || warp == 2) {
+            if (lane == 0) {
+                int s = 0;
+                unsigned phase = 1;                               // a barrier that was never used passes for the phase before its first
+                bool ok = true;
+                int ahead = !GROUPED && warp == 0 ? FP_STAGES : -1;       // boxes of weights that do not wait for the kernel in front
+                for (int t = cluster; ok && t < tiles; t += clusters) {
+                    const FpTile at = fp_tile<GROUPED>(a, t, row_tiles, rank);
+#pragma unroll 1
+                    for (int kb = 0; kb < ktiles; ++kb) {
+                        if (ahead >= 0 && ahead-- == 0) pdl_wait();       // the bounded waits below are not for that kernel
+                        if (!fp_wait(&empty[s], phase, a.waits, &abort_flag, a.status)) {
+                            asked = (t - cluster) / clusters * ktiles + kb;
+                            ok = false;
+                            break;
+                        }
+                        ask(at, kb, s);
+                        if (++s == FP_STAGES) s = 0, phase ^= 1;
+                    }
+                }
+                if (ok) asked = tiles > cluster ? (tiles - cluster + clusters - 1) / clusters * ktiles : 0;
+                asked_s[warp >> 1] = asked;
+            }
+            __syncwarp();
+        } else if (warp == 1 && rank == 0) {
+            const unsigned lead = elect_one();
+            const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024);
+            const unsigned idesc = f8_idesc(256, 256);
+            int s = 0;
+            unsigned phase = 0, buf = 0, acc_phase = 1;
+            bool ok = true;
+            for (int t = cluster; ok && t < tiles; t += clusters) {
+#pragma unroll 1
+                for (int kb = 0; kb < ktiles; ++kb) {
+                    ok = __all_sync(0xffffffffu, fp_wait_cluster(&acc_empty[buf], acc_phase, a.waits, &abort_flag, a.status) &&
+                                                     fp_wait(&full[s], phase, a.waits, &abort_flag, a.status));
+                    if (!ok) break;
+                    t5_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        fp_mma_lead(lead, tmem + buf * 256, xd + s * (F8_TILE >> 4) + 2 * k, wd + s * (F8_TILE >> 4) + 2 * k, idesc, k ? 1u : 0u);
+                    fp_commit_lead(lead, &empty[s]);
+                    fp_commit_lead(lead, &acc_full[buf]);
+                    if (++s == FP_STAGES) s = 0, phase ^= 1;
+                    buf ^= 1;
+                    if (buf == 0) acc_phase ^= 1;
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(FP_LARGE));
+        const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+        const unsigned acc_empty_first = fp_map_to(t5_smem(&acc_empty[0]), 0);
+        unsigned char* block = out_s + (warp - 4) * FP_BLOCK;
+        // Scales are asked for AHEAD tiles of K before they are used, across the borders between tiles: a cursor of its own.
+        constexpr int AHEAD = 4;
+        float sx[AHEAD];
+        float2 sw[AHEAD];
+        float sz[AHEAD];                                          // SPLIT
+        int ct = cluster, ckb = 0;
+        const float* cx = a.x_scales;
+        const float4* cw = a.w_scales;
+        bool there = false;
+        auto cursor_to = [&](int t) {
+            if (t >= tiles) return;
+            const FpTile at = fp_tile<GROUPED>(a, t, row_tiles, 0);
+            const int r = at.row0 + static_cast<int>(rank) * 128 + row;
+            there = r < a.x_rows;
+            cx = a.x_scales + (there ? r : 0);
+            cw = a.w_scales + static_cast<long long>(at.tile + half) * ktiles;
+        };
+        auto fetch = [&](float& x, float2& w, float& z) {
+            if (ct >= tiles) return;
+            x = there ? cx[ckb * a.x_rows] : 0.0f;
+            w = *reinterpret_cast<const float2*>(cw + ckb);
+            if (SPLIT) z = cw[ckb].z;
+            if (++ckb == ktiles) {
+                ckb = 0, ct += clusters;
+                cursor_to(ct);
+            }
+        };
+        cursor_to(ct);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            sx[i] = sz[i] = 0.0f, sw[i] = make_float2(0.0f, 0.0f);
+            fetch(sx[i], sw[i], sz[i]);
+        }
+        unsigned buf = 0, acc_phase = 0, turn = 0;
+        for (int t = cluster; t < tiles; t += clusters) {
+            const FpTile at = fp_tile<GROUPED>(a, t, row_tiles, rank);
+            unsigned long long acc[64];                           // two features each
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0ull;
+            bool ok = true;
+            const int split = SPLIT ? f8_split(a.N, 2 * at.features + half) : 64;
+#pragma unroll 1
+            for (int kb = 0; kb < ktiles; ++kb) {
+                const float s0 = sx[0] * sw[0].x, s1 = sx[0] * sw[0].y, s2 = SPLIT ? sx[0] * sz[0] : s1;
+#pragma unroll
+                for (int i = 0; i + 1 < AHEAD; ++i) sx[i] = sx[i + 1], sw[i] = sw[i + 1], sz[i] = sz[i + 1];
+                fetch(sx[AHEAD - 1], sw[AHEAD - 1], sz[AHEAD - 1]);
+                ok = __all_sync(0xffffffffu, fp_wait(&acc_full[buf], acc_phase, a.waits, &abort_flag, a.status));
+                if (!ok) break;
+                t5_fence_after();
+                const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * 256 + half * 128;
+                const unsigned long long first_64 = t5_two(s0, s0), other_64 = t5_two(s1, s1);
+                unsigned r[2][32];
+                t5_ld32(from, r[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    t5_wait_ld();
+                    if (c < 3) t5_ld32(from + 32 * (c + 1), r[(c + 1) & 1]);
+                    else {                                        // all of it is in registers
+                        t5_fence_before();
+                        __syncwarp();
+                        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int f = (c - 2) * 32 + 2 * i;       // of the up features
+                        const unsigned long long s = c < 2 ? first_64 : SPLIT ? t5_two(f < split ? s1 : s2, f + 1 < split ? s1 : s2) : other_64;
+                        acc[c * 16 + i] = t5_fma2(t5_two(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s, acc[c * 16 + i]);
+                    }
+                }
+                buf ^= 1;
+                if (buf == 0) acc_phase ^= 1;
+            }
+            if constexpr (MODE == F8_GATED) ok = fp_all(ok);      // the two halves of a row meet below: all go on or leave together
+            if (!ok) break;                                       // what has not been computed is not stored
+            const int valid = min(at.rows - static_cast<int>(rank) * 128 - quarter * 32, 32);        // of the warp's rows
+            const long long row0 = at.row0 + static_cast<int>(rank) * 128 + quarter * 32;
+            if constexpr (MODE == F8_GATED) {
+                float w = 1.0f;
+                if (GROUPED && a.on_input && lane < valid) w = a.groups.weights[row0 + lane];
+                float v[64];
+                unsigned most = 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float g0, g1, u0, u1;
+                    t5_untwo(acc[i], g0, g1);
+                    t5_untwo(acc[32 + i], u0, u1);
+                    if (GROUPED) g0 *= w, g1 *= w, u0 *= w, u1 *= w;
+                    v[2 * i] = mx_gated(g0, u0, a.act);
+                    v[2 * i + 1] = mx_gated(g1, u1, a.act);
+                    most = max(most, max(mx_abs_bits(v[2 * i]), mx_abs_bits(v[2 * i + 1])));
+                }
+                // the other 64 features of the row are another thread's; two places in turn, so that the next tile's need not wait for these to be read
+                most_s[(turn * 2 + half) * 128 + row] = __uint_as_float(most);
+                asm volatile("bar.sync 1, 256;\n" ::: "memory");
+                most = max(most, __float_as_uint(most_s[(turn * 2 + (half ^ 1)) * 128 + row]));
+                turn ^= 1;
+                const F8Scale s = f8_scale(most);
+                if (lane < valid) {
+                    const long long to = at.features * a.y_rows + row0 + lane;
+                    uint4* codes = reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) + to * F8_K + half * 64);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        unsigned c[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float* q = v + 16 * i + 4 * j;
+                            c[j] = mx_e4m3x4(q[0] * s.inverse, q[1] * s.inverse, q[2] * s.inverse, q[3] * s.inverse);
+                        }
+                        codes[i] = make_uint4(c[0], c[1], c[2], c[3]);
+                    }
+                    if (half == 0) a.y_scales[to] = s.scale;
+                }
+            } else {
+                // 128 bytes of each of the warp's rows at a time through shared memory, in pieces of 16 bytes that the row number scatters over the banks
+                constexpr int PER = 128 / sizeof(TO);             // features of a turn
+                float w = 1.0f;
+                if (GROUPED && a.groups.weights && lane < valid) w = a.groups.weights[row0 + lane];
+                TO* y = static_cast<TO*>(a.y) + row0 * a.N;
+                const int col0 = at.features * 256 + half * 128;
+#pragma unroll
+                for (int c = 0; c < 128 / PER; ++c) {
+                    if (col0 + c * PER >= a.N) break;
+                    __syncwarp();
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) {
+                        unsigned q[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (sizeof(TO) == 4) {
+                                float lo, hi;
+                                t5_untwo(acc[(c * PER + p * 4 + i) / 2], lo, hi);
+                                q[i] = __float_as_uint((i & 1 ? hi : lo) * (GROUPED ? w : 1.0f));
+                            } else {
+                                float lo, hi;
+                                t5_untwo(acc[(c * PER + p * 8) / 2 + i], lo, hi);
+                                q[i] = GROUPED ? t5_pack(lo * w, hi * w) : t5_pack(lo, hi);
+                            }
+                        }
+                        *reinterpret_cast<uint4*>(block + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);
+                    }
+                    __syncwarp();
+                    if (a.vec) {                                  // rows of whole, aligned pieces of 16 bytes
+                        constexpr int PIECE = 16 / sizeof(TO);
+                        const int p = lane & 7, col = col0 + c * PER + p * PIECE;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = i * 4 + (lane >> 3);
+                            if (r >= valid || col >= a.N) continue;
+                            uint4 v = *reinterpret_cast<const uint4*>(block + r * 128 + ((p ^ (r & 7)) << 4));
+                            uint4* to = reinterpret_cast<uint4*>(y + static_cast<size_t>(r) * a.N + col);
+                            if constexpr (MODE == F8_ADD) {
+                                const float4 o = *reinterpret_cast<const float4*>(to);
+                                v.x = __float_as_uint(__uint_as_float(v.x) + o.x), v.y = __float_as_uint(__uint_as_float(v.y) + o.y);
+                                v.z = __float_as_uint(__uint_as_float(v.z) + o.z), v.w = __float_as_uint(__uint_as_float(v.w) + o.w);
+                            }
+                            *to = v;
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int r = 0; r < valid; ++r)
+#pragma unroll
+                            for (int j = 0; j < PER; j += 32) {
+                                const int f = j + lane, col = col0 + c * PER + f, piece = f * static_cast<int>(sizeof(TO)) / 16;
+                                if (col >= a.N) continue;
+                                TO v = *reinterpret_cast<const TO*>(block + r * 128 + ((piece ^ (r & 7)) << 4) + f * sizeof(TO) % 16);
+                                TO* to = y + static_cast<size_t>(r) * a.N + col;
+                                if constexpr (MODE == F8_ADD) v += *to;
+                                *to = v;
+                            }
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    t5_fence_before();
+    __syncthreads();
+    fp_cluster_sync();                                            // nobody signals a CTA that has left
+    if (abort_flag) {
+        // A wait ran out, both CTAs know it, and what is under way ends before they go away.  A barrier fills when all who bring its bytes have asked: those
+        // who stopped earlier ask for what the others have asked for already, at most a ring's worth, into places that the products have left
+        // (whoever asked first has waited for that).  Then the first CTA's barriers tell when all of it is there, and one more commit when the products are.
+        if ((warp == 0 || warp == 2) && lane == 0) {
+            int most = 0;
+            for (int who = 0; who < 2; ++who)
+                for (unsigned r = 0; r < 2; ++r) {
+                    int n;
+                    asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(n) : "r"(fp_map_to(t5_smem(&asked_s[who]), r)) : "memory");
+                    most = max(most, n);
+                }
+            for (; asked < most; ++asked) ask(fp_tile<GROUPED>(a, cluster + asked / ktiles * clusters, row_tiles, rank), asked % ktiles, asked % FP_STAGES);
+            if (rank == 0) f8_land_ring(full, FP_STAGES, most);
+        } else if (warp == 1) {
+            if (rank == 0) fp_commit_lead(elect_one(), &drained);         // the lane that issued: elect gives the same one for the same lanes
+            f8_land(&drained, 0);
+        }
+        __syncwarp();
+        __syncthreads();
+        fp_cluster_sync();
+    }
+    if (warp == 1) {
+        t5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+#define F8_DEVICES 64
+static int f8_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < F8_DEVICES ? dev : -1;
+}
+static int f8_sms(int dev) {
+    static int sms[F8_DEVICES] = {0};
+    if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms[dev] = 0;
+    return sms[dev];
+}
+// Lets a kernel have its shared memory, once a device (`had`: a flag for each).
+template <typename K> static int f8_allow(K kern, size_t smem, int dev, bool* had) {
+    if (had[dev]) return LLM_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    had[dev] = e == cudaSuccess;
+    return static_cast<int>(e);
+}
+static bool f8_encoder() {
+    CUtensorMap any;
+    if (g_t5_state == 0) (void)t5_encode_2d(&any, nullptr, 64, 64, 64, 64);       // finds the driver's entry point
+    return g_t5_state > 0;
+}
+// Codes of weights: lines of 128 bytes in boxes of 128.
+static bool f8_weight_map(CUtensorMap* map, const void* w, long long lines) {
+    if (!f8_encoder() || lines >= (1LL << 31)) return false;
+    const cuuint64_t dims[2] = {F8_K, static_cast<cuuint64_t>(lines)}, strides[1] = {F8_K};
+    const cuuint32_t box[2] = {F8_K, 128}, es[2] = {1u, 1u};
+    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(w), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Codes of rows [ktiles][rows][128] in boxes of `box_tiles` x `box_rows` x 128.
+static bool f8_rows_map(CUtensorMap* map, const void* x, long long rows, int ktiles, int box_rows, int box_tiles) {
+    if (!f8_encoder() || rows >= (1LL << 31)) return false;
+    const cuuint64_t dims[3] = {F8_K, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(ktiles)}, strides[2] = {F8_K, static_cast<cuuint64_t>(rows) * F8_K};
+    const cuuint32_t box[3] = {F8_K, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_tiles)}, es[3] = {1u, 1u, 1u};
+    return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(x), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.  Two CTAs an SM, less an eighth, because clusters do not
+// fill a group of SMs to the last slot.
+static int f8_parts(long long tiles, int ktiles, int sms) {
+    const int slots = 2 * sms * 7 / 8;
+    int best = 1;
+    while (best < 8 && (best + 1) * tiles <= slots && ktiles / (best + 1) >= 2) ++best;
+    return best;
+}
+struct F8Call {
+    const void* w;
+    long long w_tiles;                    // of the whole stack
+    const void* x;                        // rows of 8 bits
+    int row_tiles;                        // tiles of rows, or room for items
+};
+template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED> static int f8_few(const F8Call& c, const F8Args& a, cudaStream_t s) {
+    constexpr int WT = MODE == F8_GATED ? 2 : 1;
+    CUtensorMap w_map, x_map = {};
+    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128)) return LLM_REFUSED_SIZE;
+    if (!PLAIN && !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, NT, G)) return LLM_REFUSED_SIZE;
+    constexpr size_t smem = static_cast<size_t>(WS) * WT * F8_TILE + 2 * G * NT * (F8_K + sizeof(float)) + 1024;
+    static_assert(NT * 128 * sizeof(float) <= WS * F8_TILE, "the sums fit the weights' stages");
+    static_assert(smem <= 113 * 1024, "half of an SM's shared memory");
+    auto kern = f8_few_kernel<NT, WS, G, PLAIN, MODE, TO, GROUPED>;
+    static bool had[F8_DEVICES];
+    const int dev = f8_device();
+    if (dev < 0) return LLM_REFUSED_SIZE;
+    if (const int rc = f8_allow(kern, smem, dev, had)) return rc;
+    const int tiles = (MODE == F8_GATED ? a.tiles / 2 : (a.N + 127) / 128), sms = f8_sms(dev);
+    if (tiles > 65535 || c.row_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
+    const int parts = f8_parts(static_cast<long long>(tiles) * c.row_tiles, a.ktiles, sms);
+    launch_pdl_cluster(kern, dim3(parts, tiles, c.row_tiles), dim3(F8_FEW_THREADS(PLAIN)), smem, s, parts, w_map, x_map, a);
+    return launch_status();
+}
+template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(const F8Call& c, F8Args a, cudaStream_t s) {
+    CUtensorMap w_map, x_map;
+    const int dev = f8_device();
+    if (dev < 0 || f8_sms(dev) < 2) return LLM_REFUSED_SIZE;
+    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128) || !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, 128, 1)) return LLM_REFUSED_SIZE;
+    a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
+    constexpr size_t smem = static_cast<size_t>(FP_STAGES) * 2 * F8_TILE + 8 * FP_BLOCK + 1024;
+    static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
+    static_assert(128 * FP_SMALL + 256 * FP_LARGE <= FP_THREADS * 168, "registers of the launch");
+    auto kern = f8_pair_kernel<MODE, TO, GROUPED, SPLIT>;
+    static bool had[F8_DEVICES];
+    if (const int rc = f8_allow(kern, smem, dev, had)) return rc;
+    const long long all = static_cast<long long>(c.row_tiles) * (a.tiles / 2);
+    const int slots = f8_sms(dev) / 2;
+    if (all > (1LL << 30)) return LLM_REFUSED_SIZE;
+    const int clusters = all < slots ? static_cast<int>(all) : slots;
+    launch_pdl(kern, dim3(2 * clusters), dim3(FP_THREADS), smem, s, w_map, x_map, a, c.row_tiles, static_cast<int>(all));
+    return launch_status();
+}
+
+// Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself.
+#define F8_PLAIN_ROWS 16
+// Rows from which on pairs of CTAs take over.
+#define F8_PAIR_ROWS 129
+// How a product of T rows runs: the rows of a tile.
+extern "C" int llm_f8_way(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T < F8_PAIR_ROWS ? 64 : 256; }
+
+template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const F8Args& a, int per, cudaStream_t s) {
+    if (!GROUPED) c.row_tiles = (a.T + per - 1) / per;
+    if (per == 256) return MODE == F8_GATED && a.N % 64 ? f8_pair<MODE, TO, GROUPED, MODE == F8_GATED>(c, a, s) : f8_pair<MODE, TO, GROUPED, false>(c, a, s);
+    if constexpr (MODE == F8_GATED) {
+        if (per == 16) return a.plain ? f8_few<16, 3, 2, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 3, 2, false, MODE, TO, GROUPED>(c, a, s);
+        if (per == 32) return f8_few<32, 3, 1, false, MODE, TO, GROUPED>(c, a, s);
+        return f8_few<64, 2, 2, false, MODE, TO, GROUPED>(c, a, s);
+    } else {
+        if (per == 16) return a.plain ? f8_few<16, 5, 4, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 5, 4, false, MODE, TO, GROUPED>(c, a, s);
+        if (per == 32) return f8_few<32, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
+        return f8_few<64, 4, 2, false, MODE, TO, GROUPED>(c, a, s);
+    }
+}
+
+// One product.  rows: of 8 bits [T, K] (`padded` of them), or null and `plain` a bfloat16 matrix [tokens, K] of whole, aligned pieces of eight values, for tiles of 16 rows;
+// w: a weight's codes and, behind them, its scales.
+//   which 0: y [T, N] float32 or bfloat16; add: y (float32) holds a summand already
+//   which 1: y the codes and scales of act(x gate^T) * (x up^T) as rows of 8 bits [T, N], `y_padded` of them; w gated
+// counts (null: one matrix): rows sorted by expert, `per` rows an item at most, room for `room` items; T: rows in all at most.  weights: of the rows, or null; they multiply
+// the result, with on_input the gate and up values.
+extern "C" int llm_linear_f8(int which, void* rows, long long padded, const void* plain, const void* w, const void* w_scales, int E, int tiles, void* y, int out_dtype,
+                             int add, long long y_padded, int T, int N, int K, int act, float limit, const int32_t* counts, const void* items,
+                             const int32_t* tokens, const float* weights, int on_input, int per, int room, int waits, int32_t* status, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    if (N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 20) || T > (1 << 24) || E <= 0 || status == nullptr || (which != 0 && which != 1)) return LLM_REFUSED_SIZE;
+    if (tiles != (which ? 2 * ((N + 127) / 128) : (N + 255) / 256 * 2)) return LLM_REFUSED_SIZE;
+    if (!aligned16(w) || !aligned16(w_scales) || !aligned16(rows) || (which && !aligned16(y))) return LLM_REFUSED_ALIGN;
+    if (!rows && !(plain && K % 8 == 0 && aligned16(plain))) return LLM_REFUSED_ALIGN;
+    if (out_dtype != LLM_DT_F32 && (out_dtype != LLM_DT_BF16 || add)) return LLM_REFUSED_DTYPE;
+    F8Args a = {};
+    if (!counts) per = llm_f8_way(T);
+    if ((per != 16 && per != 32 && per != 64 && per != 256) || (!rows && per != 16) || (rows && padded < T)) return LLM_REFUSED_SIZE;
+    if (counts && (!items || !tokens || room <= 0 || add)) return LLM_REFUSED_SIZE;
+    a.w_scales = static_cast<const float4*>(w_scales);
+    a.ktiles = f8_tiles(K), a.tiles = tiles;
+    a.x_scales = rows ? f8_row_scales(rows, padded, a.ktiles) : nullptr, a.x_rows = padded;
+    a.y = y, a.y_rows = y_padded;
+    a.T = T, a.N = N, a.K = K, a.waits = waits, a.status = status;
+    a.plain = rows ? nullptr : static_cast<const bf16*>(plain);
+    a.groups = {counts, static_cast<const int4*>(items), tokens, weights};
+    a.on_input = on_input;
+    const F8Call c = {w, static_cast<long long>(E) * tiles, rows, room};
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (which == 1) {
+        if (!mx_act(act, limit, &a.act)) return LLM_REFUSED_SIZE;
+        a.y_scales = f8_row_scales(y, y_padded, (N + 127) / 128);
+        return counts ? f8_way<F8_GATED, float, true>(c, a, per, s) : f8_way<F8_GATED, float, false>(c, a, per, s);
+    }
+    a.vec = N % 4 == 0 && aligned16(y);
+    if (counts) return out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, true>(c, a, per, s) : f8_way<F8_STORE, bf16, true>(c, a, per, s);
+    if (add) return f8_way<F8_ADD, float, false>(c, a, per, s);
+    return out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, false>(c, a, per, s) : f8_way<F8_STORE, bf16, false>(c, a, per, s);
+}

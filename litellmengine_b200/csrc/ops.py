@@ -2591,6 +2591,250 @@ def _mx_count() -> None:
     launch_count += 1                         # the kernel that takes a matrix to 8 bits
 
 
+# ---- products of 8 bits, a scale for each block of 128 -----------------------------------------------
+# A weight has one float32 scale for each block of 128 x 128 values, a row one for each 128 neighbouring values: the block's largest
+# magnitude / 448.  csrc/f8_blocks.cuh says how codes are rounded and where the bytes lie.
+F8_BLOCK = 128
+# Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself.
+F8_PLAIN_ROWS = 16
+_MX_SIGNATURES.update({
+    "llm_f8_rows": ("blocks_f8", [_P, _I, _P, _L, _I, _I, _P, _I, _P]),
+    "llm_f8_weight": ("blocks_f8", [_P, _I, _P, _P, _I, _I, _I, _I, _I, _L, _L, _P]),
+    "llm_f8_values": ("blocks_f8", [_P, _P, _P, _I, _I, _I, _I, _I, _L, _I, _P]),
+    "llm_f8_sort": ("blocks_f8", [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "llm_f8_add_up": ("blocks_f8", [_P, _I, _P, _P, _P, _I, _I, _I, _P]),
+    "llm_linear_f8": ("blocks_f8", [_I, _P, _L, _P, _P, _P, _I, _I, _P, _I, _I, _L, _I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
+})
+
+
+def f8_padded_rows(T: int) -> int:
+    """Rows that stand behind T rows of 8 bits: the products read whole tiles, and nobody minds what stands there."""
+    if T <= 64:
+        return 16 if T <= 16 else 32 if T <= 32 else 64
+    return (T + 127) // 128 * 128
+
+
+class F8Rows:
+    """Rows [T, K] in 8 bits (e4m3) with a float32 scale per 128 values: what `linear_f8` and `linear_silu_mul_f8` read.  Made by
+    `f8_rows` and `linear_silu_mul_f8`.  `codes`: uint8 [tiles of K, rows padded, 128]; `scales`: float32 [tiles of K, rows padded]; `values`
+    gives the rows as a matrix again."""
+
+    __slots__ = ("shape", "device", "padded", "buffer")
+
+    def __init__(self, T: int, K: int, device: torch.device):
+        self.shape = (T, K)
+        self.device = device
+        self.padded = f8_padded_rows(T)
+        # one allocation: the codes, then the scales
+        self.buffer = torch.empty((K + 127) // 128 * self.padded * 132, dtype=torch.uint8, device=device)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        tiles = (self.shape[1] + 127) // 128
+        return self.buffer[:tiles * self.padded * 128].view(tiles, self.padded, 128)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        tiles = (self.shape[1] + 127) // 128
+        return self.buffer[tiles * self.padded * 128:].view(torch.float32).view(tiles, self.padded)
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        T, K = self.shape
+        _here(self.buffer)
+        out, at = _mx_matrix(T, K, dtype, self.device), self.buffer.data_ptr()
+        _check(_mx_call("llm_f8_values")(at, at + (K + 127) // 128 * self.padded * 128, out.data_ptr(), _dt(out), T, 0, K, 0, self.padded, 0, _stream()),
+               "values of rows in 8 bits")
+        return out
+
+
+class F8Weight:
+    """A weight [N, K], or a stack of them [E, N, K], in 8 bits (e4m3) with a float32 scale per block of 128 x 128 values, stored tile by
+    tile.  Made by `f8_weight`; `gated`: it is [gate; up], gate and up rows stored beside each other for `linear_silu_mul_f8`; the values are
+    the same."""
+
+    def __init__(self, shape, gated: bool, device: torch.device):
+        self.shape = tuple(shape)
+        self.gated = gated
+        self.device = device
+        self.experts = shape[0] if len(shape) == 3 else 1
+        N, K = shape[-2:]
+        # tiles of 128 rows: an even number of a matrix, because products of many rows take two at a time
+        self.tiles = n, tiles = 2 * ((N // 2 + 127) // 128 if gated else (N + 255) // 256), (K + 127) // 128
+        # one allocation: the codes, then three scales and room for a fourth for each tile
+        self.scales_behind = self.experts * n * tiles * 128 * 128
+        self.buffer = torch.empty(self.scales_behind + self.experts * n * tiles * 16, dtype=torch.uint8, device=device)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        n, tiles = self.tiles
+        return self.buffer[:self.scales_behind].view(self.experts, n, tiles, 128, 128)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        n, tiles = self.tiles
+        return self.buffer[self.scales_behind:].view(torch.float32).view(self.experts, n, tiles, 4)
+
+    @property
+    def nbytes(self) -> int:
+        return self.buffer.numel()
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        N, K = self.shape[-2:]
+        _here(self.buffer)
+        out, at = _mx_matrix(self.experts * N, K, dtype, self.device), self.buffer.data_ptr()
+        _check(_mx_call("llm_f8_values")(at, at + self.scales_behind, out.data_ptr(), _dt(out), self.experts * N, N // 2 if self.gated else N, K, self.tiles[0], 0,
+                                         2 if self.gated else 1, _stream()), "values of a weight in 8 bits")
+        return out.view(self.shape)
+
+
+def f8_weight(weight: torch.Tensor, gated: bool = False) -> F8Weight:
+    """A weight [N, K], or a stack [E, N, K], float32 or bfloat16, in 8 bits.  With `gated`, a matrix is [gate; up] and serves `linear_silu_mul_f8`.
+    Rows and matrices may lie any distance apart, a row's values side by side."""
+    if not weight.is_cuda:
+        raise KernelError("tensor is not on a CUDA device; the engine has no CPU path")
+    if weight.dim() not in (2, 3) or min(weight.shape) < 1 or (gated and weight.shape[-2] % 2):
+        raise KernelError("a weight in 8 bits is a matrix or a stack of them; a gated one has as many gate as up rows")
+    N, K = weight.shape[-2:]
+    if K > 1 and weight.stride(-1) != 1:
+        raise KernelError("a row's values lie side by side")
+    dt = _dt(weight)
+    _here(weight.as_strided((1,), (1,)))
+    made = F8Weight(weight.shape, gated, weight.device)
+    at = made.buffer.data_ptr()
+    _check(_mx_call("llm_f8_weight")(weight.data_ptr(), dt, at, at + made.scales_behind, made.experts, N // 2 if gated else N, K, made.tiles[0], int(gated),
+                                     weight.stride(-2), weight.stride(0) if weight.dim() == 3 else 0, _stream()), "f8_weight")
+    return made
+
+
+def f8_rows(x: torch.Tensor) -> F8Rows:
+    """x [T, K] (float32 or bfloat16) as rows of 8 bits."""
+    _here(x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError("rows of 8 bits are made of a matrix [T, K]")
+    T, K = x.shape
+    dt = _dt(x)
+    made = F8Rows(T, K, x.device)
+    _check(_mx_call("llm_f8_rows")(x.data_ptr(), dt, made.buffer.data_ptr(), made.padded, T, K, None, 1, _stream()), "f8_rows")
+    return made
+
+
+def _f8_operands(x, weight: F8Weight, gated: bool):
+    """(rows of 8 bits or None, the matrix that the product takes to 8 bits itself or None) of a product's x."""
+    if not isinstance(weight, F8Weight) or weight.gated != gated or len(weight.shape) != 2:
+        raise KernelError("the product takes an F8Weight of one matrix" + (" made with gated=True" if gated else " that is not a gated one"))
+    if not isinstance(x, (F8Rows, torch.Tensor)):
+        raise KernelError("the product takes rows of 8 bits or a matrix")
+    if len(x.shape) != 2 or x.shape[1] != weight.shape[1]:
+        raise KernelError("x and weight disagree on K")
+    if type(x) is F8Rows:
+        _here(x.buffer, weight.buffer)
+        return x, None
+    _here(x, weight.buffer)
+    if x.shape[0] <= F8_PLAIN_ROWS and _dt(x) == 1 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0:
+        return None, x
+    return f8_rows(x), None
+
+
+def linear_f8(x, weight: F8Weight, out_dtype: torch.dtype = torch.float32, residual: Optional[torch.Tensor] = None,
+              waits: int = STREAM_WAITS) -> torch.Tensor:
+    """x [T, K] @ weight[N, K]^T with weight and x in 8 bits under float32 scales (`F8Rows`; a matrix is taken to 8 bits first), products exact,
+    sums in float32, on the tcgen05 products.  The result is float32 or bfloat16 [T, N]; with `residual` (float32 [T, N]) it is added to
+    that in place, which is returned.  Where a wait runs out (`stream_status`), what was not computed is neither stored nor added."""
+    rows, plain = _f8_operands(x, weight, False)
+    (T, K), N = x.shape, weight.shape[0]
+    if residual is not None:
+        _here(residual)
+        if residual.dtype != torch.float32 or residual.shape != (T, N):
+            raise KernelError("the product joins a float32 residual of its shape")
+        y, od = residual, 0
+    else:
+        y = _mx_matrix(T, N, out_dtype, weight.device)
+        od = _dt(y)
+    at = weight.buffer.data_ptr()
+    _check(_mx_call("llm_linear_f8")(0, rows.buffer.data_ptr() if rows is not None else None, rows.padded if rows is not None else 0, _ptr(plain), at,
+                                     at + weight.scales_behind, 1, weight.tiles[0], y.data_ptr(), od, residual is not None, 0, T, N, K, 0, 0.0, None, None, None, None,
+                                     0, 0, 0, waits, _mx_status_ptr(weight.device), _stream()), "linear_f8")
+    return y
+
+
+def linear_silu_mul_f8(x, weight: F8Weight, activation: str = "silu", limit: float = 0.0, waits: int = STREAM_WAITS) -> F8Rows:
+    """act(x @ gate^T) * (x @ up^T) as rows of 8 bits [T, I] for a gated weight [2I, K] in 8 bits, act as in `silu_and_mul`, in the
+    product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits."""
+    act = ACTIVATIONS[activation]
+    rows, plain = _f8_operands(x, weight, True)
+    (T, K), inter = x.shape, weight.shape[0] // 2
+    made = F8Rows(T, inter, weight.device)
+    at = weight.buffer.data_ptr()
+    _check(_mx_call("llm_linear_f8")(1, rows.buffer.data_ptr() if rows is not None else None, rows.padded if rows is not None else 0, _ptr(plain), at,
+                                     at + weight.scales_behind, 1, weight.tiles[0], made.buffer.data_ptr(), 0, 0, made.padded, T, inter, K, act, limit, None, None, None,
+                                     None, 0, 0, 0, waits, _mx_status_ptr(weight.device), _stream()), "linear_silu_mul_f8")
+    return made
+
+
+def _f8_item_rows(picks: int, experts: int) -> int:
+    """Rows of an expert that a grouped product takes at a time: by how many it has on average."""
+    if picks <= 16 * experts:
+        return 16
+    return 32 if picks <= 32 * experts else 64 if picks <= 64 * experts else 256
+
+
+def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Tensor, weights: torch.Tensor, activation: str = "silu", limit: float = 0.0,
+           on_input: bool = False, base: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32, waits: int = STREAM_WAITS) -> torch.Tensor:
+    """The routed feed-forward with the experts' matrices in 8 bits, for any number of tokens: x [T, W] (float32 or bfloat16), `w_gate_up` a gated stack [E, 2 ff, W],
+    `w_down` a stack [E, W, ff], `ids` (int32) and `weights` (float32) [T, top] from `moe_route` (an id that is none of 0 .. E - 1: a pick without an expert).
+    The picks are sorted by expert on the device, each expert's rows go through its own matrices as in `linear_silu_mul_f8` and `linear_f8`, and a
+    token's rows are added up in float32 in the order of its choices, times their weights (`on_input`: the weight multiplies the expert's input, that is
+    its gate and up values, instead), onto `base` (float32 [T, W]) where there is one.  The result is float32 or bfloat16 [T, W]; for bfloat16 the experts' rows
+    are rounded to it before they are added up, as `moe_sorted` rounds its."""
+    act = ACTIVATIONS[activation]
+    _here(x, ids, weights, base)
+    _i32(ids, "ids")
+    if not (isinstance(w_gate_up, F8Weight) and isinstance(w_down, F8Weight)) or not w_gate_up.gated or w_down.gated or len(w_gate_up.shape) != 3 or len(w_down.shape) != 3:
+        raise KernelError("routed experts in 8 bits: a gated stack [E, 2 ff, W] and a stack [E, W, ff] made by f8_weight")
+    _here(w_gate_up.buffer, w_down.buffer)
+    E, two_ff, W = w_gate_up.shape
+    ff = two_ff // 2
+    if w_down.shape != (E, W, ff) or x.dim() != 2 or x.shape[1] != W:
+        raise KernelError("x and the experts' matrices disagree")
+    T = x.shape[0]
+    if ids.dim() != 2 or ids.shape[0] != T or ids.shape[1] < 1 or weights.shape != ids.shape or weights.dtype != torch.float32:
+        raise KernelError("moe_f8: int32 ids and float32 weights [T, top]")
+    if base is not None and (base.dtype != torch.float32 or base.shape != (T, W)):
+        raise KernelError("moe_f8: the base must be float32 [T, W]")
+    out = _mx_matrix(T, W, out_dtype, x.device)
+    od, dt = _dt(out), _dt(x)
+    if T == 0:
+        return out
+    top = ids.shape[1]
+    picks = T * top
+    per = _f8_item_rows(picks, E)
+    room = min(E, picks) + picks // per
+    # one allocation for what the sorting makes: items (16 bytes each), counts, places, tokens, weights
+    plan = torch.empty(4 * room + 4 + 3 * picks, dtype=torch.int32, device=x.device)
+    items = plan.data_ptr()
+    counts = items + 16 * room
+    places = counts + 16
+    tokens, row_weights = places + 4 * picks, places + 8 * picks
+    stream, status = _stream(), _mx_status_ptr(x.device)
+    _check(_mx_call("llm_f8_sort")(ids.data_ptr(), weights.data_ptr(), picks, top, E, per, counts, items, places, tokens, row_weights, stream), "f8_sort")
+    rows, plain = None, None
+    if per == 16 and dt == 1 and W % 8 == 0 and x.data_ptr() % 16 == 0:
+        plain = x
+    else:
+        rows = F8Rows(picks, W, x.device)
+        _check(_mx_call("llm_f8_rows")(x.data_ptr(), dt, rows.buffer.data_ptr(), rows.padded, T, W, places, top, stream), "f8_rows")
+    middle = F8Rows(picks, ff, x.device)
+    product, at = _mx_call("llm_linear_f8"), w_gate_up.buffer.data_ptr()
+    _check(product(1, rows.buffer.data_ptr() if rows is not None else None, rows.padded if rows is not None else 0, _ptr(plain), at, at + w_gate_up.scales_behind, E,
+                   w_gate_up.tiles[0], middle.buffer.data_ptr(), 0, 0, middle.padded, picks, ff, W, act, limit, counts, items, tokens, row_weights, int(on_input), per, room,
+                   waits, status, stream), "gate and up of experts in 8 bits")
+    y, at = _mx_matrix(picks, W, out_dtype, x.device), w_down.buffer.data_ptr()
+    _check(product(0, middle.buffer.data_ptr(), middle.padded, None, at, at + w_down.scales_behind, E, w_down.tiles[0], y.data_ptr(), od, 0, 0, picks, W, ff, 0, 0.0,
+                   counts, items, tokens, None if on_input else row_weights, 0, per, room, waits, status, stream), "down of experts in 8 bits")
+    _check(_mx_call("llm_f8_add_up")(y.data_ptr(), od, places, _ptr(base), out.data_ptr(), T, W, top, stream), "f8_add_up")
+    return out
+
+
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:
     """residual (float32 [T, N]) += x @ weight^T in the product's epilogue, if the paired kernel or, for a weight in 4 bits, the
     microscaled one takes these operands; False, and nothing done, if not."""
