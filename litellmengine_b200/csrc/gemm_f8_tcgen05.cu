@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
                 if (g == 0) turn ^= 1;
             }
         }
-        t5_commit_lead(lead, &drained);                           // what was issued has ended
+        t5_commit_lead(lead, &drained);                           // what was issued has ended, and all of it has been told
+        f8_land(&drained, 0);
     } else if (warp < 6) {
         const int quarter = warp & 3, feature = quarter * 32 + lane;
         pdl_wait();
@@ -439,15 +440,21 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
 
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 // The two CTAs of a cluster compute a tile of 256 rows x 256 features together (cta_group::2): each brings its own 128 rows and half of the features, and
-// reads both halves.  A tile of K's products fill one of two accumulators while 256 threads, a row and 128 features each, take the other out, so that tensor
-// memory is all in use and the sums are in registers.  The clusters are persistent; the products go on into the next tile while the threads
-// write a finished one.  Tiles are numbered row tile fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.  Of
-// rows sorted by expert the features are fastest: an expert's rows and weights are few.
-#define FP_STAGES 6
-#define FP_THREADS 384            // weights, products, rows, none; 8 warps for the sums
+// reads both halves.  Tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them, one after the other, while 256
+// threads, a row and 128 features each, take out those of the tile of K before, so that the sums are in registers.  The products of a tile of K take 512 clocks,
+// which is what an accumulator's way round (its products 256, telling 200, taking out 350, telling 200) leaves room for; with two accumulators of 256 features
+// that way is twice 600.  The clusters are persistent; the products go on into the next tile while the threads write a finished one.  Tiles are numbered row tile
+// fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's
+// rows and weights are few.
+// Warp 0 feeds the weights, 2 the rows, 3 the scales; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
+#define FP_STAGES 5
+#define FP_THREADS 384
 #define FP_BLOCK 4096             // a warp's rows on their way out: 32 of 128 bytes
-#define FP_SMALL 56               // registers of a thread that takes no sums, and of one that does: (128 * 56 + 256 * 224) = 384 * 168
-#define FP_LARGE 224
+#define FP_RING 3                 // groups of tiles of K whose scales are there
+#define FP_GROUP 4
+#define FP_SCALES (128 * 4 + 2 * 16)      // bytes of a tile of K's: 128 rows', two tiles of weights'
+#define FP_SMALL 40               // registers of a thread that takes no sums, and of one that does: (128 * 40 + 256 * 232) = 384 * 168
+#define FP_LARGE 232
 
 __device__ __forceinline__ unsigned fp_rank() {
     unsigned r;
@@ -474,15 +481,23 @@ __device__ __forceinline__ bool fp_wait(unsigned long long* bar, unsigned parity
     }
     return fp_give_up(abort_flag, status);
 }
-__device__ __forceinline__ bool fp_wait_cluster(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
-    for (int i = 0; i < waits; ++i) {
-        unsigned ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                     : "=r"(ok) : "r"(t5_smem(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-        if (*abort_flag) return false;
-    }
-    return fp_give_up(abort_flag, status);
+// Whether a barrier's phase is complete, without waiting for it; and the wait of a warp that has looked.  A look takes 100 clocks until its answer is there, so what is
+// likely to be complete is asked for ahead of what can run without it; a vote over the lanes would take another 45.  All lanes come out of it together:
+// what follows are instructions of whole warps.
+__device__ __forceinline__ bool fp_look(unsigned long long* bar, unsigned parity) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(t5_smem(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool fp_wait_warp(bool seen, unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+    bool ok = true;
+    if (!seen) ok = fp_wait(bar, parity, waits, abort_flag, status);
+    __syncwarp();
+    return ok;
+}
+// acc += a * b of two float32 values each, where it stands: between what is asked for in front of it and used behind it.
+__device__ __forceinline__ void fp_fma2(unsigned long long& acc, unsigned long long a, unsigned long long b) {
+    asm volatile("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(acc) : "l"(a), "l"(b));
 }
 // Boxes into this CTA's shared memory, counted on a barrier of the pair's first CTA.
 __device__ __forceinline__ void fp_tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
@@ -506,6 +521,8 @@ __device__ __forceinline__ void fp_mma_lead(unsigned lead, unsigned d_tmem, unsi
 __device__ __forceinline__ void fp_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// The pair's warps meet: nobody signals a CTA that has left.  WHO (a text) keeps the places apart.
+#define fp_meet(WHO) asm volatile("// " WHO "\nbarrier.cta.sync.aligned 0;\nbarrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory")
 // Whether all of the eight warps that take sums say so.
 __device__ __forceinline__ bool fp_all(bool yes) {
     unsigned r;
@@ -518,30 +535,32 @@ __device__ __forceinline__ bool fp_all(bool yes) {
 struct FpTile {
     int row0, rows;                       // of the pair: first, and how many there are from it on (more than 256 where it goes on)
     int features;                         // number of the 256 features of a matrix
-    int tile;                             // number of this CTA's tile of the weight
+    int tile;                             // number of the first of the two tiles of the weight
 };
-template <bool GROUPED> __device__ __forceinline__ FpTile fp_tile(const F8Args& a, int t, int row_tiles, int rank) {
+template <bool GROUPED> __device__ __forceinline__ FpTile fp_tile(const F8Args& a, int t, int row_tiles) {
     if constexpr (GROUPED) {
         const int per = a.tiles / 2, i = t / per, f = t - i * per;
         const int4 item = a.groups.items[i];
-        return {item.y, item.z, f, item.x * a.tiles + 2 * f + rank};
+        return {item.y, item.z, f, item.x * a.tiles + 2 * f};
     } else {
         const int f = t / row_tiles, r = t - f * row_tiles;
-        return {r * 256, a.T - r * 256, f, 2 * f + rank};
+        return {r * 256, a.T - r * 256, f, 2 * f};
     }
 }
 
 // SPLIT: gated, and the up features of a tile may lie in two blocks.
 template <int MODE, typename TO, bool GROUPED, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pair_kernel(const __grid_constant__ CUtensorMap w_map,
-                                                                                         const __grid_constant__ CUtensorMap x_map, const F8Args a, int row_tiles,
+                                                                                         const __grid_constant__ CUtensorMap x_map,
+                                                                                         const __grid_constant__ CUtensorMap y_map, const F8Args a, int row_tiles,
                                                                                          int all_tiles) {
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     unsigned char* x_s = w_s + FP_STAGES * F8_TILE;               // [STAGES][128 rows][128]
     unsigned char* out_s = x_s + FP_STAGES * F8_TILE;             // a block for each of the eight warps
     float* most_s = reinterpret_cast<float*>(out_s);              // gated: [2][2][128]
-    __shared__ __align__(8) unsigned long long full[FP_STAGES], empty[FP_STAGES], acc_full[2], acc_empty[2], drained;
+    unsigned char* scales_s = out_s + 8 * FP_BLOCK;               // [RING]
+    __shared__ __align__(8) unsigned long long full[FP_STAGES], empty[FP_STAGES], acc_full[4], acc_empty[2], s_full[FP_RING], s_empty[FP_RING], drained;
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag, asked_s[2];                        // asked_s: boxes of weights, of rows that were asked for
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -550,7 +569,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < FP_STAGES; ++s) { t5_mbar_init(&full[s], 2); t5_mbar_init(&empty[s], 1); }      // weights and rows
-        for (int s = 0; s < 2; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 16); }     // 8 warps of 2 CTAs
+        for (int s = 0; s < 4; ++s) t5_mbar_init(&acc_full[s], 1);
+        for (int s = 0; s < 2; ++s) t5_mbar_init(&acc_empty[s], 16);      // 8 warps of 2 CTAs
+        for (int s = 0; s < FP_RING; ++s) { t5_mbar_init(&s_full[s], 32); t5_mbar_init(&s_empty[s], 8); }
         t5_mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -567,13 +588,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     if (GROUPED || warp != 0) pdl_wait();                         // weights are nobody's output, the items are
     const int tiles = GROUPED ? a.groups.counts[0] * (a.tiles / 2) : all_tiles;
 
-    // One box of this thread's (of weights or rows) for tile at and tile of K kb, into stage s.
+    // This thread's box (or two of weights: 64 features of either tile, so that a product's two halves are a tile) for tile at and tile of K kb, into stage s.
     const unsigned first = fp_map_to(t5_smem(full), 0);           // the first CTA's barriers
     auto ask = [&](const FpTile& at, int kb, int s) {
         if (rank == 0) t5_expect_tx(&full[s], 2 * F8_TILE);       // of both CTAs
         const unsigned bar = first + s * 8;
-        if (warp == 0) fp_tma_2d(w_s + s * F8_TILE, &w_map, 0, (at.tile * ktiles + kb) * 128, bar);
-        else fp_tma_3d(x_s + s * F8_TILE, &x_map, 0, at.row0 + static_cast<int>(rank) * 128, kb, bar);
+        if (warp == 0) {
+            const int line = (at.tile * ktiles + kb) * 128 + static_cast<int>(rank) * 64;
+            fp_tma_2d(w_s + s * F8_TILE, &w_map, 0, line, bar);
+            fp_tma_2d(w_s + s * F8_TILE + F8_TILE / 2, &w_map, 0, line + ktiles * 128, bar);
+        } else fp_tma_3d(x_s + s * F8_TILE, &x_map, 0, at.row0 + static_cast<int>(rank) * 128, kb, bar);
     };
     int asked = 0;                                                // boxes, in the thread that asks
 
@@ -586,7 +610,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 bool ok = true;
                 int ahead = !GROUPED && warp == 0 ? FP_STAGES : -1;       // boxes of weights that do not wait for the kernel in front
                 for (int t = cluster; ok && t < tiles; t += clusters) {
-                    const FpTile at = fp_tile<GROUPED>(a, t, row_tiles, rank);
+                    const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
 #pragma unroll 1
                     for (int kb = 0; kb < ktiles; ++kb) {
                         if (ahead >= 0 && ahead-- == 0) pdl_wait();       // the bounded waits below are not for that kernel
@@ -601,111 +625,182 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 }
                 if (ok) asked = tiles > cluster ? (tiles - cluster + clusters - 1) / clusters * ktiles : 0;
                 asked_s[warp >> 1] = asked;
+                // The products tell both CTAs that they have read a stage, and none may leave before it has been told.
+                if (warp == 0 && ok) f8_land_ring(empty, FP_STAGES, asked);
             }
             __syncwarp();
         } else if (warp == 1 && rank == 0) {
             const unsigned lead = elect_one();
             const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024);
-            const unsigned idesc = f8_idesc(256, 256);
+            const unsigned idesc = f8_idesc(256, 128);
             int s = 0;
             unsigned phase = 0, buf = 0, acc_phase = 1;
-            bool ok = true;
+            bool ok = true, seen = false;
             for (int t = cluster; ok && t < tiles; t += clusters) {
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; ++kb) {
-                    ok = __all_sync(0xffffffffu, fp_wait_cluster(&acc_empty[buf], acc_phase, a.waits, &abort_flag, a.status) &&
-                                                     fp_wait(&full[s], phase, a.waits, &abort_flag, a.status));
+                    ok = fp_wait_warp(seen, &full[s], phase, a.waits, &abort_flag, a.status);
+                    ok = __all_sync(0xffffffffu, fp_wait_warp(false, &acc_empty[buf], acc_phase, a.waits, &abort_flag, a.status) && ok);
                     if (!ok) break;
                     t5_fence_after();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        fp_mma_lead(lead, tmem + buf * 256, xd + s * (F8_TILE >> 4) + 2 * k, wd + s * (F8_TILE >> 4) + 2 * k, idesc, k ? 1u : 0u);
-                    fp_commit_lead(lead, &empty[s]);
-                    fp_commit_lead(lead, &acc_full[buf]);
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)               // of the features' first or other halves in both CTAs
+                            fp_mma_lead(lead, tmem + buf * 256 + h * 128, xd + s * (F8_TILE >> 4) + 2 * k, wd + ((s * F8_TILE + h * (F8_TILE / 2)) >> 4) + 2 * k, idesc, k ? 1u : 0u);
+                        if (h == 1) fp_commit_lead(lead, &empty[s]);
+                        fp_commit_lead(lead, &acc_full[2 * buf + h]);
+                    }
                     if (++s == FP_STAGES) s = 0, phase ^= 1;
+                    seen = fp_look(&full[s], phase);
                     buf ^= 1;
                     if (buf == 0) acc_phase ^= 1;
                 }
             }
+        } else if (warp == 3) {
+            // A tile of K's scales: four rows a lane, and of the weights' the first two lanes', copied without a register between.
+            int slot = 0;
+            unsigned phase = 1;
+            bool ok = true;
+            for (int t = cluster; ok && t < tiles; t += clusters) {
+                const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
+                const int r0 = at.row0 + static_cast<int>(rank) * 128 + lane;
+                const float* cx = a.x_scales;
+                const float4* cw = a.w_scales + (at.tile + (lane & 1)) * static_cast<long long>(ktiles);
+                int rows[4], bytes[4];                            // beyond the last row: zeros
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bytes[i] = r0 + 32 * i < a.x_rows ? 4 : 0, rows[i] = bytes[i] ? r0 + 32 * i : 0;
+#pragma unroll 1
+                for (int kb0 = 0; kb0 < ktiles; kb0 += FP_GROUP) {
+                    ok = __all_sync(0xffffffffu, fp_wait(&s_empty[slot], phase, a.waits, &abort_flag, a.status));
+                    if (!ok) break;
+                    unsigned to = t5_smem(scales_s) + slot * (FP_GROUP * FP_SCALES);
+#pragma unroll 1
+                    for (int kb = kb0; kb < min(kb0 + FP_GROUP, ktiles); ++kb, to += FP_SCALES) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + (lane + 32 * i) * 4), "l"(cx + rows[i]), "r"(bytes[i]) : "memory");
+                        if (lane < 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 512 + lane * 16), "l"(cw + kb) : "memory");
+                        cx += a.x_rows;
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(t5_smem(&s_full[slot])) : "memory");
+                    if (++slot == FP_RING) slot = 0, phase ^= 1;
+                }
+            }
+            asm volatile("cp.async.wait_all;\n" ::: "memory");
+        }
+        // The two kinds of warps meet at the end from code of their own: what stands behind a place where they come together again is not held to the few registers
+        // that these have left.
+        __syncwarp();
+        t5_fence_before();
+        fp_meet("feeding");
+        if (*static_cast<volatile int*>(&abort_flag)) {
+            // A wait ran out, both CTAs know it, and what is under way ends before they go away.  A barrier fills when all who bring its bytes have asked: those
+            // who stopped earlier ask for what the others have asked for already, at most a ring's worth, into places that the products have left
+            // (whoever asked first has waited for that).  Then the first CTA's barriers tell when all of it is there, and one more commit when the products are.
+            if ((warp == 0 || warp == 2) && lane == 0) {
+                int most = 0;
+                for (int who = 0; who < 2; ++who)
+                    for (unsigned r = 0; r < 2; ++r) {
+                        int n;
+                        asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(n) : "r"(fp_map_to(t5_smem(&asked_s[who]), r)) : "memory");
+                        most = max(most, n);
+                    }
+                for (; asked < most; ++asked) ask(fp_tile<GROUPED>(a, cluster + asked / ktiles * clusters, row_tiles), asked % ktiles, asked % FP_STAGES);
+                if (rank == 0) f8_land_ring(full, FP_STAGES, most);
+            } else if (warp == 1) {
+                if (rank == 0) fp_commit_lead(elect_one(), &drained);     // the lane that issued: elect gives the same one for the same lanes
+                f8_land(&drained, 0);
+            }
+            __syncwarp();
+            fp_meet("feeding");
+        }
+        if (warp == 1) {
+            t5_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(FP_LARGE));
         const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
         const unsigned acc_empty_first = fp_map_to(t5_smem(&acc_empty[0]), 0);
         unsigned char* block = out_s + (warp - 4) * FP_BLOCK;
-        // Scales are asked for AHEAD tiles of K before they are used, across the borders between tiles: a cursor of its own.
-        constexpr int AHEAD = 4;
-        float sx[AHEAD];
-        float2 sw[AHEAD];
-        float sz[AHEAD];                                          // SPLIT
-        int ct = cluster, ckb = 0;
-        const float* cx = a.x_scales;
-        const float4* cw = a.w_scales;
-        bool there = false;
-        auto cursor_to = [&](int t) {
-            if (t >= tiles) return;
-            const FpTile at = fp_tile<GROUPED>(a, t, row_tiles, 0);
-            const int r = at.row0 + static_cast<int>(rank) * 128 + row;
-            there = r < a.x_rows;
-            cx = a.x_scales + (there ? r : 0);
-            cw = a.w_scales + static_cast<long long>(at.tile + half) * ktiles;
-        };
-        auto fetch = [&](float& x, float2& w, float& z) {
-            if (ct >= tiles) return;
-            x = there ? cx[ckb * a.x_rows] : 0.0f;
-            w = *reinterpret_cast<const float2*>(cw + ckb);
-            if (SPLIT) z = cw[ckb].z;
-            if (++ckb == ktiles) {
-                ckb = 0, ct += clusters;
-                cursor_to(ct);
-            }
-        };
-        cursor_to(ct);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            sx[i] = sz[i] = 0.0f, sw[i] = make_float2(0.0f, 0.0f);
-            fetch(sx[i], sw[i], sz[i]);
-        }
-        unsigned buf = 0, acc_phase = 0, turn = 0;
+        const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + half * 128;
+        unsigned buf = 0, acc_phase = 0, slot = 0, s_phase = 0, turn = 0;
         for (int t = cluster; t < tiles; t += clusters) {
-            const FpTile at = fp_tile<GROUPED>(a, t, row_tiles, rank);
+            const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
             unsigned long long acc[64];                           // two features each
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0ull;
             bool ok = true;
+            // What stands on the way from one accumulator to the next (is it full, its scales, its numbers) is asked for in front of additions and used behind
+            // them.  One that gives up goes on with what there is, and stores nothing.
             const int split = SPLIT ? f8_split(a.N, 2 * at.features + half) : 64;
+            float sx, s0, s1, s2;
+            float4 sw;
+            auto scales = [&](int kb) {
+                const unsigned char* p = scales_s + (slot * FP_GROUP + kb % FP_GROUP) * FP_SCALES;
+                sx = *reinterpret_cast<const float*>(p + row * 4);
+                sw = *reinterpret_cast<const float4*>(p + 512 + half * 16);
+            };
+            ok = fp_wait_warp(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status);
+            scales(0);
+            ok = fp_wait_warp(false, &acc_full[2 * buf + half], acc_phase, a.waits, &abort_flag, a.status) && ok;
+            t5_fence_after();
+            unsigned r[2][32];
+            t5_ld32(from + buf * 256, r[0]);
+            t5_ld32(from + buf * 256 + 32, r[1]);
 #pragma unroll 1
             for (int kb = 0; kb < ktiles; ++kb) {
-                const float s0 = sx[0] * sw[0].x, s1 = sx[0] * sw[0].y, s2 = SPLIT ? sx[0] * sz[0] : s1;
-#pragma unroll
-                for (int i = 0; i + 1 < AHEAD; ++i) sx[i] = sx[i + 1], sw[i] = sw[i + 1], sz[i] = sz[i + 1];
-                fetch(sx[AHEAD - 1], sw[AHEAD - 1], sz[AHEAD - 1]);
-                ok = __all_sync(0xffffffffu, fp_wait(&acc_full[buf], acc_phase, a.waits, &abort_flag, a.status));
-                if (!ok) break;
-                t5_fence_after();
-                const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * 256 + half * 128;
+                const bool last = kb + 1 == ktiles;
+                s0 = sx * sw.x;
+                s1 = MODE == F8_GATED ? sx * sw.y : s0;
+                s2 = SPLIT ? sx * sw.z : s1;
                 const unsigned long long first_64 = t5_two(s0, s0), other_64 = t5_two(s1, s1);
-                unsigned r[2][32];
-                t5_ld32(from, r[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    t5_wait_ld();
-                    if (c < 3) t5_ld32(from + 32 * (c + 1), r[(c + 1) & 1]);
-                    else {                                        // all of it is in registers
-                        t5_fence_before();
-                        __syncwarp();
-                        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
-                    }
+                auto add = [&](int c) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int f = (c - 2) * 32 + 2 * i;       // of the up features
                         const unsigned long long s = c < 2 ? first_64 : SPLIT ? t5_two(f < split ? s1 : s2, f + 1 < split ? s1 : s2) : other_64;
-                        acc[c * 16 + i] = t5_fma2(t5_two(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s, acc[c * 16 + i]);
+                        fp_fma2(acc[c * 16 + i], t5_two(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s);
                     }
+                };
+                const unsigned now = from + buf * 256;
+                t5_wait_ld();
+                add(0);
+                t5_ld32(now + 64, r[0]);
+                add(1);
+                t5_ld32(now + 96, r[1]);
+                if (kb % FP_GROUP == FP_GROUP - 1 || last) {      // the group's scales are in registers
+                    __syncwarp();
+                    if (lane == 0) t5_arrive(&s_empty[slot]);
+                    __syncwarp();
+                    if (++slot == FP_RING) slot = 0, s_phase ^= 1;
+                    if (!last) ok = fp_wait_warp(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
                 }
+                if (!last) scales(kb + 1);
+                t5_wait_ld();
+                // All of it is in registers: the accumulator is free again, with half of the additions still to do.
+                t5_fence_before();
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
+                __syncwarp();
                 buf ^= 1;
                 if (buf == 0) acc_phase ^= 1;
+                if (last) {
+                    add(2);
+                    add(3);
+                    break;
+                }
+                unsigned long long* const next = &acc_full[2 * buf + half];
+                const bool seen = fp_look(next, acc_phase);
+                add(2);
+                ok = fp_wait_warp(seen, next, acc_phase, a.waits, &abort_flag, a.status) && ok;
+                t5_fence_after();
+                t5_ld32(from + buf * 256, r[0]);
+                add(3);
+                t5_ld32(from + buf * 256 + 32, r[1]);
             }
+            ok = __all_sync(0xffffffffu, ok);
             if constexpr (MODE == F8_GATED) ok = fp_all(ok);      // the two halves of a row meet below: all go on or leave together
             if (!ok) break;                                       // what has not been computed is not stored
             const int valid = min(at.rows - static_cast<int>(rank) * 128 - quarter * 32, 32);        // of the warp's rows
@@ -733,7 +828,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 const F8Scale s = f8_scale(most);
                 if (lane < valid) {
                     const long long to = at.features * a.y_rows + row0 + lane;
-                    uint4* codes = reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) + to * F8_K + half * 64);
+                    unsigned char* codes = static_cast<unsigned char*>(a.y) + to * F8_K + half * 64;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         unsigned c[4];
@@ -742,47 +837,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                             const float* q = v + 16 * i + 4 * j;
                             c[j] = mx_e4m3x4(q[0] * s.inverse, q[1] * s.inverse, q[2] * s.inverse, q[3] * s.inverse);
                         }
-                        codes[i] = make_uint4(c[0], c[1], c[2], c[3]);
+                        *reinterpret_cast<uint4*>(codes + i * 16) = make_uint4(c[0], c[1], c[2], c[3]);
                     }
                     if (half == 0) a.y_scales[to] = s.scale;
                 }
             } else {
-                // 128 bytes of each of the warp's rows at a time through shared memory, in pieces of 16 bytes that the row number scatters over the banks
-                constexpr int PER = 128 / sizeof(TO);             // features of a turn
+                // 32 neighbouring features of each of the warp's rows at a time through shared memory, in pieces of 16 bytes that the row number scatters over the banks (the copy engine's swizzle).  The copy engine takes them out, adds, and leaves out what is beyond the matrix;
+                // rows of an expert that end within these 32, and rows that it cannot address, leave by the lanes.
+                constexpr int LINE = 32 * sizeof(TO), PIECES = LINE / 16, BLOCKS = FP_BLOCK / (32 * LINE);       // bytes of a row, its pieces, blocks in turn
                 float w = 1.0f;
                 if (GROUPED && a.groups.weights && lane < valid) w = a.groups.weights[row0 + lane];
                 TO* y = static_cast<TO*>(a.y) + row0 * a.N;
-                const int col0 = at.features * 256 + half * 128;
+                const bool copies = a.vec && (!GROUPED || valid == 32);
+                auto place = [&](int r, int piece) { return r * LINE + ((PIECES == 8 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) << 4); };
 #pragma unroll
-                for (int c = 0; c < 128 / PER; ++c) {
-                    if (col0 + c * PER >= a.N) break;
+                for (int c = 0; c < 4; ++c) {
+                    const int col0 = at.features * 256 + half * 128 + c * 32;
+                    if (col0 >= a.N) break;
+                    unsigned char* to_s = block + turn % BLOCKS * (32 * LINE);
+                    // the block has been read
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(BLOCKS - 1) : "memory");
                     __syncwarp();
 #pragma unroll
-                    for (int p = 0; p < 8; ++p) {
+                    for (int p = 0; p < PIECES; ++p) {
                         unsigned q[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
+                            float lo, hi;
                             if constexpr (sizeof(TO) == 4) {
-                                float lo, hi;
-                                t5_untwo(acc[(c * PER + p * 4 + i) / 2], lo, hi);
+                                t5_untwo(acc[c * 16 + p * 2 + i / 2], lo, hi);
                                 q[i] = __float_as_uint((i & 1 ? hi : lo) * (GROUPED ? w : 1.0f));
                             } else {
-                                float lo, hi;
-                                t5_untwo(acc[(c * PER + p * 8) / 2 + i], lo, hi);
+                                t5_untwo(acc[c * 16 + p * 4 + i], lo, hi);
                                 q[i] = GROUPED ? t5_pack(lo * w, hi * w) : t5_pack(lo, hi);
                             }
                         }
-                        *reinterpret_cast<uint4*>(block + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);
+                        *reinterpret_cast<uint4*>(to_s + place(lane, p)) = make_uint4(q[0], q[1], q[2], q[3]);
+                    }
+                    if (copies) {
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (valid > 0) {
+                                if (MODE == F8_ADD)
+                                    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(t5_smem(to_s)),
+                                                 "r"(col0), "r"(static_cast<int>(row0)) : "memory");
+                                else
+                                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(t5_smem(to_s)),
+                                                 "r"(col0), "r"(static_cast<int>(row0)) : "memory");
+                            }
+                            asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+                        }
+                        __syncwarp();
+                        ++turn;
+                        continue;
                     }
                     __syncwarp();
                     if (a.vec) {                                  // rows of whole, aligned pieces of 16 bytes
                         constexpr int PIECE = 16 / sizeof(TO);
-                        const int p = lane & 7, col = col0 + c * PER + p * PIECE;
+                        const int p = lane % PIECES, col = col0 + p * PIECE;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int r = i * 4 + (lane >> 3);
+                        for (int i = 0; i < PIECES; ++i) {
+                            const int r = i * (32 / PIECES) + lane / PIECES;
                             if (r >= valid || col >= a.N) continue;
-                            uint4 v = *reinterpret_cast<const uint4*>(block + r * 128 + ((p ^ (r & 7)) << 4));
+                            uint4 v = *reinterpret_cast<const uint4*>(to_s + place(r, p));
                             uint4* to = reinterpret_cast<uint4*>(y + static_cast<size_t>(r) * a.N + col);
                             if constexpr (MODE == F8_ADD) {
                                 const float4 o = *reinterpret_cast<const float4*>(to);
@@ -792,51 +910,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                             *to = v;
                         }
                     } else {
+                        const int col = col0 + lane;
+                        if (col < a.N)
 #pragma unroll 1
-                        for (int r = 0; r < valid; ++r)
-#pragma unroll
-                            for (int j = 0; j < PER; j += 32) {
-                                const int f = j + lane, col = col0 + c * PER + f, piece = f * static_cast<int>(sizeof(TO)) / 16;
-                                if (col >= a.N) continue;
-                                TO v = *reinterpret_cast<const TO*>(block + r * 128 + ((piece ^ (r & 7)) << 4) + f * sizeof(TO) % 16);
+                            for (int r = 0; r < valid; ++r) {
+                                TO v = *reinterpret_cast<const TO*>(to_s + place(r, lane * static_cast<int>(sizeof(TO)) / 16) + lane * sizeof(TO) % 16);
                                 TO* to = y + static_cast<size_t>(r) * a.N + col;
                                 if constexpr (MODE == F8_ADD) v += *to;
                                 *to = v;
                             }
                     }
+                    __syncwarp();
                 }
             }
         }
-    }
-    __syncwarp();
-    t5_fence_before();
-    __syncthreads();
-    fp_cluster_sync();                                            // nobody signals a CTA that has left
-    if (abort_flag) {
-        // A wait ran out, both CTAs know it, and what is under way ends before they go away.  A barrier fills when all who bring its bytes have asked: those
-        // who stopped earlier ask for what the others have asked for already, at most a ring's worth, into places that the products have left
-        // (whoever asked first has waited for that).  Then the first CTA's barriers tell when all of it is there, and one more commit when the products are.
-        if ((warp == 0 || warp == 2) && lane == 0) {
-            int most = 0;
-            for (int who = 0; who < 2; ++who)
-                for (unsigned r = 0; r < 2; ++r) {
-                    int n;
-                    asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(n) : "r"(fp_map_to(t5_smem(&asked_s[who]), r)) : "memory");
-                    most = max(most, n);
-                }
-            for (; asked < most; ++asked) ask(fp_tile<GROUPED>(a, cluster + asked / ktiles * clusters, row_tiles, rank), asked % ktiles, asked % FP_STAGES);
-            if (rank == 0) f8_land_ring(full, FP_STAGES, most);
-        } else if (warp == 1) {
-            if (rank == 0) fp_commit_lead(elect_one(), &drained);         // the lane that issued: elect gives the same one for the same lanes
-            f8_land(&drained, 0);
-        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");       // the result is there before this grid is over
         __syncwarp();
-        __syncthreads();
-        fp_cluster_sync();
-    }
-    if (warp == 1) {
-        t5_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+        t5_fence_before();
+        fp_meet("sums");
+        if (*static_cast<volatile int*>(&abort_flag)) fp_meet("sums");
     }
 }
 
@@ -863,11 +955,11 @@ static bool f8_encoder() {
     if (g_t5_state == 0) (void)t5_encode_2d(&any, nullptr, 64, 64, 64, 64);       // finds the driver's entry point
     return g_t5_state > 0;
 }
-// Codes of weights: lines of 128 bytes in boxes of 128.
-static bool f8_weight_map(CUtensorMap* map, const void* w, long long lines) {
+// Codes of weights: lines of 128 bytes.
+static bool f8_weight_map(CUtensorMap* map, const void* w, long long lines, int box_lines) {
     if (!f8_encoder() || lines >= (1LL << 31)) return false;
     const cuuint64_t dims[2] = {F8_K, static_cast<cuuint64_t>(lines)}, strides[1] = {F8_K};
-    const cuuint32_t box[2] = {F8_K, 128}, es[2] = {1u, 1u};
+    const cuuint32_t box[2] = {F8_K, static_cast<cuuint32_t>(box_lines)}, es[2] = {1u, 1u};
     return g_t5_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(w), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -897,7 +989,7 @@ struct F8Call {
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED> static int f8_few(const F8Call& c, const F8Args& a, cudaStream_t s) {
     constexpr int WT = MODE == F8_GATED ? 2 : 1;
     CUtensorMap w_map, x_map = {};
-    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128)) return LLM_REFUSED_SIZE;
+    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128, 128)) return LLM_REFUSED_SIZE;
     if (!PLAIN && !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, NT, G)) return LLM_REFUSED_SIZE;
     constexpr size_t smem = static_cast<size_t>(WS) * WT * F8_TILE + 2 * G * NT * (F8_K + sizeof(float)) + 1024;
     static_assert(NT * 128 * sizeof(float) <= WS * F8_TILE, "the sums fit the weights' stages");
@@ -914,12 +1006,20 @@ template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED
     return launch_status();
 }
 template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(const F8Call& c, F8Args a, cudaStream_t s) {
-    CUtensorMap w_map, x_map;
+    CUtensorMap w_map, x_map, y_map = {};
     const int dev = f8_device();
     if (dev < 0 || f8_sms(dev) < 2) return LLM_REFUSED_SIZE;
-    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128) || !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, 128, 1)) return LLM_REFUSED_SIZE;
-    a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
-    constexpr size_t smem = static_cast<size_t>(FP_STAGES) * 2 * F8_TILE + 8 * FP_BLOCK + 1024;
+    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128, 64) || !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, 128, 1)) return LLM_REFUSED_SIZE;
+    if (MODE != F8_GATED) {                                       // [T, N] in boxes of 32 rows of 32 features
+        a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.N), static_cast<cuuint64_t>(a.T)}, strides[1] = {static_cast<cuuint64_t>(a.N) * sizeof(TO)};
+        const cuuint32_t box[2] = {32, 32}, es[2] = {1u, 1u};
+        if (a.vec && g_t5_encode(&y_map, sizeof(TO) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, strides, box, es,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, sizeof(TO) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return LLM_REFUSED_SIZE;
+    }
+    constexpr size_t smem = static_cast<size_t>(FP_STAGES) * 2 * F8_TILE + 8 * FP_BLOCK + FP_RING * FP_GROUP * FP_SCALES + 1024;
     static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
     static_assert(128 * FP_SMALL + 256 * FP_LARGE <= FP_THREADS * 168, "registers of the launch");
     auto kern = f8_pair_kernel<MODE, TO, GROUPED, SPLIT>;
@@ -929,7 +1029,7 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
     const int slots = f8_sms(dev) / 2;
     if (all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
-    launch_pdl(kern, dim3(2 * clusters), dim3(FP_THREADS), smem, s, w_map, x_map, a, c.row_tiles, static_cast<int>(all));
+    launch_pdl(kern, dim3(2 * clusters), dim3(FP_THREADS), smem, s, w_map, x_map, y_map, a, c.row_tiles, static_cast<int>(all));
     return launch_status();
 }
 
