@@ -447,11 +447,11 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
 // fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's
 // rows and weights are few.
 // Warp 0 feeds the weights, 2 the rows, 3 the scales; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
-#define FP_STAGES 5
+#define FP_STAGES 4
 #define FP_THREADS 384
-#define FP_BLOCK 4096             // a warp's rows on their way out: 32 of 128 bytes
-#define FP_RING 3                 // groups of tiles of K whose scales are there
-#define FP_GROUP 4
+#define FP_BLOCK 8192             // a warp's rows on their way out: 32 of 64 features, or of 128 in 16 bits
+#define FP_RING 2                 // groups of tiles of K whose scales are there
+#define FP_GROUP 8
 #define FP_SCALES (128 * 4 + 2 * 16)      // bytes of a tile of K's: 128 rows', two tiles of weights'
 #define FP_SMALL 40               // registers of a thread that takes no sums, and of one that does: (128 * 40 + 256 * 232) = 384 * 168
 #define FP_LARGE 232
@@ -494,6 +494,10 @@ __device__ __forceinline__ bool fp_wait_warp(bool seen, unsigned long long* bar,
     if (!seen) ok = fp_wait(bar, parity, waits, abort_flag, status);
     __syncwarp();
     return ok;
+}
+// One lane's word for the warp, without a branch that would part it from the others.
+__device__ __forceinline__ void fp_tell(unsigned bar) {
+    asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, %1, 0;\n @p mbarrier.arrive.shared::cluster.b64 _, [%0];\n}\n" ::"r"(bar), "r"(threadIdx.x & 31) : "memory");
 }
 // acc += a * b of two float32 values each, where it stands: between what is asked for in front of it and used behind it.
 __device__ __forceinline__ void fp_fma2(unsigned long long& acc, unsigned long long a, unsigned long long b) {
@@ -722,7 +726,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(FP_LARGE));
         const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
-        const unsigned acc_empty_first = fp_map_to(t5_smem(&acc_empty[0]), 0);
+        const unsigned acc_empty_first = fp_map_to(t5_smem(&acc_empty[0]), 0), s_empty_own = fp_map_to(t5_smem(&s_empty[0]), rank);
         unsigned char* block = out_s + (warp - 4) * FP_BLOCK;
         const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + half * 128;
         unsigned buf = 0, acc_phase = 0, slot = 0, s_phase = 0, turn = 0;
@@ -765,6 +769,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                     }
                 };
                 const unsigned now = from + buf * 256;
+                bool seen_s = false;
+                if (kb % FP_GROUP == FP_GROUP - 1 && !last)       // the next group's scales
+                    seen_s = slot + 1 < FP_RING ? fp_look(&s_full[slot + 1], s_phase) : fp_look(&s_full[0], s_phase ^ 1);
                 t5_wait_ld();
                 add(0);
                 t5_ld32(now + 64, r[0]);
@@ -772,18 +779,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 t5_ld32(now + 96, r[1]);
                 if (kb % FP_GROUP == FP_GROUP - 1 || last) {      // the group's scales are in registers
                     __syncwarp();
-                    if (lane == 0) t5_arrive(&s_empty[slot]);
-                    __syncwarp();
+                    fp_tell(s_empty_own + slot * 8);
                     if (++slot == FP_RING) slot = 0, s_phase ^= 1;
-                    if (!last) ok = fp_wait_warp(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
+                    if (!last) ok = fp_wait_warp(seen_s, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
                 }
                 if (!last) scales(kb + 1);
                 t5_wait_ld();
                 // All of it is in registers: the accumulator is free again, with half of the additions still to do.
                 t5_fence_before();
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(acc_empty_first + buf * 8) : "memory");
-                __syncwarp();
+                fp_tell(acc_empty_first + buf * 8);
                 buf ^= 1;
                 if (buf == 0) acc_phase ^= 1;
                 if (last) {
