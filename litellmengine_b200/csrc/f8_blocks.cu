@@ -44,7 +44,7 @@ template <bool FAST> __device__ __forceinline__ void f8_load(const float* row, i
 
 template <int U, bool FAST, typename T>
 __global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, float* __restrict__ scales, unsigned items,
-                                                             unsigned per_row, int K, int ktiles, long long padded, const int32_t* __restrict__ places, int top) {
+                                                             unsigned per_row, int K, int ktiles, int k4, long long padded, const int32_t* __restrict__ places, int top) {
     pdl_begin();
     const unsigned w = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5);
     if (w >= items) return;                                       // whole warps
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* __restrict
             const long long to = places ? static_cast<long long>(places[static_cast<size_t>(row) * top + k]) : static_cast<long long>(row);
             if (to < 0) continue;                                 // a pick without an expert
             *reinterpret_cast<uint2*>(codes + (kb * padded + to) * F8_K + (lane & 15) * 8) = c;
-            if ((lane & 15) == 0) scales[kb * padded + to] = s.scale;
+            if ((lane & 15) == 0) scales[to * k4 + kb] = s.scale;
         }
     }
 }
@@ -86,7 +86,7 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 #define LAUNCH(U, FAST, T_)                                                                                                                       \
     launch_pdl((f8_rows_kernel<U, FAST, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(x), codes, scales, static_cast<unsigned>(items), per_row, K, \
-               ktiles, padded, places, places ? top : 1)
+               ktiles, f8_k4(K), padded, places, places ? top : 1)
 #define LAUNCH_T(T_)                                        \
     if (many) { if (fast) LAUNCH(4, true, T_); else LAUNCH(4, false, T_); } \
     else { if (fast) LAUNCH(1, true, T_); else LAUNCH(1, false, T_); }
@@ -102,8 +102,8 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
 // A CTA a block of 128 x 128: sixteen lanes a row, two rows a warp and trip, eight trips that are asked for together.  It does not invite the kernel behind
 // it: products fetch weights before they wait for what is in front of them.
 template <bool FAST, typename T>
-__global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ codes, float4* __restrict__ scales, int rows, int K,
-                                                               int tiles, int ktiles, int gate_rows, long long row_stride, long long matrix_stride) {
+__global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ codes, float* __restrict__ scales, int rows, int K,
+                                                               int tiles, int ktiles, int k4, int gate_rows, long long row_stride, long long matrix_stride) {
     __shared__ unsigned most_s[F8_THREADS / 32];
     pdl_wait();
     const int kb = blockIdx.x, block = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -111,12 +111,13 @@ __global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* __restri
     const int col = kb * F8_K + (lane & 15) * 8, there = rows - block * 128;
     const long long stack = static_cast<long long>(blockIdx.z) * tiles;
     codes += stack * ktiles * F8_TILE + kb * F8_TILE + (lane & 15) * 8;
-    scales += stack * ktiles + kb;
+    scales += stack * 3 * k4 + kb;
     if (gate_rows && there <= 0) {                                // one CTA more: the rows of whole tiles that gate and up do not have
         for (int f = gate_rows + warp * 2 + (lane >> 4); f < tiles * 64; f += F8_THREADS / 16)
             for (int up = 0; up < 2; ++up) *reinterpret_cast<uint2*>(codes + static_cast<long long>(f >> 6) * ktiles * F8_TILE + (up * 64 + (f & 63)) * F8_K) = make_uint2(0u, 0u);
         const int empty = (gate_rows + 63) / 64 + threadIdx.x;    // tiles of nothing else
-        if (empty < tiles) scales[static_cast<long long>(empty) * ktiles] = make_float4(F8_LEAST, F8_LEAST, F8_LEAST, 0.0f);
+        if (empty < tiles)
+            for (int i = 0; i < 3; ++i) scales[(empty * 3LL + i) * k4] = F8_LEAST;
         return;
     }
     typename F8Raw<T>::type raw[8];
@@ -143,13 +144,13 @@ __global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* __restri
             *reinterpret_cast<uint2*>(codes + static_cast<long long>(tile) * ktiles * F8_TILE + at * F8_K) = f8_codes(raw[u], most, s.inverse);
     }
     if (!gate_rows) {
-        if (threadIdx.x == 0) scales[static_cast<long long>(block) * ktiles] = make_float4(s.scale, s.scale, s.scale, 0.0f);
+        if (threadIdx.x < 3) scales[(block * 3LL + threadIdx.x) * k4] = s.scale;
     } else if (threadIdx.x < 4) {                                 // the tiles whose gate rows, first up row or last up row lie in this block
         const int first = block * 128, i = first / 64 + threadIdx.x, j = (first - gate_rows) / 64 - 1 + static_cast<int>(threadIdx.x);
-        if (i * 64 < gate_rows && i * 64 / 128 == block) scales[static_cast<long long>(i) * ktiles].x = s.scale;
+        if (i * 64 < gate_rows && i * 64 / 128 == block) scales[i * 3LL * k4] = s.scale;
         if (j >= 0 && j * 64 < gate_rows) {
-            if ((gate_rows + j * 64) / 128 == block) scales[static_cast<long long>(j) * ktiles].y = s.scale;
-            if ((gate_rows + min(j * 64 + 63, gate_rows - 1)) / 128 == block) scales[static_cast<long long>(j) * ktiles].z = s.scale;
+            if ((gate_rows + j * 64) / 128 == block) scales[(j * 3LL + 1) * k4] = s.scale;
+            if ((gate_rows + min(j * 64 + 63, gate_rows - 1)) / 128 == block) scales[(j * 3LL + 2) * k4] = s.scale;
         }
     }
 }
@@ -168,7 +169,7 @@ extern "C" int llm_f8_weight(const void* w, int dtype, void* codes, void* scales
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 #define LAUNCH(FAST, T_)                                                                                                                              \
     launch_pdl((f8_weight_kernel<FAST, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(w), static_cast<unsigned char*>(codes), \
-               static_cast<float4*>(scales), rows, K, tiles, f8_tiles(K), gated ? N : 0, row_stride, matrix_stride)
+               static_cast<float*>(scales), rows, K, tiles, f8_tiles(K), f8_k4(K), gated ? N : 0, row_stride, matrix_stride)
     if (dtype == LLM_DT_BF16) { if (fast) LAUNCH(true, bf16); else LAUNCH(false, bf16); }
     else if (dtype == LLM_DT_F32) { if (fast) LAUNCH(true, float); else LAUNCH(false, float); }
     else return LLM_REFUSED_DTYPE;
@@ -180,7 +181,7 @@ extern "C" int llm_f8_weight(const void* w, int dtype, void* codes, void* scales
 // Eight lanes a tile's row, sixteen codes a lane, U rows a thread asked for together.
 template <int U, bool FAST, typename T>
 __global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned char* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, int rows,
-                                                               int N, int K, int ktiles, int tiles, long long padded, int kind) {
+                                                               int N, int K, int ktiles, int k4, int tiles, long long padded, int kind) {
     // kind 0: rows, 1: a weight, 2: a gated one (N: its gate rows); tiles: of 128 rows
     pdl_begin();
     const int kb = blockIdx.x % ktiles, piece = threadIdx.x & 7, col = kb * F8_K + piece * 16;
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned ch
         if (r >= rows) continue;
         if (kind == 0) {
             c[u] = *reinterpret_cast<const uint4*>(codes + (kb * padded + r) * F8_K + piece * 16);
-            s[u] = scales[kb * padded + r];
+            s[u] = scales[r * k4 + kb];
         } else {
             const int per = kind == 2 ? 2 * N : N;                // rows of a matrix of the stack
             const long long e = r / per;
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned ch
             const long long tile = e * tiles + (kind == 2 ? (i >> 6) : (i >> 7));
             const int in = kind == 2 ? up * 64 + (i & 63) : i & 127, which = !up ? 0 : (i & 63) < f8_split(N, i >> 6) ? 1 : 2;
             c[u] = *reinterpret_cast<const uint4*>(codes + ((tile * ktiles + kb) * 128 + in) * F8_K + piece * 16);
-            s[u] = scales[(tile * ktiles + kb) * 4 + which];
+            s[u] = scales[(tile * 3 + which) * k4 + kb];
         }
     }
 #pragma unroll
@@ -242,7 +243,7 @@ extern "C" int llm_f8_values(const void* codes, const void* scales, void* out, i
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 #define LAUNCH(FAST, T_)                                                                                                                              \
     launch_pdl((f8_values_kernel<U, FAST, T_>), dim3(static_cast<unsigned>(blocks)), dim3(F8_THREADS), 0, s, static_cast<const unsigned char*>(codes), \
-               static_cast<const float*>(scales), static_cast<T_*>(out), rows, N, K, ktiles, tiles, padded, kind)
+               static_cast<const float*>(scales), static_cast<T_*>(out), rows, N, K, ktiles, f8_k4(K), tiles, padded, kind)
     if (dtype == LLM_DT_BF16) { if (fast) LAUNCH(true, bf16); else LAUNCH(false, bf16); }
     else if (dtype == LLM_DT_F32) { if (fast) LAUNCH(true, float); else LAUNCH(false, float); }
     else return LLM_REFUSED_DTYPE;

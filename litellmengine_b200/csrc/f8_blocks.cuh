@@ -6,12 +6,12 @@
 // A block with an infinity or a NaN has the scale NaN: all of it reads as NaN, and so does every sum that it is in.
 //
 // Where the bytes lie: K is padded with zeros to whole tiles of 128 values.
-//   rows     codes [tile of K][rows, padded][128], float32 scales [tile of K][rows, padded] behind them: the products take a tile of K of
+//   rows     codes [tile of K][rows, padded][128], behind them float32 scales [rows, padded][tiles of K, padded to fours]: the products take a tile of K of
 //            neighbouring rows as one box, whatever row it starts at
-//   weights  codes [matrix of a stack][tile of 128 rows][tile of K][128][128], 16 KB that lie side by side; float4 scales [...][tile of K] behind
-//            them.  An even number of tiles.  A gated weight [gate; up] has 64 gate rows and the 64 up rows beside them in a tile; its values are those
-//            of the same matrix without that, whose blocks count from the first row of gate.  So the 64 up rows may lie in two blocks, where the number of
-//            gate rows is no multiple of 64: the scales of a tile are those of its first 64 rows, of its 65th, and of its last
+//   weights  codes [matrix of a stack][tile of 128 rows][tile of K][128][128], 16 KB that lie side by side; behind them float32 scales
+//            [...][3][tiles of K, padded to fours].  An even number of tiles.  A gated weight [gate; up] has 64 gate rows and the 64 up rows beside them in a tile; its
+//            values are those of the same matrix without that, whose blocks count from the first row of gate.  So the 64 up rows may lie in two blocks, where the
+//            number of gate rows is no multiple of 64: the three scales of a tile are those of its first 64 rows, of its 65th, and of its last
 #pragma once
 
 #include "microscaling.cuh"
@@ -24,6 +24,7 @@
 // Rows that stand behind T rows: hardly a box of a product (16, 32, 64 or 128 rows) then reaches beyond them, which takes longer.
 static inline long long f8_padded_rows(long long T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : (T + 127) / 128 * 128; }
 static inline int f8_tiles(int k) { return (k + F8_K - 1) / F8_K; }
+static inline int f8_k4(int k) { return (f8_tiles(k) + 3) / 4 * 4; }       // room for a row's scales
 // Gated: the first of a tile's 64 up rows that lie in the second of two blocks; 64: none does.  i: the tile's number in its matrix.
 __host__ __device__ __forceinline__ int f8_split(int gate_rows, int i) {
     const int at = 128 - (gate_rows + 64 * i) % 128;

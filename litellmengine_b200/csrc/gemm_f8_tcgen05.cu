@@ -49,13 +49,13 @@ __host__ __device__ constexpr unsigned f8_idesc(int m, int n) {
 }
 
 struct F8Args {
-    const float4* w_scales;               // [tiles][ktiles] of a tile's first 64 features, its 65th, its last
-    const float* x_scales;                // [ktiles][x_rows]
+    const float* w_scales;                // [tiles][first 64 features, 65th, last][K4]
+    const float* x_scales;                // [x_rows][K4]
     long long x_rows;
     void* y;                              // [T, N]; gated: the codes [tiles / 2][y_rows][128]
-    float* y_scales;                      // gated: [tiles / 2][y_rows]
+    float* y_scales;                      // gated: [y_rows][y_k4]
     long long y_rows;
-    int T, N, K, ktiles, tiles, vec, waits;       // tiles: of a matrix of the stack; N gated: features of the result
+    int T, N, K, ktiles, k4, y_k4, tiles, vec, waits;       // k4: room for a row's scales; tiles: of a matrix of the stack; N gated: features of the result
     int32_t* status;
     MxAct act;
     const bf16* plain;                    // a matrix [tokens, K] that the kernel takes to 8 bits itself
@@ -194,10 +194,9 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
             if ((kb & 31) == 0)
 #pragma unroll
                 for (int w = 0; w < WT; ++w) {
-                    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (kb + lane < kbs) s = a.w_scales[(first_tile + w) * static_cast<long long>(a.ktiles) + kb0 + kb + lane];
-                    mine[w][0] = quarter < 2 ? s.x : s.y;
-                    if (WS_ == 2) mine[w][WS_ - 1] = quarter < 2 ? s.x : s.z;
+                    const float* s = a.w_scales + (first_tile + w) * 3LL * a.k4 + kb0 + kb + lane;
+#pragma unroll
+                    for (int i = 0; i < WS_; ++i) mine[w][i] = kb + lane < kbs ? s[WS_ == 1 || quarter < 2 ? 0 : (1 + i) * a.k4] : 0.0f;
                 }
             ok = __all_sync(0xffffffffu, (q || f8_wait(&x_full[g], turn, a.waits, &abort_flag, a.status)) &&
                                              f8_wait(&acc_full[slot], acc_phase, a.waits, &abort_flag, a.status));
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
                 const int i = lane + 32 * j, kb = first + i / NT;
-                s[j] = i < G * NT && kb < a.ktiles && row0 + i % NT < a.x_rows ? a.x_scales[kb * a.x_rows + row0 + i % NT] : 0.0f;
+                s[j] = i < G * NT && kb < a.ktiles && row0 + i % NT < a.x_rows ? a.x_scales[(row0 + i % NT) * static_cast<long long>(a.k4) + kb] : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < EACH; ++j)
@@ -374,7 +373,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
         };
         if constexpr (MODE == F8_GATED) {
             // a warp a row, four features a lane, all of a block
-            const int f = 4 * lane, block = blockIdx.y;
+            const int f = 4 * lane;
+            const long long block = blockIdx.y;
             unsigned char* codes = static_cast<unsigned char*>(a.y);
 #pragma unroll 1
             for (int r = first_row; r < rows; r += THREADS / 32 * parts) {
@@ -389,9 +389,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
                 most = __reduce_max_sync(0xffffffffu, most);
                 const F8Scale s = f8_scale(most);
                 if (!__any_sync(0xffffffffu, quit)) {
-                    const size_t at = block * a.y_rows + row0 + r;
-                    *reinterpret_cast<unsigned*>(codes + at * F8_K + f) = mx_e4m3x4(v[0] * s.inverse, v[1] * s.inverse, v[2] * s.inverse, v[3] * s.inverse);
-                    if (lane == 0) a.y_scales[at] = s.scale;
+                    *reinterpret_cast<unsigned*>(codes + (block * a.y_rows + row0 + r) * F8_K + f) = mx_e4m3x4(v[0] * s.inverse, v[1] * s.inverse, v[2] * s.inverse, v[3] * s.inverse);
+                    if (lane == 0) a.y_scales[(row0 + r) * static_cast<long long>(a.y_k4) + block] = s.scale;
                 }
             }
         } else {
@@ -440,21 +439,23 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
 
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 // The two CTAs of a cluster compute a tile of 256 rows x 256 features together (cta_group::2): each brings its own 128 rows and half of the features, and
-// reads both halves.  Tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them, one after the other, while 256
-// threads, a row and 128 features each, take out those of the tile of K before, so that the sums are in registers.  The products of a tile of K take 512 clocks,
-// which is what an accumulator's way round (its products 256, telling 200, taking out 350, telling 200) leaves room for; with two accumulators of 256 features
-// that way is twice 600.  The clusters are persistent; the products go on into the next tile while the threads write a finished one.  Tiles are numbered row tile
-// fastest: what runs at one time shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's
-// rows and weights are few.
-// Warp 0 feeds the weights, 2 the rows, 3 the scales; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
+// reads both halves.  Tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them one after the other while 256 threads
+// (a row and 64 features of either each) take out those before, so that the sums are in registers.  What limits it is an accumulator's way round: its products 256
+// clocks, 300 until the threads of both CTAs know, 100 to take it out (all of it, before anything is added), 250 until the products know that it is free again: 1,000
+// of the 1,024 that four leave.  With two accumulators of 256 features, taken out and added in turns, the way is 1,700 and bounds the kernel.
+// Shared memory is busy with the products' operands (128 bytes a clock, all that it has), so that a load from it takes 200 clocks and a look at a barrier as much: the
+// threads that take the sums have their scales from memory, two tiles of K in a load and two ahead, and ask early whether the next accumulator is full.
+// The clusters are persistent; the products go on into the next tile while the threads write a finished one.  Tiles are numbered row tile fastest: what runs at one time
+// shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's rows and weights are few.
+// Warp 0 feeds the weights, 2 the rows; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
 #define FP_STAGES 4
 #define FP_THREADS 384
 #define FP_BLOCK 8192             // a warp's rows on their way out: 32 of 64 features, or of 128 in 16 bits
 #define FP_RING 2                 // groups of tiles of K whose scales are there
 #define FP_GROUP 8
-#define FP_SCALES (128 * 4 + 2 * 16)      // bytes of a tile of K's: 128 rows', two tiles of weights'
-#define FP_SMALL 40               // registers of a thread that takes no sums, and of one that does: (128 * 40 + 256 * 232) = 384 * 168
-#define FP_LARGE 232
+#define FP_SCALES (128 * 4 + 2 * 16)      // bytes of a tile of K's: 128 rows', three of either tile of weights
+#define FP_SMALL 56               // registers of a thread that takes no sums, and of one that does: (128 * 56 + 256 * 224) = 384 * 168
+#define FP_LARGE 224
 
 __device__ __forceinline__ unsigned fp_rank() {
     unsigned r;
@@ -498,10 +499,6 @@ __device__ __forceinline__ bool fp_wait_warp(bool seen, unsigned long long* bar,
 // One lane's word for the warp, without a branch that would part it from the others.
 __device__ __forceinline__ void fp_tell(unsigned bar) {
     asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, %1, 0;\n @p mbarrier.arrive.shared::cluster.b64 _, [%0];\n}\n" ::"r"(bar), "r"(threadIdx.x & 31) : "memory");
-}
-// acc += a * b of two float32 values each, where it stands: between what is asked for in front of it and used behind it.
-__device__ __forceinline__ void fp_fma2(unsigned long long& acc, unsigned long long a, unsigned long long b) {
-    asm volatile("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(acc) : "l"(a), "l"(b));
 }
 // Boxes into this CTA's shared memory, counted on a barrier of the pair's first CTA.
 __device__ __forceinline__ void fp_tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
@@ -564,7 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     unsigned char* out_s = x_s + FP_STAGES * F8_TILE;             // a block for each of the eight warps
     float* most_s = reinterpret_cast<float*>(out_s);              // gated: [2][2][128]
     unsigned char* scales_s = out_s + 8 * FP_BLOCK;               // [RING]
-    __shared__ __align__(8) unsigned long long full[FP_STAGES], empty[FP_STAGES], acc_full[4], acc_empty[2], s_full[FP_RING], s_empty[FP_RING], drained;
+    __shared__ __align__(8) unsigned long long full[FP_STAGES], empty[FP_STAGES], acc_full[4], acc_empty[4], s_full[FP_RING], s_empty[FP_RING], drained;
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag, asked_s[2];                        // asked_s: boxes of weights, of rows that were asked for
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -573,8 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < FP_STAGES; ++s) { t5_mbar_init(&full[s], 2); t5_mbar_init(&empty[s], 1); }      // weights and rows
-        for (int s = 0; s < 4; ++s) t5_mbar_init(&acc_full[s], 1);
-        for (int s = 0; s < 2; ++s) t5_mbar_init(&acc_empty[s], 16);      // 8 warps of 2 CTAs
+        for (int s = 0; s < 4; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 8); }      // 4 warps of 2 CTAs
         for (int s = 0; s < FP_RING; ++s) { t5_mbar_init(&s_full[s], 32); t5_mbar_init(&s_empty[s], 8); }
         t5_mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -592,7 +588,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     if (GROUPED || warp != 0) pdl_wait();                         // weights are nobody's output, the items are
     const int tiles = GROUPED ? a.groups.counts[0] * (a.tiles / 2) : all_tiles;
 
-    // This thread's box (or two of weights: 64 features of either tile, so that a product's two halves are a tile) for tile at and tile of K kb, into stage s.
+    // This thread's box (or two of weights: 64 features of either tile, so that an accumulator is a tile) for tile at and tile of K kb, into stage s.
     const unsigned first = fp_map_to(t5_smem(full), 0);           // the first CTA's barriers
     auto ask = [&](const FpTile& at, int kb, int s) {
         if (rank == 0) t5_expect_tx(&full[s], 2 * F8_TILE);       // of both CTAs
@@ -643,18 +639,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
             for (int t = cluster; ok && t < tiles; t += clusters) {
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; ++kb) {
-                    ok = fp_wait_warp(seen, &full[s], phase, a.waits, &abort_flag, a.status);
-                    ok = __all_sync(0xffffffffu, fp_wait_warp(false, &acc_empty[buf], acc_phase, a.waits, &abort_flag, a.status) && ok);
-                    if (!ok) break;
-                    t5_fence_after();
+                    ok = fp_wait_warp(seen, &full[s], phase, a.waits, &abort_flag, a.status) && ok;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        ok = fp_wait_warp(false, &acc_empty[2 * buf + h], acc_phase, a.waits, &abort_flag, a.status) && ok;
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        t5_fence_after();
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)               // of the features' first or other halves in both CTAs
+                        for (int k = 0; k < 4; ++k)
                             fp_mma_lead(lead, tmem + buf * 256 + h * 128, xd + s * (F8_TILE >> 4) + 2 * k, wd + ((s * F8_TILE + h * (F8_TILE / 2)) >> 4) + 2 * k, idesc, k ? 1u : 0u);
                         if (h == 1) fp_commit_lead(lead, &empty[s]);
                         fp_commit_lead(lead, &acc_full[2 * buf + h]);
                     }
+                    if (!ok) break;
                     if (++s == FP_STAGES) s = 0, phase ^= 1;
                     seen = fp_look(&full[s], phase);
                     buf ^= 1;
@@ -662,18 +660,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 }
             }
         } else if (warp == 3) {
-            // A tile of K's scales: four rows a lane, and of the weights' the first two lanes', copied without a register between.
+            // A tile of K's scales: four rows a lane, and of the weights' the first six lanes', copied without a register between.
             int slot = 0;
             unsigned phase = 1;
             bool ok = true;
             for (int t = cluster; ok && t < tiles; t += clusters) {
                 const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
                 const int r0 = at.row0 + static_cast<int>(rank) * 128 + lane;
-                const float* cx = a.x_scales;
-                const float4* cw = a.w_scales + (at.tile + (lane & 1)) * static_cast<long long>(ktiles);
-                int rows[4], bytes[4];                            // beyond the last row: zeros
+                const float* cw = a.w_scales + (at.tile * 3LL + min(lane, 5)) * a.k4;
+                const float* cx[4];
+                int bytes[4];                                     // beyond the last row: zeros
 #pragma unroll
-                for (int i = 0; i < 4; ++i) bytes[i] = r0 + 32 * i < a.x_rows ? 4 : 0, rows[i] = bytes[i] ? r0 + 32 * i : 0;
+                for (int i = 0; i < 4; ++i) bytes[i] = r0 + 32 * i < a.x_rows ? 4 : 0, cx[i] = a.x_scales + (bytes[i] ? (r0 + 32 * i) * static_cast<long long>(a.k4) : 0);
 #pragma unroll 1
                 for (int kb0 = 0; kb0 < ktiles; kb0 += FP_GROUP) {
                     ok = __all_sync(0xffffffffu, fp_wait(&s_empty[slot], phase, a.waits, &abort_flag, a.status));
@@ -683,9 +681,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                     for (int kb = kb0; kb < min(kb0 + FP_GROUP, ktiles); ++kb, to += FP_SCALES) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + (lane + 32 * i) * 4), "l"(cx + rows[i]), "r"(bytes[i]) : "memory");
-                        if (lane < 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 512 + lane * 16), "l"(cw + kb) : "memory");
-                        cx += a.x_rows;
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + (lane + 32 * i) * 4), "l"(cx[i] + (bytes[i] ? kb : 0)), "r"(bytes[i]) : "memory");
+                        if (lane < 6) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to + 512 + (lane / 3 * 4 + lane % 3) * 4), "l"(cw + kb) : "memory");
                     }
                     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(t5_smem(&s_full[slot])) : "memory");
                     if (++slot == FP_RING) slot = 0, phase ^= 1;
@@ -735,75 +732,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
             unsigned long long acc[64];                           // two features each
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0ull;
-            bool ok = true;
-            // What stands on the way from one accumulator to the next (is it full, its scales, its numbers) is asked for in front of additions and used behind
-            // them.  One that gives up goes on with what there is, and stores nothing.
             const int split = SPLIT ? f8_split(a.N, 2 * at.features + half) : 64;
-            float sx, s0, s1, s2;
+            float sx;
             float4 sw;
             auto scales = [&](int kb) {
                 const unsigned char* p = scales_s + (slot * FP_GROUP + kb % FP_GROUP) * FP_SCALES;
                 sx = *reinterpret_cast<const float*>(p + row * 4);
                 sw = *reinterpret_cast<const float4*>(p + 512 + half * 16);
             };
-            ok = fp_wait_warp(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status);
+            // One that gives up goes on with what there is, and stores nothing.
+            bool ok = fp_wait_warp(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status);
             scales(0);
             ok = fp_wait_warp(false, &acc_full[2 * buf + half], acc_phase, a.waits, &abort_flag, a.status) && ok;
             t5_fence_after();
             unsigned r[2][32];
             t5_ld32(from + buf * 256, r[0]);
-            t5_ld32(from + buf * 256 + 32, r[1]);
 #pragma unroll 1
             for (int kb = 0; kb < ktiles; ++kb) {
-                const bool last = kb + 1 == ktiles;
-                s0 = sx * sw.x;
-                s1 = MODE == F8_GATED ? sx * sw.y : s0;
-                s2 = SPLIT ? sx * sw.z : s1;
+                // The wait for numbers waits for all that a thread has asked for.  So what the next tile of K needs (its scales, whether its accumulator is full) is asked
+                // for together with them, with additions in between.
+                const bool last = kb + 1 == ktiles, group_ends = kb % FP_GROUP == FP_GROUP - 1 || last;
+                const float s0 = sx * sw.x, s1 = MODE == F8_GATED ? sx * sw.y : s0, s2 = SPLIT ? sx * sw.z : s1;
                 const unsigned long long first_64 = t5_two(s0, s0), other_64 = t5_two(s1, s1);
                 auto add = [&](int c) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int f = (c - 2) * 32 + 2 * i;       // of the up features
                         const unsigned long long s = c < 2 ? first_64 : SPLIT ? t5_two(f < split ? s1 : s2, f + 1 < split ? s1 : s2) : other_64;
-                        fp_fma2(acc[c * 16 + i], t5_two(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s);
+                        acc[c * 16 + i] = t5_fma2(t5_two(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s, acc[c * 16 + i]);
                     }
                 };
                 const unsigned now = from + buf * 256;
-                bool seen_s = false;
-                if (kb % FP_GROUP == FP_GROUP - 1 && !last)       // the next group's scales
-                    seen_s = slot + 1 < FP_RING ? fp_look(&s_full[slot + 1], s_phase) : fp_look(&s_full[0], s_phase ^ 1);
                 t5_wait_ld();
-                add(0);
-                t5_ld32(now + 64, r[0]);
-                add(1);
-                t5_ld32(now + 96, r[1]);
-                if (kb % FP_GROUP == FP_GROUP - 1 || last) {      // the group's scales are in registers
+                t5_ld32(now + 32, r[1]);
+                bool seen_s = true;
+                if (group_ends) {
                     __syncwarp();
                     fp_tell(s_empty_own + slot * 8);
                     if (++slot == FP_RING) slot = 0, s_phase ^= 1;
-                    if (!last) ok = fp_wait_warp(seen_s, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
+                    if (!last) seen_s = fp_look(&s_full[slot], s_phase);
                 }
-                if (!last) scales(kb + 1);
+                add(0);
                 t5_wait_ld();
-                // All of it is in registers: the accumulator is free again, with half of the additions still to do.
+                t5_ld32(now + 64, r[0]);
+                if (!last) {
+                    if (group_ends) ok = fp_wait_warp(seen_s, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
+                    scales(kb + 1);
+                }
+                add(1);
+                t5_wait_ld();
+                t5_ld32(now + 96, r[1]);
+                unsigned long long* const next = &acc_full[2 * (buf ^ 1) + half];
+                const unsigned next_phase = buf ? acc_phase ^ 1 : acc_phase;
+                const bool seen = last || fp_look(next, next_phase);
+                add(2);
+                t5_wait_ld();
+                // All of it is in registers: the accumulator is free again, with a quarter of the additions still to do.
                 t5_fence_before();
                 __syncwarp();
-                fp_tell(acc_empty_first + buf * 8);
+                fp_tell(acc_empty_first + (2 * buf + half) * 8);
                 buf ^= 1;
-                if (buf == 0) acc_phase ^= 1;
-                if (last) {
-                    add(2);
-                    add(3);
-                    break;
+                acc_phase = next_phase;
+                if (!last) {
+                    ok = fp_wait_warp(seen, next, next_phase, a.waits, &abort_flag, a.status) && ok;
+                    t5_fence_after();
+                    t5_ld32(from + buf * 256, r[0]);
                 }
-                unsigned long long* const next = &acc_full[2 * buf + half];
-                const bool seen = fp_look(next, acc_phase);
-                add(2);
-                ok = fp_wait_warp(seen, next, acc_phase, a.waits, &abort_flag, a.status) && ok;
-                t5_fence_after();
-                t5_ld32(from + buf * 256, r[0]);
                 add(3);
-                t5_ld32(from + buf * 256 + 32, r[1]);
             }
             ok = __all_sync(0xffffffffu, ok);
             if constexpr (MODE == F8_GATED) ok = fp_all(ok);      // the two halves of a row meet below: all go on or leave together
@@ -844,7 +839,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                         }
                         *reinterpret_cast<uint4*>(codes + i * 16) = make_uint4(c[0], c[1], c[2], c[3]);
                     }
-                    if (half == 0) a.y_scales[to] = s.scale;
+                    if (half == 0) a.y_scales[(row0 + lane) * a.y_k4 + at.features] = s.scale;
                 }
             } else {
                 // 32 neighbouring features of each of the warp's rows at a time through shared memory, in pieces of 16 bytes that the row number scatters over the banks (the copy engine's swizzle).  The copy engine takes them out, adds, and leaves out what is beyond the matrix;
@@ -1078,8 +1073,8 @@ extern "C" int llm_linear_f8(int which, void* rows, long long padded, const void
     if (!counts) per = llm_f8_way(T);
     if ((per != 16 && per != 32 && per != 64 && per != 256) || (!rows && per != 16) || (rows && padded < T)) return LLM_REFUSED_SIZE;
     if (counts && (!items || !tokens || room <= 0 || add)) return LLM_REFUSED_SIZE;
-    a.w_scales = static_cast<const float4*>(w_scales);
-    a.ktiles = f8_tiles(K), a.tiles = tiles;
+    a.w_scales = static_cast<const float*>(w_scales);
+    a.ktiles = f8_tiles(K), a.k4 = f8_k4(K), a.y_k4 = f8_k4(N), a.tiles = tiles;
     a.x_scales = rows ? f8_row_scales(rows, padded, a.ktiles) : nullptr, a.x_rows = padded;
     a.y = y, a.y_rows = y_padded;
     a.T = T, a.N = N, a.K = K, a.waits = waits, a.status = status;

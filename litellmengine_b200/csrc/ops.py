@@ -2616,8 +2616,8 @@ def f8_padded_rows(T: int) -> int:
 
 class F8Rows:
     """Rows [T, K] in 8 bits (e4m3) with a float32 scale per 128 values: what `linear_f8` and `linear_silu_mul_f8` read.  Made by
-    `f8_rows` and `linear_silu_mul_f8`.  `codes`: uint8 [tiles of K, rows padded, 128]; `scales`: float32 [tiles of K, rows padded]; `values`
-    gives the rows as a matrix again."""
+    `f8_rows` and `linear_silu_mul_f8`.  `codes`: uint8 [tiles of K, rows padded, 128]; `scales`: float32 [rows padded, tiles of K padded to fours];
+    `values` gives the rows as a matrix again."""
 
     __slots__ = ("shape", "device", "padded", "buffer")
 
@@ -2626,7 +2626,8 @@ class F8Rows:
         self.device = device
         self.padded = f8_padded_rows(T)
         # one allocation: the codes, then the scales
-        self.buffer = torch.empty((K + 127) // 128 * self.padded * 132, dtype=torch.uint8, device=device)
+        tiles = (K + 127) // 128
+        self.buffer = torch.empty(self.padded * (tiles * 128 + (tiles + 3) // 4 * 16), dtype=torch.uint8, device=device)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -2636,7 +2637,7 @@ class F8Rows:
     @property
     def scales(self) -> torch.Tensor:
         tiles = (self.shape[1] + 127) // 128
-        return self.buffer[tiles * self.padded * 128:].view(torch.float32).view(tiles, self.padded)
+        return self.buffer[tiles * self.padded * 128:].view(torch.float32).view(self.padded, (tiles + 3) // 4 * 4)
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         T, K = self.shape
@@ -2660,9 +2661,9 @@ class F8Weight:
         N, K = shape[-2:]
         # tiles of 128 rows: an even number of a matrix, because products of many rows take two at a time
         self.tiles = n, tiles = 2 * ((N // 2 + 127) // 128 if gated else (N + 255) // 256), (K + 127) // 128
-        # one allocation: the codes, then three scales and room for a fourth for each tile
+        # one allocation: the codes, then three scales for each tile
         self.scales_behind = self.experts * n * tiles * 128 * 128
-        self.buffer = torch.empty(self.scales_behind + self.experts * n * tiles * 16, dtype=torch.uint8, device=device)
+        self.buffer = torch.empty(self.scales_behind + self.experts * n * ((tiles + 3) // 4 * 4) * 12, dtype=torch.uint8, device=device)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -2672,7 +2673,7 @@ class F8Weight:
     @property
     def scales(self) -> torch.Tensor:
         n, tiles = self.tiles
-        return self.buffer[self.scales_behind:].view(torch.float32).view(self.experts, n, tiles, 4)
+        return self.buffer[self.scales_behind:].view(torch.float32).view(self.experts, n, 3, (tiles + 3) // 4 * 4)
 
     @property
     def nbytes(self) -> int:
