@@ -15,6 +15,8 @@
 #include "f8_blocks.cuh"
 #include "tcgen05_attention.cuh"
 
+#include <type_traits>
+
 #define F8_STATUS 10
 
 __device__ __forceinline__ bool f8_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
@@ -532,6 +534,29 @@ __device__ __forceinline__ bool fp_all(bool yes) {
     return r != 0;
 }
 
+// mx_gated (microscaling.cuh) with the fast exponential and reciprocal as they are, off by less than 8 + 1.5 |z| units of 2^-24, of eight values step by step: the products
+// wait for 64 of these a thread and tile, which one after the other take 8,000 clocks.  SILU: z = g, no clamps, no shift.
+template <bool SILU> __device__ __forceinline__ void fp_gated8(float (&g)[8], float (&u)[8], const MxAct& a, float* out) {
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (!SILU) {
+            g[i] = g[i] > a.limit ? a.limit : g[i];
+            u[i] = (u[i] > a.limit ? a.limit : u[i] < -a.limit ? -a.limit : u[i]) + a.shift;
+            s[i] = g[i] * (a.alpha + a.beta * g[i] * g[i]) * -1.4426950408889634f;
+        } else {
+            s[i] = g[i] * -1.4426950408889634f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = t5_ex2(s[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = 1.0f + s[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("rcp.approx.ftz.f32 %0, %0;\n" : "+f"(s[i]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = g[i] * s[i] * u[i];
+}
 // What a tile of the launch is.
 struct FpTile {
     int row0, rows;                       // of the pair: first, and how many there are from it on (more than 256 where it goes on)
@@ -810,16 +835,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 if (GROUPED && a.on_input && lane < valid) w = a.groups.weights[row0 + lane];
                 float v[64];
                 unsigned most = 0;
+                auto gated = [&](auto silu) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    float g0, g1, u0, u1;
-                    t5_untwo(acc[i], g0, g1);
-                    t5_untwo(acc[32 + i], u0, u1);
-                    if (GROUPED) g0 *= w, g1 *= w, u0 *= w, u1 *= w;
-                    v[2 * i] = mx_gated(g0, u0, a.act);
-                    v[2 * i + 1] = mx_gated(g1, u1, a.act);
-                    most = max(most, max(mx_abs_bits(v[2 * i]), mx_abs_bits(v[2 * i + 1])));
-                }
+                    for (int i = 0; i < 8; ++i) {
+                        float g[8], u[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) t5_untwo(acc[i * 4 + j], g[2 * j], g[2 * j + 1]), t5_untwo(acc[32 + i * 4 + j], u[2 * j], u[2 * j + 1]);
+                        if (GROUPED)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) g[j] *= w, u[j] *= w;
+                        fp_gated8<decltype(silu)::value>(g, u, a.act, v + 8 * i);
+                    }
+                };
+                if (a.act.beta == 0.0f && a.act.shift == 0.0f) gated(std::true_type());       // without clamps too (mx_act)
+                else gated(std::false_type());
+#pragma unroll
+                for (int i = 0; i < 64; ++i) most = max(most, mx_abs_bits(v[i]));
                 // the other 64 features of the row are another thread's; two places in turn, so that the next tile's need not wait for these to be read
                 most_s[(turn * 2 + half) * 128 + row] = __uint_as_float(most);
                 asm volatile("bar.sync 1, 256;\n" ::: "memory");
