@@ -873,83 +873,89 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                     if (half == 0) a.y_scales[(row0 + lane) * a.y_k4 + at.features] = s.scale;
                 }
             } else {
-                // 32 neighbouring features of each of the warp's rows at a time through shared memory, in pieces of 16 bytes that the row number scatters over the banks (the copy engine's swizzle).  The copy engine takes them out, adds, and leaves out what is beyond the matrix;
-                // rows of an expert that end within these 32, and rows that it cannot address, leave by the lanes.
-                constexpr int LINE = 32 * sizeof(TO), PIECES = LINE / 16, BLOCKS = FP_BLOCK / (32 * LINE);       // bytes of a row, its pieces, blocks in turn
+                // 32 neighbouring features of each of the warp's rows make a block in shared memory, in pieces of 16 bytes that the row number scatters over the banks (the
+                // copy engine's swizzle).  The copy engine takes blocks out, adds, and leaves out what is beyond the matrix; rows of an expert that end
+                // within these 32, and rows that it cannot address, leave by the lanes.
+                constexpr int LINE = 32 * sizeof(TO), PIECES = LINE / 16, BLOCKS = FP_BLOCK / (32 * LINE);       // bytes of a row, its pieces, blocks that there is room for
                 float w = 1.0f;
                 if (GROUPED && a.groups.weights && lane < valid) w = a.groups.weights[row0 + lane];
                 TO* y = static_cast<TO*>(a.y) + row0 * a.N;
                 const bool copies = a.vec && (!GROUPED || valid == 32);
                 auto place = [&](int r, int piece) { return r * LINE + ((PIECES == 8 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) << 4); };
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int col0 = at.features * 256 + half * 128 + c * 32;
-                    if (col0 >= a.N) break;
-                    unsigned char* to_s = block + turn % BLOCKS * (32 * LINE);
-                    // the block has been read
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(BLOCKS - 1) : "memory");
+                for (int c0 = 0; c0 < 4; c0 += BLOCKS) {
+                    const int first_col = at.features * 256 + half * 128 + c0 * 32, blocks = min((a.N - first_col + 31) / 32, BLOCKS);
+                    if (blocks <= 0 || valid <= 0) break;
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");       // the blocks have been read
                     __syncwarp();
 #pragma unroll
-                    for (int p = 0; p < PIECES; ++p) {
-                        unsigned q[4];
+                    for (int c = 0; c < BLOCKS; ++c)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float lo, hi;
-                            if constexpr (sizeof(TO) == 4) {
-                                t5_untwo(acc[c * 16 + p * 2 + i / 2], lo, hi);
-                                q[i] = __float_as_uint((i & 1 ? hi : lo) * (GROUPED ? w : 1.0f));
-                            } else {
-                                t5_untwo(acc[c * 16 + p * 4 + i], lo, hi);
-                                q[i] = GROUPED ? t5_pack(lo * w, hi * w) : t5_pack(lo, hi);
+                        for (int p = 0; p < PIECES; ++p) {
+                            unsigned q[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float lo, hi;
+                                if constexpr (sizeof(TO) == 4) {
+                                    t5_untwo(acc[(c0 + c) * 16 + p * 2 + i / 2], lo, hi);
+                                    q[i] = __float_as_uint((i & 1 ? hi : lo) * (GROUPED ? w : 1.0f));
+                                } else {
+                                    t5_untwo(acc[(c0 + c) * 16 + p * 4 + i], lo, hi);
+                                    q[i] = GROUPED ? t5_pack(lo * w, hi * w) : t5_pack(lo, hi);
+                                }
                             }
+                            *reinterpret_cast<uint4*>(block + c * (32 * LINE) + place(lane, p)) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
-                        *reinterpret_cast<uint4*>(to_s + place(lane, p)) = make_uint4(q[0], q[1], q[2], q[3]);
-                    }
                     if (copies) {
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
-                            if (valid > 0) {
-                                if (MODE == F8_ADD)
-                                    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(t5_smem(to_s)),
-                                                 "r"(col0), "r"(static_cast<int>(row0)) : "memory");
-                                else
-                                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map), "r"(t5_smem(to_s)),
-                                                 "r"(col0), "r"(static_cast<int>(row0)) : "memory");
-                            }
+#pragma unroll
+                            for (int c = 0; c < BLOCKS; ++c)
+                                if (c < blocks) {
+                                    if (MODE == F8_ADD)
+                                        asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map),
+                                                     "r"(t5_smem(block + c * (32 * LINE))), "r"(first_col + c * 32), "r"(static_cast<int>(row0)) : "memory");
+                                    else
+                                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(&y_map),
+                                                     "r"(t5_smem(block + c * (32 * LINE))), "r"(first_col + c * 32), "r"(static_cast<int>(row0)) : "memory");
+                                }
                             asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                         }
                         __syncwarp();
-                        ++turn;
                         continue;
                     }
                     __syncwarp();
-                    if (a.vec) {                                  // rows of whole, aligned pieces of 16 bytes
-                        constexpr int PIECE = 16 / sizeof(TO);
-                        const int p = lane % PIECES, col = col0 + p * PIECE;
-#pragma unroll
-                        for (int i = 0; i < PIECES; ++i) {
-                            const int r = i * (32 / PIECES) + lane / PIECES;
-                            if (r >= valid || col >= a.N) continue;
-                            uint4 v = *reinterpret_cast<const uint4*>(to_s + place(r, p));
-                            uint4* to = reinterpret_cast<uint4*>(y + static_cast<size_t>(r) * a.N + col);
-                            if constexpr (MODE == F8_ADD) {
-                                const float4 o = *reinterpret_cast<const float4*>(to);
-                                v.x = __float_as_uint(__uint_as_float(v.x) + o.x), v.y = __float_as_uint(__uint_as_float(v.y) + o.y);
-                                v.z = __float_as_uint(__uint_as_float(v.z) + o.z), v.w = __float_as_uint(__uint_as_float(v.w) + o.w);
-                            }
-                            *to = v;
-                        }
-                    } else {
-                        const int col = col0 + lane;
-                        if (col < a.N)
 #pragma unroll 1
-                            for (int r = 0; r < valid; ++r) {
-                                TO v = *reinterpret_cast<const TO*>(to_s + place(r, lane * static_cast<int>(sizeof(TO)) / 16) + lane * sizeof(TO) % 16);
-                                TO* to = y + static_cast<size_t>(r) * a.N + col;
-                                if constexpr (MODE == F8_ADD) v += *to;
+                    for (int c = 0; c < blocks; ++c) {
+                        const unsigned char* from_s = block + c * (32 * LINE);
+                        if (a.vec) {                              // rows of whole, aligned pieces of 16 bytes
+                            constexpr int PIECE = 16 / sizeof(TO);
+                            const int p = lane % PIECES, col = first_col + c * 32 + p * PIECE;
+#pragma unroll
+                            for (int i = 0; i < PIECES; ++i) {
+                                const int r = i * (32 / PIECES) + lane / PIECES;
+                                if (r >= valid || col >= a.N) continue;
+                                uint4 v = *reinterpret_cast<const uint4*>(from_s + place(r, p));
+                                uint4* to = reinterpret_cast<uint4*>(y + static_cast<size_t>(r) * a.N + col);
+                                if constexpr (MODE == F8_ADD) {
+                                    const float4 o = *reinterpret_cast<const float4*>(to);
+                                    v.x = __float_as_uint(__uint_as_float(v.x) + o.x), v.y = __float_as_uint(__uint_as_float(v.y) + o.y);
+                                    v.z = __float_as_uint(__uint_as_float(v.z) + o.z), v.w = __float_as_uint(__uint_as_float(v.w) + o.w);
+                                }
                                 *to = v;
                             }
+                        } else {
+                            const int col = first_col + c * 32 + lane;
+                            if (col < a.N)
+#pragma unroll 4
+                                for (int r = 0; r < valid; ++r) {
+                                    TO v = *reinterpret_cast<const TO*>(from_s + place(r, lane * static_cast<int>(sizeof(TO)) / 16) + lane * sizeof(TO) % 16);
+                                    TO* to = y + static_cast<size_t>(r) * a.N + col;
+                                    if constexpr (MODE == F8_ADD) v += *to;
+                                    *to = v;
+                                }
+                        }
                     }
                     __syncwarp();
                 }
