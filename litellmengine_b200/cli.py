@@ -36,7 +36,7 @@ Options:
   --seed <int>             Seed of the sampling stream and of --random-weights, default: 0
   --device <str>           cuda, cuda:N, gpu or auto (there is no CPU path)
   --dtype <str>            bfloat16 (default) or float32
-  --weight-format <str>    stored (default), or mxfp4: softmax attention's and dense feed-forwards' matrices in 4 bits
+  --weight-format <str>    stored (default); mxfp4: softmax attention's and dense feed-forwards' matrices in 4 bits; fp8: those and routed experts' in 8 bits
   --eos-token-id <int>     Stop generation when this token id is generated
   --page-size <N>          Paged KV cache page size, default 16
   --max-total-tokens <N>   Tokens the cache pool holds, default: prompt + max tokens + 16
@@ -144,10 +144,10 @@ def parse_args(argv: List[str]) -> Args:
         raise ArgError("--page-size must be positive")
     if a.dtype not in ("bfloat16", "bf16", "float32", "fp32"):
         raise ArgError("--dtype must be bfloat16 or float32")
-    if a.weight_format not in ("stored", "mxfp4"):
-        raise ArgError("--weight-format must be stored or mxfp4")
-    if a.weight_format == "mxfp4" and a.dtype in ("float32", "fp32"):
-        raise ArgError("--weight-format mxfp4 is for --dtype bfloat16")
+    if a.weight_format not in ("stored", "mxfp4", "fp8"):
+        raise ArgError("--weight-format must be stored, mxfp4 or fp8")
+    if a.weight_format != "stored" and a.dtype in ("float32", "fp32"):
+        raise ArgError(f"--weight-format {a.weight_format} is for --dtype bfloat16")
     return a
 
 

@@ -6,6 +6,9 @@
 //   sorting   (token, choice) pairs by expert, and the experts' rows cut into tiles
 //   adding up a token's rows, in the order of its choices
 // Everything is bound by memory: each value is read once and each code written once.
+//
+// No pointer here is __restrict__: a load of what is const and restricted counts as one of constant memory, and may move in front of the wait for the kernel that
+// writes it (the sorting's picks did, where several kernels of a step were under way).
 #include "f8_blocks.cuh"
 
 #define F8_THREADS 256
@@ -43,8 +46,8 @@ template <bool FAST> __device__ __forceinline__ void f8_load(const float* row, i
 }
 
 template <int U, bool FAST, typename T>
-__global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, float* __restrict__ scales, unsigned items,
-                                                             unsigned per_row, int K, int ktiles, int k4, long long padded, const int32_t* __restrict__ places, int top) {
+__global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* x, unsigned char* codes, float* scales, unsigned items,
+                                                             unsigned per_row, int K, int ktiles, int k4, long long padded, const int32_t* places, int top) {
     pdl_begin();
     const unsigned w = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5);
     if (w >= items) return;                                       // whole warps
@@ -102,7 +105,7 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
 // A CTA a block of 128 x 128: sixteen lanes a row, two rows a warp and trip, eight trips that are asked for together.  It does not invite the kernel behind
 // it: products fetch weights before they wait for what is in front of them.
 template <bool FAST, typename T>
-__global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ codes, float* __restrict__ scales, int rows, int K,
+__global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* w, unsigned char* codes, float* scales, int rows, int K,
                                                                int tiles, int ktiles, int k4, int gate_rows, long long row_stride, long long matrix_stride) {
     __shared__ unsigned most_s[F8_THREADS / 32];
     pdl_wait();
@@ -180,7 +183,7 @@ extern "C" int llm_f8_weight(const void* w, int dtype, void* codes, void* scales
 // ---- values ---------------------------------------------------------------------------------------------------------
 // Eight lanes a tile's row, sixteen codes a lane, U rows a thread asked for together.
 template <int U, bool FAST, typename T>
-__global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned char* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, int rows,
+__global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned char* codes, const float* scales, T* out, int rows,
                                                                int N, int K, int ktiles, int k4, int tiles, long long padded, int kind) {
     // kind 0: rows, 1: a weight, 2: a gated one (N: its gate rows); tiles: of 128 rows
     pdl_begin();
@@ -259,9 +262,9 @@ extern "C" int llm_f8_values(const void* codes, const void* scales, void* out, i
 #define F8_SORT_CTAS 8
 #define F8_SORT_PICKS 4           // picks of a thread that stay in registers
 
-__global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* __restrict__ ids, const float* __restrict__ weights, int picks, int top, int E, int per,
-                                                       int32_t* __restrict__ counts, int4* __restrict__ items, int32_t* __restrict__ places,
-                                                       int32_t* __restrict__ tokens, float* __restrict__ row_weights) {
+__global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* ids, const float* weights, int picks, int top, int E, int per,
+                                                       int32_t* counts, int4* items, int32_t* places,
+                                                       int32_t* tokens, float* row_weights) {
     extern __shared__ int counted_s[];                            // [E] this CTA's picks, [E] the next row of an expert
     __shared__ int2 warps_s[32];
     int* next_s = counted_s + E;
@@ -360,8 +363,8 @@ extern "C" int llm_f8_sort(const int32_t* ids, const float* weights, int picks, 
 
 // out[token] = base[token] + the token's rows of y in the order of its choices, in 32 bits.
 template <typename TY, typename TO>
-__global__ void __launch_bounds__(128) f8_add_up_kernel(const TY* __restrict__ y, const int32_t* __restrict__ places, TO* __restrict__ out, int N, int top, int vec,
-                                                        const float* __restrict__ base) {
+__global__ void __launch_bounds__(128) f8_add_up_kernel(const TY* y, const int32_t* places, TO* out, int N, int top, int vec,
+                                                        const float* base) {
     pdl_begin();
     const size_t t = blockIdx.x;
     if (vec) {

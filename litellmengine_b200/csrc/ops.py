@@ -2837,12 +2837,15 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
 
 
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:
-    """residual (float32 [T, N]) += x @ weight^T in the product's epilogue, if the paired kernel or, for a weight in 4 bits, the
-    microscaled one takes these operands; False, and nothing done, if not."""
+    """residual (float32 [T, N]) += x @ weight^T in the product's epilogue, if the paired kernel or, for a weight in 4 or 8 bits, its
+    own takes these operands; False, and nothing done, if not."""
     if residual.dtype != torch.float32 or not residual.is_contiguous() or residual.shape != (x.shape[0], weight.shape[0]):
         return False
     if isinstance(weight, MxWeight):
         linear_mx(x, weight, residual=residual)
+        return True
+    if isinstance(weight, F8Weight):
+        linear_f8(x, weight, residual=residual)
         return True
     if not _pair_takes(x, weight, weight.shape[0], "into"):
         return False
@@ -2854,9 +2857,11 @@ def linear_silu_mul(x: torch.Tensor, w_gate_up: torch.Tensor, out_dtype: torch.d
                     limit: float = 0.0):
     """act(x @ gate^T) * (x @ up^T) for w_gate_up = [gate; up]: one kernel where the paired product
     takes it, else the product (which may stay a sum of k-splits) followed by the activation kernel.  A weight in 4 bits
-    (`MxWeight`): rows of 8 bits (`MxRows`)."""
+    (`MxWeight`): rows of 8 bits (`MxRows`); one in 8 bits (`F8Weight`): `F8Rows`."""
     if isinstance(w_gate_up, MxWeight):
         return linear_silu_mul_mx(x, w_gate_up, activation=activation, limit=limit)
+    if isinstance(w_gate_up, F8Weight):
+        return linear_silu_mul_f8(x, w_gate_up, activation=activation, limit=limit)
     if out_dtype == torch.bfloat16 and (isinstance(x, PendingRows) or (x.dtype == torch.bfloat16 and x.is_contiguous() and x.data_ptr() % 16 == 0
                                                                        and small_product(x.shape[0], w_gate_up, gated=True))):
         return linear_small(x, w_gate_up, out_dtype, activation=activation, limit=limit)
@@ -2932,9 +2937,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     keeps its product in true float32 (no TF32), whatever x is: up to 16 rows in the engine's own streaming kernel, more rows of large matrices
     on the tensor cores as sums of three bfloat16 values each, as near as float32 sums.  bfloat16 weights and those in 4 bits may be read before the
     kernel in front of the product in the stream has finished (they are nobody's output); float32 ones are not.  A weight in 4
-    bits (`MxWeight`) goes to `linear_mx`, which also takes `MxRows` (their result is bfloat16 without an `out_dtype`)."""
+    bits (`MxWeight`) goes to `linear_mx`, which also takes `MxRows` (their result is bfloat16 without an `out_dtype`), one in 8 (`F8Weight`) to
+    `linear_f8`, which also takes `F8Rows`."""
     if isinstance(weight, MxWeight):
         return linear_mx(x, weight, out_dtype or getattr(x, "dtype", torch.bfloat16))
+    if isinstance(weight, F8Weight):
+        return linear_f8(x, weight, out_dtype or getattr(x, "dtype", torch.bfloat16))
     if isinstance(x, PendingRows):
         return linear_small(x, weight, out_dtype or x.dtype)
     _dev(x, weight)

@@ -32,8 +32,8 @@ class PagedGenerateEngine:
                  chunk: Optional[int] = None, verbose: bool = False, seed: int = 0, pipelined: bool = True,
                  weight_format: str = "stored"):
         """`model`: a model folder (config.json + *.safetensors), a typed configuration (random
-        weights from `seed`, drawn on the device), or a ready `ModelRunner`.  `weight_format` 'mxfp4': matrices held in
-        4 bits, as `Model` has it (a ready runner's model has its own)."""
+        weights from `seed`, drawn on the device), or a ready `ModelRunner`.  `weight_format` 'mxfp4' or 'fp8': matrices held in
+        4 or 8 bits, as `Model` has it (a ready runner's model has its own)."""
         if isinstance(model, ModelRunner):
             self.runner = model
         else:

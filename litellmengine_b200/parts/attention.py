@@ -136,6 +136,11 @@ class AttentionMixer:
         self.w_qkv, self.w_o = ops.mx_weight(self.w_qkv), ops.mx_weight(self.w_o)
         return 2
 
+    def hold_in_8_bits(self) -> int:
+        """The same in 8 bits (`ops.F8Weight`)."""
+        self.w_qkv, self.w_o = ops.f8_weight(self.w_qkv), ops.f8_weight(self.w_o)
+        return 2
+
     def cache_need(self):
         if not self.spec.has_kv:
             return None
@@ -441,6 +446,11 @@ class GatedAttentionMixer(BranchMixer):
     def hold_in_4_bits(self) -> int:
         """As `AttentionMixer.hold_in_4_bits`."""
         self.w_in, self.w_o = ops.mx_weight(self.w_in), ops.mx_weight(self.w_o)
+        return 2
+
+    def hold_in_8_bits(self) -> int:
+        """As `AttentionMixer.hold_in_8_bits`."""
+        self.w_in, self.w_o = ops.f8_weight(self.w_in), ops.f8_weight(self.w_o)
         return 2
 
     def large_rows(self, between: bool):

@@ -189,14 +189,17 @@ class Block:
                 out[f"{prefix}.{name}" if name else prefix] = p      # '' : the tensor is named like the part
         return out
 
-    def parts_in_4_bits(self):
-        """The parts whose matrices a model of 4-bit weights holds in that form."""
-        return [p for p in self.parts() if speaks_for_forward(p, "hold_in_4_bits")]
+    HOLDS = {"mxfp4": "hold_in_4_bits", "fp8": "hold_in_8_bits"}      # weight format -> what a part says that holds its matrices so
 
-    def load(self, tensors: Dict[str, torch.Tensor], in_4_bits: bool = False) -> int:
-        """Bind the tensors; with `in_4_bits` the matrices of `parts_in_4_bits` are held so from then on (how many those were)."""
+    def parts_that_hold(self, weight_format: str):
+        """The parts whose matrices a model of this weight format holds in it."""
+        name = self.HOLDS.get(weight_format)
+        return [p for p in self.parts() if name is not None and speaks_for_forward(p, name)]
+
+    def load(self, tensors: Dict[str, torch.Tensor], weight_format: str = "stored") -> int:
+        """Bind the tensors; the matrices of `parts_that_hold(weight_format)` are held so from then on (how many those were)."""
         from ..csrc import ops
-        converted = self.parts_in_4_bits() if in_4_bits else []
+        converted = self.parts_that_hold(weight_format)
         for prefix, part in self._children():
             mine = {n[len(prefix) + 1:]: t for n, t in tensors.items() if n.startswith(prefix + ".")}
             if prefix in tensors and "" in part.parameters():
@@ -206,7 +209,7 @@ class Block:
         if self.layer_scales is not None or self.branch_scale != 1.0:
             for norm, ls in zip(self._output_norms(), self.layer_scales or (None, None)):
                 norm.scale_output(self.branch_scale if ls is None else ls.weight * self.branch_scale)
-        return sum(part.hold_in_4_bits() for part in converted)
+        return sum(getattr(part, self.HOLDS[weight_format])() for part in converted)
 
     def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor], ctx: StageContext
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -222,7 +225,7 @@ def _normed(norm, part, h: torch.Tensor, delta, dtype: torch.dtype):
         if isinstance(weight, ops.MxWeight):
             if speaks_for_forward(norm, "makes_mx_rows") and (delta is None or isinstance(delta, (torch.Tensor, ops.PartialSum))):
                 return h, norm.forward_mx(h, delta)
-        elif ops.rows_worth_leaving(h, delta) and speaks_for_forward(norm, "products_apply_it"):
+        elif not isinstance(weight, ops.F8Weight) and ops.rows_worth_leaving(h, delta) and speaks_for_forward(norm, "products_apply_it"):
             rows = ops.pending_rows(h, delta, norm, weight, dtype, gated)
             if rows is not None:
                 return rows.stream, rows

@@ -57,6 +57,11 @@ class SwiGLU:
         self.w_gate_up, self.w_down = ops.mx_weight(self.w_gate_up, gated=True), ops.mx_weight(self.w_down)
         return 2
 
+    def hold_in_8_bits(self) -> int:
+        """The same in 8 bits (`ops.F8Weight`)."""
+        self.w_gate_up, self.w_down = ops.f8_weight(self.w_gate_up, gated=True), ops.f8_weight(self.w_down)
+        return 2
+
     supports_partials = True   # forward(x, partials_ok=True) may return an ops.PartialSum
     supports_residual = True   # forward(x, residual=h) may add its result to h itself and return None
 
@@ -79,7 +84,8 @@ class RoutedExperts:
     The result is the weighted sum of the chosen experts' outputs.
 
     The experts' [gate; up] matrices are stacked into one and their down matrices stand side by side along the
-    input axis.  Three ways to run, chosen by the step's size; all give the same sums up to rounding.
+    input axis.  Three ways to run, chosen by the step's size; all give the same sums up to rounding.  (In 8 bits there is one,
+    `ops.moe_f8`: each expert's rows through its own matrices, whatever the step's size.)
     Prompt portions in bfloat16: the (token, choice) pairs are sorted by expert and each expert's rows go through
     its own matrices in the library's grouped matrix product (exactly the chosen experts' flops).  Steps whose
     pairs are fewer than the experts (decode steps of a model with many experts): two kernels that read only the
@@ -161,7 +167,7 @@ class RoutedExperts:
             count, keep = self.groups
             if self.E % count or not 0 < keep <= count or keep * (self.E // count) < self.top:
                 raise ValueError("the expert groups do not fit the experts that are chosen")
-        self.w_router = self.w_gate_up = self.w_down = None
+        self.w_router = self.w_gate_up = self.w_down = self.w_shared_gate_up = None
 
     def parameters(self) -> Dict[str, ParamSpec]:
         out = {"router": ParamSpec((self.E + self.identity, self.hidden), role="scale", init=("normal", 0.5))}
@@ -207,6 +213,15 @@ class RoutedExperts:
         ops.prepare_streaming(self.w_gate_up)
         ops.prepare_streaming(self.w_down)
 
+    def hold_in_8_bits(self) -> int:
+        """From now on the experts' matrices are stacks in 8 bits (`ops.F8Weight`), and the shared expert's are too.  How many matrices that are."""
+        rows, ff = self.E * 2 * self.ff, self.ff
+        if self.joined is not None:
+            self.w_shared_gate_up, self.w_shared_down = ops.f8_weight(self.w_gate_up[rows:]), ops.f8_weight(self.w_shared_down)
+        down = self.w_down.as_strided((self.E, self.hidden, ff), (ff, self.w_down.stride(0), 1))
+        self.w_gate_up, self.w_down = ops.f8_weight(self.w_gate_up[:rows].view(self.E, 2 * ff, self.hidden), gated=True), ops.f8_weight(down)
+        return 2 + (2 if self.joined is not None else 0) + (self.shared.hold_in_8_bits() if self.shared is not None else 0)
+
     def _route(self, x: torch.Tensor, lists: bool):
         """(dense weights, ids, weights, the tokens' share of their own input or None, the shared expert's weights or None)."""
         got = ops.moe_route(x, self.w_router, self.top, self.groups, self.route_scale, lists=lists, score=self.score,
@@ -219,7 +234,8 @@ class RoutedExperts:
 
     def _shared_alone(self, x: torch.Tensor, share, partials_ok: bool):
         n, limit = self.joined
-        gate_up = ops.linear(x, self.w_gate_up[self.E * 2 * self.ff:], out_dtype=torch.float32, partials_ok=True)
+        w = self.w_gate_up[self.E * 2 * self.ff:] if isinstance(self.w_gate_up, torch.Tensor) else self.w_shared_gate_up
+        gate_up = ops.linear(x, w, out_dtype=torch.float32, partials_ok=True)
         a = ops.moe_act(gate_up, None, 0, 0, 1.0, self.act_alpha, self.dtype, shift=self.act_shift, shared=(n, limit, share))
         return ops.linear(a, self.w_shared_down, out_dtype=torch.float32, partials_ok=partials_ok)
 
@@ -229,7 +245,11 @@ class RoutedExperts:
         plain = self.identity == 0 and self.shared is None        # nothing joins the experts' sum (a joined one is in it)
         routed_rows, routed_cols = self.E * 2 * self.ff, self.E * self.ff
         joined = None                                             # a joined expert's output where it ran alone
-        if (T * self.top < self.E and x.dtype == self.w_gate_up.dtype == self.w_down.dtype and self.hidden <= 12288
+        if isinstance(self.w_gate_up, ops.F8Weight):
+            _, ids, weights, own, share = self._route(x, True)
+            base = self._shared_alone(x, share, False) if self.joined is not None else None
+            out = ops.moe_f8(x, self.w_gate_up, self.w_down, ids, weights, activation=self.activation, limit=self.limit, on_input=self.on_input, base=base)
+        elif (T * self.top < self.E and x.dtype == self.w_gate_up.dtype == self.w_down.dtype and self.hidden <= 12288
                 and self.top * self.ff <= 12288):
             _, ids, weights, own, share = self._route(x, True)
             out = ops.moe_sparse(x, self.w_gate_up[:routed_rows], self.w_down[:, :routed_cols], ids, weights, self.ff, *act,

@@ -33,20 +33,22 @@ class Model:
     kernels and the cache are in the compute dtype (bfloat16 or float32); logits are float32.
     """
 
-    WEIGHT_FORMATS = ("stored", "mxfp4")
+    WEIGHT_FORMATS = ("stored", "mxfp4", "fp8")
 
     def __init__(self, plan: ModelPlan, dtype="bfloat16", device="cuda", weight_format: str = "stored"):
         """`weight_format` 'mxfp4': the matrices of the parts that can (`hold_in_4_bits`: softmax attention's projections, dense
         feed-forwards) are taken to 4 bits with a scale per 32 values when they are loaded, and multiply rows of 8 bits; all others (routed
         experts, recurrent and latent mixers, the embedding, the output head) stay as stored.  Layers of width 1,024 lose the products that make
-        their own input by it: decode steps of up to 16 requests take 2 to 9 % longer, larger ones and prompts less time, as all steps of width 2,048 do."""
+        their own input by it: decode steps of up to 16 requests take 2 to 9 % longer, larger ones and prompts less time, as all steps of width 2,048 do.
+        'fp8': the matrices of the parts with `hold_in_8_bits` (the same ones, and routed experts) are taken to 8 bits with a float32 scale per block of
+        128 x 128 values, and multiply rows of 8 bits with a scale per 128."""
         plan.validate()
         self.plan = plan
         self.dtype = _compute_dtype(dtype)
         if weight_format not in self.WEIGHT_FORMATS:
             raise ValueError(f"weight_format {weight_format!r}: one of {self.WEIGHT_FORMATS}")
         if weight_format != "stored" and self.dtype != torch.bfloat16:
-            raise ValueError("weights in 4 bits are for bfloat16 models")
+            raise ValueError("weights in 4 or 8 bits are for bfloat16 models")
         self.weight_format = weight_format
         self.device = torch.device(device)
         self.blocks: List[Block] = [Block(b, plan.hidden_size, self.dtype, self.device) for b in plan.blocks]
@@ -81,11 +83,10 @@ class Model:
                                        optional_alias=p.embedding_name if p.tie_word_embeddings else None)
         return out
 
-    def _names_in_4_bits(self) -> set:
-        """The tensors whose matrices are held in 4 bits once they are loaded."""
-        if self.weight_format != "mxfp4":
-            return set()
-        return {f"{spec.weight_prefix}.{name}" for spec, block in zip(self.plan.blocks, self.blocks) for name in block.parameters(block.parts_in_4_bits())}
+    def _names_held(self) -> set:
+        """The tensors whose matrices are held in the model's weight format once they are loaded."""
+        return {f"{spec.weight_prefix}.{name}" for spec, block in zip(self.plan.blocks, self.blocks)
+                for name in block.parameters(block.parts_that_hold(self.weight_format))}
 
     @staticmethod
     def _norm_tensor(prefix: str, k: int, name: str) -> str:
@@ -99,8 +100,8 @@ class Model:
         params = self.parameters()
         aliased = check_source(params, source, where)
         if self.dtype == torch.bfloat16:               # one decision for all of the model's matrices
-            in_4_bits = self._names_in_4_bits()
-            ops.begin_model(sum(ps.shape[0] * ps.shape[1] * 17 // 32 if n in in_4_bits else 2 * ps.shape[0] * ps.shape[1] for n, ps in params.items()
+            held_names, share = self._names_held(), {"mxfp4": 17 / 32, "fp8": 1.0}.get(self.weight_format, 2.0)
+            ops.begin_model(sum(int(ps.shape[0] * ps.shape[1] * share) if n in held_names else 2 * ps.shape[0] * ps.shape[1] for n, ps in params.items()
                                 if len(ps.shape) == 2 and n not in aliased), self.device)
         get = lambda n: fetch_tensor(source, n, params[n], self.dtype, self.device)
         have = set(source.names())
@@ -108,11 +109,11 @@ class Model:
         held = 0
         for spec, block in zip(p.blocks, self.blocks):
             # a tensor that may be absent and is: the part is handed nothing for it
-            # (in 4 bits: a layer's stored matrices are gone before the next one's come)
+            # (in 4 or 8 bits: a layer's stored matrices are gone before the next one's come)
             held += block.load({n: get(f"{spec.weight_prefix}.{n}") for n, ps in block.parameters().items()
-                                if not (ps.optional and f"{spec.weight_prefix}.{n}" not in have)}, in_4_bits=self.weight_format == "mxfp4")
-        if self.weight_format == "mxfp4" and not held:
-            raise ValueError("weight_format 'mxfp4': no part of this model holds its matrices in 4 bits")
+                                if not (ps.optional and f"{spec.weight_prefix}.{n}" not in have)}, weight_format=self.weight_format)
+        if self.weight_format != "stored" and not held:
+            raise ValueError(f"weight_format {self.weight_format!r}: no part of this model holds its matrices so")
         for norm, prefix in ((self.final_norm, p.final_norm_name), (self.embedding_norm, p.embedding_norm_name)):
             if norm is not None:
                 norm.load({name: get(self._norm_tensor(prefix, k, name)) for k, name in enumerate(norm.parameters())})
@@ -176,7 +177,7 @@ class Model:
                 for v in vars(part).values():
                     if isinstance(v, torch.Tensor) and v.dim() in (2, 3):
                         add(v)
-                    elif isinstance(v, ops.MxWeight):
+                    elif isinstance(v, (ops.MxWeight, ops.F8Weight)):
                         add(v.buffer)
         if self.rejoin is not None:
             for w in self.rejoin.matrices():
