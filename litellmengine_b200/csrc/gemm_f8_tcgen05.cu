@@ -67,17 +67,19 @@ struct F8Args {
 enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-#define F8_MAKERS 8               // warps that make rows of a matrix
-#define F8_FEW_THREADS(PLAIN) (32 * (6 + ((PLAIN) ? F8_MAKERS : 1)))
+// Warps: two that feed weights and issue, four for the sums of each of a CTA's tiles of the weight, and those that make rows of a matrix, or one that feeds rows.
+#define F8_MAKERS(WT) ((WT) == 2 ? 6 : 8)
+#define F8_FEW_CTAS(NT, WT) ((NT) * (WT) > 64 ? 1 : 2)          // on an SM: sums of 64 rows of two tiles need the registers of both
+#define F8_FEW_THREADS(PLAIN, WT) (32 * (2 + 4 * (WT) + ((PLAIN) ? F8_MAKERS(WT) : 1)))
 
 // grid (parts of K, tiles of features, tiles of rows or items), a cluster the parts of a tile.  WS: stages of weights; G: stages whose rows come together, two
 // such groups at a time.  A CTA's tile is 128 features, gated 64 + 64 gate and as many up features, of two tiles of the weight.
-// Warp 0 feeds the weights, warp 1 issues, warps 2 to 5 take the sums, warp 6 feeds the rows and their scales; or, PLAIN, x comes as a matrix and warps 6 to 13 make
+// Warp 0 feeds the weights, warp 1 issues, warps from 2 on take the sums, the last feeds the rows and their scales; or, PLAIN, x comes as a matrix and the last warps make
 // the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED>
-__global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+__global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1), F8_FEW_CTAS(NT, MODE == F8_GATED ? 2 : 1)) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                                          const F8Args a) {
-    constexpr int THREADS = F8_FEW_THREADS(PLAIN), WT = MODE == F8_GATED ? 2 : 1, FEATURES = 128 * WT;
+    constexpr int WT = MODE == F8_GATED ? 2 : 1, THREADS = F8_FEW_THREADS(PLAIN, WT), MAKERS = F8_MAKERS(WT), LAST = 2 + 4 * WT, FEATURES = 128 * WT;
     constexpr unsigned W_BYTES = WT * F8_TILE, X_BYTES = NT * F8_K, SLOT = NT * WT;
     constexpr unsigned SLOTS = 256 / SLOT < 4 ? 256 / SLOT : 4, COLS = SLOT * SLOTS < 32 ? 32 : SLOT * SLOTS;      // accumulators in turn; two CTAs share tensor memory
     static_assert(COLS <= 256 && SLOTS >= 2, "tensor memory");
@@ -108,8 +110,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < WS; ++s) { t5_mbar_init(&full[s], 1); t5_mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { t5_mbar_init(&x_full[s], PLAIN ? F8_MAKERS : 2); t5_mbar_init(&x_empty[s], 5); }      // the products and four warps of sums
-        for (int s = 0; s < static_cast<int>(SLOTS); ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 4); }
+        for (int s = 0; s < 2; ++s) { t5_mbar_init(&x_full[s], PLAIN ? MAKERS : 2); t5_mbar_init(&x_empty[s], 1 + 4 * WT); }      // the products and the warps of sums
+        for (int s = 0; s < static_cast<int>(SLOTS); ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 4 * WT); }
         t5_mbar_init(&drained, 1);
         t5_mbar_init(&fed, PLAIN ? 1 : 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -174,63 +176,54 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
         }
         t5_commit_lead(lead, &drained);                           // what was issued has ended, and all of it has been told
         f8_land(&drained, 0);
-    } else if (warp < 6) {
-        const int quarter = warp & 3, feature = quarter * 32 + lane;
+    } else if (warp < LAST) {
+        const int quarter = warp & 3, w = (warp - 2) >> 2, feature = quarter * 32 + lane;
         pdl_wait();
-        float acc[WT][NT];
+        float acc[NT];
 #pragma unroll
-        for (int w = 0; w < WT; ++w)
-#pragma unroll
-            for (int i = 0; i < NT; ++i) acc[w][i] = 0.0f;
+        for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
         // A lane has the weights' scales of every 32nd tile of K; of up rows two, where these 64 lie in two blocks.
-        constexpr int WS_ = MODE == F8_GATED ? 2 : 1;
-        float mine[WT][WS_];
-        bool second[WT];
-#pragma unroll
-        for (int w = 0; w < WT; ++w) second[w] = WS_ == 2 && quarter >= 2 && feature - 64 >= f8_split(a.N, blockIdx.y * WT + w);
+        constexpr int HELD = MODE == F8_GATED ? 2 : 1;
+        float mine[HELD];
+        const bool second = HELD == 2 && quarter >= 2 && feature - 64 >= f8_split(a.N, blockIdx.y * WT + w);
         int slot = 0, q = 0, g = 0;
         unsigned turn = 0, acc_phase = 0;
         bool ok = true;
 #pragma unroll 1
         for (int kb = 0; kb < kbs; ++kb) {
-            if ((kb & 31) == 0)
+            if ((kb & 31) == 0) {
+                const float* s = a.w_scales + (first_tile + w) * 3LL * a.k4 + kb0 + kb + lane;
 #pragma unroll
-                for (int w = 0; w < WT; ++w) {
-                    const float* s = a.w_scales + (first_tile + w) * 3LL * a.k4 + kb0 + kb + lane;
-#pragma unroll
-                    for (int i = 0; i < WS_; ++i) mine[w][i] = kb + lane < kbs ? s[WS_ == 1 || quarter < 2 ? 0 : (1 + i) * a.k4] : 0.0f;
-                }
+                for (int i = 0; i < HELD; ++i) mine[i] = kb + lane < kbs ? s[HELD == 1 || quarter < 2 ? 0 : (1 + i) * a.k4] : 0.0f;
+            }
             ok = __all_sync(0xffffffffu, (q || f8_wait(&x_full[g], turn, a.waits, &abort_flag, a.status)) &&
                                              f8_wait(&acc_full[slot], acc_phase, a.waits, &abort_flag, a.status));
             if (!ok) break;
             t5_fence_after();
-            const unsigned at = tmem + (static_cast<unsigned>(quarter * 32) << 16) + slot * SLOT;
+            const unsigned at = tmem + (static_cast<unsigned>(quarter * 32) << 16) + slot * SLOT + w * NT;
             const float* sx = sx_s + (g * G + q) * NT;
+            float sw = __shfl_sync(0xffffffffu, mine[0], kb & 31);
+            if constexpr (HELD == 2) {
+                const float other = __shfl_sync(0xffffffffu, mine[HELD - 1], kb & 31);
+                if (second) sw = other;
+            }
 #pragma unroll
-            for (int w = 0; w < WT; ++w) {
-                float sw = __shfl_sync(0xffffffffu, mine[w][0], kb & 31);
-                if constexpr (WS_ == 2) {
-                    const float other = __shfl_sync(0xffffffffu, mine[w][WS_ - 1], kb & 31);
-                    if (second[w]) sw = other;
+            for (int c = 0; c < NT; c += 16) {
+                unsigned r[16];
+                t5_ld16(at + c, r);
+                t5_wait_ld();
+                if (c + 16 == NT) {                               // all of it is in registers
+                    t5_fence_before();
+                    __syncwarp();
+                    if (lane == 0) t5_arrive(&acc_empty[slot]);
                 }
 #pragma unroll
-                for (int c = 0; c < NT; c += 16) {
-                    unsigned r[16];
-                    t5_ld16(at + w * NT + c, r);
-                    t5_wait_ld();
-                    if (w == WT - 1 && c + 16 == NT) {            // all of it is in registers
-                        t5_fence_before();
-                        __syncwarp();
-                        if (lane == 0) t5_arrive(&acc_empty[slot]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 s = *reinterpret_cast<const float4*>(sx + c + i);
-                        acc[w][c + i] = fmaf(__uint_as_float(r[i]), s.x * sw, acc[w][c + i]);
-                        acc[w][c + i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y * sw, acc[w][c + i + 1]);
-                        acc[w][c + i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z * sw, acc[w][c + i + 2]);
-                        acc[w][c + i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w * sw, acc[w][c + i + 3]);
-                    }
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 s = *reinterpret_cast<const float4*>(sx + c + i);
+                    acc[c + i] = fmaf(__uint_as_float(r[i]), s.x * sw, acc[c + i]);
+                    acc[c + i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y * sw, acc[c + i + 1]);
+                    acc[c + i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z * sw, acc[c + i + 2]);
+                    acc[c + i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w * sw, acc[c + i + 3]);
                 }
             }
             if (++slot == static_cast<int>(SLOTS)) slot = 0, acc_phase ^= 1;
@@ -243,10 +236,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
         }
         if (ok) {
 #pragma unroll
-            for (int w = 0; w < WT; ++w)
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-                    if (i < rows) sums[i * FEATURES + w * 128 + feature] = acc[w][i];
+            for (int i = 0; i < NT; ++i)
+                if (i < rows) sums[i * FEATURES + w * 128 + feature] = acc[i];
         } else {
             // A wait ran out.  Who asks for copies has stopped; the copies (the stages are where the sums go) and the products end; then NaNs tell
             // whoever adds the parts up that these sums are not there.  Nothing of it is in the way of a product that does not give up.
@@ -254,20 +245,19 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
             f8_land_ring(full, WS, asked_s[0]);
             if (!PLAIN) f8_land_ring(x_full, 2, asked_s[1]);
             f8_land(&drained, 0);
-            for (int i = 0; i < rows; ++i)
-                for (int w = 0; w < WT; ++w) sums[i * FEATURES + w * 128 + feature] = __uint_as_float(0x7fffffffu);
+            for (int i = 0; i < rows; ++i) sums[i * FEATURES + w * 128 + feature] = __uint_as_float(0x7fffffffu);
         }
     } else if constexpr (PLAIN) {                                 // rows beyond the last keep what stands there, nobody minds
         // A warp takes two stages of a row at a time, sixteen lanes each, and has the next group's values on their way while it makes this one's.
         static_assert(G % 2 == 0, "stages go in pairs");
-        constexpr int BATCH = (NT * G / 2 + F8_MAKERS - 1) / F8_MAKERS;       // units of a group that a warp has at most
+        constexpr int BATCH = (NT * G / 2 + MAKERS - 1) / MAKERS;       // units of a group that a warp has at most
         const int p = lane & 15, units = rows * (G / 2);
         const int left = a.K - kb0 * F8_K - (lane >> 4) * F8_K - p * 8;       // values of the row from the lane's first on
         const bf16* from[BATCH];
         pdl_wait();
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            const int u = warp - 6 + j * F8_MAKERS;
+            const int u = warp - LAST + j * MAKERS;
             long long r = 0;
             if (u < units) r = GROUPED ? a.groups.tokens[row0 + u / (G / 2)] : row0 + u / (G / 2);
             from[j] = a.plain + r * a.K + kb0 * F8_K + (lane >> 4) * F8_K + p * 8 + u % (G / 2) * 2 * F8_K;
@@ -276,7 +266,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
         auto fetch = [&](int grp) {
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const int u = warp - 6 + j * F8_MAKERS, at = grp * G * F8_K;
+                const int u = warp - LAST + j * MAKERS, at = grp * G * F8_K;
                 raw[j] = u < units && at + u % (G / 2) * 2 * F8_K < left ? *reinterpret_cast<const uint4*>(from[j] + at) : make_uint4(0u, 0u, 0u, 0u);
             }
         };
@@ -291,7 +281,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN), 2) f8_few_kernel(const 
             fetch(grp + 1);                                       // beyond the part: not used, and beyond the row not read
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const int u = warp - 6 + j * F8_MAKERS, r = u / (G / 2), q = u % (G / 2) * 2 + (lane >> 4);
+                const int u = warp - LAST + j * MAKERS, r = u / (G / 2), q = u % (G / 2) * 2 + (lane >> 4);
                 if (u >= units) break;                            // for the whole warp
                 const unsigned most = f8_most16(mx_most8(now[j]));
                 const F8Scale s = f8_scale(most);
@@ -1009,28 +999,33 @@ static bool f8_rows_map(CUtensorMap* map, const void* x, long long rows, int kti
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.  Two CTAs an SM, less an eighth, because clusters do not
+// Into how many parts K is cut: the most, up to 8 (a cluster), with which all clusters run at once.  One or two CTAs an SM, less an eighth, because clusters do not
 // fill a group of SMs to the last slot.
-static int f8_parts(long long tiles, int ktiles, int sms) {
-    const int slots = 2 * sms * 7 / 8;
+static int f8_parts(long long tiles, int ktiles, int sms, int ctas) {
+    const int slots = ctas * sms * 7 / 8;
     int best = 1;
     while (best < 8 && (best + 1) * tiles <= slots && ktiles / (best + 1) >= 2) ++best;
     return best;
 }
+// A weight as the host knows it: what its products need of it, the copy engine's maps included, put together once (llm_f8_describe).
+struct F8Weight {
+    CUtensorMap whole, halves;            // its codes in boxes of a tile, of half a tile
+    const void* codes;
+    const float* scales;
+    int E, N, K, tiles, gated, ready;     // N: of a matrix; gated: of its gate; tiles: of 128 rows of a matrix
+};
 struct F8Call {
-    const void* w;
-    long long w_tiles;                    // of the whole stack
+    const F8Weight* w;
     const void* x;                        // rows of 8 bits
     int row_tiles;                        // tiles of rows, or room for items
 };
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED> static int f8_few(const F8Call& c, const F8Args& a, cudaStream_t s) {
     constexpr int WT = MODE == F8_GATED ? 2 : 1;
-    CUtensorMap w_map, x_map = {};
-    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128, 128)) return LLM_REFUSED_SIZE;
+    CUtensorMap x_map = {};
     if (!PLAIN && !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, NT, G)) return LLM_REFUSED_SIZE;
     constexpr size_t smem = static_cast<size_t>(WS) * WT * F8_TILE + 2 * G * NT * (F8_K + sizeof(float)) + 1024;
     static_assert(NT * 128 * sizeof(float) <= WS * F8_TILE, "the sums fit the weights' stages");
-    static_assert(smem <= 113 * 1024, "half of an SM's shared memory");
+    static_assert(smem * F8_FEW_CTAS(NT, WT) <= 226 * 1024, "an SM's shared memory");
     auto kern = f8_few_kernel<NT, WS, G, PLAIN, MODE, TO, GROUPED>;
     static bool had[F8_DEVICES];
     const int dev = f8_device();
@@ -1038,15 +1033,15 @@ template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED
     if (const int rc = f8_allow(kern, smem, dev, had)) return rc;
     const int tiles = (MODE == F8_GATED ? a.tiles / 2 : (a.N + 127) / 128), sms = f8_sms(dev);
     if (tiles > 65535 || c.row_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
-    const int parts = f8_parts(static_cast<long long>(tiles) * c.row_tiles, a.ktiles, sms);
-    launch_pdl_cluster(kern, dim3(parts, tiles, c.row_tiles), dim3(F8_FEW_THREADS(PLAIN)), smem, s, parts, w_map, x_map, a);
+    const int parts = f8_parts(static_cast<long long>(tiles) * c.row_tiles, a.ktiles, sms, F8_FEW_CTAS(NT, WT));
+    launch_pdl_cluster(kern, dim3(parts, tiles, c.row_tiles), dim3(F8_FEW_THREADS(PLAIN, WT)), smem, s, parts, c.w->whole, x_map, a);
     return launch_status();
 }
 template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(const F8Call& c, F8Args a, cudaStream_t s) {
-    CUtensorMap w_map, x_map, y_map = {};
+    CUtensorMap x_map, y_map = {};
     const int dev = f8_device();
     if (dev < 0 || f8_sms(dev) < 2) return LLM_REFUSED_SIZE;
-    if (!f8_weight_map(&w_map, c.w, c.w_tiles * a.ktiles * 128, 64) || !f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, 128, 1)) return LLM_REFUSED_SIZE;
+    if (!f8_rows_map(&x_map, c.x, a.x_rows, a.ktiles, 128, 1)) return LLM_REFUSED_SIZE;
     if (MODE != F8_GATED) {                                       // [T, N] in boxes of 32 rows of 32 features
         a.vec = a.vec && a.N * sizeof(TO) % 16 == 0;
         const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.N), static_cast<cuuint64_t>(a.T)}, strides[1] = {static_cast<cuuint64_t>(a.N) * sizeof(TO)};
@@ -1066,7 +1061,7 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
     const int slots = f8_sms(dev) / 2;
     if (all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
-    launch_pdl(kern, dim3(2 * clusters), dim3(FP_THREADS), smem, s, w_map, x_map, y_map, a, c.row_tiles, static_cast<int>(all));
+    launch_pdl(kern, dim3(2 * clusters), dim3(FP_THREADS), smem, s, c.w->halves, x_map, y_map, a, c.row_tiles, static_cast<int>(all));
     return launch_status();
 }
 
@@ -1083,7 +1078,7 @@ template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const
     if constexpr (MODE == F8_GATED) {
         if (per == 16) return a.plain ? f8_few<16, 3, 2, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 3, 2, false, MODE, TO, GROUPED>(c, a, s);
         if (per == 32) return f8_few<32, 3, 1, false, MODE, TO, GROUPED>(c, a, s);
-        return f8_few<64, 2, 2, false, MODE, TO, GROUPED>(c, a, s);
+        return f8_few<64, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
     } else {
         if (per == 16) return a.plain ? f8_few<16, 5, 4, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 5, 4, false, MODE, TO, GROUPED>(c, a, s);
         if (per == 32) return f8_few<32, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
@@ -1091,42 +1086,139 @@ template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const
     }
 }
 
-// One product.  rows: of 8 bits [T, K] (`padded` of them), or null and `plain` a bfloat16 matrix [tokens, K] of whole, aligned pieces of eight values, for tiles of 16 rows;
-// w: a weight's codes and, behind them, its scales.
-//   which 0: y [T, N] float32 or bfloat16; add: y (float32) holds a summand already
-//   which 1: y the codes and scales of act(x gate^T) * (x up^T) as rows of 8 bits [T, N], `y_padded` of them; w gated
-// counts (null: one matrix): rows sorted by expert, `per` rows an item at most, room for `room` items; T: rows in all at most.  weights: of the rows, or null; they multiply
-// the result, with on_input the gate and up values.
-extern "C" int llm_linear_f8(int which, void* rows, long long padded, const void* plain, const void* w, const void* w_scales, int E, int tiles, void* y, int out_dtype,
-                             int add, long long y_padded, int T, int N, int K, int act, float limit, const int32_t* counts, const void* items,
-                             const int32_t* tokens, const float* weights, int on_input, int per, int room, int waits, int32_t* status, uintptr_t stream) {
+extern "C" int llm_f8_weight_size() { return static_cast<int>(sizeof(F8Weight)); }
+// room: llm_f8_weight_size() bytes on the host, 64-byte aligned; codes, scales: of a stack of E matrices of N rows (gated: N gate and N up rows).
+extern "C" int llm_f8_describe(void* room, const void* codes, const void* scales, int E, int N, int K, int gated) {
+    if (reinterpret_cast<uintptr_t>(room) % 64 || !aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
+    if (E <= 0 || N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 20)) return LLM_REFUSED_SIZE;
+    F8Weight w = {};
+    w.codes = codes, w.scales = static_cast<const float*>(scales);
+    w.E = E, w.N = N, w.K = K, w.gated = gated, w.tiles = gated ? 2 * ((N + 127) / 128) : (N + 255) / 256 * 2;
+    const long long lines = static_cast<long long>(E) * w.tiles * f8_tiles(K) * 128;
+    if (!f8_weight_map(&w.whole, codes, lines, 128) || !f8_weight_map(&w.halves, codes, lines, 64)) return LLM_REFUSED_SIZE;
+    w.ready = 1;
+    *static_cast<F8Weight*>(room) = w;
+    return LLM_OK;
+}
+
+static bool f8_takes_plain(const void* plain, int dtype, int T, int K) { return T <= F8_PLAIN_ROWS && dtype == LLM_DT_BF16 && K % 8 == 0 && aligned16(plain); }
+static int f8_args(F8Args* a, const F8Weight* w, int gated, const void* rows, long long padded, int T, int waits, int32_t* status) {
+    if (!w || !w->ready || w->gated != gated || status == nullptr || T > (1 << 24)) return LLM_REFUSED_SIZE;
+    if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
+    if (rows && padded < T) return LLM_REFUSED_SIZE;
+    *a = {};
+    a->w_scales = w->scales;
+    a->N = w->N, a->K = w->K, a->ktiles = f8_tiles(w->K), a->k4 = f8_k4(w->K), a->y_k4 = f8_k4(w->N), a->tiles = w->tiles;
+    a->x_scales = rows ? f8_row_scales(const_cast<void*>(rows), padded, a->ktiles) : nullptr, a->x_rows = padded;
+    a->T = T, a->waits = waits, a->status = status;
+    return LLM_OK;
+}
+// The rows of a product's x: those that are there; made of the matrix `plain` where there is room for them; or none, and the product makes them.
+static int f8_operand(F8Args* a, void* rows, long long padded, const void* plain, int dtype, uintptr_t stream) {
+    if (!plain) return rows ? LLM_OK : LLM_REFUSED_ALIGN;
+    if (rows) return llm_f8_rows(plain, dtype, rows, padded, a->T, a->K, nullptr, 1, stream);
+    if (!f8_takes_plain(plain, dtype, a->T, a->K)) return LLM_REFUSED_ALIGN;
+    a->plain = static_cast<const bf16*>(plain);
+    return LLM_OK;
+}
+
+// rows: of 8 bits [T, K], `padded` of them, or room for them (null: none, for up to F8_PLAIN_ROWS rows of a bfloat16 matrix of whole, aligned pieces of eight values) and
+// `plain` a matrix [T, K] of `dtype`; y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
+extern "C" int llm_linear_f8(const void* weight, void* rows, long long padded, const void* plain, int dtype, void* y, int out_dtype, int add, int T, int waits,
+                             int32_t* status, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
-    if (N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 20) || T > (1 << 24) || E <= 0 || status == nullptr || (which != 0 && which != 1)) return LLM_REFUSED_SIZE;
-    if (tiles != (which ? 2 * ((N + 127) / 128) : (N + 255) / 256 * 2)) return LLM_REFUSED_SIZE;
-    if (!aligned16(w) || !aligned16(w_scales) || !aligned16(rows) || (which && !aligned16(y))) return LLM_REFUSED_ALIGN;
-    if (!rows && !(plain && K % 8 == 0 && aligned16(plain))) return LLM_REFUSED_ALIGN;
     if (out_dtype != LLM_DT_F32 && (out_dtype != LLM_DT_BF16 || add)) return LLM_REFUSED_DTYPE;
-    F8Args a = {};
-    if (!counts) per = llm_f8_way(T);
-    if ((per != 16 && per != 32 && per != 64 && per != 256) || (!rows && per != 16) || (rows && padded < T)) return LLM_REFUSED_SIZE;
-    if (counts && (!items || !tokens || room <= 0 || add)) return LLM_REFUSED_SIZE;
-    a.w_scales = static_cast<const float*>(w_scales);
-    a.ktiles = f8_tiles(K), a.k4 = f8_k4(K), a.y_k4 = f8_k4(N), a.tiles = tiles;
-    a.x_scales = rows ? f8_row_scales(rows, padded, a.ktiles) : nullptr, a.x_rows = padded;
-    a.y = y, a.y_rows = y_padded;
-    a.T = T, a.N = N, a.K = K, a.waits = waits, a.status = status;
-    a.plain = rows ? nullptr : static_cast<const bf16*>(plain);
-    a.groups = {counts, static_cast<const int4*>(items), tokens, weights};
-    a.on_input = on_input;
-    const F8Call c = {w, static_cast<long long>(E) * tiles, rows, room};
+    const F8Weight* w = static_cast<const F8Weight*>(weight);
+    F8Args a;
+    if (const int rc = f8_args(&a, w, 0, rows, padded, T, waits, status)) return rc;
+    if (const int rc = f8_operand(&a, rows, padded, plain, dtype, stream)) return rc;
+    a.y = y;
+    a.vec = a.N % 4 == 0 && aligned16(y);
+    const F8Call c = {w, rows, 0};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (which == 1) {
-        if (!mx_act(act, limit, &a.act)) return LLM_REFUSED_SIZE;
-        a.y_scales = f8_row_scales(y, y_padded, (N + 127) / 128);
-        return counts ? f8_way<F8_GATED, float, true>(c, a, per, s) : f8_way<F8_GATED, float, false>(c, a, per, s);
-    }
-    a.vec = N % 4 == 0 && aligned16(y);
-    if (counts) return out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, true>(c, a, per, s) : f8_way<F8_STORE, bf16, true>(c, a, per, s);
+    const int per = llm_f8_way(T);
     if (add) return f8_way<F8_ADD, float, false>(c, a, per, s);
     return out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, false>(c, a, per, s) : f8_way<F8_STORE, bf16, false>(c, a, per, s);
 }
+
+// weight gated; made: act(x gate^T) * (x up^T) as rows of 8 bits [T, N], `made_padded` of them.
+extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long padded, const void* plain, int dtype, void* made, long long made_padded, int T, int act,
+                                      float limit, int waits, int32_t* status, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    const F8Weight* w = static_cast<const F8Weight*>(weight);
+    F8Args a;
+    if (const int rc = f8_args(&a, w, 1, rows, padded, T, waits, status)) return rc;
+    if (!mx_act(act, limit, &a.act) || made_padded < T) return LLM_REFUSED_SIZE;
+    if (!aligned16(made)) return LLM_REFUSED_ALIGN;
+    if (const int rc = f8_operand(&a, rows, padded, plain, dtype, stream)) return rc;
+    a.y = made, a.y_rows = made_padded;
+    a.y_scales = f8_row_scales(made, made_padded, f8_tiles(a.N));
+    return f8_way<F8_GATED, float, false>({w, rows, 0}, a, llm_f8_way(T), reinterpret_cast<cudaStream_t>(stream));
+}
+
+// Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
+// work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
+// middle's rows, the experts' results.
+static int f8_item_rows(long long picks, int E) { return picks <= 16LL * E ? 16 : picks <= 32LL * E ? 32 : picks <= 64LL * E ? 64 : 256; }
+static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
+struct F8Work {
+    int per, room, rows;                  // rows: of x are made in memory
+    long long items, counts, places, tokens, weights, x, middle, y, all;
+};
+static F8Work f8_work(long long picks, int E, int W, int ff, bool plain, int out_dtype) {
+    F8Work k = {};
+    k.per = f8_item_rows(picks, E);
+    k.room = static_cast<int>((E < picks ? E : picks) + picks / k.per);
+    k.rows = !(plain && k.per == 16);
+    const long long padded = f8_padded_rows(picks);
+    auto rows_bytes = [&](int n) { return padded * (f8_tiles(n) * F8_K + f8_k4(n) * 4LL); };
+    k.counts = f8_up(16LL * k.room);
+    k.places = k.counts + 256, k.tokens = k.places + f8_up(4 * picks), k.weights = k.tokens + f8_up(4 * picks);
+    k.x = k.weights + f8_up(4 * picks);
+    k.middle = k.x + (k.rows ? f8_up(rows_bytes(W)) : 0);
+    k.y = k.middle + f8_up(rows_bytes(ff));
+    k.all = k.y + picks * W * (out_dtype == LLM_DT_F32 ? 4 : 2);
+    return k;
+}
+static bool f8_plain_experts(const void* x, int dtype, int W) { return dtype == LLM_DT_BF16 && W % 8 == 0 && aligned16(x); }
+extern "C" long long llm_moe_f8_work(const void* x, int dtype, int T, int top, int E, int W, int ff, int out_dtype) {
+    return f8_work(static_cast<long long>(T) * top, E, W, ff, f8_plain_experts(x, dtype, W), out_dtype).all;
+}
+extern "C" int llm_f8_sort(const int32_t*, const float*, int, int, int, int, int32_t*, void*, int32_t*, int32_t*, float*, uintptr_t);
+extern "C" int llm_f8_add_up(const void*, int, const int32_t*, const float*, void*, int, int, int, uintptr_t);
+extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, int dtype, const int32_t* ids, const float* weights, int T, int top, void* work,
+                          const float* base, void* out, int out_dtype, int act, float limit, int on_input, int waits, int32_t* status, uintptr_t stream) {
+    if (T <= 0) return LLM_OK;
+    if (top <= 0 || static_cast<long long>(T) * top > (1 << 24)) return LLM_REFUSED_SIZE;
+    if (out_dtype != LLM_DT_F32 && out_dtype != LLM_DT_BF16) return LLM_REFUSED_DTYPE;
+    if (reinterpret_cast<uintptr_t>(work) % 256) return LLM_REFUSED_ALIGN;
+    const F8Weight *g = static_cast<const F8Weight*>(gate_up), *d = static_cast<const F8Weight*>(down);
+    if (!g || !d || g->E != d->E || g->N != d->K || g->K != d->N) return LLM_REFUSED_SIZE;
+    const int picks = T * top, W = g->K, ff = g->N;
+    const F8Work k = f8_work(picks, g->E, W, ff, f8_plain_experts(x, dtype, W), out_dtype);
+    unsigned char* at = static_cast<unsigned char*>(work);
+    int32_t *counts = reinterpret_cast<int32_t*>(at + k.counts), *places = reinterpret_cast<int32_t*>(at + k.places), *tokens = reinterpret_cast<int32_t*>(at + k.tokens);
+    float* row_weights = reinterpret_cast<float*>(at + k.weights);
+    const long long padded = f8_padded_rows(picks);
+    if (const int rc = llm_f8_sort(ids, weights, picks, top, g->E, k.per, counts, at, places, tokens, row_weights, stream)) return rc;
+    if (k.rows)
+        if (const int rc = llm_f8_rows(x, dtype, at + k.x, padded, T, W, places, top, stream)) return rc;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    F8Args a;
+    if (const int rc = f8_args(&a, g, 1, k.rows ? at + k.x : nullptr, padded, picks, waits, status)) return rc;
+    if (!mx_act(act, limit, &a.act)) return LLM_REFUSED_SIZE;
+    a.plain = k.rows ? nullptr : static_cast<const bf16*>(x);
+    a.y = at + k.middle, a.y_rows = padded, a.y_scales = f8_row_scales(at + k.middle, padded, f8_tiles(ff));
+    a.groups = {counts, reinterpret_cast<const int4*>(at), tokens, row_weights};
+    a.on_input = on_input;
+    if (const int rc = f8_way<F8_GATED, float, true>({g, k.rows ? at + k.x : nullptr, k.room}, a, k.per, s)) return rc;
+    if (const int rc = f8_args(&a, d, 0, at + k.middle, padded, picks, waits, status)) return rc;
+    a.y = at + k.y;
+    a.vec = W % 4 == 0;
+    a.groups = {counts, reinterpret_cast<const int4*>(at), tokens, on_input ? nullptr : row_weights};
+    const F8Call c = {d, at + k.middle, k.room};
+    if (const int rc = out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, true>(c, a, k.per, s) : f8_way<F8_STORE, bf16, true>(c, a, k.per, s)) return rc;
+    return llm_f8_add_up(at + k.y, out_dtype, places, base, out, T, W, top, stream);
+}
+// Kernels that llm_moe_f8 launches.
+extern "C" int llm_moe_f8_launches(const void* x, int dtype, int picks, int E, int W) { return 4 + (f8_work(picks, E, W, 1, f8_plain_experts(x, dtype, W), 0).rows ? 1 : 0); }

@@ -2601,9 +2601,11 @@ _MX_SIGNATURES.update({
     "llm_f8_rows": ("blocks_f8", [_P, _I, _P, _L, _I, _I, _P, _I, _P]),
     "llm_f8_weight": ("blocks_f8", [_P, _I, _P, _P, _I, _I, _I, _I, _I, _L, _L, _P]),
     "llm_f8_values": ("blocks_f8", [_P, _P, _P, _I, _I, _I, _I, _I, _L, _I, _P]),
-    "llm_f8_sort": ("blocks_f8", [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
-    "llm_f8_add_up": ("blocks_f8", [_P, _I, _P, _P, _P, _I, _I, _I, _P]),
-    "llm_linear_f8": ("blocks_f8", [_I, _P, _L, _P, _P, _P, _I, _I, _P, _I, _I, _L, _I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "llm_f8_weight_size": ("blocks_f8", []),
+    "llm_f8_describe": ("blocks_f8", [_P, _P, _P, _I, _I, _I, _I]),
+    "llm_linear_f8": ("blocks_f8", [_P, _P, _L, _P, _I, _P, _I, _I, _I, _I, _P, _P]),
+    "llm_linear_f8_silu_mul": ("blocks_f8", [_P, _P, _L, _P, _I, _P, _L, _I, _I, _F, _I, _P, _P]),
+    "llm_moe_f8": ("blocks_f8", [_P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _F, _I, _I, _P, _P]),
 })
 
 
@@ -2679,6 +2681,23 @@ class F8Weight:
     def nbytes(self) -> int:
         return self.buffer.numel()
 
+    def __getstate__(self):                       # a copy has an address, and so a description, of its own
+        return {k: v for k, v in self.__dict__.items() if k != "_described"}
+
+    def described(self) -> int:
+        """The address, on the host, of what the kernels' launches need to know of the weight: put together once, for its address on the device."""
+        at, known = self.buffer.data_ptr(), self.__dict__.get("_described")
+        if known is None or known[0] != at:
+            size = _mx_call("llm_f8_weight_size")()
+            room = ctypes.create_string_buffer(size + 64)
+            here = (ctypes.addressof(room) + 63) // 64 * 64
+            N, K = self.shape[-2:]
+            code = _mx_call("llm_f8_describe")(here, at, at + self.scales_behind, self.experts, N // 2 if self.gated else N, K, int(self.gated))
+            if code:
+                raise KernelError(f"a weight in 8 bits that no product takes: {_REFUSALS.get(code, code)}")
+            known = self._described = (at, here, room)
+        return known[1]
+
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         N, K = self.shape[-2:]
         _here(self.buffer)
@@ -2720,20 +2739,22 @@ def f8_rows(x: torch.Tensor) -> F8Rows:
 
 
 def _f8_operands(x, weight: F8Weight, gated: bool):
-    """(rows of 8 bits or None, the matrix that the product takes to 8 bits itself or None) of a product's x."""
+    """(rows of 8 bits or room for them or None, the address of a matrix that they are still to be made of or None, its dtype) of a product's x."""
     if not isinstance(weight, F8Weight) or weight.gated != gated or len(weight.shape) != 2:
         raise KernelError("the product takes an F8Weight of one matrix" + (" made with gated=True" if gated else " that is not a gated one"))
-    if not isinstance(x, (F8Rows, torch.Tensor)):
-        raise KernelError("the product takes rows of 8 bits or a matrix")
-    if len(x.shape) != 2 or x.shape[1] != weight.shape[1]:
+    shape = getattr(x, "shape", ())
+    if len(shape) != 2 or shape[1] != weight.shape[1]:
         raise KernelError("x and weight disagree on K")
     if type(x) is F8Rows:
         _here(x.buffer, weight.buffer)
-        return x, None
+        return x, None, 0
+    if not isinstance(x, torch.Tensor):
+        raise KernelError("the product takes rows of 8 bits or a matrix")
     _here(x, weight.buffer)
-    if x.shape[0] <= F8_PLAIN_ROWS and _dt(x) == 1 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0:
-        return None, x
-    return f8_rows(x), None
+    at, dt = x.data_ptr(), _dt(x)
+    if shape[0] <= F8_PLAIN_ROWS and dt == 1 and shape[1] % 8 == 0 and at % 16 == 0:
+        return None, at, dt
+    return F8Rows(shape[0], shape[1], weight.device), at, dt
 
 
 def linear_f8(x, weight: F8Weight, out_dtype: torch.dtype = torch.float32, residual: Optional[torch.Tensor] = None,
@@ -2741,8 +2762,8 @@ def linear_f8(x, weight: F8Weight, out_dtype: torch.dtype = torch.float32, resid
     """x [T, K] @ weight[N, K]^T with weight and x in 8 bits under float32 scales (`F8Rows`; a matrix is taken to 8 bits first), products exact,
     sums in float32, on the tcgen05 products.  The result is float32 or bfloat16 [T, N]; with `residual` (float32 [T, N]) it is added to
     that in place, which is returned.  Where a wait runs out (`stream_status`), what was not computed is neither stored nor added."""
-    rows, plain = _f8_operands(x, weight, False)
-    (T, K), N = x.shape, weight.shape[0]
+    rows, plain, dt = _f8_operands(x, weight, False)
+    T, N = x.shape[0], weight.shape[0]
     if residual is not None:
         _here(residual)
         if residual.dtype != torch.float32 or residual.shape != (T, N):
@@ -2751,10 +2772,11 @@ def linear_f8(x, weight: F8Weight, out_dtype: torch.dtype = torch.float32, resid
     else:
         y = _mx_matrix(T, N, out_dtype, weight.device)
         od = _dt(y)
-    at = weight.buffer.data_ptr()
-    _check(_mx_call("llm_linear_f8")(0, rows.buffer.data_ptr() if rows is not None else None, rows.padded if rows is not None else 0, _ptr(plain), at,
-                                     at + weight.scales_behind, 1, weight.tiles[0], y.data_ptr(), od, residual is not None, 0, T, N, K, 0, 0.0, None, None, None, None,
-                                     0, 0, 0, waits, _mx_status_ptr(weight.device), _stream()), "linear_f8")
+    at, padded = (None, 0) if rows is None else (rows.buffer.data_ptr(), rows.padded)
+    _check(_mx_call("llm_linear_f8")(weight.described(), at, padded, plain, dt, y.data_ptr(), od, residual is not None, T, waits, _mx_status_ptr(weight.device), _stream()),
+           "linear_f8")
+    if plain is not None and rows is not None:
+        _mx_count()
     return y
 
 
@@ -2762,21 +2784,15 @@ def linear_silu_mul_f8(x, weight: F8Weight, activation: str = "silu", limit: flo
     """act(x @ gate^T) * (x @ up^T) as rows of 8 bits [T, I] for a gated weight [2I, K] in 8 bits, act as in `silu_and_mul`, in the
     product's epilogue: sums and activation in 32-bit until they are rounded to 8 bits."""
     act = ACTIVATIONS[activation]
-    rows, plain = _f8_operands(x, weight, True)
-    (T, K), inter = x.shape, weight.shape[0] // 2
-    made = F8Rows(T, inter, weight.device)
-    at = weight.buffer.data_ptr()
-    _check(_mx_call("llm_linear_f8")(1, rows.buffer.data_ptr() if rows is not None else None, rows.padded if rows is not None else 0, _ptr(plain), at,
-                                     at + weight.scales_behind, 1, weight.tiles[0], made.buffer.data_ptr(), 0, 0, made.padded, T, inter, K, act, limit, None, None, None,
-                                     None, 0, 0, 0, waits, _mx_status_ptr(weight.device), _stream()), "linear_silu_mul_f8")
+    rows, plain, dt = _f8_operands(x, weight, True)
+    T = x.shape[0]
+    made = F8Rows(T, weight.shape[0] // 2, weight.device)
+    at, padded = (None, 0) if rows is None else (rows.buffer.data_ptr(), rows.padded)
+    _check(_mx_call("llm_linear_f8_silu_mul")(weight.described(), at, padded, plain, dt, made.buffer.data_ptr(), made.padded, T, act, limit, waits,
+                                              _mx_status_ptr(weight.device), _stream()), "linear_silu_mul_f8")
+    if plain is not None and rows is not None:
+        _mx_count()
     return made
-
-
-def _f8_item_rows(picks: int, experts: int) -> int:
-    """Rows of an expert that a grouped product takes at a time: by how many it has on average."""
-    if picks <= 16 * experts:
-        return 16
-    return 32 if picks <= 32 * experts else 64 if picks <= 64 * experts else 256
 
 
 def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Tensor, weights: torch.Tensor, activation: str = "silu", limit: float = 0.0,
@@ -2807,33 +2823,23 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
     if T == 0:
         return out
     top = ids.shape[1]
-    picks = T * top
-    per = _f8_item_rows(picks, E)
-    room = min(E, picks) + picks // per
-    # one allocation for what the sorting makes: items (16 bytes each), counts, places, tokens, weights
-    plan = torch.empty(4 * room + 4 + 3 * picks, dtype=torch.int32, device=x.device)
-    items = plan.data_ptr()
-    counts = items + 16 * room
-    places = counts + 16
-    tokens, row_weights = places + 4 * picks, places + 8 * picks
-    stream, status = _stream(), _mx_status_ptr(x.device)
-    _check(_mx_call("llm_f8_sort")(ids.data_ptr(), weights.data_ptr(), picks, top, E, per, counts, items, places, tokens, row_weights, stream), "f8_sort")
-    rows, plain = None, None
-    if per == 16 and dt == 1 and W % 8 == 0 and x.data_ptr() % 16 == 0:
-        plain = x
-    else:
-        rows = F8Rows(picks, W, x.device)
-        _check(_mx_call("llm_f8_rows")(x.data_ptr(), dt, rows.buffer.data_ptr(), rows.padded, T, W, places, top, stream), "f8_rows")
-    middle = F8Rows(picks, ff, x.device)
-    product, at = _mx_call("llm_linear_f8"), w_gate_up.buffer.data_ptr()
-    _check(product(1, rows.buffer.data_ptr() if rows is not None else None, rows.padded if rows is not None else 0, _ptr(plain), at, at + w_gate_up.scales_behind, E,
-                   w_gate_up.tiles[0], middle.buffer.data_ptr(), 0, 0, middle.padded, picks, ff, W, act, limit, counts, items, tokens, row_weights, int(on_input), per, room,
-                   waits, status, stream), "gate and up of experts in 8 bits")
-    y, at = _mx_matrix(picks, W, out_dtype, x.device), w_down.buffer.data_ptr()
-    _check(product(0, middle.buffer.data_ptr(), middle.padded, None, at, at + w_down.scales_behind, E, w_down.tiles[0], y.data_ptr(), od, 0, 0, picks, W, ff, 0, 0.0,
-                   counts, items, tokens, None if on_input else row_weights, 0, per, room, waits, status, stream), "down of experts in 8 bits")
-    _check(_mx_call("llm_f8_add_up")(y.data_ptr(), od, places, _ptr(base), out.data_ptr(), T, W, top, stream), "f8_add_up")
+    key = (T, top, E, W, ff, dt, od, x.data_ptr() % 16)
+    sizes = _f8_sizes.get(key)
+    if sizes is None:
+        work = _fn("blocks_f8", "llm_moe_f8_work", [_P, _I, _I, _I, _I, _I, _I, _I], c_longlong)(x.data_ptr(), dt, T, top, E, W, ff, od)
+        launches = _fn("blocks_f8", "llm_moe_f8_launches", [_P, _I, _I, _I, _I])(x.data_ptr(), dt, T * top, E, W)
+        if len(_f8_sizes) > 4096:
+            _f8_sizes.clear()
+        sizes = _f8_sizes[key] = work, launches
+    work = torch.empty(sizes[0], dtype=torch.uint8, device=x.device)
+    _check(_mx_call("llm_moe_f8")(w_gate_up.described(), w_down.described(), x.data_ptr(), dt, ids.data_ptr(), weights.data_ptr(), T, top, work.data_ptr(), _ptr(base),
+                                  out.data_ptr(), od, act, limit, int(on_input), waits, _mx_status_ptr(x.device), _stream()), "moe_f8")
+    global launch_count
+    launch_count += sizes[1] - 1
     return out
+
+
+_f8_sizes: Dict[tuple, tuple] = {}        # of a call of `moe_f8`: its workspace's bytes, its launches
 
 
 def linear_into(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor) -> bool:

@@ -51,8 +51,12 @@ def test_a_residual_that_the_product_does_not_take_is_declined():
     refuses(ops.linear_into, x, W, torch.ones(4, 32))             # one that it takes: no device here
 
 
-def test_rows_of_an_expert_at_a_time():
-    assert [ops._f8_item_rows(p, 8) for p in (1, 128, 129, 256, 257, 512, 513, 100000)] == [16, 16, 32, 32, 64, 64, 256, 256]
+def test_a_copy_of_a_weight_is_described_for_itself():
+    import copy
+    w = ops.F8Weight((32, 64), False, CPU)
+    w._described = (w.buffer.data_ptr(), 1, None)
+    other = copy.deepcopy(w)
+    assert w.described() == 1 and "_described" not in other.__dict__ and other.buffer.data_ptr() != w.buffer.data_ptr() and other.shape == w.shape
 
 
 def test_matrices_are_held_in_8_bits_by_parts_that_say_so_of_their_own_forward(monkeypatch):
