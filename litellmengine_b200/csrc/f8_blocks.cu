@@ -21,10 +21,17 @@ __device__ __forceinline__ unsigned f8_most(const uint4& r) { return mx_most8(r)
 __device__ __forceinline__ unsigned f8_most(const F8Raw<float>::type& r) { return mx_most8(r.v); }
 __device__ __forceinline__ uint2 f8_codes(const uint4& r, unsigned most, float inverse) { return f8_codes8(r, most, inverse); }
 __device__ __forceinline__ uint2 f8_codes(const F8Raw<float>::type& r, unsigned most, float inverse) { return f8_codes8(r.v, most, inverse); }
-template <bool FAST> __device__ __forceinline__ void f8_load(const bf16* row, int col, int n, uint4& r) {
+// vec 8: rows of whole, aligned pieces of eight values; 2: of pairs; 1: any.
+template <int VEC> __device__ __forceinline__ void f8_load(const bf16* row, int col, int n, uint4& r) {
     r = make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (FAST) {
+    if constexpr (VEC == 8) {
         if (col < n) mx_raw8(row + col, r);
+    } else if constexpr (VEC == 2) {
+        unsigned h[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + 2 * i < n) h[i] = *reinterpret_cast<const unsigned*>(row + col + 2 * i);
+        r = make_uint4(h[0], h[1], h[2], h[3]);
     } else {
         unsigned short h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
@@ -33,11 +40,18 @@ template <bool FAST> __device__ __forceinline__ void f8_load(const bf16* row, in
         r = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
 }
-template <bool FAST> __device__ __forceinline__ void f8_load(const float* row, int col, int n, F8Raw<float>::type& r) {
+template <int VEC> __device__ __forceinline__ void f8_load(const float* row, int col, int n, F8Raw<float>::type& r) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = 0.0f;
-    if constexpr (FAST) {
+    if constexpr (VEC == 8) {
         if (col < n) load8(row + col, r.v);
+    } else if constexpr (VEC == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            if (col + i < n) {
+                const float2 f = *reinterpret_cast<const float2*>(row + col + i);
+                r.v[i] = f.x, r.v[i + 1] = f.y;
+            }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -45,7 +59,7 @@ template <bool FAST> __device__ __forceinline__ void f8_load(const float* row, i
     }
 }
 
-template <int U, bool FAST, typename T>
+template <int U, int VEC, typename T>
 __global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* x, unsigned char* codes, float* scales, unsigned items,
                                                              unsigned per_row, int K, int ktiles, int k4, long long padded, const int32_t* places, int top) {
     pdl_begin();
@@ -55,7 +69,7 @@ __global__ void __launch_bounds__(F8_THREADS) f8_rows_kernel(const T* x, unsigne
     const int lane = threadIdx.x & 31, first = (w - row * per_row) * (2 * U) + (lane >> 4);       // of the lane's tiles of K
     typename F8Raw<T>::type raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) f8_load<FAST>(x + static_cast<size_t>(row) * K, (first + 2 * u) * F8_K + (lane & 15) * 8, K, raw[u]);
+    for (int u = 0; u < U; ++u) f8_load<VEC>(x + static_cast<size_t>(row) * K, (first + 2 * u) * F8_K + (lane & 15) * 8, K, raw[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int kb = first + 2 * u;
@@ -76,8 +90,7 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
     if (T <= 0) return LLM_OK;
     if (K <= 0 || K > (1 << 20) || T > (1 << 24) || top <= 0 || padded < T) return LLM_REFUSED_SIZE;
     if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
-    const int ktiles = f8_tiles(K), esz = dtype == LLM_DT_F32 ? 4 : 2;
-    const bool fast = K % 8 == 0 && aligned16(x) && static_cast<long long>(K) * esz % 16 == 0;
+    const int ktiles = f8_tiles(K), vec = mx_vec(K, x, dtype == LLM_DT_F32 ? 4 : 2);
     // four tiles of K a lane where that leaves every SM with enough warps
     const bool many = static_cast<long long>(T) * ktiles >= 32 * 1024;
     const unsigned u = many ? 4 : 1, per_row = (ktiles + 2 * u - 1) / (2 * u);
@@ -87,12 +100,12 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
     unsigned char* codes = static_cast<unsigned char*>(rows);
     float* scales = f8_row_scales(rows, padded, ktiles);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define LAUNCH(U, FAST, T_)                                                                                                                       \
-    launch_pdl((f8_rows_kernel<U, FAST, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(x), codes, scales, static_cast<unsigned>(items), per_row, K, \
+#define LAUNCH(U, VEC, T_)                                                                                                                       \
+    launch_pdl((f8_rows_kernel<U, VEC, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(x), codes, scales, static_cast<unsigned>(items), per_row, K, \
                ktiles, f8_k4(K), padded, places, places ? top : 1)
 #define LAUNCH_T(T_)                                        \
-    if (many) { if (fast) LAUNCH(4, true, T_); else LAUNCH(4, false, T_); } \
-    else { if (fast) LAUNCH(1, true, T_); else LAUNCH(1, false, T_); }
+    if (many) { if (vec == 8) LAUNCH(4, 8, T_); else if (vec == 2) LAUNCH(4, 2, T_); else LAUNCH(4, 1, T_); } \
+    else { if (vec == 8) LAUNCH(1, 8, T_); else if (vec == 2) LAUNCH(1, 2, T_); else LAUNCH(1, 1, T_); }
     if (dtype == LLM_DT_BF16) { LAUNCH_T(bf16) }
     else if (dtype == LLM_DT_F32) { LAUNCH_T(float) }
     else return LLM_REFUSED_DTYPE;
@@ -104,7 +117,7 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
 // ---- weights --------------------------------------------------------------------------------------------------------
 // A CTA a block of 128 x 128: sixteen lanes a row, two rows a warp and trip, eight trips that are asked for together.  It does not invite the kernel behind
 // it: products fetch weights before they wait for what is in front of them.
-template <bool FAST, typename T>
+template <int VEC, typename T>
 __global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* w, unsigned char* codes, float* scales, int rows, int K,
                                                                int tiles, int ktiles, int k4, int gate_rows, long long row_stride, long long matrix_stride) {
     __shared__ unsigned most_s[F8_THREADS / 32];
@@ -128,7 +141,7 @@ __global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* w, unsig
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         const int r = u * 16 + warp * 2 + (lane >> 4);
-        f8_load<FAST>(from + r * row_stride, col, r < there ? K : 0, raw[u]);
+        f8_load<VEC>(from + r * row_stride, col, r < there ? K : 0, raw[u]);
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) most = max(most, f8_most(raw[u]));
@@ -164,17 +177,18 @@ extern "C" int llm_f8_weight(const void* w, int dtype, void* codes, void* scales
     if (E <= 0 || E > 65535 || N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 20) || tiles != (gated ? 2 * ((N + 127) / 128) : (N + 255) / 256 * 2)) return LLM_REFUSED_SIZE;
     if (tiles > 65535 || row_stride < 0 || matrix_stride < 0) return LLM_REFUSED_SIZE;
     if (!aligned16(codes) || !aligned16(scales)) return LLM_REFUSED_ALIGN;
-    const int esz = dtype == LLM_DT_F32 ? 4 : 2;
-    const bool fast = K % 8 == 0 && aligned16(w) && row_stride * esz % 16 == 0 && matrix_stride * esz % 16 == 0;
+    const int esz = dtype == LLM_DT_F32 ? 4 : 2, strides = static_cast<int>((row_stride | matrix_stride) & 7);
+    int vec = mx_vec(K, w, esz);                                  // of rows that lie strides apart
+    if (strides) vec = strides % 2 ? 1 : vec < 2 ? 1 : 2;
     const int rows = gated ? 2 * N : N, blocks = gated ? (rows + 127) / 128 + (N % 128 ? 1 : 0) : tiles;
     if (blocks > 65535) return LLM_REFUSED_SIZE;
     const dim3 grid(f8_tiles(K), blocks, E);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define LAUNCH(FAST, T_)                                                                                                                              \
-    launch_pdl((f8_weight_kernel<FAST, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(w), static_cast<unsigned char*>(codes), \
+#define LAUNCH(VEC, T_)                                                                                                                              \
+    launch_pdl((f8_weight_kernel<VEC, T_>), grid, dim3(F8_THREADS), 0, s, static_cast<const T_*>(w), static_cast<unsigned char*>(codes), \
                static_cast<float*>(scales), rows, K, tiles, f8_tiles(K), f8_k4(K), gated ? N : 0, row_stride, matrix_stride)
-    if (dtype == LLM_DT_BF16) { if (fast) LAUNCH(true, bf16); else LAUNCH(false, bf16); }
-    else if (dtype == LLM_DT_F32) { if (fast) LAUNCH(true, float); else LAUNCH(false, float); }
+    if (dtype == LLM_DT_BF16) { if (vec == 8) LAUNCH(8, bf16); else if (vec == 2) LAUNCH(2, bf16); else LAUNCH(1, bf16); }
+    else if (dtype == LLM_DT_F32) { if (vec == 8) LAUNCH(8, float); else if (vec == 2) LAUNCH(2, float); else LAUNCH(1, float); }
     else return LLM_REFUSED_DTYPE;
 #undef LAUNCH
     return launch_status();
@@ -182,7 +196,7 @@ extern "C" int llm_f8_weight(const void* w, int dtype, void* codes, void* scales
 
 // ---- values ---------------------------------------------------------------------------------------------------------
 // Eight lanes a tile's row, sixteen codes a lane, U rows a thread asked for together.
-template <int U, bool FAST, typename T>
+template <int U, int VEC, typename T>
 __global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned char* codes, const float* scales, T* out, int rows,
                                                                int N, int K, int ktiles, int k4, int tiles, long long padded, int kind) {
     // kind 0: rows, 1: a weight, 2: a gated one (N: its gate rows); tiles: of 128 rows
@@ -224,8 +238,12 @@ __global__ void __launch_bounds__(F8_THREADS) f8_values_kernel(const unsigned ch
         T* to = out + r * K + col;
 #pragma unroll
         for (int h = 0; h < 16; h += 8) {
-            if (FAST) {
+            if constexpr (VEC == 8) {
                 if (col + h < K) store8(to + h, *reinterpret_cast<float(*)[8]>(v + h));
+            } else if constexpr (VEC == 2) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2)
+                    if (col + h + i < K) mx_store2(to + h + i, v[h + i], v[h + i + 1]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -239,16 +257,15 @@ extern "C" int llm_f8_values(const void* codes, const void* scales, void* out, i
     if (rows <= 0) return LLM_OK;
     if (K <= 0 || K > (1 << 20) || kind < 0 || kind > 2 || (kind && N <= 0)) return LLM_REFUSED_SIZE;
     constexpr int U = 4;                                          // 128 rows a CTA
-    const int esz = dtype == LLM_DT_F32 ? 4 : 2, ktiles = f8_tiles(K);
+    const int ktiles = f8_tiles(K), vec = mx_vec(K, out, dtype == LLM_DT_F32 ? 4 : 2);
     const long long blocks = (static_cast<long long>(rows) + 127) / 128 * ktiles;
     if (blocks >= (1LL << 31)) return LLM_REFUSED_SIZE;
-    const bool fast = K % 8 == 0 && aligned16(out) && static_cast<long long>(K) * esz % 16 == 0;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define LAUNCH(FAST, T_)                                                                                                                              \
-    launch_pdl((f8_values_kernel<U, FAST, T_>), dim3(static_cast<unsigned>(blocks)), dim3(F8_THREADS), 0, s, static_cast<const unsigned char*>(codes), \
+#define LAUNCH(VEC, T_)                                                                                                                              \
+    launch_pdl((f8_values_kernel<U, VEC, T_>), dim3(static_cast<unsigned>(blocks)), dim3(F8_THREADS), 0, s, static_cast<const unsigned char*>(codes), \
                static_cast<const float*>(scales), static_cast<T_*>(out), rows, N, K, ktiles, f8_k4(K), tiles, padded, kind)
-    if (dtype == LLM_DT_BF16) { if (fast) LAUNCH(true, bf16); else LAUNCH(false, bf16); }
-    else if (dtype == LLM_DT_F32) { if (fast) LAUNCH(true, float); else LAUNCH(false, float); }
+    if (dtype == LLM_DT_BF16) { if (vec == 8) LAUNCH(8, bf16); else if (vec == 2) LAUNCH(2, bf16); else LAUNCH(1, bf16); }
+    else if (dtype == LLM_DT_F32) { if (vec == 8) LAUNCH(8, float); else if (vec == 2) LAUNCH(2, float); else LAUNCH(1, float); }
     else return LLM_REFUSED_DTYPE;
 #undef LAUNCH
     return launch_status();
@@ -372,14 +389,18 @@ __global__ void __launch_bounds__(128) f8_add_up_kernel(const TY* y, const int32
         if (i >= N) return;
         float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (base) load8(base + t * N + i, sum);
-#pragma unroll 4
-        for (int k = 0; k < top; ++k) {
-            const int r = places[t * top + k];
-            if (r < 0) continue;
-            float v[8];
-            load8(y + static_cast<size_t>(r) * N + i, v);
+        for (int k0 = 0; k0 < top; k0 += 8) {                     // eight rows' places, then eight rows, in flight together
+            int r[8];
+            float v[8][8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) sum[c] += v[c];
+            for (int k = 0; k < 8; ++k) r[k] = k0 + k < top ? places[t * top + k0 + k] : -1;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (r[k] >= 0) load8(y + static_cast<size_t>(r[k]) * N + i, v[k]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) sum[c] += r[k] >= 0 ? v[k][c] : 0.0f;
         }
         store8(out + t * N + i, sum);
     } else {

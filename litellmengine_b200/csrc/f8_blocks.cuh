@@ -85,8 +85,11 @@ __device__ __forceinline__ unsigned f8_most16(unsigned most) {
     return most;
 }
 
-// Rows that a router has sorted by expert.  Items are up to a tile's rows of one expert; what stands behind the last is not read.
+// Rows that a router has sorted by expert.  Items are up to a tile's rows of one expert; what stands behind the last is not read.  Or, for a token or a few, the picks
+// as they are, each a row and an item of its own (ids, [tokens][top]; weights [tokens][top]).
 struct F8Groups {
+    const int32_t* ids;                   // or null
+    int top, E;
     const int32_t* counts;                // items, rows
     const int4* items;                    // expert, first row, rows
     const int32_t* tokens;                // [rows] the token of a row

@@ -63,6 +63,7 @@ struct F8Args {
     const bf16* plain;                    // a matrix [tokens, K] that the kernel takes to 8 bits itself
     F8Groups groups;
     int on_input;                         // a row's weight multiplies its gate and up values instead of the result
+    const float* base;                    // picks as they are: what a token's sum starts from, or null
 };
 enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
 
@@ -93,13 +94,24 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
     __shared__ int abort_flag, asked_s[2];                        // asked_s: stages of weights, groups of rows that were asked for
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int part = blockIdx.x, parts = gridDim.x;
-    const int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0;
+    int kb0 = part * a.ktiles / parts, kbs = (part + 1) * a.ktiles / parts - kb0;
     int row0 = blockIdx.z * NT, rows = min(NT, a.T - row0), first_tile = blockIdx.y * WT;
+    const bool joins = GROUPED && MODE == F8_STORE && a.groups.ids;
     if constexpr (GROUPED) {
         pdl_wait();                                               // the items are the kernel's in front
-        if (static_cast<int>(blockIdx.z) >= a.groups.counts[0]) return;       // the whole cluster
-        const int4 item = a.groups.items[blockIdx.z];
-        first_tile += item.x * a.tiles, row0 = item.y, rows = item.z;
+        if (a.groups.ids) {
+            // A pick is an item.  Behind its down product a token's picks are the parts of the sum instead of K's: the cluster adds them up.
+            row0 = joins ? blockIdx.z * parts + part : blockIdx.z;
+            const int e = a.groups.ids[row0];
+            rows = 1;
+            if (static_cast<unsigned>(e) < static_cast<unsigned>(a.groups.E)) first_tile += e * a.tiles;
+            else if (!joins) return;                              // the whole cluster
+            if (joins) kb0 = 0, kbs = static_cast<unsigned>(e) < static_cast<unsigned>(a.groups.E) ? a.ktiles : 0;
+        } else {
+            if (static_cast<int>(blockIdx.z) >= a.groups.counts[0]) return;
+            const int4 item = a.groups.items[blockIdx.z];
+            first_tile += item.x * a.tiles, row0 = item.y, rows = item.z;
+        }
     }
     const int early = min(WS, kbs);
     auto weights = [&](int kb, int s) {                           // into stage s
@@ -237,7 +249,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
         if (ok) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
-                if (i < rows) sums[i * FEATURES + w * 128 + feature] = acc[i];
+                if (i < rows) sums[i * FEATURES + w * 128 + feature] = joins && kbs && a.groups.weights ? acc[i] * a.groups.weights[row0] : acc[i];
         } else {
             // A wait ran out.  Who asks for copies has stopped; the copies (the stages are where the sums go) and the products end; then NaNs tell
             // whoever adds the parts up that these sums are not there.  Nothing of it is in the way of a product that does not give up.
@@ -259,7 +271,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
         for (int j = 0; j < BATCH; ++j) {
             const int u = warp - LAST + j * MAKERS;
             long long r = 0;
-            if (u < units) r = GROUPED ? a.groups.tokens[row0 + u / (G / 2)] : row0 + u / (G / 2);
+            if (u < units) r = !GROUPED ? row0 + u / (G / 2) : a.groups.ids ? row0 / a.groups.top : a.groups.tokens[row0 + u / (G / 2)];
             from[j] = a.plain + r * a.K + kb0 * F8_K + (lane >> 4) * F8_K + p * 8 + u % (G / 2) * 2 * F8_K;
         }
         uint4 raw[BATCH];
@@ -336,7 +348,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");       // every part's sums are there
     {
         const unsigned base = t5_smem(sums);
-        auto total = [&](int at) {                                // the parts' sums in order, four features, all parts' loads in flight at once
+        auto total = [&](int at, float4 v) {                      // what they join and the parts' sums in order, four features, all parts' loads in flight at once
             float4 f[8];
 #pragma unroll
             for (int p = 0; p < 8; ++p)
@@ -345,9 +357,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(addr) : "r"(base + 4u * at), "r"(p));
                     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(f[p].x), "=f"(f[p].y), "=f"(f[p].z), "=f"(f[p].w) : "r"(addr));
                 }
-            float4 v = f[0];
 #pragma unroll
-            for (int p = 1; p < 8; ++p)
+            for (int p = 0; p < 8; ++p)
                 if (p < parts) v.x += f[p].x, v.y += f[p].y, v.z += f[p].z, v.w += f[p].w;
             return v;
         };
@@ -370,7 +381,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
             unsigned char* codes = static_cast<unsigned char*>(a.y);
 #pragma unroll 1
             for (int r = first_row; r < rows; r += THREADS / 32 * parts) {
-                float4 g = total(r * FEATURES + (f >> 6) * 128 + (f & 63)), u = total(r * FEATURES + (f >> 6) * 128 + 64 + (f & 63));
+                const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float4 g = total(r * FEATURES + (f >> 6) * 128 + (f & 63), none), u = total(r * FEATURES + (f >> 6) * 128 + 64 + (f & 63), none);
                 const bool quit = missing(g.x + u.x);
                 if (GROUPED && a.on_input) {
                     const float w = a.groups.weights[row0 + r];
@@ -390,15 +402,21 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
             const int f = feature;
 #pragma unroll 2
             for (int r = first_row; f < a.N && r < rows; r += THREADS / 32 * parts) {
-                const float4 t = total(r * FEATURES + 4 * lane);
+                const size_t out_row = joins ? blockIdx.z : row0 + r;
+                float from[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (joins && a.base)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (f + i < a.N) from[i] = a.base[out_row * a.N + f + i];
+                const float4 t = total(r * FEATURES + 4 * lane, make_float4(from[0], from[1], from[2], from[3]));
                 if (missing(t.x)) continue;
                 float ts[4] = {t.x, t.y, t.z, t.w};
-                if (GROUPED && a.groups.weights) {
+                if (GROUPED && a.groups.weights && !joins) {
                     const float w = a.groups.weights[row0 + r];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) ts[i] *= w;
                 }
-                TO* to = y + static_cast<size_t>(row0 + r) * a.N + f;
+                TO* to = y + out_row * a.N + f;
                 if (a.vec) {                                      // N a multiple of 4, y aligned
                     if constexpr (sizeof(TO) == 4) {
                         float4 v = make_float4(ts[0], ts[1], ts[2], ts[3]);
@@ -1033,7 +1051,8 @@ template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED
     if (const int rc = f8_allow(kern, smem, dev, had)) return rc;
     const int tiles = (MODE == F8_GATED ? a.tiles / 2 : (a.N + 127) / 128), sms = f8_sms(dev);
     if (tiles > 65535 || c.row_tiles > 65535 || sms <= 0) return LLM_REFUSED_SIZE;
-    const int parts = f8_parts(static_cast<long long>(tiles) * c.row_tiles, a.ktiles, sms, F8_FEW_CTAS(NT, WT));
+    const bool joins = GROUPED && MODE == F8_STORE && a.groups.ids;
+    const int parts = joins ? a.groups.top : f8_parts(static_cast<long long>(tiles) * c.row_tiles, a.ktiles, sms, F8_FEW_CTAS(NT, WT));
     launch_pdl_cluster(kern, dim3(parts, tiles, c.row_tiles), dim3(F8_FEW_THREADS(PLAIN, WT)), smem, s, parts, c.w->whole, x_map, a);
     return launch_status();
 }
@@ -1156,6 +1175,10 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
     return f8_way<F8_GATED, float, false>({w, rows, 0}, a, llm_f8_way(T), reinterpret_cast<cudaStream_t>(stream));
 }
 
+// Tokens whose picks stay as they are: two launches instead of four, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
+// time on out of the second-level cache.
+#define F8_UNSORTED_TOKENS 4
+static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UNSORTED_TOKENS && top <= 8; }
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
 // middle's rows, the experts' results.
@@ -1165,9 +1188,10 @@ struct F8Work {
     int per, room, rows;                  // rows: of x are made in memory
     long long items, counts, places, tokens, weights, x, middle, y, all;
 };
-static F8Work f8_work(long long picks, int E, int W, int ff, bool plain, int out_dtype) {
+static F8Work f8_work(int T, int top, int E, int W, int ff, bool plain, int out_dtype) {
+    const long long picks = static_cast<long long>(T) * top;
     F8Work k = {};
-    k.per = f8_item_rows(picks, E);
+    k.per = f8_unsorted(T, top, plain) ? 16 : f8_item_rows(picks, E);
     k.room = static_cast<int>((E < picks ? E : picks) + picks / k.per);
     k.rows = !(plain && k.per == 16);
     const long long padded = f8_padded_rows(picks);
@@ -1182,7 +1206,7 @@ static F8Work f8_work(long long picks, int E, int W, int ff, bool plain, int out
 }
 static bool f8_plain_experts(const void* x, int dtype, int W) { return dtype == LLM_DT_BF16 && W % 8 == 0 && aligned16(x); }
 extern "C" long long llm_moe_f8_work(const void* x, int dtype, int T, int top, int E, int W, int ff, int out_dtype) {
-    return f8_work(static_cast<long long>(T) * top, E, W, ff, f8_plain_experts(x, dtype, W), out_dtype).all;
+    return f8_work(T, top, E, W, ff, f8_plain_experts(x, dtype, W), out_dtype).all;
 }
 extern "C" int llm_f8_sort(const int32_t*, const float*, int, int, int, int, int32_t*, void*, int32_t*, int32_t*, float*, uintptr_t);
 extern "C" int llm_f8_add_up(const void*, int, const int32_t*, const float*, void*, int, int, int, uintptr_t);
@@ -1195,12 +1219,14 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     const F8Weight *g = static_cast<const F8Weight*>(gate_up), *d = static_cast<const F8Weight*>(down);
     if (!g || !d || g->E != d->E || g->N != d->K || g->K != d->N) return LLM_REFUSED_SIZE;
     const int picks = T * top, W = g->K, ff = g->N;
-    const F8Work k = f8_work(picks, g->E, W, ff, f8_plain_experts(x, dtype, W), out_dtype);
+    const bool plain = f8_plain_experts(x, dtype, W), unsorted = f8_unsorted(T, top, plain);
+    const F8Work k = f8_work(T, top, g->E, W, ff, plain, out_dtype);
     unsigned char* at = static_cast<unsigned char*>(work);
     int32_t *counts = reinterpret_cast<int32_t*>(at + k.counts), *places = reinterpret_cast<int32_t*>(at + k.places), *tokens = reinterpret_cast<int32_t*>(at + k.tokens);
     float* row_weights = reinterpret_cast<float*>(at + k.weights);
     const long long padded = f8_padded_rows(picks);
-    if (const int rc = llm_f8_sort(ids, weights, picks, top, g->E, k.per, counts, at, places, tokens, row_weights, stream)) return rc;
+    if (!unsorted)
+        if (const int rc = llm_f8_sort(ids, weights, picks, top, g->E, k.per, counts, at, places, tokens, row_weights, stream)) return rc;
     if (k.rows)
         if (const int rc = llm_f8_rows(x, dtype, at + k.x, padded, T, W, places, top, stream)) return rc;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -1209,16 +1235,22 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     if (!mx_act(act, limit, &a.act)) return LLM_REFUSED_SIZE;
     a.plain = k.rows ? nullptr : static_cast<const bf16*>(x);
     a.y = at + k.middle, a.y_rows = padded, a.y_scales = f8_row_scales(at + k.middle, padded, f8_tiles(ff));
-    a.groups = {counts, reinterpret_cast<const int4*>(at), tokens, row_weights};
+    const F8Groups groups = {unsorted ? ids : nullptr, top, g->E, counts, reinterpret_cast<const int4*>(at), tokens, unsorted ? weights : row_weights};
+    a.groups = groups;
     a.on_input = on_input;
-    if (const int rc = f8_way<F8_GATED, float, true>({g, k.rows ? at + k.x : nullptr, k.room}, a, k.per, s)) return rc;
+    if (const int rc = f8_way<F8_GATED, float, true>({g, k.rows ? at + k.x : nullptr, unsorted ? picks : k.room}, a, k.per, s)) return rc;
     if (const int rc = f8_args(&a, d, 0, at + k.middle, padded, picks, waits, status)) return rc;
-    a.y = at + k.y;
-    a.vec = W % 4 == 0;
-    a.groups = {counts, reinterpret_cast<const int4*>(at), tokens, on_input ? nullptr : row_weights};
-    const F8Call c = {d, at + k.middle, k.room};
+    a.y = unsorted ? out : at + k.y;
+    a.vec = W % 4 == 0 && aligned16(a.y);
+    a.groups = groups;
+    if (on_input) a.groups.weights = nullptr;
+    a.base = base;
+    const F8Call c = {d, at + k.middle, unsorted ? T : k.room};
     if (const int rc = out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, true>(c, a, k.per, s) : f8_way<F8_STORE, bf16, true>(c, a, k.per, s)) return rc;
-    return llm_f8_add_up(at + k.y, out_dtype, places, base, out, T, W, top, stream);
+    return unsorted ? LLM_OK : llm_f8_add_up(at + k.y, out_dtype, places, base, out, T, W, top, stream);
 }
 // Kernels that llm_moe_f8 launches.
-extern "C" int llm_moe_f8_launches(const void* x, int dtype, int picks, int E, int W) { return 4 + (f8_work(picks, E, W, 1, f8_plain_experts(x, dtype, W), 0).rows ? 1 : 0); }
+extern "C" int llm_moe_f8_launches(const void* x, int dtype, int T, int top, int E, int W) {
+    const bool plain = f8_plain_experts(x, dtype, W);
+    return f8_unsorted(T, top, plain) ? 2 : 4 + f8_work(T, top, E, W, 1, plain, 0).rows;
+}
