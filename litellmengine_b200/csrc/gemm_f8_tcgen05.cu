@@ -506,9 +506,10 @@ __device__ __forceinline__ bool fp_wait_warp(bool seen, unsigned long long* bar,
     __syncwarp();
     return ok;
 }
-// One lane's word for the warp, without a branch that would part it from the others.
-__device__ __forceinline__ void fp_tell(unsigned bar) {
-    asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, %1, 0;\n @p mbarrier.arrive.shared::cluster.b64 _, [%0];\n}\n" ::"r"(bar), "r"(threadIdx.x & 31) : "memory");
+// One lane's word for the warp, if `ok`, without a branch that would part it from the others.  A warp that has given up tells nobody that a place is free: it may not
+// have been its turn, and others still read there.
+__device__ __forceinline__ void fp_tell(unsigned bar, bool ok) {
+    asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, %1, 0;\n @p mbarrier.arrive.shared::cluster.b64 _, [%0];\n}\n" ::"r"(bar), "r"(ok ? threadIdx.x & 31 : 1u) : "memory");
 }
 // Boxes into this CTA's shared memory, counted on a barrier of the pair's first CTA.
 __device__ __forceinline__ void fp_tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
@@ -658,8 +659,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 }
                 if (ok) asked = tiles > cluster ? (tiles - cluster + clusters - 1) / clusters * ktiles : 0;
                 asked_s[warp >> 1] = asked;
-                // The products tell both CTAs that they have read a stage, and none may leave before it has been told.
-                if (warp == 0 && ok) f8_land_ring(empty, FP_STAGES, asked);
+                // The products tell both CTAs that they have read a stage, and none may leave before it has been told (of products that stop, the last commit tells).
+                if (warp == 0 && ok)
+                    for (int i = max(0, asked - FP_STAGES); i < asked; ++i)
+                        for (int j = 0; j < T5_WAIT_LIMIT && !t5_try_wait(&empty[i % FP_STAGES], (i / FP_STAGES) & 1) && !*static_cast<volatile int*>(&abort_flag); ++j) {}
             }
             __syncwarp();
         } else if (warp == 1 && rank == 0) {
@@ -801,7 +804,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 bool seen_s = true;
                 if (group_ends) {
                     __syncwarp();
-                    fp_tell(s_empty_own + slot * 8);
+                    fp_tell(s_empty_own + slot * 8, ok);
                     if (++slot == FP_RING) slot = 0, s_phase ^= 1;
                     if (!last) seen_s = fp_look(&s_full[slot], s_phase);
                 }
@@ -823,7 +826,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 // All of it is in registers: the accumulator is free again, with a quarter of the additions still to do.
                 t5_fence_before();
                 __syncwarp();
-                fp_tell(acc_empty_first + (2 * buf + half) * 8);
+                fp_tell(acc_empty_first + (2 * buf + half) * 8, ok);
                 buf ^= 1;
                 acc_phase = next_phase;
                 if (!last) {
@@ -1086,13 +1089,22 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
 
 // Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself.
 #define F8_PLAIN_ROWS 16
-// Rows from which on pairs of CTAs take over.
-#define F8_PAIR_ROWS 129
-// How a product of T rows runs: the rows of a tile.
-extern "C" int llm_f8_way(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T < F8_PAIR_ROWS ? 64 : 256; }
+// How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 64 rows one tile of rows reads the weight once.  Beyond that tiles of 64
+// rows go on as long as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which pairs of CTAs (256) do not do.  Measured, rows of 8 bits by tiles of 64 and of pairs (us): 65 rows of 4,096 by
+// 6,144 15.6 and 16.8, 197 rows 27.3 and 17.3; 256 by 4,096 15.8 and 17.2, 320 27.0 and 17.2; 256 rows of 12,288 by 4,096 37.8 and 42.5; 65 rows of 2,048 by 12,288 15.8 and
+// 11.1; 197 rows of 1,358 by 2,501 7.5 and 11.3, 512 12.9 and 11.4; gated, 320 rows of 1,358 by 2 x 1,450 9.9 and 12.4, 512 14.3 and 12.5.
+static int f8_tile_rows(int T, int tiles, int sms) {
+    if (T <= 64) return T <= 16 ? 16 : T <= 32 ? 32 : 64;
+    return static_cast<long long>((T + 63) / 64) * tiles <= sms ? 64 : 256;
+}
 
-template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const F8Args& a, int per, cudaStream_t s) {
-    if (!GROUPED) c.row_tiles = (a.T + per - 1) / per;
+template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const F8Args& a, int per, cudaStream_t s) {         // per: rows of an item
+    if (!GROUPED) {
+        const int dev = f8_device();
+        if (dev < 0) return LLM_REFUSED_SIZE;
+        per = f8_tile_rows(a.T, (MODE == F8_GATED ? 2 : 1) * ((a.N + 127) / 128), f8_sms(dev));
+        c.row_tiles = (a.T + per - 1) / per;
+    }
     if (per == 256) return MODE == F8_GATED && a.N % 64 ? f8_pair<MODE, TO, GROUPED, MODE == F8_GATED>(c, a, s) : f8_pair<MODE, TO, GROUPED, false>(c, a, s);
     if constexpr (MODE == F8_GATED) {
         if (per == 16) return a.plain ? f8_few<16, 3, 2, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 3, 2, false, MODE, TO, GROUPED>(c, a, s);
@@ -1155,9 +1167,8 @@ extern "C" int llm_linear_f8(const void* weight, void* rows, long long padded, c
     a.vec = a.N % 4 == 0 && aligned16(y);
     const F8Call c = {w, rows, 0};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int per = llm_f8_way(T);
-    if (add) return f8_way<F8_ADD, float, false>(c, a, per, s);
-    return out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, false>(c, a, per, s) : f8_way<F8_STORE, bf16, false>(c, a, per, s);
+    if (add) return f8_way<F8_ADD, float, false>(c, a, 0, s);
+    return out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, false>(c, a, 0, s) : f8_way<F8_STORE, bf16, false>(c, a, 0, s);
 }
 
 // weight gated; made: act(x gate^T) * (x up^T) as rows of 8 bits [T, N], `made_padded` of them.
@@ -1172,7 +1183,7 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
     if (const int rc = f8_operand(&a, rows, padded, plain, dtype, stream)) return rc;
     a.y = made, a.y_rows = made_padded;
     a.y_scales = f8_row_scales(made, made_padded, f8_tiles(a.N));
-    return f8_way<F8_GATED, float, false>({w, rows, 0}, a, llm_f8_way(T), reinterpret_cast<cudaStream_t>(stream));
+    return f8_way<F8_GATED, float, false>({w, rows, 0}, a, 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
 // Tokens whose picks stay as they are: two launches instead of four, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
@@ -1182,7 +1193,10 @@ static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UN
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
 // middle's rows, the experts' results.
-static int f8_item_rows(long long picks, int E) { return picks <= 16LL * E ? 16 : picks <= 32LL * E ? 32 : picks <= 64LL * E ? 64 : 256; }
+// Rows of an item, by how many picks an expert has on average: fewer fit most experts' picks into one item, whose weights are read once.  Measured (us, 64 experts, 8 a
+// token, 1,024 by 2,048): 8 picks an expert 91 (16), 92 (32), 131 (256); 12: 112, 99, 136; 32: 180, 133, 147; 48: 160 (64), 148 (256); 64: 179, 159; 256: 533, 242.
+// Of 8 experts, 2 a token, 2,048 by 4,096: 8: 54 (16), 52 (32), 68 (256); 32: 67 (32), 62 (64), 72 (256); 48: 73, 63, 75; 64: 97 (64), 77 (256).
+static int f8_item_rows(long long picks, int E) { return picks <= 8LL * E ? 16 : picks <= 32LL * E ? 32 : picks <= 48LL * E ? 64 : 256; }
 static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
 struct F8Work {
     int per, room, rows;                  // rows: of x are made in memory
