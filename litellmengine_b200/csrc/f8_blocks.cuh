@@ -17,6 +17,7 @@
 #include "microscaling.cuh"
 
 #define F8_K 128                  // values of a tile's row
+#define F8_MOST_EXPERTS 4096      // that a call routes to
 #define F8_TILE (128 * F8_K)      // bytes of a weight's tile
 #define F8_TOP 448.0f
 #define F8_LEAST 1.17549435082228750797e-38f          // 2^-126

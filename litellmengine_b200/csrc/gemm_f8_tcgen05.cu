@@ -76,7 +76,11 @@ enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
 // grid (parts of K, tiles of features, tiles of rows or items), a cluster the parts of a tile.  WS: stages of weights; G: stages whose rows come together, two
 // such groups at a time.  A CTA's tile is 128 features, gated 64 + 64 gate and as many up features, of two tiles of the weight.
 // Warp 0 feeds the weights, warp 1 issues, warps from 2 on take the sums, the last feeds the rows and their scales; or, PLAIN, x comes as a matrix and the last warps make
-// the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.
+// the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.  With up to 32 rows that is
+// slower than a launch for the rows (24 rows of 12,288 by 4,096 16.0 us instead of 13.0; by 24,576 of 4,096 33.8 instead of 21.5).
+// Measured (us): a row of 4,096 by 6,144 6.95 (25 MB, 3.6 TB/s); 8 rows of 8 bits, 12,288 by 4,096, 10.2 (50 MB, 5.0 TB/s), 4,096 by 24,576 18.0 (101 MB, 5.6 TB/s); gated, 8 rows of
+// 4,096 by 2 x 12,288 21.5 (4.7 TB/s); 48 tokens' picks, 8 of 64 experts, 1,024 by 2,048 88 (4.6 TB/s of the weights), 51 of them gate and up and 32 down.  Three CTAs an SM with three
+// stages for the latter, so that more of them begin while others end, came out 84 to 88 there and slower for 8 large experts (49 instead of 45 us).
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED>
 __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1), F8_FEW_CTAS(NT, MODE == F8_GATED ? 2 : 1)) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                                          const F8Args a) {
@@ -449,15 +453,19 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
 
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 // The two CTAs of a cluster compute a tile of 256 rows x 256 features together (cta_group::2): each brings its own 128 rows and half of the features, and
-// reads both halves.  Tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them one after the other while 256 threads
-// (a row and 64 features of either each) take out those before, so that the sums are in registers.  What limits it is an accumulator's way round: its products 256
-// clocks, 300 until the threads of both CTAs know, 100 to take it out (all of it, before anything is added), 250 until the products know that it is free again: 1,000
-// of the 1,024 that four leave.  With two accumulators of 256 features, taken out and added in turns, the way is 1,700 and bounds the kernel.
-// Shared memory is busy with the products' operands (128 bytes a clock, all that it has), so that a load from it takes 200 clocks and a look at a barrier as much: the
-// threads that take the sums have their scales from memory, two tiles of K in a load and two ahead, and ask early whether the next accumulator is full.
-// The clusters are persistent; the products go on into the next tile while the threads write a finished one.  Tiles are numbered row tile fastest: what runs at one time
+// reads both halves.  A CTA's tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them, one for each tile of the weight,
+// while those of the tile before are taken out.  Each has barriers and four warps of its own (a row and 128 features a thread, 64 pairs of sums in registers), so that
+// its way round (products, the word of them, taking out, the word that it is free) overlaps the other three's.  Taking out (tcgen05.ld) and adding (fma of two at a time)
+// alternate in quarters of 32 features; the accumulator is free again with the last quarter's additions still to do.
+// Shared memory is busy with the products' operands, so that a load from it or a look at a barrier takes 100 to 200 clocks: what the next tile of K needs (its scales,
+// whether its accumulator is full) is asked for between additions.  Scales come by a warp's asynchronous copies, eight tiles of K at a time into a ring of two: loads of the
+// threads that need them would wait together with tcgen05.ld, whose wait is for all.
+// Measured: a tile of K takes 700 clocks, its products 512.  4,096 rows of 4,096 by 24,576: 380 to 410 us with the clocks that the power limit leaves (1.3 to 1.5 GHz), 2.0 to
+// 2.15 PFLOP/s; 1,024 rows by 4,096 21 us; gated, 2,045 rows of 4,096 by 2 x 12,288 205 to 220 us.  Two accumulators of 256 features, taken out and added in turns, made it 1,700 clocks a
+// tile of K.
+// The clusters are persistent: the copies go on into the next tile while the threads write a finished one.  Tiles are numbered row tile fastest: what runs at one time
 // shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's rows and weights are few.
-// Warp 0 feeds the weights, 2 the rows; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
+// Warp 0 feeds the weights, 2 the rows, 3 the scales; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
 #define FP_STAGES 4
 #define FP_THREADS 384
 #define FP_BLOCK 8192             // a warp's rows on their way out: 32 of 64 features, or of 128 in 16 bits
@@ -1087,7 +1095,7 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
     return launch_status();
 }
 
-// Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself.
+// Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself (see f8_few_kernel).
 #define F8_PLAIN_ROWS 16
 // How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 64 rows one tile of rows reads the weight once.  Beyond that tiles of 64
 // rows go on as long as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which pairs of CTAs (256) do not do.  Measured, rows of 8 bits by tiles of 64 and of pairs (us): 65 rows of 4,096 by
@@ -1187,7 +1195,8 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
 }
 
 // Tokens whose picks stay as they are: two launches instead of four, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
-// time on out of the second-level cache.
+// time on out of the second-level cache.  Measured, as they are and sorted (us), 1, 2, 4, 5 and 8 tokens: 64 experts, 8 a token, 1,024 by 2,048 17.1 and 21.1, 21.2 and 28.0, 38.1 and 41.4,
+// 55.1 and 46.8, 69.6 and 65.4; 8 experts, 2 a token, 2,048 by 4,096 19.4 and 22.6, 23.7 and 28.4, 31.7 and 36.0, 48.2 and 44.0, 50.8 and 43.3.  Up to eight picks: a cluster adds them up.
 #define F8_UNSORTED_TOKENS 4
 static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UNSORTED_TOKENS && top <= 8; }
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
@@ -1231,7 +1240,7 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     if (out_dtype != LLM_DT_F32 && out_dtype != LLM_DT_BF16) return LLM_REFUSED_DTYPE;
     if (reinterpret_cast<uintptr_t>(work) % 256) return LLM_REFUSED_ALIGN;
     const F8Weight *g = static_cast<const F8Weight*>(gate_up), *d = static_cast<const F8Weight*>(down);
-    if (!g || !d || g->E != d->E || g->N != d->K || g->K != d->N) return LLM_REFUSED_SIZE;
+    if (!g || !d || g->E != d->E || g->E > F8_MOST_EXPERTS || g->N != d->K || g->K != d->N) return LLM_REFUSED_SIZE;
     const int picks = T * top, W = g->K, ff = g->N;
     const bool plain = f8_plain_experts(x, dtype, W), unsorted = f8_unsorted(T, top, plain);
     const F8Work k = f8_work(T, top, g->E, W, ff, plain, out_dtype);
