@@ -45,6 +45,11 @@ __device__ __forceinline__ void f8_mma_lead(unsigned lead, unsigned d_tmem, unsi
                  " @q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::
                      "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
 }
+__device__ __forceinline__ unsigned long long f8_mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 // Instruction descriptor: e4m3 x e4m3 -> float32, M x N, both K-major.
 __host__ __device__ constexpr unsigned f8_idesc(int m, int n) {
     return (1u << 4) | (static_cast<unsigned>(n >> 3) << 17) | (static_cast<unsigned>(m >> 4) << 24);
@@ -85,6 +90,10 @@ template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED
 __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1), F8_FEW_CTAS(NT, MODE == F8_GATED ? 2 : 1)) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                                          const F8Args a) {
     constexpr int WT = MODE == F8_GATED ? 2 : 1, THREADS = F8_FEW_THREADS(PLAIN, WT), MAKERS = F8_MAKERS(WT), LAST = 2 + 4 * WT, FEATURES = 128 * WT;
+    constexpr bool TOGETHER = MODE != F8_GATED && !PLAIN;         // a row's scale comes times its tile of weights' (gate and up rows have one each)
+    // Rows of an accumulator that are asked for together.  Of 64 rows' sums half (their registers leave no room for scales ahead): 64 rows of 4,096 by 24,576 26.9 us, in pieces of 16 with
+    // scales ahead 27.9; 32 rows 20.5 and 20.2, gated 27.4 and 21.8.
+    constexpr int PIECE = NT == 64 && MODE != F8_GATED ? 32 : 16;
     constexpr unsigned W_BYTES = WT * F8_TILE, X_BYTES = NT * F8_K, SLOT = NT * WT;
     constexpr unsigned SLOTS = 256 / SLOT < 4 ? 256 / SLOT : 4, COLS = SLOT * SLOTS < 32 ? 32 : SLOT * SLOTS;      // accumulators in turn; two CTAs share tensor memory
     static_assert(COLS <= 256 && SLOTS >= 2, "tensor memory");
@@ -195,9 +204,9 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
     } else if (warp < LAST) {
         const int quarter = warp & 3, w = (warp - 2) >> 2, feature = quarter * 32 + lane;
         pdl_wait();
-        float acc[NT];
+        unsigned long long acc[NT / 2];                           // two rows each
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+        for (int i = 0; i < NT / 2; ++i) acc[i] = 0ull;
         // A lane has the weights' scales of every 32nd tile of K; of up rows two, where these 64 lie in two blocks.
         constexpr int HELD = MODE == F8_GATED ? 2 : 1;
         float mine[HELD];
@@ -207,39 +216,58 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
         bool ok = true;
 #pragma unroll 1
         for (int kb = 0; kb < kbs; ++kb) {
-            if ((kb & 31) == 0) {
+            if (!TOGETHER && (kb & 31) == 0) {
                 const float* s = a.w_scales + (first_tile + w) * 3LL * a.k4 + kb0 + kb + lane;
 #pragma unroll
                 for (int i = 0; i < HELD; ++i) mine[i] = kb + lane < kbs ? s[HELD == 1 || quarter < 2 ? 0 : (1 + i) * a.k4] : 0.0f;
             }
-            ok = __all_sync(0xffffffffu, (q || f8_wait(&x_full[g], turn, a.waits, &abort_flag, a.status)) &&
-                                             f8_wait(&acc_full[slot], acc_phase, a.waits, &abort_flag, a.status));
-            if (!ok) break;
-            t5_fence_after();
+            if (q == 0) {
+                ok = __all_sync(0xffffffffu, f8_wait(&x_full[g], turn, a.waits, &abort_flag, a.status));
+                if (!ok) break;
+            }
             const unsigned at = tmem + (static_cast<unsigned>(quarter * 32) << 16) + slot * SLOT + w * NT;
             const float* sx = sx_s + (g * G + q) * NT;
+            // A piece's scales are asked for ahead of the wait for its sums, which no load passes; while one piece is multiplied and added the next is on its way.
+            ulonglong2 s[2][4];
+            auto scales = [&](int c) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[c & 1][i] = *reinterpret_cast<const ulonglong2*>(sx + c * PIECE + 4 * i);
+            };
+            if (PIECE == 16) scales(0);
+            ok = __all_sync(0xffffffffu, f8_wait(&acc_full[slot], acc_phase, a.waits, &abort_flag, a.status));
+            if (!ok) break;
+            t5_fence_after();
             float sw = __shfl_sync(0xffffffffu, mine[0], kb & 31);
             if constexpr (HELD == 2) {
                 const float other = __shfl_sync(0xffffffffu, mine[HELD - 1], kb & 31);
                 if (second) sw = other;
             }
+            const unsigned long long sw2 = t5_two(sw, sw);
+            unsigned r[2][PIECE];
+            auto ask = [&](int c) {
+                if constexpr (PIECE == 32) t5_ld32(at + c * PIECE, r[c & 1]);
+                else t5_ld16(at + c * PIECE, r[c & 1]);
+            };
+            ask(0);
 #pragma unroll
-            for (int c = 0; c < NT; c += 16) {
-                unsigned r[16];
-                t5_ld16(at + c, r);
+            for (int c = 0; c < NT / PIECE; ++c) {
                 t5_wait_ld();
-                if (c + 16 == NT) {                               // all of it is in registers
+                if (c + 1 < NT / PIECE) {
+                    ask(c + 1);
+                    if (PIECE == 16) scales(c + 1);
+                } else {                                            // all of it is in registers
                     t5_fence_before();
                     __syncwarp();
                     if (lane == 0) t5_arrive(&acc_empty[slot]);
                 }
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 s = *reinterpret_cast<const float4*>(sx + c + i);
-                    acc[c + i] = fmaf(__uint_as_float(r[i]), s.x * sw, acc[c + i]);
-                    acc[c + i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y * sw, acc[c + i + 1]);
-                    acc[c + i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z * sw, acc[c + i + 2]);
-                    acc[c + i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w * sw, acc[c + i + 3]);
+                for (int i = 0; i < PIECE; i += 4) {
+                    unsigned long long *to = acc + (c * PIECE + i) / 2;
+                    const ulonglong2 both = PIECE == 16 ? s[c & 1][i / 4] : *reinterpret_cast<const ulonglong2*>(sx + c * PIECE + i);
+                    unsigned long long lo = both.x, hi = both.y;
+                    if (!TOGETHER) lo = f8_mul2(lo, sw2), hi = f8_mul2(hi, sw2);
+                    to[0] = t5_fma2(t5_two(__uint_as_float(r[c & 1][i]), __uint_as_float(r[c & 1][i + 1])), lo, to[0]);
+                    to[1] = t5_fma2(t5_two(__uint_as_float(r[c & 1][i + 2]), __uint_as_float(r[c & 1][i + 3])), hi, to[1]);
                 }
             }
             if (++slot == static_cast<int>(SLOTS)) slot = 0, acc_phase ^= 1;
@@ -252,8 +280,13 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
         }
         if (ok) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-                if (i < rows) sums[i * FEATURES + w * 128 + feature] = joins && kbs && a.groups.weights ? acc[i] * a.groups.weights[row0] : acc[i];
+            for (int i = 0; i < NT; i += 2) {
+                float v[2];
+                t5_untwo(acc[i / 2], v[0], v[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (i + j < rows) sums[(i + j) * FEATURES + w * 128 + feature] = joins && kbs && a.groups.weights ? v[j] * a.groups.weights[row0] : v[j];
+            }
         } else {
             // A wait ran out.  Who asks for copies has stopped; the copies (the stages are where the sums go) and the products end; then NaNs tell
             // whoever adds the parts up that these sums are not there.  Nothing of it is in the way of a product that does not give up.
@@ -326,6 +359,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
             for (int j = 0; j < EACH; ++j) {
                 const int i = lane + 32 * j, kb = first + i / NT;
                 s[j] = i < G * NT && kb < a.ktiles && row0 + i % NT < a.x_rows ? a.x_scales[(row0 + i % NT) * static_cast<long long>(a.k4) + kb] : 0.0f;
+                if (TOGETHER && kb < a.ktiles) s[j] *= a.w_scales[first_tile * 3LL * a.k4 + kb];
             }
 #pragma unroll
             for (int j = 0; j < EACH; ++j)
@@ -1098,9 +1132,10 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
 // Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself (see f8_few_kernel).
 #define F8_PLAIN_ROWS 16
 // How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 64 rows one tile of rows reads the weight once.  Beyond that tiles of 64
-// rows go on as long as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which pairs of CTAs (256) do not do.  Measured, rows of 8 bits by tiles of 64 and of pairs (us): 65 rows of 4,096 by
-// 6,144 15.6 and 16.8, 197 rows 27.3 and 17.3; 256 by 4,096 15.8 and 17.2, 320 27.0 and 17.2; 256 rows of 12,288 by 4,096 37.8 and 42.5; 65 rows of 2,048 by 12,288 15.8 and
-// 11.1; 197 rows of 1,358 by 2,501 7.5 and 11.3, 512 12.9 and 11.4; gated, 320 rows of 1,358 by 2 x 1,450 9.9 and 12.4, 512 14.3 and 12.5.
+// rows go on as long as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which pairs of CTAs (256) do not do.  Measured, rows of 8 bits by tiles of 64 and
+// of pairs (us): 65 rows of 4,096 by 6,144 15.1 and 16.8, 197 rows 27.4 and 17.4; 250 by 4,096 15.2 and 17.3, 320 27.1 and 17.2; 250 rows of 12,288 by 4,096 35.5 and 42.3; 65 rows of 2,048 by
+// 12,288 15.3 and 11.1; 197 rows of 1,358 by 2,501 7.5 and 11.3, 512 12.9 and 11.4; gated, 320 rows of 1,358 by 2 x 1,450 9.4 and 12.3, 512 14.3 and 12.5; 128 of 1,024 by 2 x 4,096 8.7 and 8.6.
+// Tiles of 128 rows by one CTA are no faster than two of 64: 65 to 128 rows by 6,144 14.5 to 16.1 and 15.1 to 15.3, by 24,576 51 to 54 and 44 to 49.
 static int f8_tile_rows(int T, int tiles, int sms) {
     if (T <= 64) return T <= 16 ? 16 : T <= 32 ? 32 : 64;
     return static_cast<long long>((T + 63) / 64) * tiles <= sms ? 64 : 256;
@@ -1117,12 +1152,13 @@ template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const
     if constexpr (MODE == F8_GATED) {
         if (per == 16) return a.plain ? f8_few<16, 3, 2, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 3, 2, false, MODE, TO, GROUPED>(c, a, s);
         if (per == 32) return f8_few<32, 3, 1, false, MODE, TO, GROUPED>(c, a, s);
-        return f8_few<64, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
+        if constexpr (!GROUPED) return f8_few<64, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
     } else {
         if (per == 16) return a.plain ? f8_few<16, 5, 4, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 5, 4, false, MODE, TO, GROUPED>(c, a, s);
         if (per == 32) return f8_few<32, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
-        return f8_few<64, 4, 2, false, MODE, TO, GROUPED>(c, a, s);
+        if constexpr (!GROUPED) return f8_few<64, 4, 2, false, MODE, TO, GROUPED>(c, a, s);
     }
+    return LLM_REFUSED_SIZE;                                      // items have 16, 32 or 256 rows
 }
 
 extern "C" int llm_f8_weight_size() { return static_cast<int>(sizeof(F8Weight)); }
@@ -1202,10 +1238,11 @@ static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UN
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
 // middle's rows, the experts' results.
-// Rows of an item, by how many picks an expert has on average: fewer fit most experts' picks into one item, whose weights are read once.  Measured (us, 64 experts, 8 a
-// token, 1,024 by 2,048): 8 picks an expert 91 (16), 92 (32), 131 (256); 12: 112, 99, 136; 32: 180, 133, 147; 48: 160 (64), 148 (256); 64: 179, 159; 256: 533, 242.
-// Of 8 experts, 2 a token, 2,048 by 4,096: 8: 54 (16), 52 (32), 68 (256); 32: 67 (32), 62 (64), 72 (256); 48: 73, 63, 75; 64: 97 (64), 77 (256).
-static int f8_item_rows(long long picks, int E) { return picks <= 8LL * E ? 16 : picks <= 32LL * E ? 32 : picks <= 48LL * E ? 64 : 256; }
+// Rows of an item, by how many picks an expert has on average: fewer fit most experts' picks into one item, whose weights are read once.  Measured (us): 64 experts, 8 a
+// token, 1,024 by 2,048, 6 picks an expert 85 (16), 86 (32), 125 (256); 12: 111, 96, 136; 32: 178, 127, 143; 48: 228, 153, 142; 96: 414, 241, 162.  8 experts, 2 a token, 2,048 by 4,096,
+// 8: 50, 49, 68; 16: 64, 52, 69; 40: 107, 69, 73; 64: 127, 97, 76; 1,450 by 1,358, 12: 28, 29, 45; 24: 32, 32, 46; 48: 45, 38, 46; 96: 60, 58, 48.  Items of 64 rows come out between the
+// latter two, or up to a tenth before both where experts are few and large.
+static int f8_item_rows(long long picks, int E) { return picks <= 8LL * E ? 16 : picks <= 40LL * E ? 32 : 256; }
 static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
 struct F8Work {
     int per, room, rows;                  // rows: of x are made in memory
