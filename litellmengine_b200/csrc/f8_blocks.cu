@@ -284,15 +284,14 @@ extern "C" int llm_f8_values(const void* codes, const void* scales, void* out, i
 
 // ---- rows sorted by expert ------------------------------------------------------------------------------------------
 // A cluster (of one CTA for few picks) counts the picks of each expert, lays the experts' rows one after another, cuts them into items of up to `per` rows, and
-// gives every pick its row: places[pick] (-1 where the pick is no expert), tokens[row], weights[row].  A CTA takes neighbouring picks and adds up the counts of those
+// gives every pick its row: places[pick] (-1 where the pick is no expert), weights[row].  A CTA takes neighbouring picks and adds up the counts of those
 // before it out of their shared memory: 32,768 picks of 64 experts 52 us by one CTA, 9 by eight.  Which of an expert's rows a pick gets is not fixed; no result depends on it,
 // a row's products being its own.
 #define F8_SORT_CTAS 8
 #define F8_SORT_PICKS 4           // picks of a thread that stay in registers
 
-__global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* ids, const float* weights, int picks, int top, int E, int per,
-                                                       int32_t* counts, int4* items, int32_t* places,
-                                                       int32_t* tokens, float* row_weights) {
+__global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* ids, const float* weights, int picks, int E, int per,
+                                                       int32_t* counts, int4* items, int32_t* places, float* row_weights) {
     extern __shared__ int counted_s[];                            // [E] this CTA's picks, [E] the next row of an expert
     __shared__ int2 warps_s[32];
     int* next_s = counted_s + E;
@@ -318,7 +317,6 @@ __global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* ids, const
         r = __shfl_sync(0xffffffffu, r, first) + __popc(same & ((1u << lane) - 1));
         if (p >= to) return;
         if (e >= 0) {
-            tokens[r] = p / top;
             row_weights[r] = weights[p];
         }
         places[p] = e >= 0 ? r : -1;
@@ -378,14 +376,14 @@ __global__ void __launch_bounds__(1024) f8_sort_kernel(const int32_t* ids, const
     if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");          // nobody leaves before
 }
 
-extern "C" int llm_f8_sort(const int32_t* ids, const float* weights, int picks, int top, int E, int per, int32_t* counts, void* items, int32_t* places, int32_t* tokens,
-                           float* row_weights, uintptr_t stream) {
+extern "C" int llm_f8_sort(const int32_t* ids, const float* weights, int picks, int E, int per, int32_t* counts, void* items, int32_t* places, float* row_weights,
+                           uintptr_t stream) {
     if (picks <= 0) return LLM_OK;
-    if (E <= 0 || E > F8_MOST_EXPERTS || top <= 0 || per <= 0) return LLM_REFUSED_SIZE;
+    if (E <= 0 || E > F8_MOST_EXPERTS || per <= 0) return LLM_REFUSED_SIZE;
     if (!aligned16(items)) return LLM_REFUSED_ALIGN;
     const int ctas = picks > 2048 ? F8_SORT_CTAS : 1, most = ctas == 1 && picks > E ? picks : E, threads = ctas > 1 || most >= 1024 ? 1024 : (most + 31) / 32 * 32;
-    launch_pdl_cluster(f8_sort_kernel, dim3(ctas), dim3(threads), 2 * E * sizeof(int), reinterpret_cast<cudaStream_t>(stream), ctas, ids, weights, picks, top, E, per, counts,
-                       static_cast<int4*>(items), places, tokens, row_weights);
+    launch_pdl_cluster(f8_sort_kernel, dim3(ctas), dim3(threads), 2 * E * sizeof(int), reinterpret_cast<cudaStream_t>(stream), ctas, ids, weights, picks, E, per, counts,
+                       static_cast<int4*>(items), places, row_weights);
     return launch_status();
 }
 

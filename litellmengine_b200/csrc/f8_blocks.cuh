@@ -93,7 +93,6 @@ struct F8Groups {
     int top, E;
     const int32_t* counts;                // items, rows
     const int4* items;                    // expert, first row, rows
-    const int32_t* tokens;                // [rows] the token of a row
     const float* weights;                 // [rows] its weight, or null
 };
 extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padded, int T, int K, const int32_t* places, int top, uintptr_t stream);

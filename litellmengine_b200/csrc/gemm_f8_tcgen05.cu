@@ -74,17 +74,19 @@ enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
 // Warps: two that feed weights and issue, four for the sums of each of a CTA's tiles of the weight, and those that make rows of a matrix, or one that feeds rows.
-#define F8_MAKERS(WT) ((WT) == 2 ? 6 : 8)
+#define F8_MAKERS(WT) ((WT) == 2 ? 4 : 8)
+#define F8_PLAIN_ROWS(GATED) ((GATED) ? 4 : 8)              // up to which a product makes its rows of a bfloat16 matrix of whole, aligned pieces of eight values itself
 #define F8_FEW_CTAS(NT, WT) ((NT) * (WT) > 64 ? 1 : 2)          // on an SM: sums of 64 rows of two tiles need the registers of both
 #define F8_FEW_THREADS(PLAIN, WT) (32 * (2 + 4 * (WT) + ((PLAIN) ? F8_MAKERS(WT) : 1)))
 
 // grid (parts of K, tiles of features, tiles of rows or items), a cluster the parts of a tile.  WS: stages of weights; G: stages whose rows come together, two
 // such groups at a time.  A CTA's tile is 128 features, gated 64 + 64 gate and as many up features, of two tiles of the weight.
 // Warp 0 feeds the weights, warp 1 issues, warps from 2 on take the sums, the last feeds the rows and their scales; or, PLAIN, x comes as a matrix and the last warps make
-// the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.  With up to 32 rows that is
-// slower than a launch for the rows (24 rows of 12,288 by 4,096 16.0 us instead of 13.0; by 24,576 of 4,096 33.8 instead of 21.5).
+// the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.  Measured, so and with a launch
+// for the rows (us): 4,096 by 6,144, a row 6.8 and 7.5, 8 rows 7.8 and 8.1, 16 rows 9.0 and 8.4; 12,288 by 4,096 10.1 and 11.1, 10.9 and 11.5, 12.8 and 12.0; gated, 4,096 by 2 x 12,288, a row
+// 20.1 and 19.3, 4 rows 20.0 and 19.6, 8 rows 21.3 and 19.7; 2,048 by 2 x 1,024 5.06 and 5.19, 5.25 and 5.26, 5.7 and 5.5.
 // Measured (us): a row of 4,096 by 6,144 6.95 (25 MB, 3.6 TB/s); 8 rows of 8 bits, 12,288 by 4,096, 10.2 (50 MB, 5.0 TB/s), 4,096 by 24,576 18.0 (101 MB, 5.6 TB/s); gated, 8 rows of
-// 4,096 by 2 x 12,288 21.5 (4.7 TB/s); 48 tokens' picks, 8 of 64 experts, 1,024 by 2,048 88 (4.6 TB/s of the weights), 51 of them gate and up and 32 down.  Three CTAs an SM with three
+// 4,096 by 2 x 12,288 18.7 (5.4 TB/s); 48 tokens' picks, 8 of 64 experts, 1,024 by 2,048 80 (5.0 TB/s of the weights) with their sorting.  Three CTAs an SM with three
 // stages for the latter, so that more of them begin while others end, came out 84 to 88 there and slower for 8 large experts (49 instead of 45 us).
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED>
 __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1), F8_FEW_CTAS(NT, MODE == F8_GATED ? 2 : 1)) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
     } else if constexpr (PLAIN) {                                 // rows beyond the last keep what stands there, nobody minds
         // A warp takes two stages of a row at a time, sixteen lanes each, and has the next group's values on their way while it makes this one's.
         static_assert(G % 2 == 0, "stages go in pairs");
-        constexpr int BATCH = (NT * G / 2 + MAKERS - 1) / MAKERS;       // units of a group that a warp has at most
+        constexpr int BATCH = (F8_PLAIN_ROWS(MODE == F8_GATED) * G / 2 + MAKERS - 1) / MAKERS;       // units of a group that a warp has at most
         const int p = lane & 15, units = rows * (G / 2);
         const int left = a.K - kb0 * F8_K - (lane >> 4) * F8_K - p * 8;       // values of the row from the lane's first on
         const bf16* from[BATCH];
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
         for (int j = 0; j < BATCH; ++j) {
             const int u = warp - LAST + j * MAKERS;
             long long r = 0;
-            if (u < units) r = !GROUPED ? row0 + u / (G / 2) : a.groups.ids ? row0 / a.groups.top : a.groups.tokens[row0 + u / (G / 2)];
+            if (u < units) r = GROUPED ? row0 / a.groups.top : row0 + u / (G / 2);        // a pick's token
             from[j] = a.plain + r * a.K + kb0 * F8_K + (lane >> 4) * F8_K + p * 8 + u % (G / 2) * 2 * F8_K;
         }
         uint4 raw[BATCH];
@@ -1129,8 +1131,6 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
     return launch_status();
 }
 
-// Rows up to which a product takes a bfloat16 matrix of whole, aligned pieces of eight values to 8 bits itself (see f8_few_kernel).
-#define F8_PLAIN_ROWS 16
 // How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 64 rows one tile of rows reads the weight once.  Beyond that tiles of 64
 // rows go on as long as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which pairs of CTAs (256) do not do.  Measured, rows of 8 bits by tiles of 64 and
 // of pairs (us): 65 rows of 4,096 by 6,144 15.1 and 16.8, 197 rows 27.4 and 17.4; 250 by 4,096 15.2 and 17.3, 320 27.1 and 17.2; 250 rows of 12,288 by 4,096 35.5 and 42.3; 65 rows of 2,048 by
@@ -1154,7 +1154,9 @@ template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const
         if (per == 32) return f8_few<32, 3, 1, false, MODE, TO, GROUPED>(c, a, s);
         if constexpr (!GROUPED) return f8_few<64, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
     } else {
-        if (per == 16) return a.plain ? f8_few<16, 5, 4, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 5, 4, false, MODE, TO, GROUPED>(c, a, s);
+        if constexpr (!GROUPED)
+            if (a.plain) return f8_few<16, 5, 4, true, MODE, TO, false>(c, a, s);
+        if (per == 16) return f8_few<16, 5, 4, false, MODE, TO, GROUPED>(c, a, s);
         if (per == 32) return f8_few<32, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
         if constexpr (!GROUPED) return f8_few<64, 4, 2, false, MODE, TO, GROUPED>(c, a, s);
     }
@@ -1176,7 +1178,7 @@ extern "C" int llm_f8_describe(void* room, const void* codes, const void* scales
     return LLM_OK;
 }
 
-static bool f8_takes_plain(const void* plain, int dtype, int T, int K) { return T <= F8_PLAIN_ROWS && dtype == LLM_DT_BF16 && K % 8 == 0 && aligned16(plain); }
+static bool f8_takes_plain(const void* plain, int dtype, int T, int K, bool gated) { return T <= F8_PLAIN_ROWS(gated) && dtype == LLM_DT_BF16 && K % 8 == 0 && aligned16(plain); }
 static int f8_args(F8Args* a, const F8Weight* w, int gated, const void* rows, long long padded, int T, int waits, int32_t* status) {
     if (!w || !w->ready || w->gated != gated || status == nullptr || T > (1 << 24)) return LLM_REFUSED_SIZE;
     if (!aligned16(rows)) return LLM_REFUSED_ALIGN;
@@ -1189,15 +1191,15 @@ static int f8_args(F8Args* a, const F8Weight* w, int gated, const void* rows, lo
     return LLM_OK;
 }
 // The rows of a product's x: those that are there; made of the matrix `plain` where there is room for them; or none, and the product makes them.
-static int f8_operand(F8Args* a, void* rows, long long padded, const void* plain, int dtype, uintptr_t stream) {
+static int f8_operand(F8Args* a, void* rows, long long padded, const void* plain, int dtype, bool gated, uintptr_t stream) {
     if (!plain) return rows ? LLM_OK : LLM_REFUSED_ALIGN;
     if (rows) return llm_f8_rows(plain, dtype, rows, padded, a->T, a->K, nullptr, 1, stream);
-    if (!f8_takes_plain(plain, dtype, a->T, a->K)) return LLM_REFUSED_ALIGN;
+    if (!f8_takes_plain(plain, dtype, a->T, a->K, gated)) return LLM_REFUSED_ALIGN;
     a->plain = static_cast<const bf16*>(plain);
     return LLM_OK;
 }
 
-// rows: of 8 bits [T, K], `padded` of them, or room for them (null: none, for up to F8_PLAIN_ROWS rows of a bfloat16 matrix of whole, aligned pieces of eight values) and
+// rows: of 8 bits [T, K], `padded` of them, or room for them (null: none, for up to F8_PLAIN_ROWS of a bfloat16 matrix of whole, aligned pieces of eight values) and
 // `plain` a matrix [T, K] of `dtype`; y: [T, N] float32 or bfloat16; add: y (float32) holds a summand already.
 extern "C" int llm_linear_f8(const void* weight, void* rows, long long padded, const void* plain, int dtype, void* y, int out_dtype, int add, int T, int waits,
                              int32_t* status, uintptr_t stream) {
@@ -1206,7 +1208,7 @@ extern "C" int llm_linear_f8(const void* weight, void* rows, long long padded, c
     const F8Weight* w = static_cast<const F8Weight*>(weight);
     F8Args a;
     if (const int rc = f8_args(&a, w, 0, rows, padded, T, waits, status)) return rc;
-    if (const int rc = f8_operand(&a, rows, padded, plain, dtype, stream)) return rc;
+    if (const int rc = f8_operand(&a, rows, padded, plain, dtype, false, stream)) return rc;
     a.y = y;
     a.vec = a.N % 4 == 0 && aligned16(y);
     const F8Call c = {w, rows, 0};
@@ -1224,13 +1226,13 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
     if (const int rc = f8_args(&a, w, 1, rows, padded, T, waits, status)) return rc;
     if (!mx_act(act, limit, &a.act) || made_padded < T) return LLM_REFUSED_SIZE;
     if (!aligned16(made)) return LLM_REFUSED_ALIGN;
-    if (const int rc = f8_operand(&a, rows, padded, plain, dtype, stream)) return rc;
+    if (const int rc = f8_operand(&a, rows, padded, plain, dtype, true, stream)) return rc;
     a.y = made, a.y_rows = made_padded;
     a.y_scales = f8_row_scales(made, made_padded, f8_tiles(a.N));
     return f8_way<F8_GATED, float, false>({w, rows, 0}, a, 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
-// Tokens whose picks stay as they are: two launches instead of four, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
+// Tokens whose picks stay as they are: two launches instead of five, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
 // time on out of the second-level cache.  Measured, as they are and sorted (us), 1, 2, 4, 5 and 8 tokens: 64 experts, 8 a token, 1,024 by 2,048 17.1 and 21.1, 21.2 and 28.0, 38.1 and 41.4,
 // 55.1 and 46.8, 69.6 and 65.4; 8 experts, 2 a token, 2,048 by 4,096 19.4 and 22.6, 23.7 and 28.4, 31.7 and 36.0, 48.2 and 44.0, 50.8 and 43.3.  Up to eight picks: a cluster adds them up.
 #define F8_UNSORTED_TOKENS 4
@@ -1245,21 +1247,20 @@ static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UN
 static int f8_item_rows(long long picks, int E) { return picks <= 8LL * E ? 16 : picks <= 40LL * E ? 32 : 256; }
 static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
 struct F8Work {
-    int per, room, rows;                  // rows: of x are made in memory
-    long long items, counts, places, tokens, weights, x, middle, y, all;
+    int per, room;
+    long long counts, places, weights, x, middle, y, all;
 };
 static F8Work f8_work(int T, int top, int E, int W, int ff, bool plain, int out_dtype) {
     const long long picks = static_cast<long long>(T) * top;
     F8Work k = {};
     k.per = f8_unsorted(T, top, plain) ? 16 : f8_item_rows(picks, E);
     k.room = static_cast<int>((E < picks ? E : picks) + picks / k.per);
-    k.rows = !(plain && k.per == 16);
     const long long padded = f8_padded_rows(picks);
     auto rows_bytes = [&](int n) { return padded * (f8_tiles(n) * F8_K + f8_k4(n) * 4LL); };
     k.counts = f8_up(16LL * k.room);
-    k.places = k.counts + 256, k.tokens = k.places + f8_up(4 * picks), k.weights = k.tokens + f8_up(4 * picks);
+    k.places = k.counts + 256, k.weights = k.places + f8_up(4 * picks);
     k.x = k.weights + f8_up(4 * picks);
-    k.middle = k.x + (k.rows ? f8_up(rows_bytes(W)) : 0);
+    k.middle = k.x + (f8_unsorted(T, top, plain) ? 0 : f8_up(rows_bytes(W)));
     k.y = k.middle + f8_up(rows_bytes(ff));
     k.all = k.y + picks * W * (out_dtype == LLM_DT_F32 ? 4 : 2);
     return k;
@@ -1268,7 +1269,7 @@ static bool f8_plain_experts(const void* x, int dtype, int W) { return dtype == 
 extern "C" long long llm_moe_f8_work(const void* x, int dtype, int T, int top, int E, int W, int ff, int out_dtype) {
     return f8_work(T, top, E, W, ff, f8_plain_experts(x, dtype, W), out_dtype).all;
 }
-extern "C" int llm_f8_sort(const int32_t*, const float*, int, int, int, int, int32_t*, void*, int32_t*, int32_t*, float*, uintptr_t);
+extern "C" int llm_f8_sort(const int32_t*, const float*, int, int, int, int32_t*, void*, int32_t*, float*, uintptr_t);
 extern "C" int llm_f8_add_up(const void*, int, const int32_t*, const float*, void*, int, int, int, uintptr_t);
 extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, int dtype, const int32_t* ids, const float* weights, int T, int top, void* work,
                           const float* base, void* out, int out_dtype, int act, float limit, int on_input, int waits, int32_t* status, uintptr_t stream) {
@@ -1282,23 +1283,24 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     const bool plain = f8_plain_experts(x, dtype, W), unsorted = f8_unsorted(T, top, plain);
     const F8Work k = f8_work(T, top, g->E, W, ff, plain, out_dtype);
     unsigned char* at = static_cast<unsigned char*>(work);
-    int32_t *counts = reinterpret_cast<int32_t*>(at + k.counts), *places = reinterpret_cast<int32_t*>(at + k.places), *tokens = reinterpret_cast<int32_t*>(at + k.tokens);
+    int32_t *counts = reinterpret_cast<int32_t*>(at + k.counts), *places = reinterpret_cast<int32_t*>(at + k.places);
     float* row_weights = reinterpret_cast<float*>(at + k.weights);
     const long long padded = f8_padded_rows(picks);
-    if (!unsorted)
-        if (const int rc = llm_f8_sort(ids, weights, picks, top, g->E, k.per, counts, at, places, tokens, row_weights, stream)) return rc;
-    if (k.rows)
-        if (const int rc = llm_f8_rows(x, dtype, at + k.x, padded, T, W, places, top, stream)) return rc;
+    void* x_rows = unsorted ? nullptr : at + k.x;
+    if (!unsorted) {
+        if (const int rc = llm_f8_sort(ids, weights, picks, g->E, k.per, counts, at, places, row_weights, stream)) return rc;
+        if (const int rc = llm_f8_rows(x, dtype, x_rows, padded, T, W, places, top, stream)) return rc;
+    }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     F8Args a;
-    if (const int rc = f8_args(&a, g, 1, k.rows ? at + k.x : nullptr, padded, picks, waits, status)) return rc;
+    if (const int rc = f8_args(&a, g, 1, x_rows, padded, picks, waits, status)) return rc;
     if (!mx_act(act, limit, &a.act)) return LLM_REFUSED_SIZE;
-    a.plain = k.rows ? nullptr : static_cast<const bf16*>(x);
+    a.plain = unsorted ? static_cast<const bf16*>(x) : nullptr;
     a.y = at + k.middle, a.y_rows = padded, a.y_scales = f8_row_scales(at + k.middle, padded, f8_tiles(ff));
-    const F8Groups groups = {unsorted ? ids : nullptr, top, g->E, counts, reinterpret_cast<const int4*>(at), tokens, unsorted ? weights : row_weights};
+    const F8Groups groups = {unsorted ? ids : nullptr, top, g->E, counts, reinterpret_cast<const int4*>(at), unsorted ? weights : row_weights};
     a.groups = groups;
     a.on_input = on_input;
-    if (const int rc = f8_way<F8_GATED, float, true>({g, k.rows ? at + k.x : nullptr, unsorted ? picks : k.room}, a, k.per, s)) return rc;
+    if (const int rc = f8_way<F8_GATED, float, true>({g, x_rows, unsorted ? picks : k.room}, a, k.per, s)) return rc;
     if (const int rc = f8_args(&a, d, 0, at + k.middle, padded, picks, waits, status)) return rc;
     a.y = unsorted ? out : at + k.y;
     a.vec = W % 4 == 0 && aligned16(a.y);
@@ -1310,7 +1312,4 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     return unsorted ? LLM_OK : llm_f8_add_up(at + k.y, out_dtype, places, base, out, T, W, top, stream);
 }
 // Kernels that llm_moe_f8 launches.
-extern "C" int llm_moe_f8_launches(const void* x, int dtype, int T, int top, int E, int W) {
-    const bool plain = f8_plain_experts(x, dtype, W);
-    return f8_unsorted(T, top, plain) ? 2 : 4 + f8_work(T, top, E, W, 1, plain, 0).rows;
-}
+extern "C" int llm_moe_f8_launches(const void* x, int dtype, int T, int top, int W) { return f8_unsorted(T, top, f8_plain_experts(x, dtype, W)) ? 2 : 5; }

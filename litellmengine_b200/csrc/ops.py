@@ -2595,8 +2595,8 @@ def _mx_count() -> None:
 # A weight has one float32 scale for each block of 128 x 128 values, a row one for each 128 neighbouring values: the block's largest
 # magnitude / 448.  csrc/f8_blocks.cuh says how codes are rounded and where the bytes lie.
 F8_BLOCK = 128
-# Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself.
-F8_PLAIN_ROWS = 16
+# Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself; one of gate and up.
+F8_PLAIN_ROWS, F8_PLAIN_ROWS_GATED = 8, 4
 _MX_SIGNATURES.update({
     "llm_f8_rows": ("blocks_f8", [_P, _I, _P, _L, _I, _I, _P, _I, _P]),
     "llm_f8_weight": ("blocks_f8", [_P, _I, _P, _P, _I, _I, _I, _I, _I, _L, _L, _P]),
@@ -2752,7 +2752,7 @@ def _f8_operands(x, weight: F8Weight, gated: bool):
         raise KernelError("the product takes rows of 8 bits or a matrix")
     _here(x, weight.buffer)
     at, dt = x.data_ptr(), _dt(x)
-    if shape[0] <= F8_PLAIN_ROWS and dt == 1 and shape[1] % 8 == 0 and at % 16 == 0:
+    if shape[0] <= (F8_PLAIN_ROWS_GATED if gated else F8_PLAIN_ROWS) and dt == 1 and shape[1] % 8 == 0 and at % 16 == 0:
         return None, at, dt
     return F8Rows(shape[0], shape[1], weight.device), at, dt
 
@@ -2827,7 +2827,7 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
     sizes = _f8_sizes.get(key)
     if sizes is None:
         work = _fn("blocks_f8", "llm_moe_f8_work", [_P, _I, _I, _I, _I, _I, _I, _I], c_longlong)(x.data_ptr(), dt, T, top, E, W, ff, od)
-        launches = _fn("blocks_f8", "llm_moe_f8_launches", [_P, _I, _I, _I, _I, _I])(x.data_ptr(), dt, T, top, E, W)
+        launches = _fn("blocks_f8", "llm_moe_f8_launches", [_P, _I, _I, _I, _I])(x.data_ptr(), dt, T, top, W)
         if len(_f8_sizes) > 4096:
             _f8_sizes.clear()
         sizes = _f8_sizes[key] = work, launches
