@@ -1233,18 +1233,18 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
 }
 
 // Tokens whose picks stay as they are: two launches instead of five, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
-// time on out of the second-level cache.  Measured, as they are and sorted (us), 1, 2, 4, 5 and 8 tokens: 64 experts, 8 a token, 1,024 by 2,048 17.1 and 21.1, 21.2 and 28.0, 38.1 and 41.4,
-// 55.1 and 46.8, 69.6 and 65.4; 8 experts, 2 a token, 2,048 by 4,096 19.4 and 22.6, 23.7 and 28.4, 31.7 and 36.0, 48.2 and 44.0, 50.8 and 43.3.  Up to eight picks: a cluster adds them up.
+// time on out of the second-level cache.  Measured, as they are and sorted (us), 1, 2, 4, 5 and 8 tokens: 64 experts, 8 a token, 1,024 by 2,048 15.7 and 21.2, 20.5 and 26.3, 38.6 and 43.7,
+// 51.8 and 47.2, 67.5 and 62.2; 8 experts, 2 a token, 2,048 by 4,096 18.5 and 20.6, 24.8 and 31.4, 36.0 and 42.7, 44.6 and 35.8, 48.2 and 44.9.  Up to eight picks: a cluster adds them up.
 #define F8_UNSORTED_TOKENS 4
 static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UNSORTED_TOKENS && top <= 8; }
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
 // middle's rows, the experts' results.
 // Rows of an item, by how many picks an expert has on average: fewer fit most experts' picks into one item, whose weights are read once.  Measured (us): 64 experts, 8 a
-// token, 1,024 by 2,048, 6 picks an expert 85 (16), 86 (32), 125 (256); 12: 111, 96, 136; 32: 178, 127, 143; 48: 228, 153, 142; 96: 414, 241, 162.  8 experts, 2 a token, 2,048 by 4,096,
-// 8: 50, 49, 68; 16: 64, 52, 69; 40: 107, 69, 73; 64: 127, 97, 76; 1,450 by 1,358, 12: 28, 29, 45; 24: 32, 32, 46; 48: 45, 38, 46; 96: 60, 58, 48.  Items of 64 rows come out between the
-// latter two, or up to a tenth before both where experts are few and large.
-static int f8_item_rows(long long picks, int E) { return picks <= 8LL * E ? 16 : picks <= 40LL * E ? 32 : 256; }
+// token, 1,024 by 2,048, 6 picks an expert 79 (16), 86 (32), 125 (256); 10: 94, 93; 12: 99, 95, 136; 24: 126, 118, 140; 32: 127 (32), 143 (256); 48: 153, 142; 96: 241, 162.  8 experts, 2 a token,
+// 2,048 by 4,096, 8: 48, 50, 68; 12: 55, 54; 24: 59, 65, 70; 40: 69, 73; 64: 97, 76; 1,450 by 1,358, 12: 29, 31, 45; 24: 31, 32, 46; 48: 38, 46; 96: 58, 48.  Items of 64 rows come out
+// between the latter two, or up to a tenth before both where experts are few and large.
+static int f8_item_rows(long long picks, int E) { return picks <= 10LL * E ? 16 : picks <= 40LL * E ? 32 : 256; }
 static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
 struct F8Work {
     int per, room;
