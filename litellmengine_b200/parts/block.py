@@ -193,6 +193,8 @@ class Block:
 
     def parts_that_hold(self, weight_format: str):
         """The parts whose matrices a model of this weight format holds in it."""
+        if weight_format != "stored" and weight_format not in self.HOLDS:
+            raise ValueError(f"weight_format {weight_format!r}: 'stored' or one of {tuple(self.HOLDS)}")
         name = self.HOLDS.get(weight_format)
         return [p for p in self.parts() if name is not None and speaks_for_forward(p, name)]
 

@@ -110,3 +110,11 @@ def test_weight_format():
     assert cli.parse_args(["--model", "m", "--weight-format=fp8"]).weight_format == "fp8"
     with pytest.raises(cli.ArgError, match="--weight-format"):
         cli.parse_args(["--model", "m", "--weight-format", "fp8", "--dtype", "float32"])
+
+
+def test_a_block_refuses_a_weight_format_that_it_does_not_know():
+    from litellmengine_b200.parts.block import Block
+    block = Block.__new__(Block)
+    for unknown in ("fp4", True, None):
+        with pytest.raises(ValueError):
+            block.parts_that_hold(unknown)
