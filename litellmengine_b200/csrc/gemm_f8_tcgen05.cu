@@ -7,7 +7,7 @@
 //   * Few rows: bytes bound the product.  The weights are the left operand (128 features a tile), the rows the right one (NT of them), so that no lane is spent
 //     on rows that are not there.  K is cut over a cluster's CTAs, which add their sums up in each other's shared memory in the parts' order;
 //     nothing is left for another kernel and no result depends on timing.
-//   * Many rows: pairs of CTAs.  The rows are the left operand, so that a lane is a row and its scale one number for 64 or 128 features.
+//   * Many rows: pairs of CTAs, or CTAs of 128 rows alone.  The rows are the left operand, so that a lane is a row and its scale one number for 64 or 128 features.
 //   * Gate and up: act(gate) * up leaves as rows of 8 bits, 128 features a scale.
 //   * Rows sorted by expert: an item (up to a tile's rows of one expert) takes the place of a tile of rows; how many there are only the device knows.
 // Waits are bounded: one that runs out sets status code 10, and the copies and products that are under way then end, which is waited for on their own barriers
@@ -487,9 +487,10 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
     }
 }
 
-// ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
+// ---- many rows: pairs of CTAs, and CTAs alone ---------------------------------------------------------------------------------------
 // The two CTAs of a cluster compute a tile of 256 rows x 256 features together (cta_group::2): each brings its own 128 rows and half of the features, and
-// reads both halves.  A CTA's tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them, one for each tile of the weight,
+// reads both halves.  Or (CTAS = 1) a CTA computes a tile of 128 rows alone and brings all of the features: for 33 to 128 rows, experts of few rows, and where rounds of pairs would be
+// half empty.  A CTA's tensor memory holds four accumulators of 128 rows x 128 features: a tile of K's products fill two of them, one for each tile of the weight,
 // while those of the tile before are taken out.  Each has barriers and four warps of its own (a row and 128 features a thread, 64 pairs of sums in registers), so that
 // its way round (products, the word of them, taking out, the word that it is free) overlaps the other three's.  Taking out (tcgen05.ld) and adding (fma of two at a time)
 // alternate in quarters of 32 features; the accumulator is free again with the last quarter's additions still to do.
@@ -501,8 +502,8 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
 // tile of K.
 // The clusters are persistent: the copies go on into the next tile while the threads write a finished one.  Tiles are numbered row tile fastest: what runs at one time
 // shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's rows and weights are few.
-// Warp 0 feeds the weights, 2 the rows, 3 the scales; warp 1 of the first CTA issues; warps 4 to 11 take the sums and write them.
-#define FP_STAGES 4
+// Warp 0 feeds the weights, 2 the rows, 3 the scales; warp 1 (of the first CTA) issues; warps 4 to 11 take the sums and write them.
+#define FP_STAGES(CTAS) ((CTAS) == 2 ? 4 : 3)
 #define FP_THREADS 384
 #define FP_BLOCK 8192             // a warp's rows on their way out: 32 of 64 features, or of 128 in 16 bits
 #define FP_RING 2                 // groups of tiles of K whose scales are there
@@ -522,19 +523,21 @@ __device__ __forceinline__ unsigned fp_map_to(unsigned smem_addr, unsigned rank)
     return r;
 }
 // A wait that ran out ends the pair's work, not one CTA's alone: the other one's flag too.
-__device__ __forceinline__ bool fp_give_up(volatile int* abort_flag, int32_t* status) {
+template <int CTAS> __device__ __forceinline__ bool fp_give_up(volatile int* abort_flag, int32_t* status) {
     *abort_flag = 1;
-    const unsigned other = fp_map_to(t5_smem(const_cast<int*>(abort_flag)), fp_rank() ^ 1);
-    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(other), "r"(1u) : "memory");
+    if (CTAS == 2) {
+        const unsigned other = fp_map_to(t5_smem(const_cast<int*>(abort_flag)), fp_rank() ^ 1);
+        asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(other), "r"(1u) : "memory");
+    }
     if (atomicCAS(status, 0, F8_STATUS) == 0) status[1] = blockIdx.x;
     return false;
 }
-__device__ __forceinline__ bool fp_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+template <int CTAS> __device__ __forceinline__ bool fp_wait(unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
     for (int i = 0; i < waits; ++i) {
         if (t5_try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
     }
-    return fp_give_up(abort_flag, status);
+    return fp_give_up<CTAS>(abort_flag, status);
 }
 // Whether a barrier's phase is complete, without waiting for it; and the wait of a warp that has looked.  A look takes 100 clocks until its answer is there, so what is
 // likely to be complete is asked for ahead of what can run without it; a vote over the lanes would take another 45.  All lanes come out of it together:
@@ -544,9 +547,9 @@ __device__ __forceinline__ bool fp_look(unsigned long long* bar, unsigned parity
     asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(t5_smem(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ bool fp_wait_warp(bool seen, unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
+template <int CTAS> __device__ __forceinline__ bool fp_wait_warp(bool seen, unsigned long long* bar, unsigned parity, int waits, volatile int* abort_flag, int32_t* status) {
     bool ok = true;
-    if (!seen) ok = fp_wait(bar, parity, waits, abort_flag, status);
+    if (!seen) ok = fp_wait<CTAS>(bar, parity, waits, abort_flag, status);
     __syncwarp();
     return ok;
 }
@@ -564,13 +567,15 @@ __device__ __forceinline__ void fp_tma_3d(void* dst, const CUtensorMap* map, int
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::
                      "r"(t5_smem(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void fp_commit_lead(unsigned lead, unsigned long long* bar) {
-    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+template <int CTAS> __device__ __forceinline__ void fp_commit_lead(unsigned lead, unsigned long long* bar) {
+    if constexpr (CTAS == 1) t5_commit_lead(lead, bar);
+    else asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
                  " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::
                      "r"(t5_smem(bar)), "h"(static_cast<unsigned short>(3)), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void fp_mma_lead(unsigned lead, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+template <int CTAS> __device__ __forceinline__ void fp_mma_lead(unsigned lead, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    if constexpr (CTAS == 1) f8_mma_lead(lead, d_tmem, a_desc, b_desc, idesc, accumulate);
+    else asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
                  " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::
                      "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
 }
@@ -616,46 +621,52 @@ struct FpTile {
     int features;                         // number of the 256 features of a matrix
     int tile;                             // number of the first of the two tiles of the weight
 };
-template <bool GROUPED> __device__ __forceinline__ FpTile fp_tile(const F8Args& a, int t, int row_tiles) {
+template <bool GROUPED, int CTAS> __device__ __forceinline__ FpTile fp_tile(const F8Args& a, int t, int row_tiles) {
     if constexpr (GROUPED) {
         const int per = a.tiles / 2, i = t / per, f = t - i * per;
         const int4 item = a.groups.items[i];
         return {item.y, item.z, f, item.x * a.tiles + 2 * f};
     } else {
         const int f = t / row_tiles, r = t - f * row_tiles;
-        return {r * 256, a.T - r * 256, f, 2 * f};
+        return {r * 128 * CTAS, a.T - r * 128 * CTAS, f, 2 * f};
     }
 }
 
 // SPLIT: gated, and the up features of a tile may lie in two blocks.
-template <int MODE, typename TO, bool GROUPED, bool SPLIT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pair_kernel(const __grid_constant__ CUtensorMap w_map,
+template <int MODE, typename TO, bool GROUPED, bool SPLIT, int CTAS>
+__global__ void __launch_bounds__(FP_THREADS, 1) f8_pair_kernel(const __grid_constant__ CUtensorMap w_map,
                                                                                          const __grid_constant__ CUtensorMap x_map,
                                                                                          const __grid_constant__ CUtensorMap y_map, const F8Args a, int row_tiles,
                                                                                          int all_tiles) {
+    constexpr int STAGES = FP_STAGES(CTAS), W_BYTES = 2 / CTAS * F8_TILE;       // of a stage of weights in this CTA
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* w_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-    unsigned char* x_s = w_s + FP_STAGES * F8_TILE;               // [STAGES][128 rows][128]
-    unsigned char* out_s = x_s + FP_STAGES * F8_TILE;             // a block for each of the eight warps
+    unsigned char* x_s = w_s + STAGES * W_BYTES;               // [STAGES][128 rows][128]
+    unsigned char* out_s = x_s + STAGES * F8_TILE;             // a block for each of the eight warps
     float* most_s = reinterpret_cast<float*>(out_s);              // gated: [2][2][128]
     unsigned char* scales_s = out_s + 8 * FP_BLOCK;               // [RING]
-    __shared__ __align__(8) unsigned long long full[FP_STAGES], empty[FP_STAGES], acc_full[4], acc_empty[4], s_full[FP_RING], s_empty[FP_RING], drained;
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[4], acc_empty[4], s_full[FP_RING], s_empty[FP_RING], drained;
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_flag, asked_s[2];                        // asked_s: boxes of weights, of rows that were asked for
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const unsigned rank = __shfl_sync(0xffffffffu, fp_rank(), 0);
-    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1, ktiles = a.ktiles;
+    const int cluster = blockIdx.x / CTAS, clusters = gridDim.x / CTAS, ktiles = a.ktiles;
     if (tid == 0) {
         abort_flag = 0;
-        for (int s = 0; s < FP_STAGES; ++s) { t5_mbar_init(&full[s], 2); t5_mbar_init(&empty[s], 1); }      // weights and rows
-        for (int s = 0; s < 4; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 8); }      // 4 warps of 2 CTAs
+        for (int s = 0; s < STAGES; ++s) { t5_mbar_init(&full[s], 2); t5_mbar_init(&empty[s], 1); }      // weights and rows
+        for (int s = 0; s < 4; ++s) { t5_mbar_init(&acc_full[s], 1); t5_mbar_init(&acc_empty[s], 4 * CTAS); }      // 4 warps of each CTA
         for (int s = 0; s < FP_RING; ++s) { t5_mbar_init(&s_full[s], 32); t5_mbar_init(&s_empty[s], 8); }
         t5_mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        if constexpr (CTAS == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(t5_smem(&tmem_base_s)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        }
     }
     t5_fence_before();
     __syncthreads();
@@ -669,7 +680,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
     // This thread's box (or two of weights: 64 features of either tile, so that an accumulator is a tile) for tile at and tile of K kb, into stage s.
     const unsigned first = fp_map_to(t5_smem(full), 0);           // the first CTA's barriers
     auto ask = [&](const FpTile& at, int kb, int s) {
-        if (rank == 0) t5_expect_tx(&full[s], 2 * F8_TILE);       // of both CTAs
+        if (rank == 0) t5_expect_tx(&full[s], warp == 0 ? 2 * F8_TILE : CTAS * F8_TILE);       // of both CTAs
+        if constexpr (CTAS == 1) {
+            if (warp == 0)
+                for (int w = 0; w < 2; ++w) t5_tma_2d(w_s + s * W_BYTES + w * F8_TILE, &w_map, 0, ((at.tile + w) * ktiles + kb) * 128, &full[s]);
+            else f8_tma_3d(x_s + s * F8_TILE, &x_map, 0, at.row0, kb, &full[s]);
+            return;
+        }
         const unsigned bar = first + s * 8;
         if (warp == 0) {
             const int line = (at.tile * ktiles + kb) * 128 + static_cast<int>(rank) * 64;
@@ -686,54 +703,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 int s = 0;
                 unsigned phase = 1;                               // a barrier that was never used passes for the phase before its first
                 bool ok = true;
-                int ahead = !GROUPED && warp == 0 ? FP_STAGES : -1;       // boxes of weights that do not wait for the kernel in front
+                int ahead = !GROUPED && warp == 0 ? STAGES : -1;       // boxes of weights that do not wait for the kernel in front
                 for (int t = cluster; ok && t < tiles; t += clusters) {
-                    const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
+                    const FpTile at = fp_tile<GROUPED, CTAS>(a, t, row_tiles);
 #pragma unroll 1
                     for (int kb = 0; kb < ktiles; ++kb) {
                         if (ahead >= 0 && ahead-- == 0) pdl_wait();       // the bounded waits below are not for that kernel
-                        if (!fp_wait(&empty[s], phase, a.waits, &abort_flag, a.status)) {
+                        if (!fp_wait<CTAS>(&empty[s], phase, a.waits, &abort_flag, a.status)) {
                             asked = (t - cluster) / clusters * ktiles + kb;
                             ok = false;
                             break;
                         }
                         ask(at, kb, s);
-                        if (++s == FP_STAGES) s = 0, phase ^= 1;
+                        if (++s == STAGES) s = 0, phase ^= 1;
                     }
                 }
                 if (ok) asked = tiles > cluster ? (tiles - cluster + clusters - 1) / clusters * ktiles : 0;
                 asked_s[warp >> 1] = asked;
                 // The products tell both CTAs that they have read a stage, and none may leave before it has been told (of products that stop, the last commit tells).
                 if (warp == 0 && ok)
-                    for (int i = max(0, asked - FP_STAGES); i < asked; ++i)
-                        for (int j = 0; j < T5_WAIT_LIMIT && !t5_try_wait(&empty[i % FP_STAGES], (i / FP_STAGES) & 1) && !*static_cast<volatile int*>(&abort_flag); ++j) {}
+                    for (int i = max(0, asked - STAGES); i < asked; ++i)
+                        for (int j = 0; j < T5_WAIT_LIMIT && !t5_try_wait(&empty[i % STAGES], (i / STAGES) & 1) && !*static_cast<volatile int*>(&abort_flag); ++j) {}
             }
             __syncwarp();
         } else if (warp == 1 && rank == 0) {
             const unsigned lead = elect_one();
             const unsigned long long wd = t5_desc(w_s, 16, 1024), xd = t5_desc(x_s, 16, 1024);
-            const unsigned idesc = f8_idesc(256, 128);
+            const unsigned idesc = f8_idesc(128 * CTAS, 128);
             int s = 0;
             unsigned phase = 0, buf = 0, acc_phase = 1;
             bool ok = true, seen = false;
             for (int t = cluster; ok && t < tiles; t += clusters) {
 #pragma unroll 1
                 for (int kb = 0; kb < ktiles; ++kb) {
-                    ok = fp_wait_warp(seen, &full[s], phase, a.waits, &abort_flag, a.status) && ok;
+                    ok = fp_wait_warp<CTAS>(seen, &full[s], phase, a.waits, &abort_flag, a.status) && ok;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        ok = fp_wait_warp(false, &acc_empty[2 * buf + h], acc_phase, a.waits, &abort_flag, a.status) && ok;
+                        ok = fp_wait_warp<CTAS>(false, &acc_empty[2 * buf + h], acc_phase, a.waits, &abort_flag, a.status) && ok;
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         t5_fence_after();
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            fp_mma_lead(lead, tmem + buf * 256 + h * 128, xd + s * (F8_TILE >> 4) + 2 * k, wd + ((s * F8_TILE + h * (F8_TILE / 2)) >> 4) + 2 * k, idesc, k ? 1u : 0u);
-                        if (h == 1) fp_commit_lead(lead, &empty[s]);
-                        fp_commit_lead(lead, &acc_full[2 * buf + h]);
+                            fp_mma_lead<CTAS>(lead, tmem + buf * 256 + h * 128, xd + s * (F8_TILE >> 4) + 2 * k, wd + ((s * W_BYTES + h * (W_BYTES / 2)) >> 4) + 2 * k, idesc, k ? 1u : 0u);
+                        if (h == 1) fp_commit_lead<CTAS>(lead, &empty[s]);
+                        fp_commit_lead<CTAS>(lead, &acc_full[2 * buf + h]);
                     }
                     if (!ok) break;
-                    if (++s == FP_STAGES) s = 0, phase ^= 1;
+                    if (++s == STAGES) s = 0, phase ^= 1;
                     seen = fp_look(&full[s], phase);
                     buf ^= 1;
                     if (buf == 0) acc_phase ^= 1;
@@ -745,7 +762,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
             unsigned phase = 1;
             bool ok = true;
             for (int t = cluster; ok && t < tiles; t += clusters) {
-                const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
+                const FpTile at = fp_tile<GROUPED, CTAS>(a, t, row_tiles);
                 const int r0 = at.row0 + static_cast<int>(rank) * 128 + lane;
                 const float* cw = a.w_scales + (at.tile * 3LL + min(lane, 5)) * a.k4;
                 const float* cx[4];
@@ -754,7 +771,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 for (int i = 0; i < 4; ++i) bytes[i] = r0 + 32 * i < a.x_rows ? 4 : 0, cx[i] = a.x_scales + (bytes[i] ? (r0 + 32 * i) * static_cast<long long>(a.k4) : 0);
 #pragma unroll 1
                 for (int kb0 = 0; kb0 < ktiles; kb0 += FP_GROUP) {
-                    ok = __all_sync(0xffffffffu, fp_wait(&s_empty[slot], phase, a.waits, &abort_flag, a.status));
+                    ok = __all_sync(0xffffffffu, fp_wait<CTAS>(&s_empty[slot], phase, a.waits, &abort_flag, a.status));
                     if (!ok) break;
                     unsigned to = t5_smem(scales_s) + slot * (FP_GROUP * FP_SCALES);
 #pragma unroll 1
@@ -782,15 +799,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
             if ((warp == 0 || warp == 2) && lane == 0) {
                 int most = 0;
                 for (int who = 0; who < 2; ++who)
-                    for (unsigned r = 0; r < 2; ++r) {
+                    for (unsigned r = 0; r < CTAS; ++r) {
                         int n;
                         asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(n) : "r"(fp_map_to(t5_smem(&asked_s[who]), r)) : "memory");
                         most = max(most, n);
                     }
-                for (; asked < most; ++asked) ask(fp_tile<GROUPED>(a, cluster + asked / ktiles * clusters, row_tiles), asked % ktiles, asked % FP_STAGES);
-                if (rank == 0) f8_land_ring(full, FP_STAGES, most);
+                for (; asked < most; ++asked) ask(fp_tile<GROUPED, CTAS>(a, cluster + asked / ktiles * clusters, row_tiles), asked % ktiles, asked % STAGES);
+                if (rank == 0) f8_land_ring(full, STAGES, most);
             } else if (warp == 1) {
-                if (rank == 0) fp_commit_lead(elect_one(), &drained);     // the lane that issued: elect gives the same one for the same lanes
+                if (rank == 0) fp_commit_lead<CTAS>(elect_one(), &drained);     // the lane that issued: elect gives the same one for the same lanes
                 f8_land(&drained, 0);
             }
             __syncwarp();
@@ -798,7 +815,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
         }
         if (warp == 1) {
             t5_fence_after();
-            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+            if constexpr (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+            else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(FP_LARGE));
@@ -808,7 +826,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
         const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + half * 128;
         unsigned buf = 0, acc_phase = 0, slot = 0, s_phase = 0, turn = 0;
         for (int t = cluster; t < tiles; t += clusters) {
-            const FpTile at = fp_tile<GROUPED>(a, t, row_tiles);
+            const FpTile at = fp_tile<GROUPED, CTAS>(a, t, row_tiles);
             unsigned long long acc[64];                           // two features each
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0ull;
@@ -821,9 +839,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 sw = *reinterpret_cast<const float4*>(p + 512 + half * 16);
             };
             // One that gives up goes on with what there is, and stores nothing.
-            bool ok = fp_wait_warp(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status);
+            bool ok = fp_wait_warp<CTAS>(false, &s_full[slot], s_phase, a.waits, &abort_flag, a.status);
             scales(0);
-            ok = fp_wait_warp(false, &acc_full[2 * buf + half], acc_phase, a.waits, &abort_flag, a.status) && ok;
+            ok = fp_wait_warp<CTAS>(false, &acc_full[2 * buf + half], acc_phase, a.waits, &abort_flag, a.status) && ok;
             t5_fence_after();
             unsigned r[2][32];
             t5_ld32(from + buf * 256, r[0]);
@@ -856,7 +874,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 t5_wait_ld();
                 t5_ld32(now + 64, r[0]);
                 if (!last) {
-                    if (group_ends) ok = fp_wait_warp(seen_s, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
+                    if (group_ends) ok = fp_wait_warp<CTAS>(seen_s, &s_full[slot], s_phase, a.waits, &abort_flag, a.status) && ok;
                     scales(kb + 1);
                 }
                 add(1);
@@ -874,7 +892,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1) f8_pa
                 buf ^= 1;
                 acc_phase = next_phase;
                 if (!last) {
-                    ok = fp_wait_warp(seen, next, next_phase, a.waits, &abort_flag, a.status) && ok;
+                    ok = fp_wait_warp<CTAS>(seen, next, next_phase, a.waits, &abort_flag, a.status) && ok;
                     t5_fence_after();
                     t5_ld32(from + buf * 256, r[0]);
                 }
@@ -1103,7 +1121,7 @@ template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED
     launch_pdl_cluster(kern, dim3(parts, tiles, c.row_tiles), dim3(F8_FEW_THREADS(PLAIN, WT)), smem, s, parts, c.w->whole, x_map, a);
     return launch_status();
 }
-template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(const F8Call& c, F8Args a, cudaStream_t s) {
+template <int MODE, typename TO, bool GROUPED, bool SPLIT, int CTAS> static int f8_pair(const F8Call& c, F8Args a, cudaStream_t s) {
     CUtensorMap x_map, y_map = {};
     const int dev = f8_device();
     if (dev < 0 || f8_sms(dev) < 2) return LLM_REFUSED_SIZE;
@@ -1117,28 +1135,32 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT> static int f8_pair(co
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return LLM_REFUSED_SIZE;
     }
-    constexpr size_t smem = static_cast<size_t>(FP_STAGES) * 2 * F8_TILE + 8 * FP_BLOCK + FP_RING * FP_GROUP * FP_SCALES + 1024;
+    constexpr size_t smem = static_cast<size_t>(FP_STAGES(CTAS)) * (2 / CTAS + 1) * F8_TILE + 8 * FP_BLOCK + FP_RING * FP_GROUP * FP_SCALES + 1024;
     static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
     static_assert(128 * FP_SMALL + 256 * FP_LARGE <= FP_THREADS * 168, "registers of the launch");
-    auto kern = f8_pair_kernel<MODE, TO, GROUPED, SPLIT>;
+    auto kern = f8_pair_kernel<MODE, TO, GROUPED, SPLIT, CTAS>;
     static bool had[F8_DEVICES];
     if (const int rc = f8_allow(kern, smem, dev, had)) return rc;
     const long long all = static_cast<long long>(c.row_tiles) * (a.tiles / 2);
-    const int slots = f8_sms(dev) / 2;
+    const int slots = f8_sms(dev) / CTAS;
     if (all > (1LL << 30)) return LLM_REFUSED_SIZE;
     const int clusters = all < slots ? static_cast<int>(all) : slots;
-    launch_pdl(kern, dim3(2 * clusters), dim3(FP_THREADS), smem, s, c.w->halves, x_map, y_map, a, c.row_tiles, static_cast<int>(all));
+    launch_pdl_cluster(kern, dim3(CTAS * clusters), dim3(FP_THREADS), smem, s, CTAS, CTAS == 2 ? c.w->halves : c.w->whole, x_map, y_map, a, c.row_tiles, static_cast<int>(all));
     return launch_status();
 }
 
-// How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 64 rows one tile of rows reads the weight once.  Beyond that tiles of 64
-// rows go on as long as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which pairs of CTAs (256) do not do.  Measured, rows of 8 bits by tiles of 64 and
-// of pairs (us): 65 rows of 4,096 by 6,144 15.1 and 16.8, 197 rows 27.4 and 17.4; 250 by 4,096 15.2 and 17.3, 320 27.1 and 17.2; 250 rows of 12,288 by 4,096 35.5 and 42.3; 65 rows of 2,048 by
-// 12,288 15.3 and 11.1; 197 rows of 1,358 by 2,501 7.5 and 11.3, 512 12.9 and 11.4; gated, 320 rows of 1,358 by 2 x 1,450 9.4 and 12.3, 512 14.3 and 12.5; 128 of 1,024 by 2 x 4,096 8.7 and 8.6.
-// Tiles of 128 rows by one CTA are no faster than two of 64: 65 to 128 rows by 6,144 14.5 to 16.1 and 15.1 to 15.3, by 24,576 51 to 54 and 44 to 49.
+// How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 32 rows one tile of rows reads the weight once.  Tiles of 64 rows go on as long
+// as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which the others do not do.  Of these, CTAs of 128 rows alone take 6/5 of the time that pairs of
+// 256 rows take for a tile of 256 features, but twice as many run at once: whoever needs less time for all.  Measured, rows of 8 bits, by tiles of 64, 128 and 256 (us): 64 rows of 4,096 by
+// 24,576 26.9, 23.6, 33.2; 65 by 6,144 15.0, 20.2, 16.9; 128 by 24,576 49, 24.5, 34.8; 197 by 6,144 26.1, 20.4, 17.4; 256 by 4,096 15.2, 20.2, 17.4; 256 rows of 12,288 by 4,096 35.6, 52.7, 42.6; 384 of
+// 4,096 by 24,576 107, 48.0, 55.7; 512 149, 64.6, 59.0; 1,024 by 4,096 (128 and 256) 22.9, 19.4; 2,048 42.5, 38.3; 65 rows of 2,048 by 12,288 15.3, 11.9, 11.2; 384 29.6, 12.7, 18.6; 197 rows of 1,358 by
+// 2,501 7.4, 11.9, 11.3; 512 12.5, 12.0, 11.5; gated, 128 rows of 4,096 by 2 x 12,288 54.7, 24.9, 36.4; 256 84.8, 43.5, 37.4; 384 of 1,358 by 2 x 1,450 13.4, 12.1, 12.5.
 static int f8_tile_rows(int T, int tiles, int sms) {
-    if (T <= 64) return T <= 16 ? 16 : T <= 32 ? 32 : 64;
-    return static_cast<long long>((T + 63) / 64) * tiles <= sms ? 64 : 256;
+    if (T <= 32) return T <= 16 ? 16 : 32;
+    if (static_cast<long long>((T + 63) / 64) * tiles <= sms) return 64;
+    const long long wide = (tiles + 1) / 2;                       // tiles of 256 features
+    const long long alone = ((T + 127) / 128 * wide + sms - 1) / sms, paired = ((T + 255) / 256 * wide + sms / 2 - 1) / (sms / 2);       // rounds
+    return 6 * alone < 5 * paired ? 128 : 256;
 }
 
 template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const F8Args& a, int per, cudaStream_t s) {         // per: rows of an item
@@ -1148,19 +1170,18 @@ template <int MODE, typename TO, bool GROUPED> static int f8_way(F8Call c, const
         per = f8_tile_rows(a.T, (MODE == F8_GATED ? 2 : 1) * ((a.N + 127) / 128), f8_sms(dev));
         c.row_tiles = (a.T + per - 1) / per;
     }
-    if (per == 256) return MODE == F8_GATED && a.N % 64 ? f8_pair<MODE, TO, GROUPED, MODE == F8_GATED>(c, a, s) : f8_pair<MODE, TO, GROUPED, false>(c, a, s);
+    if (per == 256) return MODE == F8_GATED && a.N % 64 ? f8_pair<MODE, TO, GROUPED, MODE == F8_GATED, 2>(c, a, s) : f8_pair<MODE, TO, GROUPED, false, 2>(c, a, s);
+    if (per == 128) return MODE == F8_GATED && a.N % 64 ? f8_pair<MODE, TO, GROUPED, MODE == F8_GATED, 1>(c, a, s) : f8_pair<MODE, TO, GROUPED, false, 1>(c, a, s);
     if constexpr (MODE == F8_GATED) {
         if (per == 16) return a.plain ? f8_few<16, 3, 2, true, MODE, TO, GROUPED>(c, a, s) : f8_few<16, 3, 2, false, MODE, TO, GROUPED>(c, a, s);
-        if (per == 32) return f8_few<32, 3, 1, false, MODE, TO, GROUPED>(c, a, s);
-        if constexpr (!GROUPED) return f8_few<64, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
+        if constexpr (!GROUPED) return per == 32 ? f8_few<32, 3, 1, false, MODE, TO, GROUPED>(c, a, s) : f8_few<64, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
     } else {
         if constexpr (!GROUPED)
             if (a.plain) return f8_few<16, 5, 4, true, MODE, TO, false>(c, a, s);
         if (per == 16) return f8_few<16, 5, 4, false, MODE, TO, GROUPED>(c, a, s);
-        if (per == 32) return f8_few<32, 5, 2, false, MODE, TO, GROUPED>(c, a, s);
-        if constexpr (!GROUPED) return f8_few<64, 4, 2, false, MODE, TO, GROUPED>(c, a, s);
+        if constexpr (!GROUPED) return per == 32 ? f8_few<32, 5, 2, false, MODE, TO, GROUPED>(c, a, s) : f8_few<64, 4, 2, false, MODE, TO, GROUPED>(c, a, s);
     }
-    return LLM_REFUSED_SIZE;                                      // items have 16, 32 or 256 rows
+    return LLM_REFUSED_SIZE;                                      // items have 16, 128 or 256 rows
 }
 
 extern "C" int llm_f8_weight_size() { return static_cast<int>(sizeof(F8Weight)); }
@@ -1240,11 +1261,11 @@ static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UN
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
 // middle's rows, the experts' results.
-// Rows of an item, by how many picks an expert has on average: fewer fit most experts' picks into one item, whose weights are read once.  Measured (us): 64 experts, 8 a
-// token, 1,024 by 2,048, 6 picks an expert 79 (16), 86 (32), 125 (256); 10: 94, 93; 12: 99, 95, 136; 24: 126, 118, 140; 32: 127 (32), 143 (256); 48: 153, 142; 96: 241, 162.  8 experts, 2 a token,
-// 2,048 by 4,096, 8: 48, 50, 68; 12: 55, 54; 24: 59, 65, 70; 40: 69, 73; 64: 97, 76; 1,450 by 1,358, 12: 29, 31, 45; 24: 31, 32, 46; 48: 38, 46; 96: 58, 48.  Items of 64 rows come out
-// between the latter two, or up to a tenth before both where experts are few and large.
-static int f8_item_rows(long long picks, int E) { return picks <= 10LL * E ? 16 : picks <= 40LL * E ? 32 : 256; }
+// Rows of an item, by how many picks an expert has on average.  Measured, with 16, 128 and 256 rows (us): 64 experts, 8 a token, 1,024 by 2,048, 6 picks an expert 79 (16), 12: 99, 96, 129;
+// 24: 126, 104, 142; 64: 112 and 150; 128: 145, 174; 256: 226, 242; 512: 384, 375.  8 experts, 2 a token, 2,048 by 4,096, 12: 55, 52, 69; 24: 59, 53, 69; 64: 57, 77; 128: 86, 82; 256: 119, 115;
+// 512: 172, 174; 1,450 by 1,358, 12: 29, 37, 45; 24: 31, 38, 46; 64: 39, 46; 128: 42, 50; 256: 57, 57.  Items of 32 rows come out between 16 and 128 (8 experts, 12 picks: 31, 54; 40: 37, 68), those of 64
+// behind.
+static int f8_item_rows(long long picks, int E) { return picks <= 16LL * E ? 16 : picks <= 256LL * E ? 128 : 256; }
 static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
 struct F8Work {
     int per, room;

@@ -144,6 +144,48 @@ def test_a_token_alone_gives_what_it_gives_among_others(E, top, ff, W):
                 assert torch.equal(got, o.moe_f8(x[part], G, D, ids[part], weights[part], base=base[part], on_input=on_input))
 
 
+@pytest.mark.parametrize("T", [1, 5, 11, 20, 41, 50, 64, 65, 100, 130, 200, 300])
+def test_one_expert_is_a_feed_forward(T):
+    """A stack of one expert that every token picks with weight one, against the same matrices' products."""
+    o, g = ops(), gen(T)
+    ff, W = 264, 520
+    up, down = normal(g, 2 * ff, W) * W ** -0.5, normal(g, W, ff) * ff ** -0.5
+    x = normal(g, T, W, dtype=BF16)
+    ids, weights = torch.zeros(T, 1, dtype=torch.int32, device=DEV), torch.ones(T, 1, device=DEV)
+    got = o.moe_f8(x, o.f8_weight(up[None], gated=True), o.f8_weight(down[None]), ids, weights)
+    want = o.linear_f8(o.linear_silu_mul_f8(x, o.f8_weight(up, gated=True)), o.f8_weight(down))
+    # K may be cut otherwise: the sums' order; a code may then be another, 2^-3 of a value of the middle
+    assert float((got - want).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+    # one code in 2^14, or one of these few, a step off, twice its share of the norm
+    assert float((got - want).norm()) <= 2 * 2.0 ** -3 * max(2.0 ** -14, 1.0 / (T * ff)) ** 0.5 * float(want.norm())
+
+
+@pytest.mark.parametrize("T", [33, 64, 65, 100, 128, 300])
+def test_rows_of_wide_weights(T):
+    """Tiles of 128 rows by one CTA: more tiles of weights than there are SMs, results of any alignment and added ones; up features that lie in two blocks."""
+    from test_blocks_f8_gpu import blocks, flat, half_step, middle, near, product
+    o, g = ops(), gen(T + 7)
+    for N, K in ((19201, 200), (20480, 1024)):
+        W, x = o.f8_weight(normal(g, N, K) * K ** -0.5), normal(g, T, K, dtype=BF16)
+        X = o.f8_rows(x)
+        want, carried = product(X.values(F32), W.values(F32))
+        got = o.linear_f8(X, W)
+        assert bool(((got.to(F64) - want).abs() <= near(K, carried)).all())
+        assert torch.equal(o.linear_f8(x, W), got) and torch.equal(o.linear_f8(X, W, BF16), got.to(BF16))
+        stream = normal(g, T, N)
+        total = stream + got
+        assert o.linear_f8(X, W, residual=stream) is stream and torch.equal(stream, total)
+    for N, K in ((9700, 200), (10240, 640)):
+        W, X = o.f8_weight(normal(g, 2 * N, K) * K ** -0.5, gated=True), o.f8_rows(normal(g, T, K, dtype=BF16))
+        y, carried = product(X.values(F32), W.values(F32))
+        gate, up, off = y[:, :N], y[:, N:], near(K, carried)
+        want = middle(gate, up, 0, 0.0)
+        slack = 1.7 * (off[:, :N] * (up.abs() + 1) + off[:, N:] * gate.abs()) + 32 * 2.0 ** -24 * (gate.abs() + 1) * (up.abs() + 1)
+        bound = half_step(want) * (1 + 2.0 ** -16) + 1.1 * slack + flat(blocks(slack, 1).amax(dim=3, keepdim=True).expand(-1, -1, -1, 128), T, N) * 2.0 ** -4
+        assert bool(((o.linear_silu_mul_f8(X, W).values(F32).to(F64) - want).abs() <= bound).all())
+    assert o.stream_status(torch.device(DEV)).tolist() == [0, 0]
+
+
 def test_another_stream_and_a_wrong_operand():
     o, g = ops(), gen(4)
     W = o.f8_weight(normal(g, 300, 520))
@@ -161,10 +203,11 @@ def test_another_stream_and_a_wrong_operand():
             call()
 
 
-#: (T, N, K, gated, a matrix that the product takes to 8 bits itself): tiles of 16, 32 and 64 rows with K whole and cut, pairs of CTAs with one tile and several
+#: (T, N, K, gated, a matrix that the product takes to 8 bits itself): tiles of 16, 32 and 64 rows with K whole and cut, CTAs of 128 rows, pairs of CTAs with one
+#: tile and several
 SIZES = [(4, 4096, 4096, False, False), (4, 512, 2048, True, False), (3, 1000, 4104, False, True), (16, 700, 12288, True, True), (30, 1024, 4096, False, False),
          (64, 12288, 1024, False, False), (64, 512, 4096, True, False), (250, 700, 4096, False, False), (2000, 4096, 1024, False, False), (2000, 4096, 640, True, False),
-         (2000, 2050, 640, True, False), (600, 4096, 4096, False, False), (700, 4001, 1024, False, False), (4, 128, 65536, False, False), (40, 200, 65536, False, False)]
+         (2000, 2050, 640, True, False), (600, 4096, 4096, False, False), (700, 4001, 1024, False, False), (100, 20480, 512, False, False), (100, 10240, 512, True, False), (4, 128, 65536, False, False), (40, 200, 65536, False, False)]
 #: tries of a wait: from none to enough for most waits, so that products stop in front of their first stage, among the stages, and not at all
 TRIES = [0, 1, 2, 3] + [2 ** n for n in range(2, 14)]
 
