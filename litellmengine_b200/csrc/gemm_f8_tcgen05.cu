@@ -85,7 +85,7 @@ enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
 // the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.  Measured, so and with a launch
 // for the rows (us): 4,096 by 6,144, a row 6.8 and 7.5, 8 rows 7.8 and 8.1, 16 rows 9.0 and 8.4; 12,288 by 4,096 10.1 and 11.1, 10.9 and 11.5, 12.8 and 12.0; gated, 4,096 by 2 x 12,288, a row
 // 20.1 and 19.3, 4 rows 20.0 and 19.6, 8 rows 21.3 and 19.7; 2,048 by 2 x 1,024 5.06 and 5.19, 5.25 and 5.26, 5.7 and 5.5.
-// Measured (us): a row of 4,096 by 6,144 6.95 (25 MB, 3.6 TB/s); 8 rows of 8 bits, 12,288 by 4,096, 10.2 (50 MB, 5.0 TB/s), 4,096 by 24,576 18.0 (101 MB, 5.6 TB/s); gated, 8 rows of
+// Measured (us): a row of 4,096 by 6,144 6.8 (25 MB, 3.7 TB/s); 8 rows of 8 bits, 12,288 by 4,096, 10.1 (50 MB, 5.0 TB/s), 4,096 by 24,576 17.7 (101 MB, 5.7 TB/s); gated, 8 rows of
 // 4,096 by 2 x 12,288 18.7 (5.4 TB/s); 48 tokens' picks, 8 of 64 experts, 1,024 by 2,048 80 (5.0 TB/s of the weights) with their sorting.  Three CTAs an SM with three
 // stages for the latter, so that more of them begin while others end, came out 84 to 88 there and slower for 8 large experts (49 instead of 45 us).
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED>

@@ -186,6 +186,18 @@ def test_rows_of_wide_weights(T):
     assert o.stream_status(torch.device(DEV)).tolist() == [0, 0]
 
 
+@pytest.mark.parametrize("T,E,top,ff,W", [(1, 16, 12, 96, 264), (2, 40, 9, 264, 520), (3, 20, 20, 130, 136), (4, 4097, 2, 8, 16), (300, 24, 17, 96, 264), (4300, 8, 8, 64, 136)])
+def test_more_picks_and_experts(T, E, top, ff, W):
+    """More picks a token than a cluster adds up, more than are in flight together, more tokens than the sorting keeps in registers; more experts than a call routes to are refused."""
+    from test_blocks_f8_gpu import test_experts
+    if E <= 4096:
+        return test_experts(T, E, top, ff, W, "silu", 0.0, False)
+    o, g = ops(), gen(E)
+    G, D = o.f8_weight(normal(g, E, 2 * ff, W), gated=True), o.f8_weight(normal(g, E, W, ff))
+    with pytest.raises(o.KernelError):
+        o.moe_f8(normal(g, T, W, dtype=BF16), G, D, torch.zeros(T, top, dtype=torch.int32, device=DEV), torch.ones(T, top, device=DEV))
+
+
 def test_another_stream_and_a_wrong_operand():
     o, g = ops(), gen(4)
     W = o.f8_weight(normal(g, 300, 520))
