@@ -387,9 +387,9 @@ extern "C" int llm_f8_sort(const int32_t* ids, const float* weights, int picks, 
     return launch_status();
 }
 
-// out[token] = base[token] + the token's rows of y in the order of its choices, in 32 bits.
-template <typename TY, typename TO>
-__global__ void __launch_bounds__(128) f8_add_up_kernel(const TY* y, const int32_t* places, TO* out, int N, int top, int vec,
+// out[token] = base[token] + the token's rows of y in the order of its choices, in 32 bits; rounded to the result's type once.
+template <typename TO>
+__global__ void __launch_bounds__(128) f8_add_up_kernel(const float* y, const int32_t* places, TO* out, int N, int top, int vec,
                                                         const float* base) {
     pdl_begin();
     const size_t t = blockIdx.x;
@@ -417,24 +417,24 @@ __global__ void __launch_bounds__(128) f8_add_up_kernel(const TY* y, const int32
             float sum = base ? base[t * N + i] : 0.0f;
             for (int k = 0; k < top; ++k) {
                 const int r = places[t * top + k];
-                if (r >= 0) sum += to_f32(y[static_cast<size_t>(r) * N + i]);
+                if (r >= 0) sum += y[static_cast<size_t>(r) * N + i];
             }
             out[t * N + i] = from_f32<TO>(sum);
         }
     }
 }
 
-// y [rows, N] and out [T, N] of one dtype; base (float32 [T, N]) may be null.
-extern "C" int llm_f8_add_up(const void* y, int dtype, const int32_t* places, const float* base, void* out, int T, int N, int top, uintptr_t stream) {
+// y [rows, N] in float32, out [T, N] of `dtype`; base (float32 [T, N]) may be null.
+extern "C" int llm_f8_add_up(const float* y, const int32_t* places, const float* base, void* out, int dtype, int T, int N, int top, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
     if (N <= 0 || N > (1 << 24) || top <= 0) return LLM_REFUSED_SIZE;
     const int vec = N % 8 == 0 && aligned16(y) && aligned16(out) && aligned16(base);
     const dim3 grid(T, (N + 1023) / 1024);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == LLM_DT_F32)
-        launch_pdl((f8_add_up_kernel<float, float>), grid, dim3(128), 0, s, static_cast<const float*>(y), places, static_cast<float*>(out), N, top, vec, base);
+        launch_pdl((f8_add_up_kernel<float>), grid, dim3(128), 0, s, y, places, static_cast<float*>(out), N, top, vec, base);
     else if (dtype == LLM_DT_BF16)
-        launch_pdl((f8_add_up_kernel<bf16, bf16>), grid, dim3(128), 0, s, static_cast<const bf16*>(y), places, static_cast<bf16*>(out), N, top, vec, base);
+        launch_pdl((f8_add_up_kernel<bf16>), grid, dim3(128), 0, s, y, places, static_cast<bf16*>(out), N, top, vec, base);
     else
         return LLM_REFUSED_DTYPE;
     return launch_status();

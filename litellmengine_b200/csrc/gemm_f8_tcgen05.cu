@@ -1260,7 +1260,7 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
 static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UNSORTED_TOKENS && top <= 8; }
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
-// middle's rows, the experts' results.
+// middle's rows, the experts' results in float32 (none where the picks stay as they are).
 // Rows of an item, by how many picks an expert has on average.  Measured, with 16, 128 and 256 rows (us): 64 experts, 8 a token, 1,024 by 2,048, 6 picks an expert 79 (16), 12: 99, 96, 129;
 // 24: 126, 104, 142; 64: 112 and 150; 128: 145, 174; 256: 226, 242; 512: 384, 375.  8 experts, 2 a token, 2,048 by 4,096, 12: 55, 52, 69; 24: 59, 53, 69; 64: 57, 77; 128: 86, 82; 256: 119, 115;
 // 512: 172, 174; 1,450 by 1,358, 12: 29, 37, 45; 24: 31, 38, 46; 64: 39, 46; 128: 42, 50; 256: 57, 57.  Items of 32 rows come out between 16 and 128 (8 experts, 12 picks: 31, 54; 40: 37, 68), those of 64
@@ -1271,7 +1271,7 @@ struct F8Work {
     int per, room;
     long long counts, places, weights, x, middle, y, all;
 };
-static F8Work f8_work(int T, int top, int E, int W, int ff, bool plain, int out_dtype) {
+static F8Work f8_work(int T, int top, int E, int W, int ff, bool plain) {
     const long long picks = static_cast<long long>(T) * top;
     F8Work k = {};
     k.per = f8_unsorted(T, top, plain) ? 16 : f8_item_rows(picks, E);
@@ -1283,15 +1283,15 @@ static F8Work f8_work(int T, int top, int E, int W, int ff, bool plain, int out_
     k.x = k.weights + f8_up(4 * picks);
     k.middle = k.x + (f8_unsorted(T, top, plain) ? 0 : f8_up(rows_bytes(W)));
     k.y = k.middle + f8_up(rows_bytes(ff));
-    k.all = k.y + picks * W * (out_dtype == LLM_DT_F32 ? 4 : 2);
+    k.all = k.y + (f8_unsorted(T, top, plain) ? 0 : picks * W * 4);
     return k;
 }
 static bool f8_plain_experts(const void* x, int dtype, int W) { return dtype == LLM_DT_BF16 && W % 8 == 0 && aligned16(x); }
-extern "C" long long llm_moe_f8_work(const void* x, int dtype, int T, int top, int E, int W, int ff, int out_dtype) {
-    return f8_work(T, top, E, W, ff, f8_plain_experts(x, dtype, W), out_dtype).all;
+extern "C" long long llm_moe_f8_work(const void* x, int dtype, int T, int top, int E, int W, int ff) {
+    return f8_work(T, top, E, W, ff, f8_plain_experts(x, dtype, W)).all;
 }
 extern "C" int llm_f8_sort(const int32_t*, const float*, int, int, int, int32_t*, void*, int32_t*, float*, uintptr_t);
-extern "C" int llm_f8_add_up(const void*, int, const int32_t*, const float*, void*, int, int, int, uintptr_t);
+extern "C" int llm_f8_add_up(const float*, const int32_t*, const float*, void*, int, int, int, int, uintptr_t);
 extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, int dtype, const int32_t* ids, const float* weights, int T, int top, void* work,
                           const float* base, void* out, int out_dtype, int act, float limit, int on_input, int waits, int32_t* status, uintptr_t stream) {
     if (T <= 0) return LLM_OK;
@@ -1302,7 +1302,7 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     if (!g || !d || g->E != d->E || g->E > F8_MOST_EXPERTS || g->N != d->K || g->K != d->N) return LLM_REFUSED_SIZE;
     const int picks = T * top, W = g->K, ff = g->N;
     const bool plain = f8_plain_experts(x, dtype, W), unsorted = f8_unsorted(T, top, plain);
-    const F8Work k = f8_work(T, top, g->E, W, ff, plain, out_dtype);
+    const F8Work k = f8_work(T, top, g->E, W, ff, plain);
     unsigned char* at = static_cast<unsigned char*>(work);
     int32_t *counts = reinterpret_cast<int32_t*>(at + k.counts), *places = reinterpret_cast<int32_t*>(at + k.places);
     float* row_weights = reinterpret_cast<float*>(at + k.weights);
@@ -1329,8 +1329,10 @@ extern "C" int llm_moe_f8(const void* gate_up, const void* down, const void* x, 
     if (on_input) a.groups.weights = nullptr;
     a.base = base;
     const F8Call c = {d, at + k.middle, unsorted ? T : k.room};
-    if (const int rc = out_dtype == LLM_DT_F32 ? f8_way<F8_STORE, float, true>(c, a, k.per, s) : f8_way<F8_STORE, bf16, true>(c, a, k.per, s)) return rc;
-    return unsorted ? LLM_OK : llm_f8_add_up(at + k.y, out_dtype, places, base, out, T, W, top, stream);
+    if (unsorted && out_dtype == LLM_DT_BF16) return f8_few<16, 5, 4, false, F8_STORE, bf16, true>(c, a, s);
+    // Rows stay float32 until a token's are added up, whatever the result's type: picks as they are have their sum rounded once too.
+    if (const int rc = f8_way<F8_STORE, float, true>(c, a, k.per, s)) return rc;
+    return unsorted ? LLM_OK : llm_f8_add_up(reinterpret_cast<const float*>(at + k.y), places, base, out, out_dtype, T, W, top, stream);
 }
 // Kernels that llm_moe_f8 launches.
 extern "C" int llm_moe_f8_launches(const void* x, int dtype, int T, int top, int W) { return f8_unsorted(T, top, f8_plain_experts(x, dtype, W)) ? 2 : 5; }

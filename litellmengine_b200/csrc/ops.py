@@ -2801,8 +2801,8 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
     `w_down` a stack [E, W, ff], `ids` (int32) and `weights` (float32) [T, top] from `moe_route` (an id that is none of 0 .. E - 1: a pick without an expert).
     The picks are sorted by expert on the device (those of up to four tokens stay as they are: two launches), each expert's rows go through its own matrices as in
     `linear_silu_mul_f8` and `linear_f8`, and a token's rows are added up in float32 in the order of its choices, times their weights (`on_input`: the weight multiplies the expert's input, that is
-    its gate and up values, instead), onto `base` (float32 [T, W]) where there is one.  The result is float32 or bfloat16 [T, W]; for bfloat16 the experts' rows
-    are rounded to it before they are added up, as `moe_sorted` rounds its."""
+    its gate and up values, instead), onto `base` (float32 [T, W]) where there is one.  The result is float32 or bfloat16 [T, W],
+    rounded to that once."""
     act = ACTIVATIONS[activation]
     _here(x, ids, weights, base)
     _i32(ids, "ids")
@@ -2823,10 +2823,10 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
     if T == 0:
         return out
     top = ids.shape[1]
-    key = (T, top, E, W, ff, dt, od, x.data_ptr() % 16)
+    key = (T, top, E, W, ff, dt, x.data_ptr() % 16)
     sizes = _f8_sizes.get(key)
     if sizes is None:
-        work = _fn("blocks_f8", "llm_moe_f8_work", [_P, _I, _I, _I, _I, _I, _I, _I], c_longlong)(x.data_ptr(), dt, T, top, E, W, ff, od)
+        work = _fn("blocks_f8", "llm_moe_f8_work", [_P, _I, _I, _I, _I, _I, _I], c_longlong)(x.data_ptr(), dt, T, top, E, W, ff)
         launches = _fn("blocks_f8", "llm_moe_f8_launches", [_P, _I, _I, _I, _I])(x.data_ptr(), dt, T, top, W)
         if len(_f8_sizes) > 4096:
             _f8_sizes.clear()
