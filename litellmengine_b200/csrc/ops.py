@@ -2137,6 +2137,8 @@ def linear_mid(x: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype, ac
 
 
 _stream_status: Dict[str, torch.Tensor] = {}
+# What codes in that word mean that only products write, beside those that the runner lists with the codes of a step's word.
+STREAM_STATUS_TEXT = {10: "a wait on a barrier in a product of 8 bits (dense, gated or of routed experts) ran out"}
 
 
 def stream_status(device) -> torch.Tensor:

@@ -274,4 +274,5 @@ class ModelRunner:
             code, where = word.tolist()
             if code:
                 word.zero_()
-                raise RuntimeError(f"device status {code}: {STATUS_TEXT.get(code, 'unknown')} (at index {where})")
+                text = STATUS_TEXT.get(code) or ops.STREAM_STATUS_TEXT.get(code, "unknown")
+                raise RuntimeError(f"device status {code}: {text} (at index {where})")
