@@ -2599,6 +2599,7 @@ def _mx_count() -> None:
 F8_BLOCK = 128
 # Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself; one of gate and up.
 F8_PLAIN_ROWS, F8_PLAIN_ROWS_GATED = 8, 4
+F8_MOST_EXPERTS = 4096                    # that `moe_f8` routes to
 _MX_SIGNATURES.update({
     "llm_f8_rows": ("blocks_f8", [_P, _I, _P, _L, _I, _I, _P, _I, _P]),
     "llm_f8_weight": ("blocks_f8", [_P, _I, _P, _P, _I, _I, _I, _I, _I, _L, _L, _P]),
@@ -2813,6 +2814,8 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
     _here(w_gate_up.buffer, w_down.buffer)
     E, two_ff, W = w_gate_up.shape
     ff = two_ff // 2
+    if E > F8_MOST_EXPERTS:
+        raise KernelError(f"moe_f8 routes to {F8_MOST_EXPERTS} experts at most, not {E}")
     if w_down.shape != (E, W, ff) or x.dim() != 2 or x.shape[1] != W:
         raise KernelError("x and the experts' matrices disagree")
     T = x.shape[0]

@@ -214,7 +214,10 @@ class RoutedExperts:
         ops.prepare_streaming(self.w_down)
 
     def hold_in_8_bits(self) -> int:
-        """From now on the experts' matrices are stacks in 8 bits (`ops.F8Weight`), and the shared expert's are too.  How many matrices that are."""
+        """From now on the experts' matrices are stacks in 8 bits (`ops.F8Weight`), and the shared expert's are too.  How many matrices that are.
+        More experts than `ops.moe_f8` routes to are refused here, with the stored matrices as they were."""
+        if self.E > ops.F8_MOST_EXPERTS:
+            raise ValueError(f"weight_format 'fp8': {self.E} routed experts in a layer, and {ops.F8_MOST_EXPERTS} is the most that it takes")
         rows, ff = self.E * 2 * self.ff, self.ff
         if self.joined is not None:
             self.w_shared_gate_up, self.w_shared_down = ops.f8_weight(self.w_gate_up[rows:]), ops.f8_weight(self.w_shared_down)
