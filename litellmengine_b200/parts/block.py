@@ -198,9 +198,20 @@ class Block:
         name = self.HOLDS.get(weight_format)
         return [p for p in self.parts() if name is not None and speaks_for_forward(p, name)]
 
-    def load(self, tensors: Dict[str, torch.Tensor], weight_format: str = "stored") -> int:
-        """Bind the tensors; the matrices of `parts_that_hold(weight_format)` are held so from then on (how many those were)."""
+    def parts_in_4_bits(self):
+        """Those of 'mxfp4'."""
+        return self.parts_that_hold("mxfp4")
+
+    def load(self, tensors: Dict[str, torch.Tensor], weight_format: str = "stored", in_4_bits: bool = False) -> int:
+        """Bind the tensors; the matrices of `parts_that_hold(weight_format)` are held so from then on (how many those were).  `in_4_bits`, or a truth
+        value in the format's place: 'mxfp4' or 'stored'."""
         from ..csrc import ops
+        if isinstance(weight_format, bool):
+            in_4_bits, weight_format = weight_format, "stored"
+        if in_4_bits:
+            if weight_format not in ("stored", "mxfp4"):
+                raise ValueError(f"in_4_bits and weight_format {weight_format!r}")
+            weight_format = "mxfp4"
         converted = self.parts_that_hold(weight_format)
         for prefix, part in self._children():
             mine = {n[len(prefix) + 1:]: t for n, t in tensors.items() if n.startswith(prefix + ".")}
