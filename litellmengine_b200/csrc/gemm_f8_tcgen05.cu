@@ -433,7 +433,9 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
                 most = __reduce_max_sync(0xffffffffu, most);
                 const F8Scale s = f8_scale(most);
                 if (!__any_sync(0xffffffffu, quit)) {
-                    *reinterpret_cast<unsigned*>(codes + (block * a.y_rows + row0 + r) * F8_K + f) = mx_e4m3x4(v[0] * s.inverse, v[1] * s.inverse, v[2] * s.inverse, v[3] * s.inverse);
+                    float q[4] = {v[0] * s.inverse, v[1] * s.inverse, v[2] * s.inverse, v[3] * s.inverse};
+                    f8_settle(q, v, most);
+                    *reinterpret_cast<unsigned*>(codes + (block * a.y_rows + row0 + r) * F8_K + f) = mx_e4m3x4(q[0], q[1], q[2], q[3]);
                     if (lane == 0) a.y_scales[(row0 + r) * static_cast<long long>(a.y_k4) + block] = s.scale;
                 }
             }
@@ -937,7 +939,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) f8_pair_kernel(const __grid_con
                     for (int i = 0; i < 4; ++i) {
                         unsigned c[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
+                        for (int j = 0; j < 4; ++j) {             // not settled (f8_blocks.cuh): 2,045 rows of 4,096 by 2 x 12,288 217 to 223 us with it, 4,096 of 1,024 by 2 x 4,096 46 to 51
                             const float* q = v + 16 * i + 4 * j;
                             c[j] = mx_e4m3x4(q[0] * s.inverse, q[1] * s.inverse, q[2] * s.inverse, q[3] * s.inverse);
                         }
