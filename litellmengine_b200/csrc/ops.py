@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import threading
 import weakref
 from ctypes import c_float, c_int, c_int32, c_longlong, c_uint32, c_uint64, c_void_p
 from typing import Dict, Optional
@@ -2653,6 +2654,9 @@ class F8Rows:
         return out
 
 
+_f8_describing = threading.Lock()
+
+
 class F8Weight:
     """A weight [N, K], or a stack of them [E, N, K], in 8 bits (e4m3) with a float32 scale per block of 128 x 128 values, stored tile by
     tile.  Made by `f8_weight`; `gated`: it is [gate; up], gate and up rows stored beside each other for `linear_silu_mul_f8`; the values are
@@ -2691,14 +2695,17 @@ class F8Weight:
         """The address, on the host, of what the kernels' launches need to know of the weight: put together once, for its address on the device."""
         at, known = self.buffer.data_ptr(), self.__dict__.get("_described")
         if known is None or known[0] != at:
-            size = _mx_call("llm_f8_weight_size")()
-            room = ctypes.create_string_buffer(size + 64)
-            here = (ctypes.addressof(room) + 63) // 64 * 64
-            N, K = self.shape[-2:]
-            code = _mx_call("llm_f8_describe")(here, at, at + self.scales_behind, self.experts, N // 2 if self.gated else N, K, int(self.gated))
-            if code:
-                raise KernelError(f"a weight in 8 bits that no product takes: {_REFUSALS.get(code, code)}")
-            known = self._described = (at, here, room)
+            with _f8_describing:                  # one thread's: a second description would take the first one's room from under a call that has its address
+                known = self.__dict__.get("_described")
+                if known is None or known[0] != at:
+                    size = _mx_call("llm_f8_weight_size")()
+                    room = ctypes.create_string_buffer(size + 64)
+                    here = (ctypes.addressof(room) + 63) // 64 * 64
+                    N, K = self.shape[-2:]
+                    code = _mx_call("llm_f8_describe")(here, at, at + self.scales_behind, self.experts, N // 2 if self.gated else N, K, int(self.gated))
+                    if code:
+                        raise KernelError(f"a weight in 8 bits that no product takes: {_REFUSALS.get(code, code)}")
+                    known = self._described = (at, here, room)
         return known[1]
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
