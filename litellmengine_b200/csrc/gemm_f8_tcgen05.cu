@@ -1263,11 +1263,12 @@ static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UN
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
 // work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
 // middle's rows, the experts' results in float32 (none where the picks stay as they are).
-// Rows of an item, by how many picks an expert has on average.  Measured, with 16, 128 and 256 rows (us): 64 experts, 8 a token, 1,024 by 2,048, 6 picks an expert 79 (16), 12: 99, 96, 129;
-// 24: 126, 104, 142; 64: 112 and 150; 128: 145, 174; 256: 226, 242; 512: 384, 375.  8 experts, 2 a token, 2,048 by 4,096, 12: 55, 52, 69; 24: 59, 53, 69; 64: 57, 77; 128: 86, 82; 256: 119, 115;
-// 512: 172, 174; 1,450 by 1,358, 12: 29, 37, 45; 24: 31, 38, 46; 64: 39, 46; 128: 42, 50; 256: 57, 57.  Items of 32 rows come out between 16 and 128 (8 experts, 12 picks: 31, 54; 40: 37, 68), those of 64
-// behind.
-static int f8_item_rows(long long picks, int E) { return picks <= 16LL * E ? 16 : picks <= 256LL * E ? 128 : 256; }
+// Rows of an item, by how many picks an expert has on average.  Measured, with 16, 128 and 256 rows (us): 64 experts, 8 a token, 1,024 by 2,048, 6 picks an expert 85, 99, 130; 12: 101, 106,
+// 143; 24: 129, 114, 153; 64: 240, 122, 163; 128 (128 and 256 rows): 156, 175; 256: 246, 269; 375: 334, 343; 512: 434, 440; 1,024: 789, 762.  8 experts, 2 a token, 2,048 by 4,096, 12: 49, 55, 73; 24: 59, 55,
+// 75; 40: 82, 58, 77; 64: 102, 61, 81; 256: 128, 125; 512: 183, 191; 750: 264, 267; 1,024: 346, 321; 2,048: 641, 605; 1,450 by 1,358, 12: 29, 38, 47; 24: 32, 37, 46; 40: 33, 38; 64: 49, 39, 48; 512: 91, 91; 1,024:
+// 135, 133; 512 by 1,024, 24: 20, 23; 64: 23, 26; 256: 54, 30, 31.  4 experts, 1 a token, 4,096 by 2,048, 512: 96, 106; 1,024: 172, 158.  The rule looks at picks alone: with 17 to 64 of them, small matrices would
+// take 10 to 15 % less by items of 16 rows, large ones take 7 to 50 % less as it is.  Items of 32 rows come out between 16 and 128, those of 64 behind.
+static int f8_item_rows(long long picks, int E) { return picks <= 16LL * E ? 16 : picks <= 768LL * E ? 128 : 256; }
 static long long f8_up(long long n) { return (n + 255) / 256 * 256; }
 struct F8Work {
     int per, room;

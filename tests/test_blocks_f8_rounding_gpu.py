@@ -22,7 +22,8 @@ def normal(g, *shape, dtype=F32):
 
 #: picks as they are (up to 4 tokens), and sorted into items of 16, 128 and 256 rows; results of whole, aligned pieces of eight values, of four, and of any size
 ROUNDED_ONCE = [(1, 64, 8, 64, 128), (4, 8, 2, 72, 136), (4, 8, 2, 130, 131), (2, 12, 9, 64, 128), (5, 64, 8, 64, 128), (17, 8, 2, 192, 520), (48, 64, 8, 128, 256),
-                (130, 3, 1, 200, 393), (301, 8, 2, 450, 358), (600, 5, 5, 256, 640), (90, 2, 2, 64, 12), (2000, 2, 1, 257, 515)]
+                (130, 3, 1, 200, 393), (301, 8, 2, 450, 358), (600, 5, 5, 256, 640), (90, 2, 2, 64, 12), (2000, 2, 1, 257, 515),
+                (2000, 2, 1, 256, 512), (900, 3, 3, 130, 264)]
 
 
 @pytest.mark.parametrize("T,E,top,ff,W", ROUNDED_ONCE)
