@@ -15,7 +15,7 @@
 
 // ---- rows from a matrix ---------------------------------------------------------------------------------------------
 // Sixteen lanes a block of a row, eight values a lane (16 or 32 bytes); a warp takes U times two blocks, all asked for before the first is used.
-// Measured: 4,096 rows of 12,288 in bfloat16 31.2 us (151 MB, 4.8 TB/s), of 4,096 11.5 us, 24 rows of 12,288 1.5 us.
+// Measured: 4,096 rows of 12,288 in bfloat16 31.2 us (151 MB, 4.8 TB/s), of 4,096 11.5 us, 24 rows of 12,288 1.5 us; in float32 49 us (252 MB, 5.1 TB/s), 18.4, 2.0.
 template <typename T> struct F8Raw { typedef uint4 type; };
 template <> struct F8Raw<float> { struct type { float v[8]; }; };
 __device__ __forceinline__ unsigned f8_most(const uint4& r) { return mx_most8(r); }
@@ -117,8 +117,8 @@ extern "C" int llm_f8_rows(const void* x, int dtype, void* rows, long long padde
 
 // ---- weights --------------------------------------------------------------------------------------------------------
 // A CTA a block of 128 x 128: sixteen lanes a row, two rows a warp and trip, eight trips that are asked for together.  It does not invite the kernel behind
-// it: products fetch weights before they wait for what is in front of them.  12,288 x 4,096 in bfloat16 26.6 us (151 MB, 5.7 TB/s); 1,003 x 1,358 in float32 5.9 us, 88 CTAs
-// and bound by latency.
+// it: products fetch weights before they wait for what is in front of them.  12,288 x 4,096 in bfloat16 26.4 us (151 MB, 5.7 TB/s), in float32 46.3 (252 MB, 5.4 TB/s); 1,003 x 1,358 in float32 4.6
+// us, 88 CTAs and bound by latency.
 template <int VEC, typename T>
 __global__ void __launch_bounds__(F8_THREADS) f8_weight_kernel(const T* w, unsigned char* codes, float* scales, int rows, int K,
                                                                int tiles, int ktiles, int k4, int gate_rows, long long row_stride, long long matrix_stride) {
@@ -285,7 +285,7 @@ extern "C" int llm_f8_values(const void* codes, const void* scales, void* out, i
 // ---- rows sorted by expert ------------------------------------------------------------------------------------------
 // A cluster (of one CTA for few picks) counts the picks of each expert, lays the experts' rows one after another, cuts them into items of up to `per` rows, and
 // gives every pick its row: places[pick] (-1 where the pick is no expert), weights[row].  A CTA takes neighbouring picks and adds up the counts of those
-// before it out of their shared memory: 32,768 picks of 64 experts 52 us by one CTA, 9 by eight.  Which of an expert's rows a pick gets is not fixed; no result depends on it,
+// before it out of their shared memory: 32,768 picks of 64 experts 52 us by one CTA, 9 to 12 by eight.  Which of an expert's rows a pick gets is not fixed; no result depends on it,
 // a row's products being its own.
 #define F8_SORT_CTAS 8
 #define F8_SORT_PICKS 4           // picks of a thread that stay in registers
@@ -388,6 +388,7 @@ extern "C" int llm_f8_sort(const int32_t* ids, const float* weights, int picks, 
 }
 
 // out[token] = base[token] + the token's rows of y in the order of its choices, in 32 bits; rounded to the result's type once.
+// 4,096 tokens of eight rows of 2,048: 45 us (285 MB, 6.3 TB/s), into float32 47.
 template <typename TO>
 __global__ void __launch_bounds__(128) f8_add_up_kernel(const float* y, const int32_t* places, TO* out, int N, int top, int vec,
                                                         const float* base) {

@@ -11,7 +11,8 @@
 //   * Gate and up: act(gate) * up leaves as rows of 8 bits, 128 features a scale.
 //   * Rows sorted by expert: an item (up to a tile's rows of one expert) takes the place of a tile of rows; how many there are only the device knows.
 // Waits are bounded: one that runs out sets status code 10, and the copies and products that are under way then end, which is waited for on their own barriers
-// (bounded too), before the CTA does; what was not computed is neither stored nor added.
+// (bounded too), before the CTA does; what was not computed is neither stored nor added (routed experts' rows that were not are added up as the workspace has them:
+// the status says that the result is of no use).
 #include "f8_blocks.cuh"
 #include "tcgen05_attention.cuh"
 
@@ -83,11 +84,12 @@ enum { F8_STORE = 0, F8_ADD = 1, F8_GATED = 2 };
 // such groups at a time.  A CTA's tile is 128 features, gated 64 + 64 gate and as many up features, of two tiles of the weight.
 // Warp 0 feeds the weights, warp 1 issues, warps from 2 on take the sums, the last feeds the rows and their scales; or, PLAIN, x comes as a matrix and the last warps make
 // the rows of their part of K in shared memory: one launch and no rows in memory, for steps so short that every CTA can do it while its weights come.  Measured, so and with a launch
-// for the rows (us): 4,096 by 6,144, a row 6.8 and 7.5, 8 rows 7.8 and 8.1, 16 rows 9.0 and 8.4; 12,288 by 4,096 10.1 and 11.1, 10.9 and 11.5, 12.8 and 12.0; gated, 4,096 by 2 x 12,288, a row
-// 20.1 and 19.3, 4 rows 20.0 and 19.6, 8 rows 21.3 and 19.7; 2,048 by 2 x 1,024 5.06 and 5.19, 5.25 and 5.26, 5.7 and 5.5.
-// Measured (us): a row of 4,096 by 6,144 6.8 (25 MB, 3.7 TB/s); 8 rows of 8 bits, 12,288 by 4,096, 10.1 (50 MB, 5.0 TB/s), 4,096 by 24,576 17.7 (101 MB, 5.7 TB/s); gated, 8 rows of
-// 4,096 by 2 x 12,288 18.7 (5.4 TB/s); 48 tokens' picks, 8 of 64 experts, 1,024 by 2,048 80 (5.0 TB/s of the weights) with their sorting.  Three CTAs an SM with three
-// stages for the latter, so that more of them begin while others end, came out 84 to 88 there and slower for 8 large experts (49 instead of 45 us).
+// for the rows (us): 4,096 by 6,144, a row 6.8 and 7.5, 8 rows 7.8 and 8.1, 16 rows 9.0 and 8.4; 12,288 by 4,096 10.1 and 11.1, 10.9 and 11.5, 12.8 and 12.0; gated, a row and 4 rows, 2,048 by 2 x 1,024 4.5 and 5.3,
+// 4.7 and 5.3; 1,024 by 2 x 4,096 5.0 and 5.6, 5.3 and 5.8; 2,048 by 2 x 6,144 7.6 and 8.0, 8.2 and 8.3; 4,096 by 2 x 12,288 19.2 and 19.9, 19.7 and 19.7; 2,048 by 2 x 24,576 19.2 and 19.9, 19.4 and 19.5; with the
+// down product behind it the same or up to 1.1 less, but 1,024 by 2 x 2,560 and 2,560 by 2 x 9,728, up to 0.2 of 9 and 0.4 of 19 more.  8 gated rows: 2,048 by 2 x 1,024 5.7 and 5.5.
+// Measured (us): a row of 4,096 by 6,144 6.8 to 7.3 (25 MB, 3.5 TB/s); 8 rows of 8 bits, 12,288 by 4,096, 10.1 (50 MB, 5.0 TB/s), 4,096 by 24,576 17.7 (101 MB, 5.7 TB/s); gated, 8 rows of
+// 4,096 by 2 x 12,288 18.7 (5.4 TB/s); 48 tokens' picks, 8 of 64 experts, 1,024 by 2,048 86 (4.7 TB/s of the weights) with their sorting and adding up.  Three CTAs an SM with three
+// stages for the latter, so that more of them begin while others end, came out 84 to 88 there (85 to 90 with two, rows in bfloat16) and slower for 8 large experts (49 instead of 45 us).
 template <int NT, int WS, int G, bool PLAIN, int MODE, typename TO, bool GROUPED>
 __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1), F8_FEW_CTAS(NT, MODE == F8_GATED ? 2 : 1)) f8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                                          const F8Args a) {
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(F8_FEW_THREADS(PLAIN, MODE == F8_GATED ? 2 : 1
 // whether its accumulator is full) is asked for between additions.  Scales come by a warp's asynchronous copies, eight tiles of K at a time into a ring of two: loads of the
 // threads that need them would wait together with tcgen05.ld, whose wait is for all.
 // Measured: a tile of K takes 700 clocks, its products 512.  4,096 rows of 4,096 by 24,576: 380 to 410 us with the clocks that the power limit leaves (1.3 to 1.5 GHz), 2.0 to
-// 2.15 PFLOP/s; 1,024 rows by 4,096 21 us; gated, 2,045 rows of 4,096 by 2 x 12,288 205 to 220 us.  Two accumulators of 256 features, taken out and added in turns, made it 1,700 clocks a
+// 2.15 PFLOP/s; 1,024 rows by 4,096 21 to 22 us; gated, 2,045 rows of 4,096 by 2 x 12,288 205 to 220 us.  Two accumulators of 256 features, taken out and added in turns, made it 1,700 clocks a
 // tile of K.
 // The clusters are persistent: the copies go on into the next tile while the threads write a finished one.  Tiles are numbered row tile fastest: what runs at one time
 // shares few weights, and the rows stay in the second-level cache.  Of rows sorted by expert the features are fastest: an expert's rows and weights are few.
@@ -1154,9 +1156,9 @@ template <int MODE, typename TO, bool GROUPED, bool SPLIT, int CTAS> static int 
 // How a product of T rows by `tiles` of 128 of the weight's rows runs: the rows of a tile.  Up to 32 rows one tile of rows reads the weight once.  Tiles of 64 rows go on as long
 // as every tile of rows and weight has an SM to itself; K is cut where SMs are left, which the others do not do.  Of these, CTAs of 128 rows alone take 6/5 of the time that pairs of
 // 256 rows take for a tile of 256 features, but twice as many run at once: whoever needs less time for all.  Measured, rows of 8 bits, by tiles of 64, 128 and 256 (us): 64 rows of 4,096 by
-// 24,576 26.9, 23.6, 33.2; 65 by 6,144 15.0, 20.2, 16.9; 128 by 24,576 49, 24.5, 34.8; 197 by 6,144 26.1, 20.4, 17.4; 256 by 4,096 15.2, 20.2, 17.4; 256 rows of 12,288 by 4,096 35.6, 52.7, 42.6; 384 of
-// 4,096 by 24,576 107, 48.0, 55.7; 512 149, 64.6, 59.0; 1,024 by 4,096 (128 and 256) 22.9, 19.4; 2,048 42.5, 38.3; 65 rows of 2,048 by 12,288 15.3, 11.9, 11.2; 384 29.6, 12.7, 18.6; 197 rows of 1,358 by
-// 2,501 7.4, 11.9, 11.3; 512 12.5, 12.0, 11.5; gated, 128 rows of 4,096 by 2 x 12,288 54.7, 24.9, 36.4; 256 84.8, 43.5, 37.4; 384 of 1,358 by 2 x 1,450 13.4, 12.1, 12.5.
+// 24,576 26.7, 24.1, 33.4; 65 by 6,144 15.1, 20.8, 17.5; 128 by 24,576 49, 26.4, 37.0; 197 by 6,144 25.8, 21.4, 18.6; 256 by 4,096 15.2, 21.3, 18.5; 256 rows of 12,288 by 4,096 35.6, 53.4, 43.5; 384 of
+// 4,096 by 24,576 114, 50.0, 58.5; 512 160, 73.5, 65.4; 1,024 by 4,096 (128 and 256) 23.8, 22.0; 2,048 43.7, 39.7; 65 rows of 2,048 by 12,288 15.1, 12.5, 12.0; 384 29.5, 14.0, 20.8; 197 rows of 1,358 by
+// 2,501 7.4, 12.2, 11.6; 512 12.6, 12.3, 11.8; gated, 128 rows of 4,096 by 2 x 12,288 54.9, 25.0, 35.8; 256 86.5, 44.8, 38.0; 384 of 1,358 by 2 x 1,450 13.7, 12.0, 12.4.
 static int f8_tile_rows(int T, int tiles, int sms) {
     if (T <= 32) return T <= 16 ? 16 : 32;
     if (static_cast<long long>((T + 63) / 64) * tiles <= sms) return 64;
@@ -1256,12 +1258,12 @@ extern "C" int llm_linear_f8_silu_mul(const void* weight, void* rows, long long 
 }
 
 // Tokens whose picks stay as they are: two launches instead of five, and nothing to sort or add up.  An expert that several of them pick is read once for each, from the second
-// time on out of the second-level cache.  Measured, as they are and sorted (us), 1, 2, 4, 5 and 8 tokens: 64 experts, 8 a token, 1,024 by 2,048 15.7 and 21.2, 20.5 and 26.3, 38.6 and 43.7,
-// 51.8 and 47.2, 67.5 and 62.2; 8 experts, 2 a token, 2,048 by 4,096 18.5 and 20.6, 24.8 and 31.4, 36.0 and 42.7, 44.6 and 35.8, 48.2 and 44.9.  Up to eight picks: a cluster adds them up.
+// time on out of the second-level cache.  Measured, as they are and sorted (us), 1, 2, 4, 5 and 8 tokens: 64 experts, 8 a token, 1,024 by 2,048 15.7 and 22.2, 21.6 and 30.1, 35.5 and 40.5,
+// 51.9 and 48.3, 66.4 and 52.5; 8 experts, 2 a token, 2,048 by 4,096 18.5 and 21.2, 23.1 and 28.6, 28.7 and 32.3, 43.7 and 36.6, 47.7 and 41.7.  Up to eight picks: a cluster adds them up.
 #define F8_UNSORTED_TOKENS 4
 static bool f8_unsorted(int T, int top, bool plain) { return plain && T <= F8_UNSORTED_TOKENS && top <= 8; }
 // Routed experts: picks sorted by expert, gate and up, down, each token's rows added up.  x [T, K] of `dtype`; ids, weights [T, top]; out and base as for llm_f8_add_up.
-// work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where per is 16 and the product makes them), the
+// work: room for, each from a multiple of 256 bytes on, the sorting's results (llm_moe_f8_work has the sizes), rows of x (none where the picks stay as they are: the product makes them), the
 // middle's rows, the experts' results in float32 (none where the picks stay as they are).
 // Rows of an item, by how many picks an expert has on average.  Measured, with 16, 128 and 256 rows (us): 64 experts, 8 a token, 1,024 by 2,048, 6 picks an expert 85, 99, 130; 12: 101, 106,
 // 143; 24: 129, 114, 153; 64: 240, 122, 163; 128 (128 and 256 rows): 156, 175; 256: 246, 269; 375: 334, 343; 512: 434, 440; 1,024: 789, 762.  8 experts, 2 a token, 2,048 by 4,096, 12: 49, 55, 73; 24: 59, 55,

@@ -2598,7 +2598,7 @@ def _mx_count() -> None:
 # A weight has one float32 scale for each block of 128 x 128 values, a row one for each 128 neighbouring values: the block's largest
 # magnitude / 448.  csrc/f8_blocks.cuh says how codes are rounded and where the bytes lie.
 F8_BLOCK = 128
-# Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself; one of gate and up.
+# Rows up to which a product takes a bfloat16 matrix (whole, aligned pieces of eight values) to 8 bits itself; one of gate and up (the library's numbers, which refuses others).
 F8_PLAIN_ROWS, F8_PLAIN_ROWS_GATED = 8, 4
 F8_MOST_EXPERTS = 4096                    # that `moe_f8` routes to
 _MX_SIGNATURES.update({
@@ -2812,7 +2812,7 @@ def moe_f8(x: torch.Tensor, w_gate_up: F8Weight, w_down: F8Weight, ids: torch.Te
     The picks are sorted by expert on the device (those of up to four tokens stay as they are: two launches), each expert's rows go through its own matrices as in
     `linear_silu_mul_f8` and `linear_f8`, and a token's rows are added up in float32 in the order of its choices, times their weights (`on_input`: the weight multiplies the expert's input, that is
     its gate and up values, instead), onto `base` (float32 [T, W]) where there is one.  The result is float32 or bfloat16 [T, W],
-    rounded to that once."""
+    rounded to that once.  Where a wait runs out (`stream_status`), the result is of no use: what was not computed may have been added up all the same."""
     act = ACTIVATIONS[activation]
     _here(x, ids, weights, base)
     _i32(ids, "ids")

@@ -41,8 +41,8 @@ class Model:
         experts, recurrent and latent mixers, the embedding, the output head) stay as stored.  Layers of width 1,024 lose the products that make
         their own input by it: decode steps of up to 16 requests take 2 to 9 % longer, larger ones and prompts less time, as all steps of width 2,048 do.
         'fp8': the matrices of the parts with `hold_in_8_bits` (the same ones, and routed experts) are taken to 8 bits with a float32 scale per block of
-        128 x 128 values, and multiply rows of 8 bits with a scale per 128.  Steps of layers of width 2,048 and more take less time by it, those of width 1,024
-        and up to 32 requests up to 30 % more."""
+        128 x 128 values, and multiply rows of 8 bits with a scale per 128.  Steps of layers of width 2,048 and more take less time by it, but prompt
+        portions of 512 tokens at width 2,048, which take 3 % more; those of width 1,024 and up to 32 requests take up to 30 % more."""
         plan.validate()
         self.plan = plan
         self.dtype = _compute_dtype(dtype)

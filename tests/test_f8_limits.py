@@ -34,3 +34,9 @@ def test_more_experts_than_a_call_routes_to_are_refused_when_they_would_be_held(
     assert part.w_gate_up is before[0] and part.w_down is before[1]
     part = experts(ops.F8_MOST_EXPERTS)
     assert part.hold_in_8_bits() == 2 and part.w_gate_up == ("8 bits", (4096, 2, 2))
+
+
+def test_rows_that_a_product_makes_itself():
+    """Python leaves out the room for rows where the library says that the product makes them: the same numbers on both sides."""
+    gated, others = re.fullmatch(r"\(\(GATED\) \? (\d+) : (\d+)\)", defined("F8_PLAIN_ROWS(GATED)", "gemm_f8_tcgen05.cu")).groups()
+    assert (int(others), int(gated)) == (ops.F8_PLAIN_ROWS, ops.F8_PLAIN_ROWS_GATED)
